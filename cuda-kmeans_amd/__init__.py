@@ -27,6 +27,8 @@ UPDATE_ATOMIC_SHM2, UPDATE_FAKE, UPDATE_FAKE_SHM = 5, 6, 7  # the remaining kern
 UPDATE_SERIAL_ORDER = 8  # the sums of the serial loop (ascending point number inside a cluster), bit for bit, in O(n dim)
 UPDATE_EMULATED_ATOMICS = 0x100  # flag for the point, fine and wavefront variants: compare-and-swap loops
 
+TYPE_F32, TYPE_F16, TYPE_BF16 = 0, 1, 2  # element types of the rows of the 4-bit cache
+
 KMX_OK, KMX_ERR_INVALID_ARGUMENT, KMX_ERR_UNSUPPORTED, KMX_ERR_DEVICE, KMX_ERR_NO_DEVICE = 0, 1, 2, 3, 4
 
 # every symbol include/kmx.h declares (checked by the CPU test-suite against the built library)
@@ -37,6 +39,7 @@ ABI_SYMBOLS = [
     "kmx_graph_begin", "kmx_graph_end", "kmx_graph_launch", "kmx_graph_destroy", "kmx_event_create", "kmx_event_destroy", "kmx_event_record",
     "kmx_event_elapsed_ms", "kmx_set_profiling", "kmx_last_kernel_ms", "kmx_last_error", "kmx_certificate_tau", "kmx_certificate_unmoved_threshold",
     "kmx_update_f32_noalloc", "kmx_reserve_f32", "kmx_prepare_points_f64", "kmx_forget_points_f64", "kmx_probe_matrix_chain", "kmx_set_two_level_sweep", "kmx_iteration_f32", "kmx_iteration_last_passes",
+    "kmx_cache4_sizes", "kmx_cache4_round_levels", "kmx_cache4_write", "kmx_cache4_read", "kmx_cache4_bound", "kmx_cache4_select", "kmx_cache4_attend", "kmx_cache4_reserve",
 ]
 
 
@@ -70,6 +73,19 @@ class DatasetSpec(ctypes.Structure):
                 ("iterations", ctypes.c_uint32), ("kind", ctypes.c_uint32), ("weights", ctypes.c_uint32),
                 ("centres", ctypes.c_uint32), ("lo", ctypes.c_double), ("hi", ctypes.c_double),
                 ("centre_sigma", ctypes.c_double), ("sigma", ctypes.c_double)]
+
+
+class Cache4Struct(ctypes.Structure):
+    """= kmx_cache4."""
+    _fields_ = [("blocks", ctypes.c_void_p), ("bounds", ctypes.c_void_p), ("levels", ctypes.c_void_p), ("heads", ctypes.c_uint32),
+                ("dim", ctypes.c_uint32), ("page_tokens", ctypes.c_uint32), ("page_count", ctypes.c_uint32)]
+
+
+class Cache4BatchStruct(ctypes.Structure):
+    """= kmx_cache4_batch."""
+    _fields_ = [("sequences", ctypes.c_uint32), ("query_heads", ctypes.c_uint32), ("tokens", ctypes.c_uint32), ("max_queries", ctypes.c_uint32),
+                ("max_length", ctypes.c_uint32), ("table_stride", ctypes.c_uint32), ("starts", ctypes.c_void_p), ("lengths", ctypes.c_void_p),
+                ("table", ctypes.c_void_p)]
 
 
 def build(force=True):
@@ -139,6 +155,15 @@ def hip_lib():
         lib.kmx_set_two_level_sweep.argtypes = [ctypes.c_int]
         lib.kmx_iteration_f32.argtypes = [vp, ctypes.c_int, sz, vp, vp, ctypes.c_int, sz, vp, vp, u32, u32, u32, ctypes.POINTER(ExecParams)]
         lib.kmx_iteration_last_passes.argtypes = [ctypes.POINTER(ctypes.c_int)]
+        cache, batch = ctypes.POINTER(Cache4Struct), ctypes.POINTER(Cache4BatchStruct)
+        lib.kmx_cache4_sizes.argtypes = [cache, ctypes.POINTER(sz), ctypes.POINTER(sz)]
+        lib.kmx_cache4_round_levels.argtypes = [vp, u32, vp]
+        lib.kmx_cache4_write.argtypes = [cache, ctypes.c_int, vp, vp, sz, sz, vp, u32]
+        lib.kmx_cache4_read.argtypes = lib.kmx_cache4_write.argtypes
+        lib.kmx_cache4_bound.argtypes = [cache, vp, vp, u32]
+        lib.kmx_cache4_select.argtypes = [cache, batch, ctypes.c_int, vp, sz, sz, vp, u32, u32, u32, ctypes.c_int]
+        lib.kmx_cache4_attend.argtypes = [cache, batch, ctypes.c_int, vp, sz, sz, vp, sz, sz, vp, ctypes.c_float, ctypes.c_int, vp, u32]
+        lib.kmx_cache4_reserve.argtypes = [cache, batch, u32]
         _hip = lib
     return _hip
 
@@ -272,6 +297,18 @@ class DeviceBuffer:
             self.free()
         except Exception:
             pass
+
+
+class DeviceView:
+    """Borrowed device memory (another library's allocation on the current device, a part of a DeviceBuffer): an address and its bytes."""
+
+    def __init__(self, address, nbytes):
+        self.nbytes = int(nbytes)
+        self._ptr = ctypes.c_void_p(int(address))
+
+    @property
+    def ptr(self):
+        return self._ptr
 
 
 class Event:
@@ -469,6 +506,82 @@ def last_rechecked():
     c = ctypes.c_uint64(0)
     check(hip_lib().kmx_assign_last_rechecked(ctypes.byref(c)))
     return c.value
+
+
+# ---------------------------------------------------------------- a cache in 4 bits --------------
+
+def cache4_round_levels(levels):
+    """Learned levels (..., 8), ascending within 0 and 1, as the cache takes them: 6 significant bits, float16 (kmx_cache4_round_levels)."""
+    a = np.ascontiguousarray(levels, dtype=np.float32)
+    if a.ndim == 0 or a.shape[-1] != 8:
+        raise ValueError("a set has 8 levels")
+    out = np.empty(a.shape, np.float16)
+    check(hip_lib().kmx_cache4_round_levels(a.ctypes.data, a.size // 8, out.ctypes.data))
+    return out
+
+
+class Cache4Batch:
+    """Queries of some sequences (kmx_cache4_batch): `tokens` rows in all, starts, lengths and table in device memory."""
+
+    def __init__(self, sequences, query_heads, tokens, max_queries, max_length, starts, lengths, table, table_stride):
+        self.query_heads = query_heads
+        self._buffers = (starts, lengths, table)  # kept alive
+        self._batch = Cache4BatchStruct(sequences, query_heads, tokens, max_queries, max_length, table_stride, starts.ptr, lengths.ptr, table.ptr)
+        self.ref = ctypes.byref(self._batch)
+
+
+class Cache4:
+    """Keys and values of `heads` heads in 4 bits, in `pages` pages of `page_tokens` tokens (kmx_cache4). Buffers have a .ptr (DeviceBuffer,
+    DeviceView); element strides default to rows without gaps. Calls enqueue and return."""
+
+    def __init__(self, heads, dim, page_tokens, pages, levels, blocks, bounds=None):
+        self.heads, self.dim, self.page_tokens, self.pages = heads, dim, page_tokens, pages
+        self._buffers = (levels, blocks, bounds)  # kept alive
+        self._cache = Cache4Struct(blocks.ptr, bounds.ptr if bounds is not None else None, levels.ptr, heads, dim, page_tokens, pages)
+        self.ref = ctypes.byref(self._cache)
+
+    @staticmethod
+    def sizes(heads, dim, page_tokens, pages):
+        """Bytes of `blocks` and of `bounds`."""
+        cache = Cache4Struct(None, None, None, heads, dim, page_tokens, pages)
+        blocks, bounds = ctypes.c_size_t(0), ctypes.c_size_t(0)
+        check(hip_lib().kmx_cache4_sizes(ctypes.byref(cache), ctypes.byref(blocks), ctypes.byref(bounds)))
+        return blocks.value, bounds.value
+
+    def _strides(self, heads, token_stride, head_stride):
+        head_stride = self.dim if head_stride is None else head_stride
+        return heads * head_stride if token_stride is None else token_stride, head_stride
+
+    def write(self, element_type, keys, values, slots, tokens, token_stride=None, head_stride=None):
+        """Quantises rows and keeps them at their places (kmx_cache4_write)."""
+        strides = self._strides(self.heads, token_stride, head_stride)
+        check(hip_lib().kmx_cache4_write(self.ref, element_type, keys.ptr, values.ptr, *strides, slots.ptr, tokens))
+
+    def read(self, element_type, keys, values, slots, tokens, token_stride=None, head_stride=None):
+        """The rows at the places, as the cache holds them (kmx_cache4_read)."""
+        strides = self._strides(self.heads, token_stride, head_stride)
+        check(hip_lib().kmx_cache4_read(self.ref, element_type, keys.ptr, values.ptr, *strides, slots.ptr, tokens))
+
+    def bound(self, pages, counts, count):
+        """Bounds of `count` pages with counts[] written tokens (kmx_cache4_bound)."""
+        check(hip_lib().kmx_cache4_bound(self.ref, pages.ptr, counts.ptr, count))
+
+    def select(self, batch, element_type, q, chosen, top, first=1, last=1, causal=True, q_token_stride=None, q_head_stride=None):
+        """The `top` pages that each query and head look at (kmx_cache4_select)."""
+        strides = self._strides(batch.query_heads, q_token_stride, q_head_stride)
+        check(hip_lib().kmx_cache4_select(self.ref, batch.ref, element_type, q.ptr, *strides, chosen.ptr, top, first, last, int(causal)))
+
+    def attend(self, batch, element_type, q, out, scale, causal=True, lse=None, chosen=None, top=0, q_token_stride=None, q_head_stride=None,
+               out_token_stride=None, out_head_stride=None):
+        """Attention of the queries to the cached tokens, or to those of chosen pages (kmx_cache4_attend)."""
+        strides = self._strides(batch.query_heads, q_token_stride, q_head_stride)
+        out_strides = self._strides(batch.query_heads, out_token_stride, out_head_stride)
+        check(hip_lib().kmx_cache4_attend(self.ref, batch.ref, element_type, q.ptr, *strides, out.ptr, *out_strides, lse.ptr if lse is not None else None,
+                                          scale, int(causal), chosen.ptr if chosen is not None else None, top))
+
+    def reserve(self, batch, top=0):
+        """Sizes the work space for attention on such a batch, and to `top` chosen pages (kmx_cache4_reserve)."""
+        check(hip_lib().kmx_cache4_reserve(self.ref, batch.ref, top))
 
 
 # ---------------------------------------------------------------- algorithm objects --------------

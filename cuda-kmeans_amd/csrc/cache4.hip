@@ -1,0 +1,857 @@
+/*
+ * The 4-bit cache: rows quantised as they are written and read back, bounds of its pages, the choice of pages by an 8-bit score, and the
+ * C entry points of all of it (include/kmx.h, kmx_cache4_*). The attention that reads it is in cache4_attend_impl.h.
+ */
+#include "cache4.h"
+
+#include <cmath>
+#include <cstring>
+
+namespace kmx {
+
+/* ---------------------------------------------------------------- writing and reading rows ------- */
+
+struct Rows4 {
+	Cache4 cache;
+	void* keys; void* values;
+	size_t token_stride, head_stride;
+	const int32_t* slots;
+	uint32_t tokens;
+	bool vec;
+};
+
+/* the scale of a group: its largest magnitude with 5 significant bits (ties to the even one), at most 31 * 2^11 */
+__device__ __forceinline__ _Float16 group_scale(float largest)
+{
+	uint32_t u = __builtin_bit_cast(uint32_t, fminf(largest, 65504.0f));
+	u = (u + 0x3FFFFu + ((u >> 19) & 1u)) & ~0x7FFFFu;
+	return (_Float16)fminf(__builtin_bit_cast(float, u), 63488.0f);
+}
+
+/* the 8 codes of one lane's channels, nibble i for channel i: the number of edges scale * (L_j + L_j+1) / 2 that |x| lies above (three
+ * comparisons; NaN lies above none), and the sign */
+__device__ __forceinline__ uint32_t codes8(const float x[8], float scale, const float middle[7])
+{
+	float edge[7];
+	for (int j = 0; j < 7; ++j) edge[j] = scale * middle[j];
+	uint32_t codes = 0;
+	for (int i = 0; i < 8; ++i) {
+		const float size = fabsf(x[i]);
+		const bool b2 = size > edge[3];
+		const bool b1 = size > (b2 ? edge[5] : edge[1]);
+		const float last = b2 ? (b1 ? edge[6] : edge[4]) : (b1 ? edge[2] : edge[0]);
+		const uint32_t code = (b2 ? 4u : 0u) | (b1 ? 2u : 0u) | (size > last ? 1u : 0u) | (x[i] < 0.0f ? 8u : 0u);
+		codes |= code << (4 * i);
+	}
+	return codes;
+}
+
+__device__ __forceinline__ uint32_t nibbles_to_bytes(uint32_t w) /* four nibbles, one a byte */
+{
+	w = (w | w << 8) & 0x00FF00FFu;
+	return (w | w << 4) & 0x0F0F0F0Fu;
+}
+
+/*
+ * A wavefront takes 16 tokens of one head; lane = 4 token + g holds channels 32 j + 8 g .. + 7 of each group j, so a group is four lanes and its
+ * maximum two exchanges inside them. The keys' words go out as they stand (J side by side a lane); the values' bytes pass through LDS, 16
+ * tokens of a pair side by side, and leave as 16 bytes a lane where the 16 tokens fill a block in order, else byte by byte.
+ */
+template <int J, typename T>
+__global__ void __launch_bounds__(256)
+write4_kernel(Rows4 a)
+{
+	constexpr uint32_t D = 32 * J;
+	__shared__ __attribute__((aligned(16))) uint8_t lds[4][16 * 16 * J];
+	const uint32_t wave = threadIdx.x / WAVE, lane = threadIdx.x % WAVE, t = lane / 4, g = lane % 4;
+	const uint64_t unit = (uint64_t)blockIdx.x * 4 + wave;
+	const uint32_t head = (uint32_t)(unit % a.cache.heads);
+	const uint64_t first = unit / a.cache.heads * 16;
+	if (first >= a.tokens) return; /* (no barriers below: a wavefront's LDS is its own) */
+	const uint64_t token = first + t;
+	const int32_t slot = token < a.tokens ? a.slots[token] : -1;
+	const uint64_t places = (uint64_t)a.cache.page_count << a.cache.page_shift;
+	const bool there = slot >= 0 && (uint64_t)slot < places;
+	const uint32_t page = (uint32_t)slot >> a.cache.page_shift, place = (uint32_t)slot & ((1u << a.cache.page_shift) - 1);
+	uint8_t* const block = a.cache.blocks + (there ? block_offset<J>(a.cache, page, head, place / 16) : 0);
+	const uint32_t at = place % 16;
+	uint8_t* const mine = lds[wave];
+
+	for (int which = 0; which < 2; ++which) {
+		float middle[7];
+		{
+			const uint16_t* l = a.cache.levels + ((size_t)head * 2 + which) * 8;
+			float below = (float)__builtin_bit_cast(_Float16, l[0]);
+			for (int j = 0; j < 7; ++j) {
+				const float above = (float)__builtin_bit_cast(_Float16, l[j + 1]);
+				middle[j] = (below + above) * 0.5f;
+				below = above;
+			}
+		}
+		const T* row = (const T*)(which ? a.values : a.keys) + (there ? token * a.token_stride : 0) + head * a.head_stride + 8 * g;
+		float x[J][8];
+#pragma unroll
+		for (int j = 0; j < J; ++j) {
+			if (there) load8(row + 32 * j, a.vec, x[j]);
+			else
+				for (int i = 0; i < 8; ++i) x[j][i] = 0.0f;
+		}
+		uint32_t codes[J];
+		_Float16 scale[J];
+#pragma unroll
+		for (int j = 0; j < J; ++j) {
+			float largest = 0.0f; /* fmaxf leaves NaN out */
+			for (int i = 0; i < 8; ++i) largest = fmaxf(largest, fabsf(x[j][i]));
+			largest = fmaxf(largest, dpp<DPP_XOR1>(largest));
+			largest = fmaxf(largest, dpp<DPP_XOR2>(largest));
+			scale[j] = group_scale(largest);
+			codes[j] = codes8(x[j], (float)scale[j], middle);
+		}
+		if (which == 0) {
+			if (there) {
+				uint32_t* out = (uint32_t*)(block + at * (D / 2) + g * 4 * J);
+#pragma unroll
+				for (int j = 0; j < J; ++j) out[j] = nibbles_to_bytes(codes[j] & 0xFFFFu) | nibbles_to_bytes(codes[j] >> 16) << 4;
+				if (g == 0)
+#pragma unroll
+					for (int j = 0; j < J; ++j) ((_Float16*)(block + 16 * D))[at * J + j] = scale[j];
+			}
+		} else {
+#pragma unroll
+			for (int j = 0; j < J; ++j) {
+				/* lanes g and g + 2 hold the two channels of 8 pairs: each makes the bytes of four */
+				const uint32_t other = dpp<DPP_XOR2>(codes[j]), half = g / 2;
+				const uint32_t low = (half ? other : codes[j]) >> (16 * half), high = (half ? codes[j] : other) >> (16 * half);
+				const uint32_t bytes = nibbles_to_bytes(low & 0xFFFFu) | nibbles_to_bytes(high & 0xFFFFu) << 4;
+				const uint32_t pair = 16 * j + 8 * (g & 1) + 4 * half;
+				for (int b = 0; b < 4; ++b) mine[(pair + b) * 16 + t] = (uint8_t)(bytes >> (8 * b));
+			}
+			if (there && g == 0)
+#pragma unroll
+				for (int j = 0; j < J; ++j) ((_Float16*)(block + 17 * D))[16 * j + at] = scale[j];
+			__builtin_amdgcn_wave_barrier();
+			const uint32_t slot0 = (uint32_t)__builtin_amdgcn_readfirstlane(slot);
+			if (__ballot(!there || (uint32_t)slot != slot0 + t) == 0 && slot0 % 16 == 0) {
+				for (uint32_t p = lane; p < D / 2; p += WAVE) *(u32x4*)(block + 8 * D + p * 16) = *(const u32x4*)(mine + p * 16);
+			} else {
+				for (uint32_t n = 0; n < 16; ++n) {
+					const int32_t s = __builtin_amdgcn_readlane(slot, 4 * n);
+					if (s < 0 || (uint64_t)s >= places) continue;
+					const uint32_t pl = (uint32_t)s & ((1u << a.cache.page_shift) - 1);
+					uint8_t* out = a.cache.blocks + block_offset<J>(a.cache, (uint32_t)s >> a.cache.page_shift, head, pl / 16) + 8 * D + pl % 16;
+					for (uint32_t p = lane; p < D / 2; p += WAVE) out[p * 16] = mine[p * 16 + n];
+				}
+			}
+		}
+	}
+}
+
+/* The same lanes backwards; a place outside the cache reads as zeros. */
+template <int J, typename T>
+__global__ void __launch_bounds__(256)
+read4_kernel(Rows4 a)
+{
+	constexpr uint32_t D = 32 * J, ROW = D / 2 + 8; /* LDS: the values' bytes token by token, rows 8 bytes apart in the banks */
+	__shared__ __attribute__((aligned(16))) uint8_t lds[4][16 * ROW];
+	const uint32_t wave = threadIdx.x / WAVE, lane = threadIdx.x % WAVE, t = lane / 4, g = lane % 4;
+	const uint64_t unit = (uint64_t)blockIdx.x * 4 + wave;
+	const uint32_t head = (uint32_t)(unit % a.cache.heads);
+	const uint64_t first = unit / a.cache.heads * 16;
+	if (first >= a.tokens) return;
+	const uint64_t token = first + t;
+	const int32_t slot = token < a.tokens ? a.slots[token] : -1;
+	const uint64_t places = (uint64_t)a.cache.page_count << a.cache.page_shift;
+	const bool there = slot >= 0 && (uint64_t)slot < places;
+	const uint32_t page = (uint32_t)slot >> a.cache.page_shift, place = (uint32_t)slot & ((1u << a.cache.page_shift) - 1);
+	const uint8_t* const block = a.cache.blocks + (there ? block_offset<J>(a.cache, page, head, place / 16) : 0);
+	const uint32_t at = place % 16;
+	uint8_t* const mine = lds[wave];
+
+	/* the values' bytes into LDS */
+	const uint32_t slot0 = (uint32_t)__builtin_amdgcn_readfirstlane(slot);
+	if (__ballot(!there || (uint32_t)slot != slot0 + t) == 0 && slot0 % 16 == 0) {
+		for (uint32_t p = lane; p < D / 2; p += WAVE) {
+			const u32x4 w = *(const u32x4*)(block + 8 * D + p * 16);
+			for (int n = 0; n < 16; ++n) mine[n * ROW + p] = (uint8_t)(w[n / 4] >> (8 * (n % 4)));
+		}
+	} else {
+		for (uint32_t n = 0; n < 16; ++n) {
+			const int32_t s = __builtin_amdgcn_readlane(slot, 4 * n);
+			if (s < 0 || (uint64_t)s >= places) continue;
+			const uint32_t pl = (uint32_t)s & ((1u << a.cache.page_shift) - 1);
+			const uint8_t* in = a.cache.blocks + block_offset<J>(a.cache, (uint32_t)s >> a.cache.page_shift, head, pl / 16) + 8 * D + pl % 16;
+			for (uint32_t p = lane; p < D / 2; p += WAVE) mine[n * ROW + p] = in[p * 16];
+		}
+	}
+	__builtin_amdgcn_wave_barrier();
+	if (token >= a.tokens) return;
+	for (int which = 0; which < 2; ++which) {
+		const Magnitudes m = load_magnitudes(a.cache.levels, head, which);
+		T* row = (T*)(which ? a.values : a.keys) + token * a.token_stride + head * a.head_stride + 8 * g;
+#pragma unroll
+		for (int j = 0; j < J; ++j) {
+			uint32_t w[4] = { 0, 0, 0, 0 };
+			float scale = 0.0f;
+			if (there) {
+				if (which == 0) {
+					const uint32_t c = ((const uint32_t*)(block + at * (D / 2) + g * 4 * J))[j];
+					unpack4<false>(c, m, w[0], w[1]);
+					unpack4<true>(c, m, w[2], w[3]);
+					scale = (float)((const _Float16*)(block + 16 * D))[at * J + j];
+				} else {
+					const u32x2 c = *(const u32x2*)(mine + t * ROW + 16 * j + 8 * (g & 1));
+					unpack4<false>(c[0] >> (4 * (g / 2)), m, w[0], w[1]);
+					unpack4<false>(c[1] >> (4 * (g / 2)), m, w[2], w[3]);
+					scale = (float)((const _Float16*)(block + 17 * D))[16 * j + at];
+				}
+			}
+			float x[8];
+			for (int i = 0; i < 8; ++i) x[i] = scale * (float)__builtin_bit_cast(half2v, w[i / 2])[i % 2];
+			store8(row + 32 * j, a.vec, x);
+		}
+	}
+}
+
+template <typename T>
+static int launch_rows4(bool write, const Rows4& a, uint32_t J)
+{
+	const uint64_t units = ((uint64_t)a.tokens + 15) / 16 * a.cache.heads, groups = (units + 3) / 4;
+	if (groups > 0x7FFFFFFFu) return fail(KMX_ERR_UNSUPPORTED, "kmx_cache4_%s: %u tokens of %u heads are too many for one call", write ? "write" : "read", a.tokens, a.cache.heads);
+	const dim3 grid((unsigned)groups), block(256);
+	switch (J) {
+#define KMX_CASE(N)                                                                                                     \
+	case N:                                                                                                               \
+		if (write) KMX_LAUNCH_KERNEL((write4_kernel<N, T>), grid, block, 0, stream(), a);                                  \
+		else KMX_LAUNCH_KERNEL((read4_kernel<N, T>), grid, block, 0, stream(), a);                                         \
+		break;
+		KMX_CASE(1) KMX_CASE(2) KMX_CASE(3) KMX_CASE(4) KMX_CASE(5) KMX_CASE(6) KMX_CASE(7) KMX_CASE(8)
+#undef KMX_CASE
+	}
+	KMX_LAUNCH_CHECK("write4_kernel / read4_kernel");
+	return KMX_OK;
+}
+
+/* ---------------------------------------------------------------- bounds of pages ---------------- */
+
+/* A wavefront takes a page and head: lane = 4 token + g keeps the largest and the smallest value of its channels over its tokens of all
+ * blocks, then the 16 lanes of a g join theirs. Values are products of half-precision numbers, exact in floats, and maxima know no order. */
+template <int J>
+__global__ void __launch_bounds__(256)
+bound4_kernel(Cache4 c, const int32_t* __restrict__ pages, const int32_t* __restrict__ counts, uint32_t count)
+{
+	constexpr uint32_t D = 32 * J;
+	const uint32_t wave = threadIdx.x / WAVE, lane = threadIdx.x % WAVE, t = lane / 4, g = lane % 4;
+	const uint64_t unit = (uint64_t)blockIdx.x * 4 + wave;
+	const uint64_t entry = unit / c.heads;
+	const uint32_t head = (uint32_t)(unit % c.heads);
+	if (entry >= count) return;
+	const int32_t page = pages[entry];
+	if (page < 0 || (uint32_t)page >= c.page_count) return;
+	const int32_t room = 1 << c.page_shift;
+	const int32_t tokens = counts[entry] < 0 ? 0 : counts[entry] < room ? counts[entry] : room;
+	const Magnitudes m = load_magnitudes(c.levels, head, 0);
+	float hi[8 * J], lo[8 * J];
+#pragma unroll
+	for (int i = 0; i < 8 * J; ++i) { hi[i] = -__builtin_inff(); lo[i] = __builtin_inff(); }
+	for (int32_t from = 0; from < tokens; from += 16) {
+		const uint8_t* block = c.blocks + block_offset<J>(c, (uint32_t)page, head, from / 16);
+		if (from + (int32_t)t < tokens) {
+			const uint32_t* codes = (const uint32_t*)(block + t * (D / 2) + g * 4 * J);
+			const _Float16* scales = (const _Float16*)(block + 16 * D) + t * J;
+#pragma unroll
+			for (int j = 0; j < J; ++j) {
+				uint32_t w[4];
+				unpack4<false>(codes[j], m, w[0], w[1]);
+				unpack4<true>(codes[j], m, w[2], w[3]);
+				const float scale = (float)scales[j];
+#pragma unroll
+				for (int i = 0; i < 8; ++i) {
+					const float x = scale * (float)__builtin_bit_cast(half2v, w[i / 2])[i % 2];
+					hi[8 * j + i] = fmaxf(hi[8 * j + i], x);
+					lo[8 * j + i] = fminf(lo[8 * j + i], x);
+				}
+			}
+		}
+	}
+	float largest = 0.0f;
+#pragma unroll
+	for (int i = 0; i < 8 * J; ++i) {
+		hi[i] = fmaxf(hi[i], dpp<DPP_ROR4>(hi[i]));
+		lo[i] = fminf(lo[i], dpp<DPP_ROR4>(lo[i]));
+		hi[i] = fmaxf(hi[i], dpp<DPP_ROR8>(hi[i]));
+		lo[i] = fminf(lo[i], dpp<DPP_ROR8>(lo[i]));
+		for (int x = 16; x < 64; x *= 2) {
+			hi[i] = fmaxf(hi[i], __shfl_xor(hi[i], x));
+			lo[i] = fminf(lo[i], __shfl_xor(lo[i], x));
+		}
+		if (tokens == 0) hi[i] = lo[i] = 0.0f;
+		largest = fmaxf(largest, fmaxf(fabsf(hi[i]), fabsf(lo[i])));
+	}
+	largest = fmaxf(largest, dpp<DPP_XOR1>(largest));
+	largest = fmaxf(largest, dpp<DPP_XOR2>(largest));
+	const float by = largest > 0.0f ? 127.0f / largest : 0.0f;
+	int8_t* out = c.bounds + ((size_t)page * c.heads + head) * (2 * D);
+#pragma unroll
+	for (int j = 0; j < J; ++j) {
+		if (t != (uint32_t)j) continue; /* lane 4 j + g writes group j */
+		uint32_t h[2] = { 0, 0 }, l[2] = { 0, 0 };
+#pragma unroll
+		for (int i = 0; i < 8; ++i) { /* outwards, so that a bound stays one */
+			const int up = (int)fminf(fmaxf(ceilf(hi[8 * j + i] * by), -127.0f), 127.0f);
+			const int down = (int)fminf(fmaxf(floorf(lo[8 * j + i] * by), -127.0f), 127.0f);
+			h[i / 4] |= (uint32_t)(up & 0xFF) << (8 * (i % 4));
+			l[i / 4] |= (uint32_t)(down & 0xFF) << (8 * (i % 4));
+		}
+		*(u32x2*)(out + 32 * j + 8 * g) = u32x2{ h[0], h[1] };
+		*(u32x2*)(out + D + 32 * j + 8 * g) = u32x2{ l[0], l[1] };
+	}
+	if (lane == 0) c.bound_scales[(size_t)page * c.heads + head] = largest / 127.0f;
+}
+
+/* ---------------------------------------------------------------- the choice of pages ------------ */
+
+struct Select4 {
+	Cache4 cache;
+	Batch4 batch;
+	const void* q; size_t q_token, q_head;
+	uint32_t* keys;     /* [token][head][table_stride], larger for a better page */
+	int32_t* chosen;    /* [token][head][top] */
+	uint32_t top, first, last;
+	uint32_t span;      /* query heads of a token side by side: the power of two from `group` on, at most 16 */
+	uint32_t token_tiles, chunks, chunk; /* tiles of queries a sequence; parts of the pages and how many tiles of 16 each */
+	bool bf16, vec;
+};
+
+/* floats in the order of unsigned words */
+__device__ __forceinline__ uint32_t ordered(float v)
+{
+	const uint32_t u = __builtin_bit_cast(uint32_t, v);
+	return u & 0x80000000u ? ~u : u | 0x80000000u;
+}
+
+__device__ __forceinline__ void load_query16(const Select4& a, const void* q, bool there, float x[16])
+{
+	if (!there) {
+		for (int i = 0; i < 16; ++i) x[i] = 0.0f;
+	} else if (a.bf16) {
+		load8((const __bf16*)q, a.vec, x);
+		load8((const __bf16*)q + 8, a.vec, x + 8);
+	} else {
+		load8((const _Float16*)q, a.vec, x);
+		load8((const _Float16*)q + 8, a.vec, x + 8);
+	}
+}
+
+/*
+ * The score of a page: the bound on q . k over its keys, in 8 bits. A wavefront keeps 16 rows of queries (16 / span tokens of one head of the
+ * cache) as 8-bit columns of v_mfma_i32_16x16x64_i8: the positive parts against the largest values, the negative ones against the smallest.
+ * Whole numbers below 2^24, the same in any order. Bounds are read once, 16 bytes a lane: the kernel is bound by that, and by its launch.
+ */
+template <int J>
+__global__ void __launch_bounds__(256)
+score4_kernel(Select4 a)
+{
+	constexpr uint32_t D = 32 * J;
+	const uint32_t wave = threadIdx.x / WAVE, lane = threadIdx.x % WAVE, col = lane % 16, kg = lane / 16;
+	uint32_t unit = blockIdx.x;
+	const uint32_t part = unit % a.chunks;
+	unit /= a.chunks;
+	const uint32_t head = unit % a.cache.heads;
+	unit /= a.cache.heads;
+	const uint32_t tile = unit % a.token_tiles, s = unit / a.token_tiles;
+	const Sequence seq = sequence_of(a.batch, s, a.cache.page_shift);
+	const uint32_t per = 16 / a.span, i = tile * per + col / a.span;
+	if (tile * per >= seq.queries) return;
+	const uint32_t page_tokens = 1u << a.cache.page_shift;
+	const uint32_t last_i = min(seq.queries - 1, tile * per + per - 1);
+	const uint32_t pages = (visible_to(a.batch, seq, last_i) + page_tokens - 1) >> a.cache.page_shift;
+	uint32_t p0 = (part * a.chunk * 4 + wave) * 16; /* the wavefronts of a part take its tiles in turn */
+	if (part * a.chunk * 64 >= pages) return;
+	const bool token_there = i < seq.queries;
+
+	/* the scale of the queries of each token and head: their largest magnitude, over all its query heads */
+	float largest = 0.0f;
+	const char* q = (const char*)a.q + 2 * ((size_t)(seq.first + (token_there ? i : 0)) * a.q_token + (size_t)head * a.batch.group * a.q_head);
+	float x[16];
+	for (uint32_t h0 = 0; h0 < a.batch.group; h0 += 16) {
+		const uint32_t h = h0 + col % a.span;
+		const bool there = token_there && h < a.batch.group;
+#pragma unroll
+		for (int c = 0; c < J; ++c) {
+			load_query16(a, q + 2 * ((size_t)(there ? h : 0) * a.q_head + (64 * c + 16 * kg) % D), there, x);
+			for (int n = 0; n < 16; ++n) largest = fmaxf(largest, fabsf(x[n]));
+		}
+	}
+	for (uint32_t d = 1; d < a.span; d *= 2) largest = fmaxf(largest, __shfl_xor(largest, (int)d));
+	for (int d = 16; d < 64; d *= 2) largest = fmaxf(largest, __shfl_xor(largest, d));
+	const float by = largest > 0.0f ? 127.0f / largest : 0.0f;
+
+	const uint32_t tiles = a.batch.group > 16 ? (a.batch.group + 15) / 16 : 1;
+	i32x4 q8[J];
+	for (uint32_t n = 0; n < a.chunk; ++n, p0 += 64) {
+		if (p0 >= pages) break;
+		const uint32_t p = p0 + col;
+		const int32_t page = p < pages ? a.batch.table[(size_t)s * a.batch.table_stride + p] : -1;
+		const bool there = page >= 0 && (uint32_t)page < a.cache.page_count;
+		const int8_t* bounds = a.cache.bounds + ((size_t)(there ? page : 0) * a.cache.heads + head) * (2 * D) + 16 * kg;
+		const float scale = there ? a.cache.bound_scales[(size_t)page * a.cache.heads + head] : 0.0f;
+		i32x4 b[J];
+#pragma unroll
+		for (int c = 0; c < J; ++c) b[c] = *(const i32x4*)(bounds + 64 * c);
+		int best[4] = { INT32_MIN, INT32_MIN, INT32_MIN, INT32_MIN };
+		for (uint32_t g0 = 0; g0 < tiles; ++g0) {
+			const uint32_t h = g0 * 16 + col % a.span;
+			const bool row_there = token_there && h < a.batch.group;
+			if (n == 0 || tiles > 1) {
+#pragma unroll
+				for (int c = 0; c < J; ++c) {
+					const uint32_t at = 64 * c + 16 * kg;
+					load_query16(a, q + 2 * ((size_t)(row_there ? h : 0) * a.q_head + at % D), row_there, x);
+					for (int w = 0; w < 4; ++w) {
+						uint32_t word = 0;
+						for (int e = 0; e < 4; ++e) {
+							float v = x[4 * w + e] * by;
+							v = v != v ? 0.0f : fminf(fmaxf(rintf(v), -127.0f), 127.0f);
+							v = at < D ? fmaxf(v, 0.0f) : fminf(v, 0.0f);
+							word |= (uint32_t)((int)v & 0xFF) << (8 * e);
+						}
+						q8[c][w] = (int)word;
+					}
+				}
+			}
+			i32x4 dot{ 0, 0, 0, 0 };
+#pragma unroll
+			for (int c = 0; c < J; ++c) dot = __builtin_amdgcn_mfma_i32_16x16x64_i8(b[c], q8[c], dot, 0, 0, 0);
+			/* lane: query row col, pages p0 + 4 kg + r */
+			for (int r = 0; r < 4; ++r) best[r] = max(best[r], row_there ? dot[r] : INT32_MIN);
+		}
+		for (int r = 0; r < 4; ++r) {
+			for (uint32_t d = 1; d < a.span; d *= 2) best[r] = max(best[r], __shfl_xor(best[r], (int)d));
+			const float sc = __shfl(scale, (int)(4 * kg + r)); /* (lanes 0 to 15 hold the scales of the tile's pages) */
+			const int known = __shfl(there ? 1 : 0, (int)(4 * kg + r));
+			const uint32_t pr = p0 + 4 * kg + r;
+			if (!token_there || pr >= pages || (r & (a.span - 1)) != (col & (a.span - 1) & 3) || (col % a.span) > 3) continue;
+			const uint32_t seen = (visible_to(a.batch, seq, i) + page_tokens - 1) >> a.cache.page_shift;
+			if (pr >= seen) continue;
+			const bool forced = pr < a.first || pr + a.last >= seen;
+			const float score = forced ? __builtin_inff() : known ? (float)best[r] * sc + 0.0f : -__builtin_inff(); /* (+ 0: one zero) */
+			a.keys[((size_t)(seq.first + i) * a.cache.heads + head) * a.batch.table_stride + pr] = ordered(score);
+		}
+	}
+}
+
+/*
+ * The `top` best pages of each token and head, ascending: the threshold by four passes over 8 bits of the scores, then one pass in the order
+ * of the pages that keeps what lies above it and as many at the threshold as are left, the lowest first. One work-group each.
+ */
+__global__ void __launch_bounds__(256)
+choose4_kernel(Select4 a)
+{
+	__shared__ uint32_t histogram[256];
+	__shared__ uint32_t found[2];
+	__shared__ uint32_t above[4], equal[4];
+	const uint32_t tid = threadIdx.x, wave = tid / WAVE, lane = tid % WAVE;
+	uint32_t unit = blockIdx.x;
+	const uint32_t head = unit % a.cache.heads;
+	unit /= a.cache.heads;
+	const uint32_t i = unit % a.batch.max_queries, s = unit / a.batch.max_queries;
+	const Sequence seq = sequence_of(a.batch, s, a.cache.page_shift);
+	if (i >= seq.queries) return;
+	const uint32_t n = (visible_to(a.batch, seq, i) + (1u << a.cache.page_shift) - 1) >> a.cache.page_shift;
+	const size_t row = (size_t)(seq.first + i) * a.cache.heads + head;
+	int32_t* out = a.chosen + row * a.top;
+	if (n <= a.top) {
+		for (uint32_t e = tid; e < a.top; e += 256) out[e] = e < n ? (int32_t)e : -1;
+		return;
+	}
+	const uint32_t* keys = a.keys + row * a.batch.table_stride;
+	uint32_t prefix = 0, mask = 0, rest = a.top; /* the rest-th largest among the keys that agree with the prefix */
+	for (int shift = 24; shift >= 0; shift -= 8) {
+		histogram[tid] = 0;
+		__syncthreads();
+		for (uint32_t p = tid; p < n; p += 256) {
+			const uint32_t k = keys[p];
+			if ((k & mask) == prefix) atomicAdd(&histogram[(k >> shift) & 255u], 1u);
+		}
+		__syncthreads();
+		if (wave == 0) { /* lane l: digits 255 - 4 l and the three below */
+			uint32_t sum = 0;
+			for (int e = 0; e < 4; ++e) sum += histogram[255 - 4 * lane - e];
+			uint32_t upto = sum;
+			for (int d = 1; d < WAVE; d *= 2) {
+				const uint32_t v = __shfl_up(upto, d);
+				if (lane >= (uint32_t)d) upto += v;
+			}
+			uint32_t before = upto - sum;
+			if (before < rest && rest <= upto) {
+				for (int e = 0; e < 4; ++e) {
+					const uint32_t h = histogram[255 - 4 * lane - e];
+					if (rest <= before + h) {
+						found[0] = 255 - 4 * lane - e;
+						found[1] = rest - before;
+						break;
+					}
+					before += h;
+				}
+			}
+		}
+		__syncthreads();
+		prefix |= found[0] << shift;
+		mask |= 255u << shift;
+		rest = found[1];
+		__syncthreads();
+	}
+	uint32_t written = 0, ties = 0;
+	for (uint32_t from = 0; from < n; from += 256) {
+		const uint32_t p = from + tid;
+		const uint32_t k = p < n ? keys[p] : 0;
+		const bool is_above = p < n && k > prefix, is_equal = p < n && k == prefix;
+		const uint64_t ballot_above = __ballot(is_above), ballot_equal = __ballot(is_equal);
+		if (lane == 0) { above[wave] = __popcll(ballot_above); equal[wave] = __popcll(ballot_equal); }
+		__syncthreads();
+		const uint64_t below = ((uint64_t)1 << lane) - 1;
+		uint32_t eq = ties + __popcll(ballot_equal & below), gt = __popcll(ballot_above & below);
+		uint32_t all_eq = ties, all_gt = 0;
+		for (uint32_t w = 0; w < 4; ++w) {
+			if (w < wave) { eq += equal[w]; gt += above[w]; }
+			all_eq += equal[w];
+			all_gt += above[w];
+		}
+		/* of the ties before this page, at most `rest` were kept */
+		const uint32_t kept = min(eq, rest) - min(ties, rest);
+		if (is_above || (is_equal && eq < rest)) out[written + gt + kept] = (int32_t)p;
+		written += all_gt + min(all_eq, rest) - min(ties, rest);
+		ties = all_eq;
+		__syncthreads();
+	}
+}
+
+/* ---------------------------------------------------------------- launch shapes of the attention - */
+
+/* Tiles of 16 rows, and how many parts the tokens are taken in: enough work-groups to fill the chip, none below one tile a wavefront */
+Plan4 plan_attend4(const Batch4& b, uint32_t heads, uint32_t max_length, uint32_t page_shift, uint32_t top, const DeviceInfo& dev)
+{
+	Plan4 plan;
+	plan.row_tiles = top ? b.max_queries * ((b.group + 15) / 16) : (uint32_t)(((uint64_t)b.max_queries * b.group + 15) / 16);
+	const uint64_t tokens = top ? (uint64_t)top << page_shift : max_length, units = (uint64_t)b.sequences * heads * plan.row_tiles;
+	const uint32_t tiles = (uint32_t)((tokens + 63) / 64);
+	const uint64_t want = (4 * dev.compute_units + units - 1) / (units ? units : 1), most = (tiles + 3) / 4;
+	const uint32_t splits = (uint32_t)(want < most ? want : most ? most : 1);
+	plan.tiles_per_split = tiles ? ((tiles + splits - 1) / splits + 3) / 4 * 4 : 4;
+	plan.splits = tiles ? (tiles + plan.tiles_per_split - 1) / plan.tiles_per_split : 1;
+	return plan;
+}
+
+size_t attend4_partial_floats(uint32_t J, const Batch4& b, uint32_t heads, uint32_t max_length, uint32_t page_shift, uint32_t top, const DeviceInfo& dev)
+{
+	const Plan4 plan = plan_attend4(b, heads, max_length, page_shift, top, dev);
+	return plan.splits > 1 ? (size_t)b.sequences * heads * plan.row_tiles * plan.splits * (16 * (32 * J + 2)) : 0;
+}
+
+} // namespace kmx
+
+using namespace kmx;
+
+/* ---------------------------------------------------------------- entry points ------------------- */
+
+static int check_cache4(const char* who, const kmx_cache4* cache, Cache4* out)
+{
+	if (!cache) return fail(KMX_ERR_INVALID_ARGUMENT, "%s: null cache", who);
+	if (cache->heads == 0) return fail(KMX_ERR_INVALID_ARGUMENT, "%s: heads must be positive", who);
+	if (cache->dim == 0 || cache->dim % 32 || cache->dim > 256) return fail(KMX_ERR_UNSUPPORTED, "%s: dim %u is not a multiple of 32 up to 256", who, cache->dim);
+	const uint32_t p = cache->page_tokens;
+	if (p < 16 || p > 256 || (p & (p - 1))) return fail(KMX_ERR_UNSUPPORTED, "%s: pages of %u tokens (16, 32, 64, 128 or 256)", who, p);
+	uint32_t shift = 4;
+	while ((1u << shift) < p) ++shift;
+	if ((uint64_t)cache->page_count << shift > 0x7FFFFFFFu) return fail(KMX_ERR_UNSUPPORTED, "%s: %u pages of %u tokens are more places than 31 bits count", who, cache->page_count, p);
+	if (out) {
+		if (!cache->blocks || !cache->levels) return fail(KMX_ERR_INVALID_ARGUMENT, "%s: null device pointer in the cache", who);
+		if ((uintptr_t)cache->blocks % 16 || (uintptr_t)cache->levels % 16 || (uintptr_t)cache->bounds % 16)
+			return fail(KMX_ERR_INVALID_ARGUMENT, "%s: the cache's buffers start at multiples of 16 bytes", who);
+		const size_t codes = (size_t)cache->page_count * cache->heads * 2 * cache->dim;
+		*out = Cache4{ (uint8_t*)cache->blocks, (int8_t*)cache->bounds, cache->bounds ? (float*)((int8_t*)cache->bounds + codes) : nullptr, cache->levels, cache->heads, cache->page_count, shift };
+	}
+	return KMX_OK;
+}
+
+static int check_type(const char* who, int type, bool floats)
+{
+	if (type == KMX_F16 || type == KMX_BF16 || (floats && type == KMX_F32)) return KMX_OK;
+	if (type == KMX_F32) return fail(KMX_ERR_UNSUPPORTED, "%s: queries are KMX_F16 or KMX_BF16", who);
+	return fail(KMX_ERR_INVALID_ARGUMENT, "%s: unknown element type %d", who, type);
+}
+
+static bool aligned_rows(const void* p, size_t token_stride, size_t head_stride, size_t size)
+{
+	return (uintptr_t)p % 16 == 0 && token_stride * size % 16 == 0 && head_stride * size % 16 == 0;
+}
+
+static int rows4(const char* who, bool write, const kmx_cache4* cache, int type, void* keys, void* values, size_t token_stride, size_t head_stride, const int32_t* slots, uint32_t tokens)
+{
+	Rows4 a{};
+	int rc = check_cache4(who, cache, &a.cache);
+	if (rc) return rc;
+	rc = check_type(who, type, true);
+	if (rc) return rc;
+	if (tokens == 0) return KMX_OK;
+	if (!keys || !values || !slots) return fail(KMX_ERR_INVALID_ARGUMENT, "%s: null device pointer", who);
+	if (!write && head_stride < cache->dim && cache->heads > 1) return fail(KMX_ERR_INVALID_ARGUMENT, "%s: head stride %zu < dim %u", who, head_stride, cache->dim);
+	if (!write && token_stride < cache->dim && tokens > 1) return fail(KMX_ERR_INVALID_ARGUMENT, "%s: token stride %zu < dim %u", who, token_stride, cache->dim);
+	if (cache->page_count == 0 && write) return KMX_OK; /* no place is in it */
+	const size_t size = type == KMX_F32 ? 4 : 2;
+	if ((uintptr_t)keys % size || (uintptr_t)values % size) return fail(KMX_ERR_INVALID_ARGUMENT, "%s: rows start at multiples of their element's size", who);
+	a.keys = keys;
+	a.values = values;
+	a.token_stride = token_stride;
+	a.head_stride = head_stride;
+	a.slots = slots;
+	a.tokens = tokens;
+	a.vec = aligned_rows(keys, token_stride, head_stride, size) && aligned_rows(values, token_stride, head_stride, size);
+	const uint32_t J = cache->dim / 32;
+	if (type == KMX_F32) return launch_rows4<float>(write, a, J);
+	if (type == KMX_F16) return launch_rows4<_Float16>(write, a, J);
+	return launch_rows4<__bf16>(write, a, J);
+}
+
+static int check_batch4(const char* who, const kmx_cache4* cache, const kmx_cache4_batch* batch, int causal, Batch4* out)
+{
+	if (!batch) return fail(KMX_ERR_INVALID_ARGUMENT, "%s: null batch", who);
+	if (batch->query_heads == 0 || batch->query_heads % cache->heads)
+		return fail(KMX_ERR_INVALID_ARGUMENT, "%s: %u query heads are no multiple of the cache's %u", who, batch->query_heads, cache->heads);
+	if (causal != 0 && causal != 1) return fail(KMX_ERR_INVALID_ARGUMENT, "%s: causal is 0 or 1", who);
+	if (batch->sequences && batch->tokens && batch->max_queries) {
+		if (!batch->starts || !batch->lengths || (batch->table_stride && !batch->table)) return fail(KMX_ERR_INVALID_ARGUMENT, "%s: null device pointer in the batch", who);
+		if (batch->max_length > 0x7FFFFFFFu || batch->tokens > 0x7FFFFFFFu) return fail(KMX_ERR_UNSUPPORTED, "%s: lengths and tokens are counted in 31 bits", who);
+	}
+	*out = Batch4{ batch->starts, batch->lengths, batch->table, batch->sequences, batch->tokens, batch->max_queries, batch->table_stride,
+		       batch->max_length, batch->query_heads / cache->heads, batch->query_heads, causal != 0 };
+	if (cache->page_count == 0) out->table_stride = 0; /* nothing is cached */
+	return KMX_OK;
+}
+
+static int reserve_cache4(const char* who, Workspace* ws, size_t floats)
+{
+	if (floats > ws->partials_cap && launches_recorded())
+		return fail(KMX_ERR_INVALID_ARGUMENT, "%s: the call needs a larger work space, which cannot be allocated while it is recorded: kmx_cache4_reserve, or the same call once before", who);
+	if (recording_graph()) scratch_recorded();
+	return reserve_partials(ws, floats);
+}
+
+static uint32_t table_pages(const kmx_cache4_batch* b, uint32_t page_tokens)
+{
+	const uint32_t need = b->max_length / page_tokens + (b->max_length % page_tokens ? 1 : 0);
+	return need < b->table_stride ? need : b->table_stride;
+}
+
+extern "C" {
+
+int kmx_cache4_sizes(const kmx_cache4* cache, size_t* blocks, size_t* bounds)
+{
+	clear_error();
+	int rc = check_cache4("kmx_cache4_sizes", cache, nullptr);
+	if (rc) return rc;
+	const size_t pages = (size_t)cache->page_count * cache->heads;
+	if (blocks) *blocks = pages * (cache->page_tokens / 16) * 18 * cache->dim;
+	if (bounds) *bounds = pages * (2 * cache->dim + 4);
+	return KMX_OK;
+}
+
+int kmx_cache4_round_levels(const float* in, uint32_t sets, uint16_t* out)
+{
+	clear_error();
+	if (sets == 0) return KMX_OK;
+	if (!in || !out) return fail(KMX_ERR_INVALID_ARGUMENT, "kmx_cache4_round_levels: null pointer");
+	for (uint32_t n = 0; n < sets; ++n) {
+		for (int i = 0; i < 8; ++i) {
+			const float v = in[8 * (size_t)n + i];
+			if (!(v >= 0.0f && v <= 1.0f)) return fail(KMX_ERR_INVALID_ARGUMENT, "kmx_cache4_round_levels: level %d of set %u is not within 0 and 1", i, n);
+			if (i && v < in[8 * (size_t)n + i - 1]) return fail(KMX_ERR_INVALID_ARGUMENT, "kmx_cache4_round_levels: set %u does not ascend at level %d", n, i);
+			int power = 0;
+			const float part = std::frexp(v, &power);
+			/* 6 significant bits, fewer below 2^-14, where half precision has its last place at 2^-24 */
+			const int place = power - 6 < -24 ? -24 : power - 6;
+			const float rounded = std::ldexp(std::nearbyint(std::ldexp(part, power - place)), place);
+			const _Float16 h = (_Float16)rounded;
+			std::memcpy(out + 8 * (size_t)n + i, &h, 2);
+		}
+	}
+	return KMX_OK;
+}
+
+int kmx_cache4_write(const kmx_cache4* cache, int type, const void* keys, const void* values, size_t token_stride, size_t head_stride, const int32_t* slots, uint32_t tokens)
+{
+	clear_error();
+	return rows4("kmx_cache4_write", true, cache, type, (void*)keys, (void*)values, token_stride, head_stride, slots, tokens);
+}
+
+int kmx_cache4_read(const kmx_cache4* cache, int type, void* keys, void* values, size_t token_stride, size_t head_stride, const int32_t* slots, uint32_t tokens)
+{
+	clear_error();
+	return rows4("kmx_cache4_read", false, cache, type, keys, values, token_stride, head_stride, slots, tokens);
+}
+
+int kmx_cache4_bound(const kmx_cache4* cache, const int32_t* pages, const int32_t* counts, uint32_t count)
+{
+	clear_error();
+	Cache4 c;
+	int rc = check_cache4("kmx_cache4_bound", cache, &c);
+	if (rc) return rc;
+	if (!cache->bounds) return fail(KMX_ERR_INVALID_ARGUMENT, "kmx_cache4_bound: the cache keeps no bounds");
+	if (count == 0) return KMX_OK;
+	if (!pages || !counts) return fail(KMX_ERR_INVALID_ARGUMENT, "kmx_cache4_bound: null device pointer");
+	const uint64_t groups = ((uint64_t)count * c.heads + 3) / 4;
+	if (groups > 0x7FFFFFFFu) return fail(KMX_ERR_UNSUPPORTED, "kmx_cache4_bound: %u pages of %u heads are too many for one call", count, c.heads);
+	switch (cache->dim / 32) {
+#define KMX_CASE(N)                                                                                                      \
+	case N: KMX_LAUNCH_KERNEL((bound4_kernel<N>), dim3((unsigned)groups), dim3(256), 0, stream(), c, pages, counts, count); break;
+		KMX_CASE(1) KMX_CASE(2) KMX_CASE(3) KMX_CASE(4) KMX_CASE(5) KMX_CASE(6) KMX_CASE(7) KMX_CASE(8)
+#undef KMX_CASE
+	}
+	KMX_LAUNCH_CHECK("bound4_kernel");
+	return KMX_OK;
+}
+
+int kmx_cache4_select(const kmx_cache4* cache, const kmx_cache4_batch* batch, int type, const void* q, size_t q_token_stride, size_t q_head_stride,
+                      int32_t* chosen, uint32_t top, uint32_t first, uint32_t last, int causal)
+{
+	clear_error();
+	Select4 a{};
+	int rc = check_cache4("kmx_cache4_select", cache, &a.cache);
+	if (rc) return rc;
+	if (!cache->bounds) return fail(KMX_ERR_INVALID_ARGUMENT, "kmx_cache4_select: the cache keeps no bounds");
+	rc = check_batch4("kmx_cache4_select", cache, batch, causal, &a.batch);
+	if (rc) return rc;
+	rc = check_type("kmx_cache4_select", type, false);
+	if (rc) return rc;
+	if (top == 0 || (uint64_t)first + last > top) return fail(KMX_ERR_INVALID_ARGUMENT, "kmx_cache4_select: top %u has no room for the %u first and %u last pages", top, first, last);
+	if (batch->sequences == 0 || batch->tokens == 0 || batch->max_queries == 0) return KMX_OK;
+	if (!q || !chosen) return fail(KMX_ERR_INVALID_ARGUMENT, "kmx_cache4_select: null device pointer");
+	if ((uintptr_t)q % 2) return fail(KMX_ERR_INVALID_ARGUMENT, "kmx_cache4_select: queries start at multiples of 2 bytes");
+	const uint32_t pages = table_pages(batch, cache->page_tokens);
+	a.q = q;
+	a.q_token = q_token_stride;
+	a.q_head = q_head_stride;
+	a.chosen = chosen;
+	a.top = top;
+	a.first = first;
+	a.last = last;
+	a.bf16 = type == KMX_BF16;
+	a.vec = aligned_rows(q, q_token_stride, q_head_stride, 2);
+	a.span = 1;
+	while (a.span < a.batch.group && a.span < 16) a.span *= 2;
+	a.token_tiles = (batch->max_queries + 16 / a.span - 1) / (16 / a.span);
+	const uint32_t tiles = (pages + 63) / 64; /* of 64 pages: one a wavefront */
+	const uint64_t units = (uint64_t)batch->sequences * a.token_tiles * a.cache.heads;
+	/* parts of the pages: enough work-groups to fill the chip, of 64 pages at least */
+	const uint64_t want = units < 1024 ? (1024 + units - 1) / units : 1;
+	a.chunks = (uint32_t)(want < tiles ? want : tiles ? tiles : 1);
+	a.chunk = tiles ? (tiles + a.chunks - 1) / a.chunks : 0;
+	a.chunks = a.chunk ? (tiles + a.chunk - 1) / a.chunk : 1;
+	const uint64_t groups = units * a.chunks, rows = (uint64_t)batch->sequences * batch->max_queries * a.cache.heads;
+	if (groups > 0x7FFFFFFFu || rows > 0x7FFFFFFFu) return fail(KMX_ERR_UNSUPPORTED, "kmx_cache4_select: too many queries for one call");
+	if (pages > top) { /* else every page there is gets chosen */
+		Workspace* ws = nullptr;
+		rc = workspace(&ws);
+		if (rc) return rc;
+		rc = reserve_cache4("kmx_cache4_select", ws, (size_t)batch->tokens * a.cache.heads * batch->table_stride);
+		if (rc) return rc;
+		a.keys = (uint32_t*)ws->partials;
+		switch (cache->dim / 32) {
+#define KMX_CASE(N)                                                                                                      \
+	case N: KMX_LAUNCH_KERNEL((score4_kernel<N>), dim3((unsigned)groups), dim3(256), 0, stream(), a); break;
+			KMX_CASE(1) KMX_CASE(2) KMX_CASE(3) KMX_CASE(4) KMX_CASE(5) KMX_CASE(6) KMX_CASE(7) KMX_CASE(8)
+#undef KMX_CASE
+		}
+		KMX_LAUNCH_CHECK("score4_kernel");
+	}
+	KMX_LAUNCH_KERNEL(choose4_kernel, dim3((unsigned)rows), dim3(256), 0, stream(), a);
+	KMX_LAUNCH_CHECK("choose4_kernel");
+	return KMX_OK;
+}
+
+int kmx_cache4_attend(const kmx_cache4* cache, const kmx_cache4_batch* batch, int type, const void* q, size_t q_token_stride, size_t q_head_stride,
+                      void* out, size_t out_token_stride, size_t out_head_stride, float* lse, float scale, int causal, const int32_t* chosen, uint32_t top)
+{
+	clear_error();
+	Attend4 a{};
+	int rc = check_cache4("kmx_cache4_attend", cache, &a.cache);
+	if (rc) return rc;
+	rc = check_batch4("kmx_cache4_attend", cache, batch, causal, &a.batch);
+	if (rc) return rc;
+	rc = check_type("kmx_cache4_attend", type, false);
+	if (rc) return rc;
+	if (chosen && top == 0) return fail(KMX_ERR_INVALID_ARGUMENT, "kmx_cache4_attend: chosen pages, but top is 0");
+	if (!(std::fabs(scale) <= 3.4e38f)) return fail(KMX_ERR_INVALID_ARGUMENT, "kmx_cache4_attend: the scale is not finite");
+	if (batch->sequences == 0 || batch->tokens == 0 || batch->max_queries == 0) return KMX_OK;
+	if (!q || !out) return fail(KMX_ERR_INVALID_ARGUMENT, "kmx_cache4_attend: null device pointer");
+	if ((uintptr_t)q % 2 || (uintptr_t)out % 2) return fail(KMX_ERR_INVALID_ARGUMENT, "kmx_cache4_attend: rows start at multiples of 2 bytes");
+	if (batch->query_heads > 1 && out_head_stride < cache->dim) return fail(KMX_ERR_INVALID_ARGUMENT, "kmx_cache4_attend: head stride of the output %zu < dim %u", out_head_stride, cache->dim);
+	if (batch->tokens > 1 && out_token_stride < cache->dim) return fail(KMX_ERR_INVALID_ARGUMENT, "kmx_cache4_attend: token stride of the output %zu < dim %u", out_token_stride, cache->dim);
+	a.q = q;
+	a.q_token = q_token_stride;
+	a.q_head = q_head_stride;
+	a.out = out;
+	a.out_token = out_token_stride;
+	a.out_head = out_head_stride;
+	a.lse = lse;
+	a.chosen = chosen;
+	a.top = chosen ? top : 0;
+	a.scale = scale;
+	a.bf16 = type == KMX_BF16;
+	a.vec = aligned_rows(q, q_token_stride, q_head_stride, 2) && aligned_rows(out, out_token_stride, out_head_stride, 2);
+	const uint64_t most = (uint64_t)batch->table_stride << a.cache.page_shift;
+	const uint32_t max_length = batch->max_length < most ? batch->max_length : (uint32_t)most;
+	const DeviceInfo* dev = nullptr;
+	rc = device_info(&dev);
+	if (rc) return rc;
+	Workspace* ws = nullptr;
+	rc = workspace(&ws);
+	if (rc) return rc;
+	const size_t floats = attend4_partial_floats(cache->dim / 32, a.batch, a.cache.heads, max_length, a.cache.page_shift, a.top, *dev);
+	if (floats) {
+		rc = reserve_cache4("kmx_cache4_attend", ws, floats);
+		if (rc) return rc;
+	}
+	switch (cache->dim / 32) {
+	case 1: return launch_attend4<1>(a, max_length, ws, *dev);
+	case 2: return launch_attend4<2>(a, max_length, ws, *dev);
+	case 3: return launch_attend4<3>(a, max_length, ws, *dev);
+	case 4: return launch_attend4<4>(a, max_length, ws, *dev);
+	case 5: return launch_attend4<5>(a, max_length, ws, *dev);
+	case 6: return launch_attend4<6>(a, max_length, ws, *dev);
+	case 7: return launch_attend4<7>(a, max_length, ws, *dev);
+	default: return launch_attend4<8>(a, max_length, ws, *dev);
+	}
+}
+
+int kmx_cache4_reserve(const kmx_cache4* cache, const kmx_cache4_batch* batch, uint32_t top)
+{
+	clear_error();
+	if (recording_graph()) return fail(KMX_ERR_INVALID_ARGUMENT, "kmx_cache4_reserve: not allowed between kmx_graph_begin and kmx_graph_end");
+	int rc = check_cache4("kmx_cache4_reserve", cache, nullptr);
+	if (rc) return rc;
+	if (!batch) return fail(KMX_ERR_INVALID_ARGUMENT, "kmx_cache4_reserve: null batch");
+	if (batch->query_heads == 0 || batch->query_heads % cache->heads)
+		return fail(KMX_ERR_INVALID_ARGUMENT, "kmx_cache4_reserve: %u query heads are no multiple of the cache's %u", batch->query_heads, cache->heads);
+	const DeviceInfo* dev = nullptr;
+	rc = device_info(&dev);
+	if (rc) return rc;
+	Workspace* ws = nullptr;
+	rc = workspace(&ws);
+	if (rc) return rc;
+	uint32_t shift = 4;
+	while ((1u << shift) < cache->page_tokens) ++shift;
+	const Batch4 b{ nullptr, nullptr, nullptr, batch->sequences, batch->tokens, batch->max_queries, batch->table_stride, batch->max_length, batch->query_heads / cache->heads, batch->query_heads, true };
+	const uint64_t most = (uint64_t)batch->table_stride << shift;
+	const uint32_t max_length = batch->max_length < most ? batch->max_length : (uint32_t)most;
+	size_t floats = attend4_partial_floats(cache->dim / 32, b, cache->heads, max_length, shift, 0, *dev);
+	if (top) {
+		const size_t sparse = attend4_partial_floats(cache->dim / 32, b, cache->heads, max_length, shift, top, *dev);
+		const size_t keys = (size_t)batch->tokens * cache->heads * batch->table_stride;
+		if (sparse > floats) floats = sparse;
+		if (keys > floats) floats = keys;
+	}
+	return floats ? reserve_cache4("kmx_cache4_reserve", ws, floats) : KMX_OK;
+}
+
+} // extern "C"

@@ -407,6 +407,91 @@ int kmx_certificate_unmoved_threshold(uint32_t dim, float first, float tau, floa
  */
 int kmx_probe_matrix_chain(int kind, const float* a, const float* b, const float* c, float* d, uint32_t blocks);
 
+/*
+ * ---- a cache of keys and values in 4 bits (no counterpart in the reference) ----
+ * What a k-means of one dimension and 8 centroids finds on the magnitudes of rows -- 8 learned levels -- is the codebook of a 4-bit
+ * quantiser: a sign and the nearest of the levels, times a scale for each 32 channels. Rows are quantised as they are written, stay
+ * packed (4.5 bits a number), and queries are answered from the packed rows. The cache holds `heads` heads of `dim` channels in pages of
+ * `page_tokens` tokens; place p of the cache is token p % page_tokens of page p / page_tokens.
+ *   scale of a group: the largest magnitude of its 32 channels (NaN left out) rounded to 5 significant bits (ties to the even one), at
+ *     most 63488; below 2^-14 it has the bits that half precision has there.
+ *   code: the number of j < 7 with |x| > scale (L_j + L_j+1) / 2, in floats -- the nearest level, the lower one of two as near; NaN: 0 --
+ *     and the sign (x < 0). It stands for +- scale L_code. Infinities stand for the largest number their group can hold.
+ * With levels from kmx_cache4_round_levels (6 significant bits) every such number is one of half precision.
+ * Buffers are the caller's (kmx_cache4_sizes tells how large), 16-byte aligned. Pages that no token was written to may hold anything.
+ * Bounds, where they are kept: for each page and head the largest and the smallest value of each channel of the keys, outwards in 127ths of
+ * their largest magnitude (dim + dim bytes), behind all of them those largest magnitudes over 127 (floats).
+ * Places, pages and lengths on the device are not trusted: a place or page outside the cache is left out (reads as zeros, is not attended to).
+ * kmx_cache4_select and kmx_cache4_attend use the library's work space (see kmx_cache4_reserve) under the rules of the updates.
+ */
+typedef enum kmx_type { KMX_F32 = 0, KMX_F16 = 1, KMX_BF16 = 2 } kmx_type;
+
+typedef struct kmx_cache4 {
+	void* blocks;           /* codes and scales */
+	void* bounds;           /* null: no bounds are kept, and kmx_cache4_bound and kmx_cache4_select are refused */
+	const uint16_t* levels; /* heads x (keys, values) x 8 half-precision levels, ascending within 0 and 1 */
+	uint32_t heads;
+	uint32_t dim;           /* a multiple of 32 up to 256 */
+	uint32_t page_tokens;   /* 16, 32, 64, 128 or 256 */
+	uint32_t page_count;    /* page_count * page_tokens < 2^31 */
+} kmx_cache4;
+
+/* Queries of some sequences. Sequence s has the cached tokens 0 .. lengths[s] - 1, token t in page table[s][t / page_tokens], and the queries
+ * starts[s] .. starts[s + 1] - 1 of the rows handed over, which are those of its last tokens: with `causal` query i of n sees
+ * lengths[s] - n + i + 1 tokens, else all. Device pointers; max_queries and max_length bound queries and length of a sequence (more is cut off). */
+typedef struct kmx_cache4_batch {
+	uint32_t sequences;
+	uint32_t query_heads;  /* a multiple of the cache's heads: the query heads h g .. h g + g - 1 look at head h */
+	uint32_t tokens;       /* rows of queries in all */
+	uint32_t max_queries;
+	uint32_t max_length;
+	uint32_t table_stride; /* entries of a row of the table */
+	const int32_t* starts;  /* sequences + 1, ascending from 0 */
+	const int32_t* lengths; /* sequences */
+	const int32_t* table;   /* sequences x table_stride */
+} kmx_cache4_batch;
+
+/* Bytes of the two buffers; either pointer may be null. Host only. */
+int kmx_cache4_sizes(const kmx_cache4* cache, size_t* blocks, size_t* bounds);
+
+/* sets x 8 learned levels to 6 significant bits (ties to the even one) in half precision; refused unless each set ascends within 0 and 1. Host only. */
+int kmx_cache4_round_levels(const float* levels, uint32_t sets, uint16_t* rounded);
+
+/* Rows to places: element (token, head, channel) = rows[token * token_stride + head * head_stride + channel] (strides in elements, the same for
+ * keys and values), token t to place slots[t], negative: nowhere. Places of one call are distinct. F32, F16, BF16. */
+int kmx_cache4_write(const kmx_cache4* cache, int type, const void* keys, const void* values, size_t token_stride, size_t head_stride,
+                     const int32_t* slots, uint32_t tokens);
+
+/* And back: the numbers that the cache holds, rounded to the type once. */
+int kmx_cache4_read(const kmx_cache4* cache, int type, void* keys, void* values, size_t token_stride, size_t head_stride,
+                    const int32_t* slots, uint32_t tokens);
+
+/* The bounds of pages[0 .. count), of which the first counts[] tokens are written (0: bounds of 0). After writes, before kmx_cache4_select. */
+int kmx_cache4_bound(const kmx_cache4* cache, const int32_t* pages, const int32_t* counts, uint32_t count);
+
+/*
+ * The pages that each query and head of the cache look at: chosen[token][head][top], numbers of pages inside the sequence (columns of the
+ * table), ascending, -1 behind the last. Of the pages with a token the query sees: the `first` first and `last` last ones, then those of the
+ * best score, the lower number of two as good. score = max over the query heads of the head of sum_c max(q_c hi_c, q_c lo_c), the bound on
+ * q . k over the page, in 8 bits: q_c = rint(q 127 / its largest magnitude over these heads), hi and lo as kept; a whole number, times the page's
+ * scale in floats. Queries F16 or BF16, element (token, head, channel) as above.
+ */
+int kmx_cache4_select(const kmx_cache4* cache, const kmx_cache4_batch* batch, int type, const void* q, size_t q_token_stride, size_t q_head_stride,
+                      int32_t* chosen, uint32_t top, uint32_t first, uint32_t last, int causal);
+
+/*
+ * out[token][head] = sum_t p_t v_t, p = softmax over the tokens t that the query sees of scale * q . k_t; lse (may be null): the logarithm of the
+ * softmax's sum, tokens x query_heads. A query that sees nothing gets zeros and minus infinity. chosen (may be null): only tokens of these pages,
+ * lists as kmx_cache4_select writes them (distinct). Queries and outputs F16 or BF16; products of numbers of half precision, sums in floats.
+ */
+int kmx_cache4_attend(const kmx_cache4* cache, const kmx_cache4_batch* batch, int type, const void* q, size_t q_token_stride, size_t q_head_stride,
+                      void* out, size_t out_token_stride, size_t out_head_stride, float* lse, float scale, int causal,
+                      const int32_t* chosen, uint32_t top);
+
+/* Sizes the work space for kmx_cache4_attend on such a batch, and for kmx_cache4_select and attention to `top` chosen pages (0: neither), so that
+ * they allocate nothing afterwards (recordings, serving loops). Of the batch it looks at the numbers only. */
+int kmx_cache4_reserve(const kmx_cache4* cache, const kmx_cache4_batch* batch, uint32_t top);
+
 /* Message of the last failed call on this thread ("" if none). */
 const char* kmx_last_error(void);
 
