@@ -191,7 +191,7 @@ struct Attend4 {
 	const int32_t* chosen; uint32_t top; /* pages chosen for each token and head, or null */
 	float scale;
 	bool bf16, vec;
-	uint32_t row_tiles, splits, tiles_per_split; /* (filled in by the launcher) */
+	uint32_t row_tiles, splits, tiles_per_split, rows; /* (filled in by the launcher) */
 	float* partial;
 };
 /* launch shape: tiles of 16 rows, parts of the tokens, tiles of 64 tokens a part (cache4.hip) */

@@ -535,7 +535,9 @@ Plan4 plan_attend4(const Batch4& b, uint32_t heads, uint32_t max_length, uint32_
 	plan.row_tiles = top ? b.max_queries * ((b.group + 15) / 16) : (uint32_t)(((uint64_t)b.max_queries * b.group + 15) / 16);
 	const uint64_t tokens = top ? (uint64_t)top << page_shift : max_length, units = (uint64_t)b.sequences * heads * plan.row_tiles;
 	const uint32_t tiles = (uint32_t)((tokens + 63) / 64);
-	const uint64_t want = (4 * dev.compute_units + units - 1) / (units ? units : 1), most = (tiles + 3) / 4;
+	uint64_t want = (2 * dev.compute_units + units - 1) / (units ? units : 1);
+	const uint64_t most = (tiles + 3) / 4;
+	if (want > 256) want = 256; /* (the kernel that joins them has a lane for each) */
 	const uint32_t splits = (uint32_t)(want < most ? want : most ? most : 1);
 	plan.tiles_per_split = tiles ? ((tiles + splits - 1) / splits + 3) / 4 * 4 : 4;
 	plan.splits = tiles ? (tiles + plan.tiles_per_split - 1) / plan.tiles_per_split : 1;

@@ -39,8 +39,10 @@ __device__ __forceinline__ uint32_t tiles_of(const Attend4& a, const Sequence& s
 {
 	if (a.chosen) {
 		const uint32_t token = row_tile / ((a.batch.group + 15) / 16);
-		if (token >= seq.queries || visible_to(a.batch, seq, token) == 0) return 0;
-		return (uint32_t)((((uint64_t)a.top << (a.cache.page_shift - 4)) + 3) / 4);
+		if (token >= seq.queries) return 0;
+		/* lists ascend: pages with a token that the query sees come first, and there are no more of them than the sequence has */
+		const uint32_t pages = (visible_to(a.batch, seq, token) + (1u << a.cache.page_shift) - 1) >> a.cache.page_shift;
+		return (uint32_t)((((uint64_t)min(a.top, pages) << (a.cache.page_shift - 4)) + 3) / 4);
 	}
 	const uint64_t x = (uint64_t)row_tile * 16;
 	if (x >= (uint64_t)seq.queries * a.batch.group) return 0;
@@ -81,6 +83,16 @@ __device__ __forceinline__ void load_halves(const uint8_t* p, uint32_t w[(J + 1)
 	}
 }
 
+/* 8 channels of every 32 of a row */
+template <int J, typename T>
+__device__ __forceinline__ void load_rows(const char* p, bool vec, float x[J][8])
+{
+	if (vec)
+		for (int j = 0; j < J; ++j) load8((const T*)p + 32 * j, true, x[j]);
+	else
+		for (int j = 0; j < J; ++j) load8((const T*)p + 32 * j, false, x[j]);
+}
+
 /* 4 channels of an output row */
 __device__ __forceinline__ void store_out4(const Attend4& a, char* row, uint32_t channel, const float v[4])
 {
@@ -94,38 +106,39 @@ __device__ __forceinline__ void store_out4(const Attend4& a, char* row, uint32_t
 /* What a wavefront loads for 64 tokens. A lane is row i = lane % 16 of the operands and holds their piece kg = lane / 16. */
 template <int J>
 struct Tile4 {
-	uint32_t kc[4][J];            /* codes of token 4 u + i % 4 of block i / 4, channels 32 j + 8 kg .. + 7 */
-	uint32_t ks[4][(J + 1) / 2];  /* its scales */
-	u32x4 vc[J];                  /* codes of channels 32 j + i and + 16 + i, the 16 tokens of block kg */
-	u32x4 vs[J][2];               /* the scales of the 16 tokens */
-};
-
-/* Where the blocks of a tile lie: the one that the lane loads keys of, and the one it loads values of (whose tokens are also its scores') */
-struct Where4 {
-	const uint8_t* keys; const uint8_t* values;
-	int32_t from; /* place of the first token of the values' block in the sequence */
-	bool there;
+	uint32_t kc[4][J];        /* codes of token 4 u + i % 4 of block i / 4, channels 32 j + 8 kg .. + 7 */
+	u32x4 vc[J];              /* codes of channels 32 j + i and + 16 + i, the 16 tokens of block kg */
+	u32x4 sc[(J + 3) / 4];    /* 16 bytes of the 64 J of the scales of block kg, which go through LDS to the lanes that need them */
 };
 
 /*
  * A work-group of four wavefronts takes 16 rows of one head of the cache (the query heads of a token side by side, then the next token's) and
- * a part of the tokens; a wavefront takes every fourth tile of 64 tokens, and its next tile is under way while it works on one. Both products
+ * a part of the tokens; a wavefront takes every fourth tile of 64 tokens. The registers of a tile's keys are loaded with the next tile's as soon as
+ * the scores are there, those of its values as soon as the sums are: each load has the other half of a tile's work to arrive in, and three or four
+ * wavefronts fit a SIMD. Both products
  * have the cache as their first operand (v_mfma_f32_16x16x32_f16): scores come out as [token][row], so a lane has all its 16 scores in one row
  * -- maxima and sums are its own but for two exchanges -- and its probabilities are, as they stand, its piece of the second operand of
  * [channel][row] = values . p. Tokens go to the rows of the first product such that a lane's 16 are those of one block: its values are 16 bytes
  * side by side.
  */
 template <int J>
-__global__ void __launch_bounds__(256)
+__global__ void __launch_bounds__(256, J <= 4 ? 3 : 2)
 attend4_kernel(Attend4 a)
 {
-	constexpr uint32_t D = 32 * J;
-	__shared__ f32x4 sums[2][2 * J][WAVE];
+	constexpr uint32_t D = 32 * J, SCALES = 64 * J + 32; /* bytes of a block's scales in LDS: 8 banks on from one block to the next */
+	__shared__ union {
+		struct {
+			__attribute__((aligned(16))) uint8_t scales[4][4][SCALES];
+			uint64_t places[4][2][WAVE];
+			int32_t from[4][2][WAVE];
+		};
+		f32x4 sums[2][2 * J][WAVE];
+	} lds;
 	__shared__ float most[4][16], total[4][16];
-	const uint32_t wave = threadIdx.x / WAVE, lane = threadIdx.x % WAVE, i16 = lane % 16, kg = lane / 16;
-	uint32_t unit = blockIdx.x;
-	const uint32_t part = unit % a.splits;
-	const uint32_t whole = unit / a.splits; /* sequence, head and tile of rows */
+	const uint32_t wave = (uint32_t)__builtin_amdgcn_readfirstlane((int)(threadIdx.x / WAVE)), lane = threadIdx.x % WAVE, i16 = lane % 16, kg = lane / 16;
+	/* first parts of all units before their second ones: the dies take work-groups in turn, and parts behind the end of a shorter sequence are empty */
+	const uint32_t units = gridDim.x / a.splits, part = blockIdx.x / units;
+	const uint32_t whole = blockIdx.x % units; /* sequence, head and tile of rows */
 	const uint32_t row_tile = whole % a.row_tiles, head = whole / a.row_tiles % a.cache.heads, s = whole / a.row_tiles / a.cache.heads;
 	const Sequence seq = sequence_of(a.batch, s, a.cache.page_shift);
 	const uint32_t tiles = tiles_of(a, seq, row_tile);
@@ -134,73 +147,74 @@ attend4_kernel(Attend4 a)
 	const Row4 row = row_of(a, seq, row_tile, i16);
 	if (a.splits > 1 && tiles == 0) return; /* (the kernel that joins the parts writes the zeros) */
 
-	/* queries: 8 channels a lane for each j, as halves of at most 2 in magnitude (bf16 has more exponents) */
+	/* queries: 8 channels a lane for each j, with the sign of the scale, as halves of at most 2 in magnitude (bf16 has more exponents);
+	 * row_scale takes a score of theirs to the exponent of 2 */
 	half8v q[J];
 	float row_scale;
 	{
 		float x[J][8];
 		const char* p = (const char*)a.q + 2 * ((size_t)(seq.first + (row.there ? row.token : 0)) * a.q_token + ((size_t)head * a.batch.group + (row.there ? row.head : 0)) * a.q_head + 8 * kg);
+		if (seq.queries == 0) {
+			for (int j = 0; j < J; ++j)
+				for (int e = 0; e < 8; ++e) x[j][e] = 0.0f;
+		} else if (a.bf16) load_rows<J, __bf16>(p, a.vec, x);
+		else load_rows<J, _Float16>(p, a.vec, x);
 		float largest = 0.0f;
 #pragma unroll
-		for (int j = 0; j < J; ++j) {
-			if (!row.there) {
-				for (int e = 0; e < 8; ++e) x[j][e] = 0.0f;
-			} else if (a.bf16) load8((const __bf16*)p + 32 * j, a.vec, x[j]);
-			else load8((const _Float16*)p + 32 * j, a.vec, x[j]);
+		for (int j = 0; j < J; ++j)
 			for (int e = 0; e < 8; ++e) largest = fmaxf(largest, fabsf(x[j][e]));
-		}
 		largest = fmaxf(largest, __shfl_xor(largest, 16));
 		largest = fmaxf(largest, __shfl_xor(largest, 32));
 		int power = (int)(__builtin_bit_cast(uint32_t, largest) >> 23) - 127;
 		power = power < -126 ? 0 : power > 126 ? 126 : power;
-		const float by = __builtin_bit_cast(float, (uint32_t)(127 - power) << 23);
-		row_scale = a.scale * 1.44269504088896341f * __builtin_bit_cast(float, (uint32_t)(127 + power) << 23);
+		float by = __builtin_bit_cast(float, (uint32_t)(127 - power) << 23);
+		row_scale = fmaxf(fabsf(a.scale) * 1.44269504088896341f * __builtin_bit_cast(float, (uint32_t)(127 + power) << 23), 1.2e-38f);
+		by = a.scale > 0.0f ? by : a.scale < 0.0f ? -by : 0.0f;
 #pragma unroll
 		for (int j = 0; j < J; ++j)
 			for (int e = 0; e < 8; ++e) q[j][e] = (_Float16)(x[j][e] * by);
 	}
 	const int32_t sees = row.there ? (int32_t)visible_to(a.batch, seq, row.token) : 0;
 	const Magnitudes mk = load_magnitudes(a.cache.levels, head, 0), mv = load_magnitudes(a.cache.levels, head, 1);
-	const int32_t* list = a.chosen ? a.chosen + ((size_t)(seq.first + row_tile / ((a.batch.group + 15) / 16)) * a.cache.heads + head) * a.top : nullptr;
-	const uint32_t sub_bits = a.cache.page_shift - 4;
+	const bool listed = a.chosen != nullptr;
+	const int32_t* list = a.chosen + (listed ? ((size_t)(seq.first + row_tile / ((a.batch.group + 15) / 16)) * a.cache.heads + head) * a.top : 0);
+	const int32_t* table = a.batch.table + (size_t)s * a.batch.table_stride;
+	const uint32_t sub_bits = a.cache.page_shift - 4, last_entry = (listed ? a.top : a.batch.table_stride) - 1;
 
-	/* block n of the tokens looked at: its address, and its place in the sequence */
-	auto block_at = [&](uint32_t n, int32_t* from) -> const uint8_t* {
-		const uint32_t entry = n >> sub_bits, sub = n & ((1u << sub_bits) - 1);
-		uint32_t logical = entry;
-		bool there = true;
-		if (list) {
-			const int32_t l = entry < a.top ? list[entry] : -1;
-			there = l >= 0;
-			logical = (uint32_t)l;
-		}
-		there = there && logical < a.batch.table_stride;
-		const int32_t page = there ? a.batch.table[(size_t)s * a.batch.table_stride + logical] : -1;
-		there = page >= 0 && (uint32_t)page < a.cache.page_count;
-		*from = there ? (int32_t)((logical << a.cache.page_shift) + 16 * sub) : INT32_MAX;
-		return a.cache.blocks + (there ? block_offset<J>(a.cache, (uint32_t)page, head, sub) : 0);
+	/*
+	 * Where the blocks of the wavefront's tiles lie, 16 tiles at a time, one block a lane (4 n + b: block b of the n-th tile), and their places in
+	 * the sequence (INT32_MAX: it is not there, and any block's address stands in its place). They are kept in LDS, in halves that take turns.
+	 */
+	auto find_places = [&](uint32_t first_tile, uint32_t half) {
+		const uint32_t n = 4 * (first_tile + lane / 4 * 4) + lane % 4, entry = n >> sub_bits, sub = n & ((1u << sub_bits) - 1);
+		uint32_t logical = min(entry, last_entry);
+		if (listed) logical = (uint32_t)list[logical];
+		const uint32_t page = (uint32_t)table[min(logical, a.batch.table_stride - 1)];
+		const bool there = entry <= last_entry && logical < a.batch.table_stride && page < a.cache.page_count;
+		lds.places[wave][half][lane] = block_offset<J>(a.cache, there ? page : 0, head, sub);
+		lds.from[wave][half][lane] = there ? (int32_t)((logical << a.cache.page_shift) + 16 * sub) : INT32_MAX;
 	};
-	auto where = [&](uint32_t tile) {
-		Where4 w;
-		int32_t unused;
-		w.keys = block_at(4 * tile + i16 / 4, &unused);
-		w.values = block_at(4 * tile + kg, &w.from);
-		w.there = w.from != INT32_MAX;
+	struct Where { const uint8_t* keys; const uint8_t* values; int32_t from; };
+	auto where = [&](uint32_t n) {
+		const uint64_t* at = &lds.places[wave][n / 16 % 2][4 * (n % 16)];
+		Where w;
+		w.keys = a.cache.blocks + at[i16 / 4] + (i16 % 4) * (D / 2) + kg * 4 * J;
+		w.values = a.cache.blocks + at[kg] + 8 * D + i16 * 16;
+		w.from = lds.from[wave][n / 16 % 2][4 * (n % 16) + kg];
 		return w;
 	};
-	auto fetch = [&](Tile4<J>& t, const Where4& w) {
+	auto fetch_keys = [&](Tile4<J>& t, const Where& w) {
 #pragma unroll
-		for (int u = 0; u < 4; ++u) {
-			const uint32_t token = 4 * u + i16 % 4;
-			load_words<J>(w.keys + token * (D / 2) + kg * 4 * J, t.kc[u]);
-			load_halves<J>(w.keys + 16 * D + token * 2 * J, t.ks[u]);
-		}
+		for (int u = 0; u < 4; ++u) load_words<J>(w.keys + u * (2 * D), t.kc[u]);
+	};
+	auto fetch_values = [&](Tile4<J>& t, const Where& w) {
 #pragma unroll
-		for (int j = 0; j < J; ++j) {
-			t.vc[j] = *(const u32x4*)(w.values + 8 * D + (16 * j + i16) * 16);
-			t.vs[j][0] = *(const u32x4*)(w.values + 17 * D + 32 * j);
-			t.vs[j][1] = *(const u32x4*)(w.values + 17 * D + 32 * j + 16);
-		}
+		for (int j = 0; j < J; ++j) t.vc[j] = *(const u32x4*)(w.values + 256 * j);
+	};
+	auto fetch_scales = [&](Tile4<J>& t, const Where& w) {
+#pragma unroll
+		for (int n = 0; n < (J + 3) / 4; ++n)
+			if (4 * J - 16 * n >= 16 || (int)i16 < 4 * J - 16 * n) t.sc[n] = *(const u32x4*)(w.values + 8 * D + 256 * n);
 	};
 
 	float m = -__builtin_inff(), l = 0.0f; /* of the lane's row: the maximum of all its lanes, the sum of the lane's own tokens */
@@ -208,16 +222,35 @@ attend4_kernel(Attend4 a)
 #pragma unroll
 	for (int c = 0; c < 2 * J; ++c) o[c] = f32x4{ 0.0f, 0.0f, 0.0f, 0.0f };
 
-	auto work = [&](Tile4<J>& t, int32_t from, bool there) {
-		const int32_t limit = there ? sees - from : 0; /* tokens of the lane's block that its row sees */
-		if (!__any(limit > 0)) return;
+	auto work = [&](Tile4<J>& t, int32_t from, const Where& next) { /* ... and leaves the next tile's loads under way */
+		const int32_t limit = from == INT32_MAX ? 0 : sees - from; /* tokens of the lane's block that its row sees */
+		uint8_t* const scales = lds.scales[wave][0]; /* (a wavefront's own: LDS takes its accesses in their order) */
+		/* what lies behind the last token may hold anything: the scales of its values become zeros */
+		const int32_t written = from == INT32_MAX ? 0 : (int32_t)seq.length - from;
+		const bool cut = __any(written < 16);
+#pragma unroll
+		for (int n = 0; n < (J + 3) / 4; ++n)
+			if (4 * J - 16 * n >= 16 || (int)i16 < 4 * J - 16 * n) {
+				if (cut && (int)i16 + 16 * n >= 2 * J) { /* scales of values: 8 tokens */
+#pragma unroll
+					for (int d = 0; d < 4; ++d) {
+						const int first = 8 * ((int)i16 & 1) + 2 * d;
+						t.sc[n][d] &= written >= first + 2 ? 0xFFFFFFFFu : written == first + 1 ? 0xFFFFu : 0u;
+					}
+				}
+				*(u32x4*)(scales + kg * SCALES + 256 * n + 16 * i16) = t.sc[n];
+			}
+		__builtin_amdgcn_wave_barrier();
+		fetch_scales(t, next);
 		float sc[16];
 #pragma unroll
 		for (int u = 0; u < 4; ++u) {
+			uint32_t ks[(J + 1) / 2];
+			load_halves<J>(scales + (i16 / 4) * SCALES + (4 * u + i16 % 4) * 2 * J, ks);
 			f32x4 acc{ 0.0f, 0.0f, 0.0f, 0.0f };
 #pragma unroll
 			for (int j = 0; j < J; ++j) {
-				const uint32_t scale = twice(t.ks[u][j / 2], j % 2);
+				const uint32_t scale = twice(ks[j / 2], j % 2);
 				u32x4 w;
 				uint32_t p[4];
 				unpack4<false>(t.kc[u][j], mk, p[0], p[1]);
@@ -225,7 +258,12 @@ attend4_kernel(Attend4 a)
 				for (int e = 0; e < 4; ++e) w[e] = times(p[e], scale);
 				acc = __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(half8v, w), q[j], acc, 0, 0, 0);
 			}
-			for (int r = 0; r < 4; ++r) sc[4 * u + r] = 4 * u + r < limit ? acc[r] * row_scale : -__builtin_inff();
+			for (int r = 0; r < 4; ++r) sc[4 * u + r] = acc[r];
+		}
+		fetch_keys(t, next);
+		if (__any(limit < 16)) {
+#pragma unroll
+			for (int e = 0; e < 16; ++e) sc[e] = e < limit ? sc[e] : -__builtin_inff();
 		}
 		float top = sc[0];
 #pragma unroll
@@ -234,74 +272,59 @@ attend4_kernel(Attend4 a)
 		top = fmaxf(top, __shfl_xor(top, 32));
 		const float now = fmaxf(m, top);
 		if (__any(now > m)) {
-			const float less = m == now ? 1.0f : exp2_(m - now); /* (both -inf: nothing seen yet) */
+			const float less = m == now ? 1.0f : exp2_((m - now) * row_scale); /* (both -inf: nothing seen yet) */
 			l *= less;
 #pragma unroll
 			for (int c = 0; c < 2 * J; ++c) o[c] *= less;
 			m = now;
 		}
-		const float base = m == -__builtin_inff() ? 0.0f : m;
+		const float base = m == -__builtin_inff() ? 0.0f : -m * row_scale;
 		half8v p[2];
 #pragma unroll
 		for (int e = 0; e < 16; ++e) {
-			const float v = exp2_(sc[e] - base);
+			const float v = exp2_(fmaf(sc[e], row_scale, base));
 			l += v;
 			p[e / 8][e % 8] = (_Float16)v; /* 11 bits: the error of a probability is below that of the result's type, and sums of them are kept in 32 */
-		}
-		/* what lies behind the last token may hold anything: its scales become zeros */
-		const int32_t written = there ? (int32_t)seq.length - from : 0;
-		if (__any(written < 16)) {
-#pragma unroll
-			for (int d = 0; d < 8; ++d) {
-				const uint32_t keep = written >= 2 * d + 2 ? 0xFFFFFFFFu : written == 2 * d + 1 ? 0xFFFFu : 0u;
-#pragma unroll
-				for (int j = 0; j < J; ++j) t.vs[j][d / 4][d % 4] &= keep;
-			}
 		}
 #pragma unroll
 		for (int j = 0; j < J; ++j) {
 #pragma unroll
 			for (int half = 0; half < 2; ++half) { /* tokens 0 to 7 of the lane's block, then 8 to 15 */
+				const u32x4 vs = *(const u32x4*)(scales + kg * SCALES + 32 * J + 32 * j + 16 * half);
 				u32x4 low, high;
 				for (int d = 0; d < 2; ++d) {
 					uint32_t x, y;
 					const uint32_t code = t.vc[j][2 * half + d];
 					unpack4<false>(code, mv, x, y);
-					low[2 * d] = times(x, t.vs[j][half][2 * d]);
-					low[2 * d + 1] = times(y, t.vs[j][half][2 * d + 1]);
+					low[2 * d] = times(x, vs[2 * d]);
+					low[2 * d + 1] = times(y, vs[2 * d + 1]);
 					unpack4<true>(code, mv, x, y);
-					high[2 * d] = times(x, t.vs[j][half][2 * d]);
-					high[2 * d + 1] = times(y, t.vs[j][half][2 * d + 1]);
+					high[2 * d] = times(x, vs[2 * d]);
+					high[2 * d + 1] = times(y, vs[2 * d + 1]);
 				}
 				o[2 * j] = __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(half8v, low), p[half], o[2 * j], 0, 0, 0);
 				o[2 * j + 1] = __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(half8v, high), p[half], o[2 * j + 1], 0, 0, 0);
 			}
 		}
+		fetch_values(t, next);
 	};
 
-	uint32_t tile = begin + wave;
-	if (tile < end) {
-		Tile4<J> even, odd;
-		Where4 w0 = where(tile);
-		fetch(even, w0);
-		Where4 w1 = where(tile + 4);
-		for (;;) {
-			const bool more = tile + 4 < end;
-			if (more) fetch(odd, w1);
-			const int32_t from0 = w0.from;
-			const bool there0 = w0.there;
-			if (more) w0 = where(tile + 8);
-			work(even, from0, there0);
-			if (!more) break;
-			tile += 4;
-			const bool again = tile + 4 < end;
-			if (again) fetch(even, w0);
-			const int32_t from1 = w1.from;
-			const bool there1 = w1.there;
-			if (again) w1 = where(tile + 8);
-			work(odd, from1, there1);
-			if (!again) break;
-			tile += 4;
+	const uint32_t count = end > begin + wave ? (end - begin - wave + 3) / 4 : 0; /* tiles of this wavefront */
+	if (count) {
+		Tile4<J> t;
+		const uint32_t tile0 = begin + wave;
+		find_places(tile0, 0);
+		__builtin_amdgcn_wave_barrier();
+		Where w = where(0);
+		fetch_scales(t, w);
+		fetch_keys(t, w);
+		fetch_values(t, w);
+		for (uint32_t n = 0; n < count; ++n) {
+			const int32_t from = w.from;
+			if (n % 16 == 7 && n + 9 < count) find_places(tile0 + 4 * (n + 9), (n + 9) / 16 % 2);
+			__builtin_amdgcn_wave_barrier();
+			w = where(min(n + 1, count - 1)); /* (the last tile is fetched twice: a fetch under a condition would make the compiler wait for everything) */
+			work(t, from, w);
 		}
 	}
 
@@ -309,36 +332,36 @@ attend4_kernel(Attend4 a)
 	l += __shfl_xor(l, 16);
 	l += __shfl_xor(l, 32);
 	if (kg == 0) { most[wave][i16] = m; total[wave][i16] = l; }
-	__syncthreads();
+	__syncthreads(); /* (from here on LDS holds sums) */
 	float all = most[0][i16];
 	for (int w = 1; w < 4; ++w) all = fmaxf(all, most[w][i16]);
 	const float base = all == -__builtin_inff() ? 0.0f : all;
-	const float mine = exp2_(m - base);
+	const float mine = exp2_((m - base) * row_scale);
 	float sum = 0.0f;
-	for (int w = 0; w < 4; ++w) sum += total[w][i16] * exp2_(most[w][i16] - base);
+	for (int w = 0; w < 4; ++w) sum += total[w][i16] * exp2_((most[w][i16] - base) * row_scale);
 #pragma unroll
 	for (int c = 0; c < 2 * J; ++c) o[c] *= mine;
 	if (wave >= 2)
 #pragma unroll
-		for (int c = 0; c < 2 * J; ++c) sums[wave - 2][c][lane] = o[c];
+		for (int c = 0; c < 2 * J; ++c) lds.sums[wave - 2][c][lane] = o[c];
 	__syncthreads();
 	if (wave < 2)
 #pragma unroll
-		for (int c = 0; c < 2 * J; ++c) o[c] += sums[wave][c][lane];
+		for (int c = 0; c < 2 * J; ++c) o[c] += lds.sums[wave][c][lane];
 	__syncthreads();
 	if (wave == 1)
 #pragma unroll
-		for (int c = 0; c < 2 * J; ++c) sums[0][c][lane] = o[c];
+		for (int c = 0; c < 2 * J; ++c) lds.sums[0][c][lane] = o[c];
 	__syncthreads();
 	if (wave != 0 || !row.there) return;
 #pragma unroll
-	for (int c = 0; c < 2 * J; ++c) o[c] += sums[0][c][lane];
+	for (int c = 0; c < 2 * J; ++c) o[c] += lds.sums[0][c][lane];
 
 	if (a.splits > 1) {
-		float* to = a.partial + (size_t)blockIdx.x * (16 * (D + 2));
+		float* to = a.partial + ((size_t)whole * a.splits + part) * (16 * (D + 2));
 #pragma unroll
 		for (int c = 0; c < 2 * J; ++c) *(f32x4*)(to + i16 * D + 16 * c + 4 * kg) = o[c];
-		if (kg == 0) { to[16 * D + i16] = all; to[16 * D + 16 + i16] = sum; }
+		if (kg == 0) { to[16 * D + i16] = all * row_scale; to[16 * D + 16 + i16] = sum; }
 		return;
 	}
 	const float by = sum > 0.0f ? 1.0f / sum : sum == sum ? 0.0f : sum; /* a row that sees nothing is zero; NaN stays */
@@ -350,51 +373,56 @@ attend4_kernel(Attend4 a)
 		for (int r = 0; r < 4; ++r) v[r] = o[c][r] * by;
 		store_out4(a, to, 16 * c + 4 * kg, v);
 	}
-	if (kg == 0 && a.lse) a.lse[token * a.batch.query_heads + query_head] = sum == 0.0f ? -__builtin_inff() : (all + log2f(sum)) * 0.693147180559945309f;
+	if (kg == 0 && a.lse) a.lse[token * a.batch.query_heads + query_head] = sum == 0.0f ? -__builtin_inff() : (all * row_scale + log2f(sum)) * 0.693147180559945309f;
 }
 
-/* Joins the parts of a row: a wavefront each, its lanes 4 channels of every (64 / lanes a row)-th part. */
+/* Joins the parts of a row, a work-group each: the parts' weights first, one a lane, then its wavefronts take the parts in turn, 8 J lanes four
+ * channels each. */
 template <int J>
 __global__ void __launch_bounds__(256)
 join4_kernel(Attend4 a)
 {
-	constexpr uint32_t D = 32 * J, LANES = 8 * J, GROUPS = WAVE / LANES;
-	const uint32_t wave = threadIdx.x / WAVE, lane = threadIdx.x % WAVE;
-	const uint64_t unit = (uint64_t)blockIdx.x * 4 + wave;
-	const uint32_t r = (uint32_t)(unit % 16), whole = (uint32_t)(unit / 16);
+	constexpr uint32_t D = 32 * J, LANES = 8 * J, GROUPS = 256 / LANES;
+	__shared__ float weights[256], most[4], sums[4];
+	__shared__ f32x4 o[GROUPS][LANES];
+	const uint32_t tid = threadIdx.x, wave = tid / WAVE, lane = tid % WAVE;
+	const uint32_t r = blockIdx.x % a.rows, whole = blockIdx.x / a.rows;
 	const uint32_t row_tile = whole % a.row_tiles, head = whole / a.row_tiles % a.cache.heads, s = whole / a.row_tiles / a.cache.heads;
-	if (s >= a.batch.sequences) return;
 	const Sequence seq = sequence_of(a.batch, s, a.cache.page_shift);
 	const Row4 row = row_of(a, seq, row_tile, r);
 	if (!row.there) return;
 	const uint32_t tiles = tiles_of(a, seq, row_tile);
-	const uint32_t parts = (tiles + a.tiles_per_split - 1) / a.tiles_per_split;
+	const uint32_t parts = (tiles + a.tiles_per_split - 1) / a.tiles_per_split; /* at most 256 */
 	const float* from = a.partial + (size_t)whole * a.splits * (16 * (D + 2));
-	float all = -__builtin_inff();
-	for (uint32_t p = lane; p < parts; p += WAVE) all = fmaxf(all, from[(size_t)p * (16 * (D + 2)) + 16 * D + r]);
+	const float m = tid < parts ? from[(size_t)tid * (16 * (D + 2)) + 16 * D + r] : -__builtin_inff();
+	float l = tid < parts ? from[(size_t)tid * (16 * (D + 2)) + 16 * D + 16 + r] : 0.0f;
+	float all = m;
 	for (int d = 1; d < WAVE; d *= 2) all = fmaxf(all, __shfl_xor(all, d));
-	const float base = all == -__builtin_inff() ? 0.0f : all;
-	float sum = 0.0f;
-	f32x4 o{ 0.0f, 0.0f, 0.0f, 0.0f };
-	const uint32_t group = lane / LANES, at = lane % LANES;
-	if (group < GROUPS)
-		for (uint32_t p = group; p < parts; p += GROUPS) {
-			const float* part = from + (size_t)p * (16 * (D + 2));
-			const float by = exp2_(part[16 * D + r] - base);
-			sum += part[16 * D + 16 + r] * by;
-			o += *(const f32x4*)(part + r * D + 4 * at) * by;
-		}
-	for (uint32_t g = 1; g < GROUPS; ++g) { /* the groups' sums, in their order */
-		const int other = (int)(at + g * LANES);
-		const f32x4 more{ __shfl(o[0], other), __shfl(o[1], other), __shfl(o[2], other), __shfl(o[3], other) };
-		const float more_sum = __shfl(sum, other);
-		if (group == 0) { o += more; sum += more_sum; }
+	if (lane == 0) most[wave] = all;
+	__syncthreads();
+	all = fmaxf(fmaxf(most[0], most[1]), fmaxf(most[2], most[3]));
+	const float weight = exp2_(m - (all == -__builtin_inff() ? 0.0f : all));
+	weights[tid] = weight;
+	l *= weight;
+	for (int d = 1; d < WAVE; d *= 2) l += __shfl_xor(l, d);
+	if (lane == 0) sums[wave] = l;
+	__syncthreads();
+	const float sum = sums[0] + sums[1] + sums[2] + sums[3];
+	const uint32_t group = tid / LANES, at = tid % LANES;
+	if (group < GROUPS) {
+		f32x4 mine{ 0.0f, 0.0f, 0.0f, 0.0f };
+#pragma unroll 4
+		for (uint32_t p = group; p < parts; p += GROUPS) mine += *(const f32x4*)(from + (size_t)p * (16 * (D + 2)) + r * D + 4 * at) * weights[p];
+		o[group][at] = mine;
 	}
-	if (group != 0) return;
+	__syncthreads();
+	if (tid >= LANES) return;
+	f32x4 whole_row = o[0][at];
+	for (uint32_t g = 1; g < GROUPS; ++g) whole_row += o[g][at];
 	const float by = sum > 0.0f ? 1.0f / sum : sum == sum ? 0.0f : sum;
 	const size_t token = seq.first + row.token, query_head = (size_t)head * a.batch.group + row.head;
 	float v[4];
-	for (int e = 0; e < 4; ++e) v[e] = o[e] * by;
+	for (int e = 0; e < 4; ++e) v[e] = whole_row[e] * by;
 	store_out4(a, (char*)a.out + 2 * (token * a.out_token + query_head * a.out_head), 4 * at, v);
 	if (at == 0 && a.lse) a.lse[token * a.batch.query_heads + query_head] = sum == 0.0f ? -__builtin_inff() : (all + log2f(sum)) * 0.693147180559945309f;
 }
@@ -408,11 +436,13 @@ int launch_attend4(Attend4 a, uint32_t max_length, Workspace* ws, const DeviceIn
 	a.tiles_per_split = plan.tiles_per_split;
 	a.partial = ws->partials;
 	const uint64_t units = (uint64_t)a.batch.sequences * a.cache.heads * a.row_tiles;
-	if (units * a.splits > 0x7FFFFFFFu) return fail(KMX_ERR_UNSUPPORTED, "kmx_cache4_attend: too many queries for one call");
+	if (units * (a.splits < 16 ? 16 : a.splits) > 0x7FFFFFFFu) return fail(KMX_ERR_UNSUPPORTED, "kmx_cache4_attend: too many queries for one call");
 	KMX_LAUNCH_KERNEL((attend4_kernel<J>), dim3((unsigned)(units * a.splits)), dim3(256), 0, stream(), a);
 	KMX_LAUNCH_CHECK("attend4_kernel");
 	if (a.splits > 1) {
-		KMX_LAUNCH_KERNEL((join4_kernel<J>), dim3((unsigned)(units * 4)), dim3(256), 0, stream(), a);
+		const uint64_t rows_of_tile = a.chosen ? a.batch.group : (uint64_t)a.batch.max_queries * a.batch.group;
+		a.rows = (uint32_t)(rows_of_tile < 16 ? rows_of_tile : 16);
+		KMX_LAUNCH_KERNEL((join4_kernel<J>), dim3((unsigned)(units * a.rows)), dim3(256), 0, stream(), a);
 		KMX_LAUNCH_CHECK("join4_kernel");
 	}
 	return KMX_OK;
