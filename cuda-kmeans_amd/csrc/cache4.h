@@ -191,9 +191,11 @@ struct Attend4 {
 	const int32_t* chosen; uint32_t top; /* pages chosen for each token and head, or null */
 	float scale;
 	bool bf16, vec;
-	uint32_t row_tiles, splits, tiles_per_split, rows; /* (filled in by the launcher) */
-	float* partial;
+	uint32_t row_tiles, splits, tiles_per_split; /* (filled in by the launcher) */
+	float* partial; uint32_t* tickets;
 };
+constexpr uint32_t MOST_PARTS = 128; /* of the tokens of a row */
+constexpr uint32_t TICKETS = 8192;   /* units (sequence, head, tile of rows) of a call that takes its tokens in parts */
 /* launch shape: tiles of 16 rows, parts of the tokens, tiles of 64 tokens a part (cache4.hip) */
 struct Plan4 { uint32_t row_tiles, splits, tiles_per_split; };
 Plan4 plan_attend4(const Batch4& b, uint32_t heads, uint32_t max_length, uint32_t page_shift, uint32_t top, const DeviceInfo& dev);

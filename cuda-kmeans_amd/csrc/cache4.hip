@@ -537,7 +537,8 @@ Plan4 plan_attend4(const Batch4& b, uint32_t heads, uint32_t max_length, uint32_
 	const uint32_t tiles = (uint32_t)((tokens + 63) / 64);
 	uint64_t want = (2 * dev.compute_units + units - 1) / (units ? units : 1);
 	const uint64_t most = (tiles + 3) / 4;
-	if (want > 256) want = 256; /* (the kernel that joins them has a lane for each) */
+	if (want > MOST_PARTS) want = MOST_PARTS;
+	if (units > TICKETS) want = 1;
 	const uint32_t splits = (uint32_t)(want < most ? want : most ? most : 1);
 	plan.tiles_per_split = tiles ? ((tiles + splits - 1) / splits + 3) / 4 * 4 : 4;
 	plan.splits = tiles ? (tiles + plan.tiles_per_split - 1) / plan.tiles_per_split : 1;
@@ -633,10 +634,11 @@ static int check_batch4(const char* who, const kmx_cache4* cache, const kmx_cach
 
 static int reserve_cache4(const char* who, Workspace* ws, size_t floats)
 {
-	if (floats > ws->partials_cap && launches_recorded())
+	if ((floats > ws->partials_cap || !ws->tickets) && launches_recorded())
 		return fail(KMX_ERR_INVALID_ARGUMENT, "%s: the call needs a larger work space, which cannot be allocated while it is recorded: kmx_cache4_reserve, or the same call once before", who);
 	if (recording_graph()) scratch_recorded();
-	return reserve_partials(ws, floats);
+	const int rc = reserve_tickets(ws, TICKETS);
+	return rc ? rc : reserve_partials(ws, floats);
 }
 
 static uint32_t table_pages(const kmx_cache4_batch* b, uint32_t page_tokens)

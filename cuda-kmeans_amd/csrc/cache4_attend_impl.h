@@ -10,6 +10,8 @@
 
 #include "cache4.h"
 
+#include <type_traits>
+
 namespace kmx {
 
 /* 2^v by the instruction: results below 2^-126 are 0, which no sum here notices */
@@ -33,6 +35,16 @@ __device__ __forceinline__ Row4 row_of(const Attend4& a, const Sequence& seq, ui
 	}
 	return row;
 }
+
+/* rows of a tile that are there: the first ones */
+__device__ __forceinline__ uint32_t rows_of(const Attend4& a, const Sequence& seq, uint32_t row_tile)
+{
+	if (a.chosen) return min(16u, a.batch.group - row_tile % ((a.batch.group + 15) / 16) * 16);
+	const uint64_t rows = (uint64_t)seq.queries * a.batch.group, first = (uint64_t)row_tile * 16;
+	return first < rows ? (uint32_t)min((uint64_t)16, rows - first) : 0;
+}
+
+__device__ __forceinline__ uint64_t pair_of(float x, float y) { return (uint64_t)__builtin_bit_cast(uint32_t, y) << 32 | __builtin_bit_cast(uint32_t, x); }
 
 /* tiles of 64 tokens that a tile of rows looks at */
 __device__ __forceinline__ uint32_t tiles_of(const Attend4& a, const Sequence& seq, uint32_t row_tile)
@@ -133,7 +145,10 @@ attend4_kernel(Attend4 a)
 			int32_t from[4][2][WAVE];
 		};
 		f32x4 sums[2][2 * J][WAVE];
+		float weights[MOST_PARTS][16]; /* of the parts of the rows */
 	} lds;
+	__shared__ f32x4 shares[256];
+	__shared__ bool last;
 	__shared__ float most[4][16], total[4][16];
 	const uint32_t wave = (uint32_t)__builtin_amdgcn_readfirstlane((int)(threadIdx.x / WAVE)), lane = threadIdx.x % WAVE, i16 = lane % 16, kg = lane / 16;
 	/* first parts of all units before their second ones: the dies take work-groups in turn, and parts behind the end of a shorter sequence are empty */
@@ -144,8 +159,8 @@ attend4_kernel(Attend4 a)
 	const uint32_t tiles = tiles_of(a, seq, row_tile);
 	const uint32_t begin = part * a.tiles_per_split, end = min(tiles, begin + a.tiles_per_split);
 	if (part > 0 && begin >= tiles) return;
+	const uint32_t parts = tiles > a.tiles_per_split ? (tiles + a.tiles_per_split - 1) / a.tiles_per_split : 1;
 	const Row4 row = row_of(a, seq, row_tile, i16);
-	if (a.splits > 1 && tiles == 0) return; /* (the kernel that joins the parts writes the zeros) */
 
 	/* queries: 8 channels a lane for each j, with the sign of the scale, as halves of at most 2 in magnitude (bf16 has more exponents);
 	 * row_scale takes a score of theirs to the exponent of 2 */
@@ -353,78 +368,107 @@ attend4_kernel(Attend4 a)
 #pragma unroll
 		for (int c = 0; c < 2 * J; ++c) lds.sums[0][c][lane] = o[c];
 	__syncthreads();
-	if (wave != 0 || !row.there) return;
+	if (wave == 0) {
 #pragma unroll
-	for (int c = 0; c < 2 * J; ++c) o[c] += lds.sums[0][c][lane];
-
-	if (a.splits > 1) {
-		float* to = a.partial + ((size_t)whole * a.splits + part) * (16 * (D + 2));
+		for (int c = 0; c < 2 * J; ++c) o[c] += lds.sums[0][c][lane];
+	}
+	if (parts == 1) {
+		if (wave != 0 || !row.there) return;
+		const float by = sum > 0.0f ? 1.0f / sum : sum == sum ? 0.0f : sum; /* a row that sees nothing is zero; NaN stays */
+		const size_t token = seq.first + row.token, query_head = (size_t)head * a.batch.group + row.head;
+		char* to = (char*)a.out + 2 * (token * a.out_token + query_head * a.out_head);
 #pragma unroll
-		for (int c = 0; c < 2 * J; ++c) *(f32x4*)(to + i16 * D + 16 * c + 4 * kg) = o[c];
-		if (kg == 0) { to[16 * D + i16] = all * row_scale; to[16 * D + 16 + i16] = sum; }
+		for (int c = 0; c < 2 * J; ++c) {
+			float v[4];
+			for (int r = 0; r < 4; ++r) v[r] = o[c][r] * by;
+			store_out4(a, to, 16 * c + 4 * kg, v);
+		}
+		if (kg == 0 && a.lse) a.lse[token * a.batch.query_heads + query_head] = sum == 0.0f ? -__builtin_inff() : (all * row_scale + log2f(sum)) * 0.693147180559945309f;
 		return;
 	}
-	const float by = sum > 0.0f ? 1.0f / sum : sum == sum ? 0.0f : sum; /* a row that sees nothing is zero; NaN stays */
-	const size_t token = seq.first + row.token, query_head = (size_t)head * a.batch.group + row.head;
-	char* to = (char*)a.out + 2 * (token * a.out_token + query_head * a.out_head);
-#pragma unroll
-	for (int c = 0; c < 2 * J; ++c) {
-		float v[4];
-		for (int r = 0; r < 4; ++r) v[r] = o[c][r] * by;
-		store_out4(a, to, 16 * c + 4 * kg, v);
-	}
-	if (kg == 0 && a.lse) a.lse[token * a.batch.query_heads + query_head] = sum == 0.0f ? -__builtin_inff() : (all * row_scale + log2f(sum)) * 0.693147180559945309f;
-}
 
-/* Joins the parts of a row, a work-group each: the parts' weights first, one a lane, then its wavefronts take the parts in turn, 8 J lanes four
- * channels each. */
-template <int J>
-__global__ void __launch_bounds__(256)
-join4_kernel(Attend4 a)
-{
-	constexpr uint32_t D = 32 * J, LANES = 8 * J, GROUPS = 256 / LANES;
-	__shared__ float weights[256], most[4], sums[4];
-	__shared__ f32x4 o[GROUPS][LANES];
-	const uint32_t tid = threadIdx.x, wave = tid / WAVE, lane = tid % WAVE;
-	const uint32_t r = blockIdx.x % a.rows, whole = blockIdx.x / a.rows;
-	const uint32_t row_tile = whole % a.row_tiles, head = whole / a.row_tiles % a.cache.heads, s = whole / a.row_tiles / a.cache.heads;
-	const Sequence seq = sequence_of(a.batch, s, a.cache.page_shift);
-	const Row4 row = row_of(a, seq, row_tile, r);
-	if (!row.there) return;
-	const uint32_t tiles = tiles_of(a, seq, row_tile);
-	const uint32_t parts = (tiles + a.tiles_per_split - 1) / a.tiles_per_split; /* at most 256 */
-	const float* from = a.partial + (size_t)whole * a.splits * (16 * (D + 2));
-	const float m = tid < parts ? from[(size_t)tid * (16 * (D + 2)) + 16 * D + r] : -__builtin_inff();
-	float l = tid < parts ? from[(size_t)tid * (16 * (D + 2)) + 16 * D + 16 + r] : 0.0f;
-	float all = m;
-	for (int d = 1; d < WAVE; d *= 2) all = fmaxf(all, __shfl_xor(all, d));
-	if (lane == 0) most[wave] = all;
+	/*
+	 * The parts of the rows: each work-group leaves its sums, and the last one to do so joins them, in their order. Stores of device scope pass
+	 * the L2 of the die by, so a part is there for everybody once they have completed.
+	 */
+	uint64_t* const all_parts = (uint64_t*)a.partial + (size_t)whole * a.splits * (16 * (D / 2 + 1)); /* [part]: [16][D / 2] pairs, [16] of maximum and sum */
+	const uint32_t rows = rows_of(a, seq, row_tile);
+	if (wave == 0 && row.there) {
+		uint64_t* to = all_parts + (size_t)part * (16 * (D / 2 + 1));
+#pragma unroll
+		for (int c = 0; c < 2 * J; ++c)
+			for (int h = 0; h < 2; ++h)
+				__hip_atomic_store(to + i16 * (D / 2) + 8 * c + 2 * kg + h, pair_of(o[c][2 * h], o[c][2 * h + 1]), __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+		if (kg == 0) __hip_atomic_store(to + 16 * (D / 2) + i16, pair_of(all * row_scale, sum), __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+	}
+	asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
 	__syncthreads();
-	all = fmaxf(fmaxf(most[0], most[1]), fmaxf(most[2], most[3]));
-	const float weight = exp2_(m - (all == -__builtin_inff() ? 0.0f : all));
-	weights[tid] = weight;
-	l *= weight;
-	for (int d = 1; d < WAVE; d *= 2) l += __shfl_xor(l, d);
-	if (lane == 0) sums[wave] = l;
+	const uint32_t tid = threadIdx.x;
+	if (tid == 0) last = atomicAdd(&a.tickets[whole], 1u) == parts - 1;
 	__syncthreads();
-	const float sum = sums[0] + sums[1] + sums[2] + sums[3];
-	const uint32_t group = tid / LANES, at = tid % LANES;
-	if (group < GROUPS) {
-		f32x4 mine{ 0.0f, 0.0f, 0.0f, 0.0f };
-#pragma unroll 4
-		for (uint32_t p = group; p < parts; p += GROUPS) mine += *(const f32x4*)(from + (size_t)p * (16 * (D + 2)) + r * D + 4 * at) * weights[p];
-		o[group][at] = mine;
+	if (!last) return;
+	__builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "agent"); /* (nothing below is read ahead of the ticket, nor from a cache that was filled before it) */
+	if (tid == 0) __hip_atomic_store(&a.tickets[whole], 0u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT); /* for the next call */
+	const float* const left = (const float*)all_parts;
+	constexpr size_t PART = 2 * 16 * (D / 2 + 1);
+	{ /* weights: 16 lanes a row, all their parts under way at once */
+		constexpr uint32_t EACH = MOST_PARTS / 16;
+		const uint32_t r = tid / 16, from = tid % 16;
+		float2 v[EACH];
+		float top = -__builtin_inff(), s1 = 0.0f;
+#pragma unroll
+		for (uint32_t u = 0; u < EACH; ++u) {
+			v[u] = float2{ -__builtin_inff(), 0.0f };
+			if (from + 16 * u < parts && r < rows) v[u] = *(const float2*)(left + (from + 16 * u) * PART + 16 * D + 2 * r);
+		}
+#pragma unroll
+		for (uint32_t u = 0; u < EACH; ++u) top = fmaxf(top, v[u].x);
+		for (int d = 1; d < 16; d *= 2) top = fmaxf(top, __shfl_xor(top, d));
+		const float lowest = top == -__builtin_inff() ? 0.0f : top;
+#pragma unroll
+		for (uint32_t u = 0; u < EACH; ++u) {
+			const float weight = exp2_(v[u].x - lowest);
+			lds.weights[from + 16 * u][r] = weight;
+			s1 += v[u].y * weight;
+		}
+		for (int d = 1; d < 16; d *= 2) s1 += __shfl_xor(s1, d);
+		if (from == 0) { most[0][r] = top; total[0][r] = s1; }
 	}
 	__syncthreads();
-	if (tid >= LANES) return;
-	f32x4 whole_row = o[0][at];
-	for (uint32_t g = 1; g < GROUPS; ++g) whole_row += o[g][at];
-	const float by = sum > 0.0f ? 1.0f / sum : sum == sum ? 0.0f : sum;
-	const size_t token = seq.first + row.token, query_head = (size_t)head * a.batch.group + row.head;
-	float v[4];
-	for (int e = 0; e < 4; ++e) v[e] = whole_row[e] * by;
-	store_out4(a, (char*)a.out + 2 * (token * a.out_token + query_head * a.out_head), 4 * at, v);
-	if (at == 0 && a.lse) a.lse[token * a.batch.query_heads + query_head] = sum == 0.0f ? -__builtin_inff() : (all + log2f(sum)) * 0.693147180559945309f;
+	const uint32_t quads = rows * (D / 4), across = min(quads, 256u), groups = 256 / across, group = tid / across;
+	for (uint32_t e0 = 0; e0 < quads; e0 += across) {
+		const uint32_t e = e0 + tid % across, r = min(e, quads - 1) / (D / 4);
+		f32x4 mine{ 0.0f, 0.0f, 0.0f, 0.0f };
+		auto add = [&](auto batch) { /* the group's parts, so many under way */
+			constexpr uint32_t BATCH = decltype(batch)::value;
+			for (uint32_t p = group; p < parts; p += BATCH * groups) {
+				f32x4 v[BATCH];
+#pragma unroll
+				for (uint32_t u = 0; u < BATCH; ++u) v[u] = *(const f32x4*)(left + min(p + u * groups, parts - 1) * PART + 4 * e);
+#pragma unroll
+				for (uint32_t u = 0; u < BATCH; ++u)
+					if (p + u * groups < parts) mine += v[u] * lds.weights[p + u * groups][r];
+			}
+		};
+		if (group < groups && e < quads) {
+			if (parts > 4 * groups) add(std::integral_constant<uint32_t, 16>{});
+			else add(std::integral_constant<uint32_t, 4>{});
+		}
+		if (groups > 1) { /* (then this loop has one turn) */
+			shares[tid] = mine;
+			__syncthreads();
+			if (group == 0)
+				for (uint32_t g = 1; g < groups; ++g) mine += shares[g * across + tid];
+		}
+		if (group != 0 || e >= quads) continue;
+		const float s1 = total[0][r], by = s1 > 0.0f ? 1.0f / s1 : s1 == s1 ? 0.0f : s1;
+		const Row4 to_row = row_of(a, seq, row_tile, r);
+		const size_t token = seq.first + to_row.token, query_head = (size_t)head * a.batch.group + to_row.head;
+		float v[4];
+		for (int i = 0; i < 4; ++i) v[i] = mine[i] * by;
+		store_out4(a, (char*)a.out + 2 * (token * a.out_token + query_head * a.out_head), 4 * (e % (D / 4)), v);
+		if (e % (D / 4) == 0 && a.lse) a.lse[token * a.batch.query_heads + query_head] = s1 == 0.0f ? -__builtin_inff() : (most[0][r] + log2f(s1)) * 0.693147180559945309f;
+	}
 }
 
 template <int J>
@@ -435,16 +479,11 @@ int launch_attend4(Attend4 a, uint32_t max_length, Workspace* ws, const DeviceIn
 	a.splits = plan.splits;
 	a.tiles_per_split = plan.tiles_per_split;
 	a.partial = ws->partials;
+	a.tickets = ws->tickets;
 	const uint64_t units = (uint64_t)a.batch.sequences * a.cache.heads * a.row_tiles;
-	if (units * (a.splits < 16 ? 16 : a.splits) > 0x7FFFFFFFu) return fail(KMX_ERR_UNSUPPORTED, "kmx_cache4_attend: too many queries for one call");
+	if (units * a.splits > 0x7FFFFFFFu) return fail(KMX_ERR_UNSUPPORTED, "kmx_cache4_attend: too many queries for one call");
 	KMX_LAUNCH_KERNEL((attend4_kernel<J>), dim3((unsigned)(units * a.splits)), dim3(256), 0, stream(), a);
 	KMX_LAUNCH_CHECK("attend4_kernel");
-	if (a.splits > 1) {
-		const uint64_t rows_of_tile = a.chosen ? a.batch.group : (uint64_t)a.batch.max_queries * a.batch.group;
-		a.rows = (uint32_t)(rows_of_tile < 16 ? rows_of_tile : 16);
-		KMX_LAUNCH_KERNEL((join4_kernel<J>), dim3((unsigned)(units * a.rows)), dim3(256), 0, stream(), a);
-		KMX_LAUNCH_CHECK("join4_kernel");
-	}
 	return KMX_OK;
 }
 
