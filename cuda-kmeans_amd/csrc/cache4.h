@@ -197,7 +197,7 @@ struct Attend4 {
 constexpr uint32_t MOST_PARTS = 128; /* of the tokens of a row */
 constexpr uint32_t TICKETS = 8192;   /* units (sequence, head, tile of rows) of a call that takes its tokens in parts */
 /* launch shape: tiles of 16 rows, parts of the tokens, tiles of 64 tokens a part (cache4.hip) */
-struct Plan4 { uint32_t row_tiles, splits, tiles_per_split; };
+struct Plan4 { uint32_t row_tiles, splits, tiles_per_split; bool many; };
 Plan4 plan_attend4(const Batch4& b, uint32_t heads, uint32_t max_length, uint32_t page_shift, uint32_t top, const DeviceInfo& dev);
 template <int J> int launch_attend4(Attend4 a, uint32_t max_length, Workspace* ws, const DeviceInfo& dev);
 size_t attend4_partial_floats(uint32_t J, const Batch4& b, uint32_t heads, uint32_t max_length, uint32_t page_shift, uint32_t top, const DeviceInfo& dev);

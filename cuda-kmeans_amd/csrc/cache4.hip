@@ -528,19 +528,22 @@ choose4_kernel(Select4 a)
 
 /* ---------------------------------------------------------------- launch shapes of the attention - */
 
-/* Tiles of 16 rows, and how many parts the tokens are taken in: enough work-groups to fill the chip, none below one tile a wavefront */
+/* Tiles of 16 rows, or of 256 where there are many, and how many parts the tokens are taken in: enough work-groups to fill the chip, none below
+ * one tile a wavefront */
 Plan4 plan_attend4(const Batch4& b, uint32_t heads, uint32_t max_length, uint32_t page_shift, uint32_t top, const DeviceInfo& dev)
 {
 	Plan4 plan;
-	plan.row_tiles = top ? b.max_queries * ((b.group + 15) / 16) : (uint32_t)(((uint64_t)b.max_queries * b.group + 15) / 16);
+	const uint64_t rows = (uint64_t)b.max_queries * b.group;
+	plan.many = !top && rows > 64;
+	plan.row_tiles = top ? b.max_queries * ((b.group + 15) / 16) : (uint32_t)(plan.many ? (rows + 255) / 256 : (rows + 15) / 16);
 	const uint64_t tokens = top ? (uint64_t)top << page_shift : max_length, units = (uint64_t)b.sequences * heads * plan.row_tiles;
-	const uint32_t tiles = (uint32_t)((tokens + 63) / 64);
-	uint64_t want = (2 * dev.compute_units + units - 1) / (units ? units : 1);
-	const uint64_t most = (tiles + 3) / 4;
+	const uint32_t tiles = (uint32_t)((tokens + 63) / 64), step = plan.many ? 1 : 4, least = plan.many ? 16 : 4;
+	uint64_t want = ((plan.many ? 1 : 2) * dev.compute_units + units - 1) / (units ? units : 1);
+	const uint64_t most = (tiles + least - 1) / least;
 	if (want > MOST_PARTS) want = MOST_PARTS;
 	if (units > TICKETS) want = 1;
 	const uint32_t splits = (uint32_t)(want < most ? want : most ? most : 1);
-	plan.tiles_per_split = tiles ? ((tiles + splits - 1) / splits + 3) / 4 * 4 : 4;
+	plan.tiles_per_split = tiles ? ((tiles + splits - 1) / splits + step - 1) / step * step : step;
 	plan.splits = tiles ? (tiles + plan.tiles_per_split - 1) / plan.tiles_per_split : 1;
 	return plan;
 }
@@ -548,7 +551,7 @@ Plan4 plan_attend4(const Batch4& b, uint32_t heads, uint32_t max_length, uint32_
 size_t attend4_partial_floats(uint32_t J, const Batch4& b, uint32_t heads, uint32_t max_length, uint32_t page_shift, uint32_t top, const DeviceInfo& dev)
 {
 	const Plan4 plan = plan_attend4(b, heads, max_length, page_shift, top, dev);
-	return plan.splits > 1 ? (size_t)b.sequences * heads * plan.row_tiles * plan.splits * (16 * (32 * J + 2)) : 0;
+	return plan.splits > 1 ? (size_t)b.sequences * heads * plan.row_tiles * plan.splits * ((plan.many ? 256 : 16) * (32 * J + 2)) : 0;
 }
 
 } // namespace kmx

@@ -105,6 +105,29 @@ __device__ __forceinline__ void load_rows(const char* p, bool vec, float x[J][8]
 		for (int j = 0; j < J; ++j) load8((const T*)p + 32 * j, false, x[j]);
 }
 
+template <int N, typename T>
+__device__ __forceinline__ void load_steps(const char* p, bool vec, float x[N][8]) /* of every 16 */
+{
+	if (vec)
+		for (int c = 0; c < N; ++c) load8((const T*)p + 16 * c, true, x[c]);
+	else
+		for (int c = 0; c < N; ++c) load8((const T*)p + 16 * c, false, x[c]);
+}
+
+template <int J>
+constexpr int values_words() { return J > 4 * ((J + 3) / 4) ? J : 4 * ((J + 3) / 4); } /* words of codes a lane holds: J of keys, or 4 for each of its pairs of channels */
+
+/* What queries of that largest magnitude are multiplied with to become halves of at most 2 in magnitude (bf16 has more exponents), with the sign
+ * of the scale; *row_scale takes a score of theirs to the exponent of 2 */
+__device__ __forceinline__ float query_scale(float scale, float largest, float* row_scale)
+{
+	int power = (int)(__builtin_bit_cast(uint32_t, largest) >> 23) - 127;
+	power = power < -126 ? 0 : power > 126 ? 126 : power;
+	const float by = __builtin_bit_cast(float, (uint32_t)(127 - power) << 23);
+	*row_scale = fmaxf(fabsf(scale) * 1.44269504088896341f * __builtin_bit_cast(float, (uint32_t)(127 + power) << 23), 1.2e-38f);
+	return scale > 0.0f ? by : scale < 0.0f ? -by : 0.0f;
+}
+
 /* 4 channels of an output row */
 __device__ __forceinline__ void store_out4(const Attend4& a, char* row, uint32_t channel, const float v[4])
 {
@@ -162,8 +185,7 @@ attend4_kernel(Attend4 a)
 	const uint32_t parts = tiles > a.tiles_per_split ? (tiles + a.tiles_per_split - 1) / a.tiles_per_split : 1;
 	const Row4 row = row_of(a, seq, row_tile, i16);
 
-	/* queries: 8 channels a lane for each j, with the sign of the scale, as halves of at most 2 in magnitude (bf16 has more exponents);
-	 * row_scale takes a score of theirs to the exponent of 2 */
+	/* queries: 8 channels a lane for each j */
 	half8v q[J];
 	float row_scale;
 	{
@@ -180,11 +202,7 @@ attend4_kernel(Attend4 a)
 			for (int e = 0; e < 8; ++e) largest = fmaxf(largest, fabsf(x[j][e]));
 		largest = fmaxf(largest, __shfl_xor(largest, 16));
 		largest = fmaxf(largest, __shfl_xor(largest, 32));
-		int power = (int)(__builtin_bit_cast(uint32_t, largest) >> 23) - 127;
-		power = power < -126 ? 0 : power > 126 ? 126 : power;
-		float by = __builtin_bit_cast(float, (uint32_t)(127 - power) << 23);
-		row_scale = fmaxf(fabsf(a.scale) * 1.44269504088896341f * __builtin_bit_cast(float, (uint32_t)(127 + power) << 23), 1.2e-38f);
-		by = a.scale > 0.0f ? by : a.scale < 0.0f ? -by : 0.0f;
+		const float by = query_scale(a.scale, largest, &row_scale);
 #pragma unroll
 		for (int j = 0; j < J; ++j)
 			for (int e = 0; e < 8; ++e) q[j][e] = (_Float16)(x[j][e] * by);
@@ -471,6 +489,269 @@ attend4_kernel(Attend4 a)
 	}
 }
 
+/* ---------------------------------------------------------------- many rows ---------------------- */
+
+typedef float f32x16 __attribute__((ext_vector_type(16)));
+
+/*
+ * Many rows (pieces of prompts): a work-group of eight wavefronts takes 256 rows of one head, 32 a wavefront, and a part of the tokens. Tiles of 64
+ * tokens become half-precision numbers once for all of them: wavefront w < 4 unpacks the keys of block w, wavefront 4 + w its values, into LDS,
+ * into one of two buffers while everybody works on the other. Scores are [token][row] as above (v_mfma_f32_32x32x16_f16, 16 tokens a lane and
+ * half of the tile), so that probabilities stay in their registers: the values' tokens lie in LDS in the order in which a lane has them. Rows of
+ * LDS are 16 bytes longer than their contents: 8 lanes one below the other read 8 different groups of banks.
+ */
+template <int J>
+__global__ void __launch_bounds__(512, 2)
+attend4_many_kernel(Attend4 a)
+{
+	constexpr uint32_t D = 32 * J, KROW = 2 * D + 16, VROW = 144, TILE = 64 * KROW + D * VROW;
+	extern __shared__ __attribute__((aligned(16))) uint8_t many[]; /* two tiles: keys [token][channel], values [channel][token] */
+	const uint32_t wave = (uint32_t)__builtin_amdgcn_readfirstlane((int)(threadIdx.x / WAVE)), lane = threadIdx.x % WAVE, n32 = lane % 32, h = lane / 32;
+	const uint32_t units = gridDim.x / a.splits, part = blockIdx.x / units, whole = blockIdx.x % units;
+	const uint32_t row_tile = whole % a.row_tiles, head = whole / a.row_tiles % a.cache.heads, s = whole / a.row_tiles / a.cache.heads;
+	const Sequence seq = sequence_of(a.batch, s, a.cache.page_shift);
+	const uint64_t all_rows = (uint64_t)seq.queries * a.batch.group, first_row = (uint64_t)row_tile * 256;
+	if (first_row >= all_rows) return;
+	const uint32_t rows = (uint32_t)min((uint64_t)256, all_rows - first_row);
+	const uint32_t tiles = (visible_to(a.batch, seq, (uint32_t)((first_row + rows - 1) / a.batch.group)) + 63) / 64;
+	const uint32_t begin = part * a.tiles_per_split, end = min(tiles, begin + a.tiles_per_split);
+	if (part > 0 && begin >= tiles) return;
+	const uint32_t parts = tiles > a.tiles_per_split ? (tiles + a.tiles_per_split - 1) / a.tiles_per_split : 1;
+
+	/* the lane's row, and what the rows of its wavefront see at least and at most */
+	const uint32_t wave_rows = rows > 32 * wave ? min(32u, rows - 32 * wave) : 0;
+	const bool there = n32 < wave_rows;
+	const uint64_t x_row = first_row + 32 * wave + (there ? n32 : 0);
+	const uint32_t token = there ? (uint32_t)(x_row / a.batch.group) : 0, query_head = (uint32_t)(head * a.batch.group + (there ? x_row % a.batch.group : 0));
+	const int32_t sees = there ? (int32_t)visible_to(a.batch, seq, token) : 0;
+	const int32_t least = wave_rows ? (int32_t)visible_to(a.batch, seq, (uint32_t)((first_row + 32 * wave) / a.batch.group)) : 0;
+	const int32_t seen = wave_rows ? (int32_t)visible_to(a.batch, seq, (uint32_t)((first_row + 32 * wave + wave_rows - 1) / a.batch.group)) : 0;
+
+	half8v q[2 * J]; /* channels 16 c + 8 h .. + 7 */
+	float row_scale;
+	{
+		float x[2 * J][8];
+		const char* p = (const char*)a.q + 2 * ((size_t)(seq.first + token) * a.q_token + (size_t)query_head * a.q_head + 8 * h);
+		if (a.bf16) load_steps<2 * J, __bf16>(p, a.vec, x);
+		else load_steps<2 * J, _Float16>(p, a.vec, x);
+		float largest = 0.0f;
+#pragma unroll
+		for (int c = 0; c < 2 * J; ++c)
+			for (int e = 0; e < 8; ++e) largest = fmaxf(largest, fabsf(x[c][e]));
+		largest = fmaxf(largest, __shfl_xor(largest, 32));
+		const float by = query_scale(a.scale, largest, &row_scale);
+#pragma unroll
+		for (int c = 0; c < 2 * J; ++c)
+			for (int e = 0; e < 8; ++e) q[c][e] = (_Float16)(x[c][e] * by);
+	}
+
+	const uint32_t b = wave % 4, sub_bits = a.cache.page_shift - 4; /* the block of a tile that this wavefront unpacks */
+	const bool values = wave >= 4;
+	const Magnitudes mag = load_magnitudes(a.cache.levels, head, values ? 1 : 0);
+	const int32_t* table = a.batch.table + (size_t)s * a.batch.table_stride;
+	constexpr int VITEMS = (16 * J + WAVE - 1) / WAVE; /* pairs of channels a lane */
+	struct { uint32_t codes[values_words<J>()]; u32x4 scales[VITEMS][2]; uint32_t key_scales[(J + 1) / 2]; } in;
+	int32_t written = 0; /* tokens of the block that are there */
+	auto fetch = [&](uint32_t tile) {
+		const uint32_t n = 4 * tile + b, entry = n >> sub_bits, sub = n & ((1u << sub_bits) - 1);
+		const uint32_t page = (uint32_t)table[min(entry, a.batch.table_stride - 1)];
+		const bool known = entry < a.batch.table_stride && page < a.cache.page_count;
+		written = known ? (int32_t)seq.length - (int32_t)(16 * n) : 0;
+		const uint8_t* block = a.cache.blocks + block_offset<J>(a.cache, known ? page : 0, head, sub);
+		if (!values) {
+			load_words<J>(block + lane * 4 * J, in.codes); /* lane = 4 token + kg */
+			load_halves<J>(block + 16 * D + lane / 4 * 2 * J, in.key_scales);
+		} else {
+#pragma unroll
+			for (int i = 0; i < VITEMS; ++i) {
+				const uint32_t pair = min(lane + WAVE * i, 16u * J - 1);
+				const u32x4 w = *(const u32x4*)(block + 8 * D + 16 * pair);
+				for (int e = 0; e < 4; ++e) in.codes[4 * i + e] = w[e];
+				in.scales[i][0] = *(const u32x4*)(block + 17 * D + 32 * (pair / 16));
+				in.scales[i][1] = *(const u32x4*)(block + 17 * D + 32 * (pair / 16) + 16);
+			}
+		}
+	};
+	auto unpack = [&](uint8_t* tile) {
+		if (!values) {
+			uint8_t* row = tile + (16 * b + lane / 4) * KROW + 16 * (lane % 4);
+#pragma unroll
+			for (int j = 0; j < J; ++j) {
+				uint32_t w[4];
+				unpack4<false>(in.codes[j], mag, w[0], w[1]);
+				unpack4<true>(in.codes[j], mag, w[2], w[3]);
+				const uint32_t scale = twice(in.key_scales[j / 2], j % 2);
+				*(u32x4*)(row + 64 * j) = u32x4{ times(w[0], scale), times(w[1], scale), times(w[2], scale), times(w[3], scale) };
+			}
+		} else {
+#pragma unroll
+			for (int i = 0; i < VITEMS; ++i) {
+				if (written < 16) { /* what lies behind the last token may hold anything: scales of zero */
+#pragma unroll
+					for (int d = 0; d < 8; ++d) in.scales[i][d / 4][d % 4] &= written >= 2 * d + 2 ? 0xFFFFFFFFu : written == 2 * d + 1 ? 0xFFFFu : 0u;
+				}
+				const uint32_t pair = lane + WAVE * i;
+				if (16 * J % WAVE && pair >= 16 * J) continue;
+				uint32_t low[8], high[8];
+#pragma unroll
+				for (int d = 0; d < 4; ++d) {
+					unpack4<false>(in.codes[4 * i + d], mag, low[2 * d], low[2 * d + 1]);
+					unpack4<true>(in.codes[4 * i + d], mag, high[2 * d], high[2 * d + 1]);
+					for (int e = 0; e < 2; ++e) {
+						const uint32_t scale = in.scales[i][d / 2][2 * (d % 2) + e];
+						low[2 * d + e] = times(low[2 * d + e], scale);
+						high[2 * d + e] = times(high[2 * d + e], scale);
+					}
+				}
+				/* tokens 0 to 3 and 8 to 11 are those of the lanes with h = 0, the others of h = 1 */
+				uint8_t* row = tile + 64 * KROW + (32 * (pair / 16) + pair % 16) * VROW + 32 * b;
+				*(u32x4*)row = u32x4{ low[0], low[1], low[4], low[5] };
+				*(u32x4*)(row + 16) = u32x4{ low[2], low[3], low[6], low[7] };
+				*(u32x4*)(row + 16 * VROW) = u32x4{ high[0], high[1], high[4], high[5] };
+				*(u32x4*)(row + 16 * VROW + 16) = u32x4{ high[2], high[3], high[6], high[7] };
+			}
+		}
+	};
+
+	float m = -__builtin_inff(), l = 0.0f;
+	f32x16 o[J];
+#pragma unroll
+	for (int j = 0; j < J; ++j)
+		for (int e = 0; e < 16; ++e) o[j][e] = 0.0f;
+
+	auto work = [&](const uint8_t* tile, int32_t from) {
+		f32x16 sc[2];
+#pragma unroll
+		for (int t = 0; t < 2; ++t) {
+			for (int e = 0; e < 16; ++e) sc[t][e] = 0.0f;
+#pragma unroll
+			for (int c = 0; c < 2 * J; ++c)
+				sc[t] = __builtin_amdgcn_mfma_f32_32x32x16_f16(*(const half8v*)(tile + (32 * t + n32) * KROW + 32 * c + 16 * h), q[c], sc[t], 0, 0, 0);
+		}
+		if (from + 64 > least) {
+#pragma unroll
+			for (int e = 0; e < 32; ++e) {
+				const int32_t place = from + 32 * (e / 16) + 8 * (e % 16 / 4) + 4 * (int32_t)h + e % 4;
+				sc[e / 16][e % 16] = place < sees ? sc[e / 16][e % 16] : -__builtin_inff();
+			}
+		}
+		float top = sc[0][0];
+#pragma unroll
+		for (int e = 1; e < 32; ++e) top = fmaxf(top, sc[e / 16][e % 16]);
+		top = fmaxf(top, __shfl_xor(top, 32));
+		const float now = fmaxf(m, top);
+		if (__any(now > m)) {
+			const float less = m == now ? 1.0f : exp2_((m - now) * row_scale);
+			l *= less;
+#pragma unroll
+			for (int j = 0; j < J; ++j) o[j] *= less;
+			m = now;
+		}
+		const float base = m == -__builtin_inff() ? 0.0f : -m * row_scale;
+		half8v p[4];
+#pragma unroll
+		for (int e = 0; e < 32; ++e) {
+			const float v = exp2_(fmaf(sc[e / 16][e % 16], row_scale, base));
+			l += v;
+			p[e / 8][e % 8] = (_Float16)v;
+		}
+#pragma unroll
+		for (int j = 0; j < J; ++j)
+#pragma unroll
+			for (int c = 0; c < 4; ++c)
+				o[j] = __builtin_amdgcn_mfma_f32_32x32x16_f16(*(const half8v*)(tile + 64 * KROW + (32 * j + n32) * VROW + 32 * c + 16 * h), p[c], o[j], 0, 0, 0);
+	};
+
+	if (begin < end) {
+		fetch(begin);
+		unpack(many);
+		fetch(min(begin + 1, end - 1));
+		__syncthreads();
+		for (uint32_t tile = begin; tile < end; ++tile) {
+			uint8_t* const now = many + (tile - begin) % 2 * TILE;
+			uint8_t* const next = many + (tile - begin + 1) % 2 * TILE;
+			if (tile + 1 < end) unpack(next);
+			if (tile + 2 < end) fetch(tile + 2);
+			if ((int32_t)(64 * tile) < seen) work(now, (int32_t)(64 * tile));
+			__syncthreads();
+		}
+	}
+	l += __shfl_xor(l, 32);
+
+	if (parts == 1) {
+		if (!there) return;
+		const float by = l > 0.0f ? 1.0f / l : l == l ? 0.0f : l;
+		char* to = (char*)a.out + 2 * ((size_t)(seq.first + token) * a.out_token + (size_t)query_head * a.out_head);
+#pragma unroll
+		for (int j = 0; j < J; ++j)
+			for (int e = 0; e < 4; ++e) {
+				float v[4];
+				for (int r = 0; r < 4; ++r) v[r] = o[j][4 * e + r] * by;
+				store_out4(a, to, 32 * j + 8 * e + 4 * h, v);
+			}
+		if (h == 0 && a.lse) a.lse[(size_t)(seq.first + token) * a.batch.query_heads + query_head] = l == 0.0f ? -__builtin_inff() : (m * row_scale + log2f(l)) * 0.693147180559945309f;
+		return;
+	}
+
+	/* a part of the tokens: [256][D] sums, then [256] pairs of maximum and sum, for join4_kernel */
+	float* const to = a.partial + ((size_t)whole * a.splits + part) * (256 * (D + 2));
+	if (!there) return;
+	const uint32_t r = 32 * wave + n32;
+#pragma unroll
+	for (int j = 0; j < J; ++j)
+		for (int e = 0; e < 4; ++e) *(f32x4*)(to + (size_t)r * D + 32 * j + 8 * e + 4 * h) = f32x4{ o[j][4 * e], o[j][4 * e + 1], o[j][4 * e + 2], o[j][4 * e + 3] };
+	if (h == 0) *(float2*)(to + 256 * D + 2 * r) = float2{ m * row_scale, l };
+}
+
+/* Joins the parts of many rows: 256 rows of sums are more than one work-group should read alone, so they have a kernel. A wavefront takes a row, 8 J
+ * lanes 4 channels each of every (64 / 8 J)-th part. */
+template <int J>
+__global__ void __launch_bounds__(256)
+join4_kernel(Attend4 a)
+{
+	constexpr uint32_t D = 32 * J, LANES = 8 * J, GROUPS = WAVE / LANES;
+	constexpr size_t PART = 256 * (D + 2);
+	const uint32_t wave = (uint32_t)__builtin_amdgcn_readfirstlane((int)(threadIdx.x / WAVE)), lane = threadIdx.x % WAVE;
+	const uint32_t whole = blockIdx.x / 64, r = blockIdx.x % 64 * 4 + wave;
+	const uint32_t row_tile = whole % a.row_tiles, head = whole / a.row_tiles % a.cache.heads, s = whole / a.row_tiles / a.cache.heads;
+	const Sequence seq = sequence_of(a.batch, s, a.cache.page_shift);
+	const uint64_t all_rows = (uint64_t)seq.queries * a.batch.group, first_row = (uint64_t)row_tile * 256;
+	if (first_row + r >= all_rows) return;
+	const uint32_t rows = (uint32_t)min((uint64_t)256, all_rows - first_row);
+	const uint32_t tiles = (visible_to(a.batch, seq, (uint32_t)((first_row + rows - 1) / a.batch.group)) + 63) / 64;
+	if (tiles <= a.tiles_per_split) return; /* one part: written where it belongs */
+	const uint32_t parts = (tiles + a.tiles_per_split - 1) / a.tiles_per_split, group = lane / LANES, at = lane % LANES;
+	const float* left = a.partial + (size_t)whole * a.splits * PART;
+	float top = -__builtin_inff();
+	for (uint32_t p = lane; p < parts; p += WAVE) top = fmaxf(top, left[p * PART + 256 * D + 2 * r]);
+	for (int d = 1; d < WAVE; d *= 2) top = fmaxf(top, __shfl_xor(top, d));
+	const float lowest = top == -__builtin_inff() ? 0.0f : top;
+	float sum = 0.0f;
+	f32x4 mine{ 0.0f, 0.0f, 0.0f, 0.0f };
+	if (group < GROUPS)
+#pragma unroll 4
+		for (uint32_t p = group; p < parts; p += GROUPS) {
+			const float2 ml = *(const float2*)(left + p * PART + 256 * D + 2 * r);
+			const float weight = exp2_(ml.x - lowest);
+			sum += ml.y * weight;
+			mine += *(const f32x4*)(left + p * PART + (size_t)r * D + 4 * at) * weight;
+		}
+	for (uint32_t g = 1; g < GROUPS; ++g) { /* the groups' sums, in their order */
+		const int other = (int)(at + g * LANES);
+		const f32x4 more{ __shfl(mine[0], other), __shfl(mine[1], other), __shfl(mine[2], other), __shfl(mine[3], other) };
+		const float more_sum = __shfl(sum, other);
+		if (group == 0) { mine += more; sum += more_sum; }
+	}
+	if (group != 0) return;
+	const float by = sum > 0.0f ? 1.0f / sum : sum == sum ? 0.0f : sum;
+	const uint64_t x = first_row + r;
+	const size_t to_token = seq.first + x / a.batch.group, to_head = (size_t)head * a.batch.group + x % a.batch.group;
+	float v[4];
+	for (int e = 0; e < 4; ++e) v[e] = mine[e] * by;
+	store_out4(a, (char*)a.out + 2 * (to_token * a.out_token + to_head * a.out_head), 4 * at, v);
+	if (at == 0 && a.lse) a.lse[to_token * a.batch.query_heads + to_head] = sum == 0.0f ? -__builtin_inff() : (top + log2f(sum)) * 0.693147180559945309f;
+}
+
 template <int J>
 int launch_attend4(Attend4 a, uint32_t max_length, Workspace* ws, const DeviceInfo& dev)
 {
@@ -481,7 +762,22 @@ int launch_attend4(Attend4 a, uint32_t max_length, Workspace* ws, const DeviceIn
 	a.partial = ws->partials;
 	a.tickets = ws->tickets;
 	const uint64_t units = (uint64_t)a.batch.sequences * a.cache.heads * a.row_tiles;
-	if (units * a.splits > 0x7FFFFFFFu) return fail(KMX_ERR_UNSUPPORTED, "kmx_cache4_attend: too many queries for one call");
+	if (units * (a.splits < 64 ? 64 : a.splits) > 0x7FFFFFFFu) return fail(KMX_ERR_UNSUPPORTED, "kmx_cache4_attend: too many queries for one call");
+	if (plan.many) {
+		constexpr uint32_t bytes = 2 * (64 * (64 * J + 16) + 32 * J * 144);
+		static bool allowed = false; /* more LDS than a launch may ask for unannounced */
+		if (!allowed && bytes > 65536) {
+			KMX_HIP(hipFuncSetAttribute((const void*)attend4_many_kernel<J>, hipFuncAttributeMaxDynamicSharedMemorySize, (int)bytes));
+			allowed = true;
+		}
+		KMX_LAUNCH_KERNEL((attend4_many_kernel<J>), dim3((unsigned)(units * a.splits)), dim3(512), bytes, stream(), a);
+		KMX_LAUNCH_CHECK("attend4_many_kernel");
+		if (a.splits > 1) {
+			KMX_LAUNCH_KERNEL((join4_kernel<J>), dim3((unsigned)(units * 64)), dim3(256), 0, stream(), a);
+			KMX_LAUNCH_CHECK("join4_kernel");
+		}
+		return KMX_OK;
+	}
 	KMX_LAUNCH_KERNEL((attend4_kernel<J>), dim3((unsigned)(units * a.splits)), dim3(256), 0, stream(), a);
 	KMX_LAUNCH_CHECK("attend4_kernel");
 	return KMX_OK;
