@@ -70,6 +70,14 @@ __device__ __forceinline__ uint32_t twice(uint32_t half_word, bool upper) /* one
 	return __builtin_amdgcn_perm(half_word, half_word, upper ? 0x07060706u : 0x05040504u);
 }
 
+/* between what lanes of a wavefront write to LDS and what others of it read there (LDS takes a wavefront's accesses in their order; this keeps
+ * the compiler to it) */
+__device__ __forceinline__ void wave_sync()
+{
+	__builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+	__builtin_amdgcn_wave_barrier();
+}
+
 template <int CTRL>
 __device__ __forceinline__ float dpp(float v)
 {

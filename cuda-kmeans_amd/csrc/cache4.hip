@@ -129,7 +129,7 @@ write4_kernel(Rows4 a)
 			if (there && g == 0)
 #pragma unroll
 				for (int j = 0; j < J; ++j) ((_Float16*)(block + 17 * D))[16 * j + at] = scale[j];
-			__builtin_amdgcn_wave_barrier();
+			wave_sync();
 			const uint32_t slot0 = (uint32_t)__builtin_amdgcn_readfirstlane(slot);
 			if (__ballot(!there || (uint32_t)slot != slot0 + t) == 0 && slot0 % 16 == 0) {
 				for (uint32_t p = lane; p < D / 2; p += WAVE) *(u32x4*)(block + 8 * D + p * 16) = *(const u32x4*)(mine + p * 16);
@@ -183,7 +183,7 @@ read4_kernel(Rows4 a)
 			for (uint32_t p = lane; p < D / 2; p += WAVE) mine[n * ROW + p] = in[p * 16];
 		}
 	}
-	__builtin_amdgcn_wave_barrier();
+	wave_sync();
 	if (token >= a.tokens) return;
 	for (int which = 0; which < 2; ++which) {
 		const Magnitudes m = load_magnitudes(a.cache.levels, head, which);
@@ -233,79 +233,93 @@ static int launch_rows4(bool write, const Rows4& a, uint32_t J)
 
 /* ---------------------------------------------------------------- bounds of pages ---------------- */
 
-/* A wavefront takes a page and head: lane = 4 token + g keeps the largest and the smallest value of its channels over its tokens of all
- * blocks, then the 16 lanes of a g join theirs. Values are products of half-precision numbers, exact in floats, and maxima know no order. */
+/*
+ * 1, 2 or 4 wavefronts (as many as a page has blocks, at most 4) take a page and head. A wavefront unpacks a block, lane = 4 token + g as in the
+ * block, and turns it over in LDS: its lanes go on with the channels, 16 tokens each. Values are products of half-precision numbers, exact in
+ * floats, and maxima know no order.
+ */
 template <int J>
 __global__ void __launch_bounds__(256)
-bound4_kernel(Cache4 c, const int32_t* __restrict__ pages, const int32_t* __restrict__ counts, uint32_t count)
+bound4_kernel(Cache4 c, const int32_t* __restrict__ pages, const int32_t* __restrict__ counts, uint32_t count, uint32_t waves)
 {
-	constexpr uint32_t D = 32 * J;
-	const uint32_t wave = threadIdx.x / WAVE, lane = threadIdx.x % WAVE, t = lane / 4, g = lane % 4;
-	const uint64_t unit = (uint64_t)blockIdx.x * 4 + wave;
-	const uint64_t entry = unit / c.heads;
+	constexpr uint32_t D = 32 * J, ROW = D + 4;
+	__shared__ __attribute__((aligned(16))) float turned[4][16 * ROW];
+	__shared__ float high[4][D], low[4][D];
+	const uint32_t wave = (uint32_t)__builtin_amdgcn_readfirstlane((int)(threadIdx.x / WAVE)), lane = threadIdx.x % WAVE, t = lane / 4, g = lane % 4;
+	const uint32_t set = wave / waves, mine = wave % waves; /* the work-group's 4 / waves pages, and the wavefronts of each */
+	const uint64_t unit = (uint64_t)blockIdx.x * (4 / waves) + set, entry = unit / c.heads;
 	const uint32_t head = (uint32_t)(unit % c.heads);
-	if (entry >= count) return;
-	const int32_t page = pages[entry];
-	if (page < 0 || (uint32_t)page >= c.page_count) return;
+	const int32_t page = entry < count ? pages[entry] : -1;
+	const bool there = page >= 0 && (uint32_t)page < c.page_count;
 	const int32_t room = 1 << c.page_shift;
-	const int32_t tokens = counts[entry] < 0 ? 0 : counts[entry] < room ? counts[entry] : room;
+	const int32_t tokens = !there || counts[entry] < 0 ? 0 : counts[entry] < room ? counts[entry] : room;
 	const Magnitudes m = load_magnitudes(c.levels, head, 0);
-	float hi[8 * J], lo[8 * J];
+	constexpr int EACH = (D + WAVE - 1) / WAVE; /* channels a lane */
+	float hi[EACH], lo[EACH];
 #pragma unroll
-	for (int i = 0; i < 8 * J; ++i) { hi[i] = -__builtin_inff(); lo[i] = __builtin_inff(); }
-	for (int32_t from = 0; from < tokens; from += 16) {
+	for (int i = 0; i < EACH; ++i) { hi[i] = -__builtin_inff(); lo[i] = __builtin_inff(); }
+	for (int32_t from = 16 * mine; from < tokens; from += 16 * waves) {
 		const uint8_t* block = c.blocks + block_offset<J>(c, (uint32_t)page, head, from / 16);
-		if (from + (int32_t)t < tokens) {
-			const uint32_t* codes = (const uint32_t*)(block + t * (D / 2) + g * 4 * J);
-			const _Float16* scales = (const _Float16*)(block + 16 * D) + t * J;
+		uint32_t codes[J], scales[(J + 1) / 2];
+		{
+			const uint32_t* p = (const uint32_t*)(block + 4 * J * lane);
+			const uint16_t* s = (const uint16_t*)(block + 16 * D) + t * J;
 #pragma unroll
-			for (int j = 0; j < J; ++j) {
-				uint32_t w[4];
-				unpack4<false>(codes[j], m, w[0], w[1]);
-				unpack4<true>(codes[j], m, w[2], w[3]);
-				const float scale = (float)scales[j];
+			for (int j = 0; j < J; ++j) codes[j] = p[j];
 #pragma unroll
-				for (int i = 0; i < 8; ++i) {
-					const float x = scale * (float)__builtin_bit_cast(half2v, w[i / 2])[i % 2];
-					hi[8 * j + i] = fmaxf(hi[8 * j + i], x);
-					lo[8 * j + i] = fminf(lo[8 * j + i], x);
-				}
+			for (int j = 0; j < J; ++j) scales[j / 2] = j % 2 ? scales[j / 2] | (uint32_t)s[j] << 16 : s[j];
+		}
+		wave_sync();
+#pragma unroll
+		for (int j = 0; j < J; ++j) {
+			uint32_t w[4];
+			unpack4<false>(codes[j], m, w[0], w[1]);
+			unpack4<true>(codes[j], m, w[2], w[3]);
+			const float scale = (float)__builtin_bit_cast(_Float16, (uint16_t)(scales[j / 2] >> (16 * (j % 2))));
+			float x[8];
+			for (int i = 0; i < 8; ++i) x[i] = scale * (float)__builtin_bit_cast(half2v, w[i / 2])[i % 2];
+			float* row = turned[wave] + t * ROW + 32 * j + 8 * g;
+			*(f32x4*)row = f32x4{ x[0], x[1], x[2], x[3] };
+			*(f32x4*)(row + 4) = f32x4{ x[4], x[5], x[6], x[7] };
+		}
+		wave_sync();
+		const int32_t rows = min(16, tokens - from);
+#pragma unroll
+		for (int i = 0; i < EACH; ++i) {
+			const uint32_t ch = min(lane + WAVE * i, D - 1);
+#pragma unroll
+			for (int n = 0; n < 16; ++n) {
+				const float x = turned[wave][n * ROW + ch];
+				hi[i] = n < rows ? fmaxf(hi[i], x) : hi[i];
+				lo[i] = n < rows ? fminf(lo[i], x) : lo[i];
 			}
 		}
 	}
-	float largest = 0.0f;
 #pragma unroll
-	for (int i = 0; i < 8 * J; ++i) {
-		hi[i] = fmaxf(hi[i], dpp<DPP_ROR4>(hi[i]));
-		lo[i] = fminf(lo[i], dpp<DPP_ROR4>(lo[i]));
-		hi[i] = fmaxf(hi[i], dpp<DPP_ROR8>(hi[i]));
-		lo[i] = fminf(lo[i], dpp<DPP_ROR8>(lo[i]));
-		for (int x = 16; x < 64; x *= 2) {
-			hi[i] = fmaxf(hi[i], __shfl_xor(hi[i], x));
-			lo[i] = fminf(lo[i], __shfl_xor(lo[i], x));
-		}
+	for (int i = 0; i < EACH; ++i)
+		if (lane + WAVE * i < D) { high[wave][lane + WAVE * i] = hi[i]; low[wave][lane + WAVE * i] = lo[i]; }
+	__syncthreads();
+	if (mine != 0) return;
+	float top = 0.0f;
+#pragma unroll
+	for (int i = 0; i < EACH; ++i) {
+		const uint32_t ch = min(lane + WAVE * i, D - 1);
+		for (uint32_t w = 1; w < waves; ++w) { hi[i] = fmaxf(hi[i], high[wave + w][ch]); lo[i] = fminf(lo[i], low[wave + w][ch]); }
 		if (tokens == 0) hi[i] = lo[i] = 0.0f;
-		largest = fmaxf(largest, fmaxf(fabsf(hi[i]), fabsf(lo[i])));
+		if (lane + WAVE * i < D) top = fmaxf(top, fmaxf(fabsf(hi[i]), fabsf(lo[i])));
 	}
-	largest = fmaxf(largest, dpp<DPP_XOR1>(largest));
-	largest = fmaxf(largest, dpp<DPP_XOR2>(largest));
-	const float by = largest > 0.0f ? 127.0f / largest : 0.0f;
+	for (int d = 1; d < WAVE; d *= 2) top = fmaxf(top, __shfl_xor(top, d));
+	if (!there) return;
+	const float by = top > 0.0f ? 1.0f / top * 127.0f : 0.0f;
 	int8_t* out = c.bounds + ((size_t)page * c.heads + head) * (2 * D);
 #pragma unroll
-	for (int j = 0; j < J; ++j) {
-		if (t != (uint32_t)j) continue; /* lane 4 j + g writes group j */
-		uint32_t h[2] = { 0, 0 }, l[2] = { 0, 0 };
-#pragma unroll
-		for (int i = 0; i < 8; ++i) { /* outwards, so that a bound stays one */
-			const int up = (int)fminf(fmaxf(ceilf(hi[8 * j + i] * by), -127.0f), 127.0f);
-			const int down = (int)fminf(fmaxf(floorf(lo[8 * j + i] * by), -127.0f), 127.0f);
-			h[i / 4] |= (uint32_t)(up & 0xFF) << (8 * (i % 4));
-			l[i / 4] |= (uint32_t)(down & 0xFF) << (8 * (i % 4));
-		}
-		*(u32x2*)(out + 32 * j + 8 * g) = u32x2{ h[0], h[1] };
-		*(u32x2*)(out + D + 32 * j + 8 * g) = u32x2{ l[0], l[1] };
+	for (int i = 0; i < EACH; ++i) {
+		const uint32_t ch = lane + WAVE * i;
+		if (ch >= D) continue;
+		out[ch] = (int8_t)fminf(fmaxf(ceilf(hi[i] * by), -127.0f), 127.0f); /* outwards, so that a bound stays one */
+		out[D + ch] = (int8_t)fminf(fmaxf(floorf(lo[i] * by), -127.0f), 127.0f);
 	}
-	if (lane == 0) c.bound_scales[(size_t)page * c.heads + head] = largest / 127.0f;
+	if (lane == 0) c.bound_scales[(size_t)page * c.heads + head] = top / 127.0f;
 }
 
 /* ---------------------------------------------------------------- the choice of pages ------------ */
@@ -318,7 +332,8 @@ struct Select4 {
 	int32_t* chosen;    /* [token][head][top] */
 	uint32_t top, first, last;
 	uint32_t span;      /* query heads of a token side by side: the power of two from `group` on, at most 16 */
-	uint32_t token_tiles, chunks, chunk; /* tiles of queries a sequence; parts of the pages and how many tiles of 16 each */
+	uint32_t per;       /* tokens of a tile of queries: a power of two, at most 16 / span and 8 */
+	uint32_t token_tiles, chunks, chunk; /* tiles of queries a sequence; parts of the pages and how many times 64 each */
 	bool bf16, vec;
 };
 
@@ -329,30 +344,189 @@ __device__ __forceinline__ uint32_t ordered(float v)
 	return u & 0x80000000u ? ~u : u | 0x80000000u;
 }
 
-__device__ __forceinline__ void load_query16(const Select4& a, const void* q, bool there, float x[16])
+/* 8 elements as they are, two a word */
+__device__ __forceinline__ u32x4 load_raw8(const uint16_t* p, bool vec)
 {
-	if (!there) {
-		for (int i = 0; i < 16; ++i) x[i] = 0.0f;
-	} else if (a.bf16) {
-		load8((const __bf16*)q, a.vec, x);
-		load8((const __bf16*)q + 8, a.vec, x + 8);
-	} else {
-		load8((const _Float16*)q, a.vec, x);
-		load8((const _Float16*)q + 8, a.vec, x + 8);
-	}
+	if (vec) return *(const u32x4*)p;
+	u32x4 w;
+	for (int i = 0; i < 4; ++i) w[i] = p[2 * i] | (uint32_t)p[2 * i + 1] << 16;
+	return w;
+}
+__device__ __forceinline__ float raw_element(uint32_t w, bool upper, bool bf16)
+{
+	if (bf16) return __builtin_bit_cast(float, upper ? w & 0xFFFF0000u : w << 16);
+	return (float)__builtin_bit_cast(_Float16, (uint16_t)(upper ? w >> 16 : w));
 }
 
 /*
- * The score of a page: the bound on q . k over its keys, in 8 bits. A wavefront keeps 16 rows of queries (16 / span tokens of one head of the
- * cache) as 8-bit columns of v_mfma_i32_16x16x64_i8: the positive parts against the largest values, the negative ones against the smallest.
- * Whole numbers below 2^24, the same in any order. Bounds are read once, 16 bytes a lane: the kernel is bound by that, and by its launch.
+ * The scores of pages: the bound on q . k over a page, in 8 bits. 16 rows of queries (tokens of one head of the cache, their query heads side by
+ * side) are 8-bit columns of v_mfma_i32_16x16x64_i8: the positive parts against the largest values, the negative ones against the smallest.
+ * Whole numbers below 2^24, the same in any order. A lane holds 16 of each 64 of the 2 dim numbers of row or page lane % 16. The work-group
+ * rounds the rows once, in LDS, for all its wavefronts (768 instructions a wavefront if each does it for itself).
  */
+template <int J>
+struct Scorer4 {
+	static constexpr uint32_t D = 32 * J, ROW = 2 * D + 16; /* LDS: 8 rows one below the other lie in 8 different groups of banks */
+	struct Lds {
+		__attribute__((aligned(16))) int8_t rows[16 * ROW];
+		uint32_t largest[8];
+	};
+	const Select4& a;
+	const Sequence& seq;
+	uint32_t head, tile, col, kg, i; /* i: the query of the lane's row */
+	bool token_there;
+	i32x4 q8[J];
+
+	__device__ __forceinline__ Scorer4(const Select4& args, const Sequence& sequence, uint32_t cache_head, uint32_t tile_of_queries, uint32_t lane)
+	    : a(args), seq(sequence), head(cache_head), tile(tile_of_queries), col(lane % 16), kg(lane / 16), i(tile * args.per + lane % 16 / args.span)
+	{
+		token_there = lane % 16 / a.span < a.per && i < seq.queries;
+	}
+	/* 8 channels of a row of the 16 from query head g0 on; zeros where there is none */
+	__device__ __forceinline__ u32x4 load(uint32_t g0, uint32_t row, uint32_t channel) const
+	{
+		const uint32_t token = tile * a.per + row / a.span, h = g0 + row % a.span;
+		if (row / a.span >= a.per || token >= seq.queries || h >= a.batch.group) return u32x4{ 0, 0, 0, 0 };
+		return load_raw8((const uint16_t*)a.q + (size_t)(seq.first + token) * a.q_token + (size_t)(head * a.batch.group + h) * a.q_head + channel, a.vec);
+	}
+	/* the largest magnitude of each token, over all its query heads; by all threads of the work-group */
+	__device__ __forceinline__ void measure(Lds& lds, uint32_t threads) const
+	{
+		if (threadIdx.x < 8) lds.largest[threadIdx.x] = 0;
+		__syncthreads();
+		for (uint32_t g0 = 0; g0 < a.batch.group; g0 += 16)
+			for (uint32_t item = threadIdx.x; item < a.per * a.span * (D / 8); item += threads) {
+				const u32x4 raw = load(g0, item / (D / 8), item % (D / 8) * 8);
+				float largest = 0.0f;
+				for (int e = 0; e < 8; ++e) {
+					const uint32_t w = raw[e / 2];
+					largest = fmaxf(largest, fabsf(raw_element(w, e % 2, a.bf16)));
+				}
+				atomicMax(&lds.largest[item / (D / 8) / a.span], __builtin_bit_cast(uint32_t, largest)); /* (not negative: in the order of their words) */
+			}
+		__syncthreads();
+	}
+	/* the 16 rows from query head g0 on in 8 bits, into LDS and then the lanes */
+	__device__ __forceinline__ void round(Lds& lds, uint32_t g0, uint32_t threads)
+	{
+		for (uint32_t item = threadIdx.x; item < 16 * (D / 8); item += threads) {
+			const uint32_t row = item / (D / 8), channel = item % (D / 8) * 8;
+			const float largest = __builtin_bit_cast(float, lds.largest[min(row / a.span, 7u)]);
+			const float by = largest > 0.0f ? 1.0f / largest * 127.0f : 0.0f;
+			const u32x4 raw = load(g0, row, channel);
+			u32x2 up{ 0, 0 }, down{ 0, 0 };
+			for (int e = 0; e < 8; ++e) {
+				const uint32_t w = raw[e / 2];
+				float v = raw_element(w, e % 2, a.bf16) * by;
+				v = v != v ? 0.0f : fminf(fmaxf(rintf(v), -127.0f), 127.0f);
+				up[e / 4] |= (uint32_t)((int)fmaxf(v, 0.0f) & 0xFF) << (8 * (e % 4));
+				down[e / 4] |= (uint32_t)((int)fminf(v, 0.0f) & 0xFF) << (8 * (e % 4));
+			}
+			*(u32x2*)(lds.rows + row * ROW + channel) = up;
+			*(u32x2*)(lds.rows + row * ROW + D + channel) = down;
+		}
+		__syncthreads();
+#pragma unroll
+		for (int c = 0; c < J; ++c) q8[c] = *(const i32x4*)(lds.rows + col * ROW + 64 * c + 16 * kg);
+	}
+	/* the whole numbers of 16 pages: lane (col, kg) gets those of its row and the pages 4 kg + r, of the rows from query head g0 on */
+	__device__ __forceinline__ void dots(const i32x4 b[J], uint32_t g0, int best[4]) const
+	{
+		i32x4 dot{ 0, 0, 0, 0 };
+#pragma unroll
+		for (int c = 0; c < J; ++c) dot = __builtin_amdgcn_mfma_i32_16x16x64_i8(b[c], q8[c], dot, 0, 0, 0);
+		const bool there = token_there && g0 + col % a.span < a.batch.group;
+		for (int r = 0; r < 4; ++r) best[r] = there ? dot[r] : INT32_MIN;
+		for (uint32_t d = 1; d < a.span; d *= 2) /* the largest over the token's query heads */
+			for (int r = 0; r < 4; ++r) best[r] = max(best[r], __shfl_xor(best[r], (int)d));
+	}
+	/* pages of the sequence with a token that the lane's query sees */
+	__device__ __forceinline__ uint32_t seen() const { return token_there ? (visible_to(a.batch, seq, i) + (1u << a.cache.page_shift) - 1) >> a.cache.page_shift : 0; }
+	/* the lane that writes number r of its page: the lanes of a token share them out */
+	__device__ __forceinline__ bool writes(int r) const { return token_there && (col % a.span) < 4 && (uint32_t)r % min(a.span, 4u) == col % min(a.span, 4u); }
+	__device__ __forceinline__ uint32_t key(uint32_t page, uint32_t pages, int best, float scale, bool known) const
+	{
+		const bool forced = page < a.first || page + a.last >= pages;
+		return ordered(forced ? __builtin_inff() : known ? (float)best * scale + 0.0f : -__builtin_inff()); /* (+ 0: one zero) */
+	}
+};
+
+/*
+ * All scores of a work-group's pages [from, end), a wavefront 16 TILES pages at a time and `stride` pages further each time; the bounds of the next ones are under way
+ * while it works on those. put(query, page, key) takes them. More than 16 query heads to a head: again for each 16, the largest kept.
+ */
+template <int J, int TILES, typename GET, typename PUT>
+__device__ __forceinline__ void score_pages(Scorer4<J>& scorer, typename Scorer4<J>::Lds& lds, const int32_t* table, uint32_t from, uint32_t end, uint32_t pages, uint32_t stride, uint32_t threads, const GET& get, const PUT& put)
+{
+	const Select4& a = scorer.a;
+	const uint32_t col = scorer.col, kg = scorer.kg;
+	auto page_at = [&](uint32_t p) { return (uint32_t)table[min(p, pages - 1)]; };
+	uint32_t page[TILES], after[TILES];
+	float scale[TILES];
+	i32x4 b[TILES][J];
+	auto fetch = [&]() {
+#pragma unroll
+		for (int t = 0; t < TILES; ++t) {
+			const bool there = page[t] < a.cache.page_count;
+			const size_t at = (size_t)(there ? page[t] : 0) * a.cache.heads + scorer.head;
+			scale[t] = a.cache.bound_scales[at];
+			const int8_t* bounds = a.cache.bounds + at * (64 * J) + 16 * kg;
+#pragma unroll
+			for (int c = 0; c < J; ++c) b[t][c] = *(const i32x4*)(bounds + 64 * c);
+		}
+	};
+	auto begin = [&]() {
+#pragma unroll
+		for (int t = 0; t < TILES; ++t) page[t] = page_at(from + 16 * t + col);
+#pragma unroll
+		for (int t = 0; t < TILES; ++t) after[t] = page_at(from + stride + 16 * t + col);
+		fetch();
+	};
+	begin();
+	scorer.measure(lds, threads);
+	const uint32_t seen = scorer.seen();
+	for (uint32_t g0 = 0; g0 < a.batch.group; g0 += 16) {
+		if (g0) {
+			__syncthreads(); /* (the rows before have been read) */
+			begin();
+		}
+		scorer.round(lds, g0, threads);
+		for (uint32_t p0 = from; p0 < end; p0 += stride) {
+			int best[TILES][4];
+			float scales[TILES];
+			bool known[TILES];
+#pragma unroll
+			for (int t = 0; t < TILES; ++t) {
+				scorer.dots(b[t], g0, best[t]);
+				scales[t] = scale[t];
+				known[t] = page[t] < a.cache.page_count;
+				page[t] = after[t];
+			}
+			fetch();
+#pragma unroll
+			for (int t = 0; t < TILES; ++t) after[t] = page_at(p0 + 2 * stride + 16 * t + col);
+#pragma unroll
+			for (int t = 0; t < TILES; ++t)
+#pragma unroll
+				for (int r = 0; r < 4; ++r) {
+					const float sc = __shfl(scales[t], (int)(4 * kg + r)); /* (lanes 0 to 15 hold the scales of the 16 pages) */
+					const int there = __shfl(known[t] ? 1 : 0, (int)(4 * kg + r));
+					const uint32_t p = p0 + 16 * t + 4 * kg + r;
+					if (!scorer.writes(r) || p >= min(seen, end)) continue;
+					const uint32_t k = scorer.key(p, seen, best[t][r], sc, there);
+					put(p, g0 ? max(get(p), k) : k);
+				}
+		}
+	}
+}
+
+/* Many pages for few queries: scores in one kernel, a part of the pages a work-group, the choice in the next. */
 template <int J>
 __global__ void __launch_bounds__(256)
 score4_kernel(Select4 a)
 {
-	constexpr uint32_t D = 32 * J;
-	const uint32_t wave = threadIdx.x / WAVE, lane = threadIdx.x % WAVE, col = lane % 16, kg = lane / 16;
+	__shared__ typename Scorer4<J>::Lds lds;
+	const uint32_t wave = (uint32_t)__builtin_amdgcn_readfirstlane((int)(threadIdx.x / WAVE)), lane = threadIdx.x % WAVE;
 	uint32_t unit = blockIdx.x;
 	const uint32_t part = unit % a.chunks;
 	unit /= a.chunks;
@@ -360,97 +534,132 @@ score4_kernel(Select4 a)
 	unit /= a.cache.heads;
 	const uint32_t tile = unit % a.token_tiles, s = unit / a.token_tiles;
 	const Sequence seq = sequence_of(a.batch, s, a.cache.page_shift);
-	const uint32_t per = 16 / a.span, i = tile * per + col / a.span;
-	if (tile * per >= seq.queries) return;
-	const uint32_t page_tokens = 1u << a.cache.page_shift;
-	const uint32_t last_i = min(seq.queries - 1, tile * per + per - 1);
+	if (tile * a.per >= seq.queries) return;
+	const uint32_t page_tokens = 1u << a.cache.page_shift, last_i = min(seq.queries, (tile + 1) * a.per) - 1;
 	const uint32_t pages = (visible_to(a.batch, seq, last_i) + page_tokens - 1) >> a.cache.page_shift;
-	uint32_t p0 = (part * a.chunk * 4 + wave) * 16; /* the wavefronts of a part take its tiles in turn */
 	if (part * a.chunk * 64 >= pages) return;
-	const bool token_there = i < seq.queries;
-
-	/* the scale of the queries of each token and head: their largest magnitude, over all its query heads */
-	float largest = 0.0f;
-	const char* q = (const char*)a.q + 2 * ((size_t)(seq.first + (token_there ? i : 0)) * a.q_token + (size_t)head * a.batch.group * a.q_head);
-	float x[16];
-	for (uint32_t h0 = 0; h0 < a.batch.group; h0 += 16) {
-		const uint32_t h = h0 + col % a.span;
-		const bool there = token_there && h < a.batch.group;
-#pragma unroll
-		for (int c = 0; c < J; ++c) {
-			load_query16(a, q + 2 * ((size_t)(there ? h : 0) * a.q_head + (64 * c + 16 * kg) % D), there, x);
-			for (int n = 0; n < 16; ++n) largest = fmaxf(largest, fabsf(x[n]));
-		}
-	}
-	for (uint32_t d = 1; d < a.span; d *= 2) largest = fmaxf(largest, __shfl_xor(largest, (int)d));
-	for (int d = 16; d < 64; d *= 2) largest = fmaxf(largest, __shfl_xor(largest, d));
-	const float by = largest > 0.0f ? 127.0f / largest : 0.0f;
-
-	const uint32_t tiles = a.batch.group > 16 ? (a.batch.group + 15) / 16 : 1;
-	i32x4 q8[J];
-	for (uint32_t n = 0; n < a.chunk; ++n, p0 += 64) {
-		if (p0 >= pages) break;
-		const uint32_t p = p0 + col;
-		const int32_t page = p < pages ? a.batch.table[(size_t)s * a.batch.table_stride + p] : -1;
-		const bool there = page >= 0 && (uint32_t)page < a.cache.page_count;
-		const int8_t* bounds = a.cache.bounds + ((size_t)(there ? page : 0) * a.cache.heads + head) * (2 * D) + 16 * kg;
-		const float scale = there ? a.cache.bound_scales[(size_t)page * a.cache.heads + head] : 0.0f;
-		i32x4 b[J];
-#pragma unroll
-		for (int c = 0; c < J; ++c) b[c] = *(const i32x4*)(bounds + 64 * c);
-		int best[4] = { INT32_MIN, INT32_MIN, INT32_MIN, INT32_MIN };
-		for (uint32_t g0 = 0; g0 < tiles; ++g0) {
-			const uint32_t h = g0 * 16 + col % a.span;
-			const bool row_there = token_there && h < a.batch.group;
-			if (n == 0 || tiles > 1) {
-#pragma unroll
-				for (int c = 0; c < J; ++c) {
-					const uint32_t at = 64 * c + 16 * kg;
-					load_query16(a, q + 2 * ((size_t)(row_there ? h : 0) * a.q_head + at % D), row_there, x);
-					for (int w = 0; w < 4; ++w) {
-						uint32_t word = 0;
-						for (int e = 0; e < 4; ++e) {
-							float v = x[4 * w + e] * by;
-							v = v != v ? 0.0f : fminf(fmaxf(rintf(v), -127.0f), 127.0f);
-							v = at < D ? fmaxf(v, 0.0f) : fminf(v, 0.0f);
-							word |= (uint32_t)((int)v & 0xFF) << (8 * e);
-						}
-						q8[c][w] = (int)word;
-					}
-				}
-			}
-			i32x4 dot{ 0, 0, 0, 0 };
-#pragma unroll
-			for (int c = 0; c < J; ++c) dot = __builtin_amdgcn_mfma_i32_16x16x64_i8(b[c], q8[c], dot, 0, 0, 0);
-			/* lane: query row col, pages p0 + 4 kg + r */
-			for (int r = 0; r < 4; ++r) best[r] = max(best[r], row_there ? dot[r] : INT32_MIN);
-		}
-		for (int r = 0; r < 4; ++r) {
-			for (uint32_t d = 1; d < a.span; d *= 2) best[r] = max(best[r], __shfl_xor(best[r], (int)d));
-			const float sc = __shfl(scale, (int)(4 * kg + r)); /* (lanes 0 to 15 hold the scales of the tile's pages) */
-			const int known = __shfl(there ? 1 : 0, (int)(4 * kg + r));
-			const uint32_t pr = p0 + 4 * kg + r;
-			if (!token_there || pr >= pages || (r & (a.span - 1)) != (col & (a.span - 1) & 3) || (col % a.span) > 3) continue;
-			const uint32_t seen = (visible_to(a.batch, seq, i) + page_tokens - 1) >> a.cache.page_shift;
-			if (pr >= seen) continue;
-			const bool forced = pr < a.first || pr + a.last >= seen;
-			const float score = forced ? __builtin_inff() : known ? (float)best[r] * sc + 0.0f : -__builtin_inff(); /* (+ 0: one zero) */
-			a.keys[((size_t)(seq.first + i) * a.cache.heads + head) * a.batch.table_stride + pr] = ordered(score);
-		}
-	}
+	Scorer4<J> scorer(a, seq, head, tile, lane);
+	uint32_t* const keys = a.keys + ((size_t)(seq.first + (scorer.token_there ? scorer.i : 0)) * a.cache.heads + head) * a.batch.table_stride;
+	score_pages<J, 1>(scorer, lds, a.batch.table + (size_t)s * a.batch.table_stride, (part * a.chunk * 4 + wave) * 16, min(pages, (part + 1) * a.chunk * 64), pages, 64, 256,
+	                  [&](uint32_t p) { return keys[p]; }, [&](uint32_t p, uint32_t k) { keys[p] = k; });
 }
 
 /*
- * The `top` best pages of each token and head, ascending: the threshold by four passes over 8 bits of the scores, then one pass in the order
- * of the pages that keeps what lies above it and as many at the threshold as are left, the lowest first. One work-group each.
+ * The `top` best of n keys, ascending. The keys' range is cut into 512 steps, whose numbers of keys tell the step with the threshold, that step again
+ * into 512, until all of a step is wanted or its keys are equal (four passes over 8 bits each, whatever the keys, took 9 us for 1024 keys; this
+ * mostly ends after one). Then one pass in the order of the pages keeps what lies above the threshold and as many at it as are left, the lowest
+ * first. All threads of the work-group come here, `threads` of them (whole wavefronts, thread `tid` of them) to each list.
  */
-__global__ void __launch_bounds__(256)
+constexpr uint32_t FORCED_KEY = 0xFF800000u; /* ordered(infinity) */
+struct ChooseLds { uint32_t histogram[512], low, high, forced, step[3]; }; /* of a list */
+template <typename KEY>
+__device__ __forceinline__ void choose_top(const KEY& key, uint32_t n, uint32_t top, int32_t* out, uint32_t tid, uint32_t threads, ChooseLds& lds, uint32_t* above, uint32_t* equal)
+{
+	const uint32_t wave = tid / WAVE, lane = tid % WAVE, waves = threads / WAVE;
+	const bool all = n <= top; /* (n = 0 and out = null where there is no list) */
+	if (all)
+		for (uint32_t e = tid; out && e < top; e += threads) out[e] = e < n ? (int32_t)e : -1;
+	const uint32_t some = all ? 0 : n;
+	if (tid == 0) { lds.low = 0xFFFFFFFFu; lds.high = 0; lds.forced = 0; }
+	for (uint32_t e = tid; e < 512; e += threads) lds.histogram[e] = 0;
+	__syncthreads();
+	{
+		uint32_t low = 0xFFFFFFFFu, high = 0, forced = 0;
+		for (uint32_t p = tid; p < some; p += threads) {
+			const uint32_t k = key(p);
+			if (k == FORCED_KEY) ++forced;
+			else { low = min(low, k); high = max(high, k); }
+		}
+		for (int d = 1; d < WAVE; d *= 2) {
+			low = min(low, (uint32_t)__shfl_xor((int)low, d));
+			high = max(high, (uint32_t)__shfl_xor((int)high, d));
+			forced += __shfl_xor((int)forced, d);
+		}
+		if (lane == 0 && !all) { atomicMin(&lds.low, low); atomicMax(&lds.high, high); atomicAdd(&lds.forced, forced); }
+	}
+	__syncthreads();
+	/* kept: the keys above `threshold`, and the first `rest` of those equal to it */
+	uint32_t low = lds.low, width = 0xFFFFFFFFu, rest = top - (all ? top : lds.forced), threshold = lds.high; /* the threshold lies in [low, low + width) */
+	int shift = all || lds.high <= low ? 0 : 32 - __clz(lds.high - low);
+	shift = shift > 9 ? shift - 9 : 0;
+	bool done = all || rest == 0;
+	while (__syncthreads_or(!done)) {
+		if (!done)
+			for (uint32_t p = tid; p < some; p += threads) {
+				const uint32_t k = key(p);
+				if (k != FORCED_KEY && k >= low && k - low < width) atomicAdd(&lds.histogram[(k - low) >> shift], 1u);
+			}
+		__syncthreads();
+		if (wave == 0 && !done) { /* lane l: steps 511 - 8 l and the seven below */
+			uint32_t sum = 0;
+			for (int e = 0; e < 8; ++e) sum += lds.histogram[511 - 8 * lane - e];
+			uint32_t upto = sum;
+			for (int d = 1; d < WAVE; d *= 2) {
+				const uint32_t v = __shfl_up(upto, d);
+				if (lane >= (uint32_t)d) upto += v;
+			}
+			uint32_t before = upto - sum;
+			if (before < rest && rest <= upto)
+				for (int e = 0; e < 8; ++e) {
+					const uint32_t h = lds.histogram[511 - 8 * lane - e];
+					if (rest <= before + h) {
+						lds.step[0] = 511 - 8 * lane - e;
+						lds.step[1] = rest - before;
+						lds.step[2] = h;
+						break;
+					}
+					before += h;
+				}
+		}
+		__syncthreads();
+		if (!done) {
+			low += lds.step[0] << shift;
+			width = 1u << shift;
+			rest = lds.step[1];
+			if (lds.step[2] == rest) { /* all of the step */
+				threshold = low - 1;
+				rest = 0;
+				done = true;
+			} else if (shift == 0) {
+				threshold = low;
+				done = true;
+			}
+			shift = shift > 9 ? shift - 9 : 0;
+			for (uint32_t e = tid; e < 512; e += threads) lds.histogram[e] = 0;
+		}
+	}
+	/* a wavefront takes a stretch of the pages: how many of it lie above the threshold and at it, then where they go */
+	const uint32_t stretch = ((some + waves - 1) / waves + WAVE - 1) / WAVE * WAVE, from = wave * stretch, to = min(some, from + stretch);
+	uint32_t gt = 0, eq = 0;
+	for (uint32_t p0 = from; p0 < to; p0 += WAVE) {
+		const uint32_t p = p0 + lane, k = p < to ? key(p) : 0;
+		gt += __popcll(__ballot(p < to && k > threshold));
+		eq += __popcll(__ballot(p < to && k == threshold));
+	}
+	if (lane == 0) { above[wave] = gt; equal[wave] = eq; }
+	__syncthreads();
+	uint32_t written = lane < wave ? above[lane] : 0, ties = lane < wave ? equal[lane] : 0; /* before this stretch (at most 16 wavefronts) */
+	for (int d = 1; d < 16; d *= 2) { written += __shfl_xor((int)written, d); ties += __shfl_xor((int)ties, d); }
+	written = (uint32_t)__builtin_amdgcn_readfirstlane((int)written);
+	ties = (uint32_t)__builtin_amdgcn_readfirstlane((int)ties);
+	const uint64_t below = ((uint64_t)1 << lane) - 1;
+	for (uint32_t p0 = from; p0 < to; p0 += WAVE) {
+		const uint32_t p = p0 + lane, k = p < to ? key(p) : 0;
+		const bool is_above = p < to && k > threshold, is_equal = p < to && k == threshold;
+		const uint64_t ballot_above = __ballot(is_above), ballot_equal = __ballot(is_equal);
+		const uint32_t my_eq = ties + __popcll(ballot_equal & below), my_gt = written + __popcll(ballot_above & below);
+		if (is_above || (is_equal && my_eq < rest)) out[my_gt + min(my_eq, rest)] = (int32_t)p;
+		written += __popcll(ballot_above);
+		ties += __popcll(ballot_equal);
+	}
+}
+
+__global__ void __launch_bounds__(512)
 choose4_kernel(Select4 a)
 {
-	__shared__ uint32_t histogram[256];
-	__shared__ uint32_t found[2];
-	__shared__ uint32_t above[4], equal[4];
-	const uint32_t tid = threadIdx.x, wave = tid / WAVE, lane = tid % WAVE;
+	constexpr uint32_t CACHED = 8192;
+	__shared__ uint32_t above[8], equal[8], cached[CACHED];
+	__shared__ ChooseLds lds;
 	uint32_t unit = blockIdx.x;
 	const uint32_t head = unit % a.cache.heads;
 	unit /= a.cache.heads;
@@ -459,71 +668,55 @@ choose4_kernel(Select4 a)
 	if (i >= seq.queries) return;
 	const uint32_t n = (visible_to(a.batch, seq, i) + (1u << a.cache.page_shift) - 1) >> a.cache.page_shift;
 	const size_t row = (size_t)(seq.first + i) * a.cache.heads + head;
-	int32_t* out = a.chosen + row * a.top;
-	if (n <= a.top) {
-		for (uint32_t e = tid; e < a.top; e += 256) out[e] = e < n ? (int32_t)e : -1;
+	const uint32_t* keys = a.keys + row * a.batch.table_stride;
+	if (n > CACHED) {
+		choose_top([&](uint32_t p) { return keys[p]; }, n, a.top, a.chosen + row * a.top, threadIdx.x, 512, lds, above, equal);
 		return;
 	}
-	const uint32_t* keys = a.keys + row * a.batch.table_stride;
-	uint32_t prefix = 0, mask = 0, rest = a.top; /* the rest-th largest among the keys that agree with the prefix */
-	for (int shift = 24; shift >= 0; shift -= 8) {
-		histogram[tid] = 0;
-		__syncthreads();
-		for (uint32_t p = tid; p < n; p += 256) {
-			const uint32_t k = keys[p];
-			if ((k & mask) == prefix) atomicAdd(&histogram[(k >> shift) & 255u], 1u);
-		}
-		__syncthreads();
-		if (wave == 0) { /* lane l: digits 255 - 4 l and the three below */
-			uint32_t sum = 0;
-			for (int e = 0; e < 4; ++e) sum += histogram[255 - 4 * lane - e];
-			uint32_t upto = sum;
-			for (int d = 1; d < WAVE; d *= 2) {
-				const uint32_t v = __shfl_up(upto, d);
-				if (lane >= (uint32_t)d) upto += v;
-			}
-			uint32_t before = upto - sum;
-			if (before < rest && rest <= upto) {
-				for (int e = 0; e < 4; ++e) {
-					const uint32_t h = histogram[255 - 4 * lane - e];
-					if (rest <= before + h) {
-						found[0] = 255 - 4 * lane - e;
-						found[1] = rest - before;
-						break;
-					}
-					before += h;
-				}
-			}
-		}
-		__syncthreads();
-		prefix |= found[0] << shift;
-		mask |= 255u << shift;
-		rest = found[1];
-		__syncthreads();
+	if (n > a.top)
+		for (uint32_t p = threadIdx.x; p < n; p += 512) cached[p] = keys[p];
+	choose_top([&](uint32_t p) { return cached[p]; }, n, a.top, a.chosen + row * a.top, threadIdx.x, 512, lds, above, equal);
+}
+
+/*
+ * Both in one kernel, where the keys of a tile of queries fit LDS and a work-group reads them fast enough: it takes `per` tokens of one
+ * head, all pages.
+ */
+constexpr uint32_t select_threads(uint32_t J, bool small) { return small ? 256 : J <= 4 ? 1024 : 512; } /* few pages, or as many wavefronts as the registers allow */
+constexpr uint32_t SELECT_FEW = 512, SELECT_PAGES = 768;
+
+template <int J, bool FEW>
+__global__ void __launch_bounds__(select_threads(J, FEW))
+select4_kernel(Select4 a, uint32_t stride)
+{
+	extern __shared__ uint32_t keys[]; /* [per][stride] */
+	constexpr uint32_t THREADS = select_threads(J, FEW);
+	__shared__ typename Scorer4<J>::Lds lds;
+	__shared__ ChooseLds choose[8];
+	__shared__ uint32_t above[THREADS / WAVE], equal[THREADS / WAVE];
+	const uint32_t wave = (uint32_t)__builtin_amdgcn_readfirstlane((int)(threadIdx.x / WAVE)), lane = threadIdx.x % WAVE;
+	uint32_t unit = blockIdx.x;
+	const uint32_t head = unit % a.cache.heads;
+	unit /= a.cache.heads;
+	const uint32_t tile = unit % a.token_tiles, s = unit / a.token_tiles;
+	const Sequence seq = sequence_of(a.batch, s, a.cache.page_shift);
+	if (tile * a.per >= seq.queries) return;
+	const uint32_t page_tokens = 1u << a.cache.page_shift, last_i = min(seq.queries, (tile + 1) * a.per) - 1;
+	const uint32_t pages = (visible_to(a.batch, seq, last_i) + page_tokens - 1) >> a.cache.page_shift;
+	if (pages > a.top) {
+		Scorer4<J> scorer(a, seq, head, tile, lane);
+		uint32_t* const mine = keys + (scorer.token_there ? scorer.col / a.span : 0) * stride;
+		constexpr int TILES = THREADS == 512 ? 2 : 1;
+		score_pages<J, TILES>(scorer, lds, a.batch.table + (size_t)s * a.batch.table_stride, 16 * TILES * wave, pages, pages, 16 * TILES * (THREADS / WAVE), THREADS,
+		                      [&](uint32_t p) { return mine[p]; }, [&](uint32_t p, uint32_t k) { mine[p] = k; });
 	}
-	uint32_t written = 0, ties = 0;
-	for (uint32_t from = 0; from < n; from += 256) {
-		const uint32_t p = from + tid;
-		const uint32_t k = p < n ? keys[p] : 0;
-		const bool is_above = p < n && k > prefix, is_equal = p < n && k == prefix;
-		const uint64_t ballot_above = __ballot(is_above), ballot_equal = __ballot(is_equal);
-		if (lane == 0) { above[wave] = __popcll(ballot_above); equal[wave] = __popcll(ballot_equal); }
-		__syncthreads();
-		const uint64_t below = ((uint64_t)1 << lane) - 1;
-		uint32_t eq = ties + __popcll(ballot_equal & below), gt = __popcll(ballot_above & below);
-		uint32_t all_eq = ties, all_gt = 0;
-		for (uint32_t w = 0; w < 4; ++w) {
-			if (w < wave) { eq += equal[w]; gt += above[w]; }
-			all_eq += equal[w];
-			all_gt += above[w];
-		}
-		/* of the ties before this page, at most `rest` were kept */
-		const uint32_t kept = min(eq, rest) - min(ties, rest);
-		if (is_above || (is_equal && eq < rest)) out[written + gt + kept] = (int32_t)p;
-		written += all_gt + min(all_eq, rest) - min(ties, rest);
-		ties = all_eq;
-		__syncthreads();
-	}
+	__syncthreads();
+	const uint32_t threads = THREADS / a.per, list = threadIdx.x / threads, tid = threadIdx.x % threads, i = tile * a.per + list;
+	const bool there = i < seq.queries;
+	const uint32_t n = there ? (visible_to(a.batch, seq, i) + page_tokens - 1) >> a.cache.page_shift : 0;
+	int32_t* out = there ? a.chosen + ((size_t)(seq.first + i) * a.cache.heads + head) * a.top : nullptr;
+	const uint32_t* from = keys + list * stride;
+	choose_top([&](uint32_t p) { return from[p]; }, n, a.top, out, tid, threads, choose[list], above + list * (threads / WAVE), equal + list * (threads / WAVE));
 }
 
 /* ---------------------------------------------------------------- launch shapes of the attention - */
@@ -706,11 +899,12 @@ int kmx_cache4_bound(const kmx_cache4* cache, const int32_t* pages, const int32_
 	if (!cache->bounds) return fail(KMX_ERR_INVALID_ARGUMENT, "kmx_cache4_bound: the cache keeps no bounds");
 	if (count == 0) return KMX_OK;
 	if (!pages || !counts) return fail(KMX_ERR_INVALID_ARGUMENT, "kmx_cache4_bound: null device pointer");
-	const uint64_t groups = ((uint64_t)count * c.heads + 3) / 4;
+	const uint32_t waves = cache->page_tokens >= 64 ? 4 : cache->page_tokens / 16;
+	const uint64_t groups = ((uint64_t)count * c.heads + 4 / waves - 1) / (4 / waves);
 	if (groups > 0x7FFFFFFFu) return fail(KMX_ERR_UNSUPPORTED, "kmx_cache4_bound: %u pages of %u heads are too many for one call", count, c.heads);
 	switch (cache->dim / 32) {
 #define KMX_CASE(N)                                                                                                      \
-	case N: KMX_LAUNCH_KERNEL((bound4_kernel<N>), dim3((unsigned)groups), dim3(256), 0, stream(), c, pages, counts, count); break;
+	case N: KMX_LAUNCH_KERNEL((bound4_kernel<N>), dim3((unsigned)groups), dim3(256), 0, stream(), c, pages, counts, count, waves); break;
 		KMX_CASE(1) KMX_CASE(2) KMX_CASE(3) KMX_CASE(4) KMX_CASE(5) KMX_CASE(6) KMX_CASE(7) KMX_CASE(8)
 #undef KMX_CASE
 	}
@@ -746,32 +940,49 @@ int kmx_cache4_select(const kmx_cache4* cache, const kmx_cache4_batch* batch, in
 	a.vec = aligned_rows(q, q_token_stride, q_head_stride, 2);
 	a.span = 1;
 	while (a.span < a.batch.group && a.span < 16) a.span *= 2;
-	a.token_tiles = (batch->max_queries + 16 / a.span - 1) / (16 / a.span);
-	const uint32_t tiles = (pages + 63) / 64; /* of 64 pages: one a wavefront */
-	const uint64_t units = (uint64_t)batch->sequences * a.token_tiles * a.cache.heads;
-	/* parts of the pages: enough work-groups to fill the chip, of 64 pages at least */
-	const uint64_t want = units < 1024 ? (1024 + units - 1) / units : 1;
-	a.chunks = (uint32_t)(want < tiles ? want : tiles ? tiles : 1);
-	a.chunk = tiles ? (tiles + a.chunks - 1) / a.chunks : 0;
-	a.chunks = a.chunk ? (tiles + a.chunk - 1) / a.chunk : 1;
-	const uint64_t groups = units * a.chunks, rows = (uint64_t)batch->sequences * batch->max_queries * a.cache.heads;
-	if (groups > 0x7FFFFFFFu || rows > 0x7FFFFFFFu) return fail(KMX_ERR_UNSUPPORTED, "kmx_cache4_select: too many queries for one call");
-	if (pages > top) { /* else every page there is gets chosen */
-		Workspace* ws = nullptr;
-		rc = workspace(&ws);
-		if (rc) return rc;
-		rc = reserve_cache4("kmx_cache4_select", ws, (size_t)batch->tokens * a.cache.heads * batch->table_stride);
-		if (rc) return rc;
-		a.keys = (uint32_t*)ws->partials;
+	/* Scores and choice in one kernel where the pages are few, by 4 wavefronts or by 16 (64 sequences of 128 pages: 65 us by 16, 57 in two kernels; two
+	 * sequences of 625 pages, 128 queries: 37 us against 41); two kernels where one work-group would read for long (1 x 1024 pages: 29 us against 34) */
+	const bool one = pages <= SELECT_PAGES, few = pages <= SELECT_FEW;
+	a.per = 1;
+	while (a.per < batch->max_queries && a.per < (one && few ? 4 : 8) && a.per * a.span < 16) a.per *= 2;
+	a.token_tiles = (batch->max_queries + a.per - 1) / a.per;
+	const uint64_t units = (uint64_t)batch->sequences * a.token_tiles * a.cache.heads, rows = (uint64_t)batch->sequences * batch->max_queries * a.cache.heads;
+	if (units > 0x7FFFFFFFu || rows > 0x7FFFFFFFu) return fail(KMX_ERR_UNSUPPORTED, "kmx_cache4_select: too many queries for one call");
+	if (one) {
+		const uint32_t stride = pages | 1, bytes = 4 * a.per * stride; /* at most 24.6 KB */
 		switch (cache->dim / 32) {
 #define KMX_CASE(N)                                                                                                      \
-	case N: KMX_LAUNCH_KERNEL((score4_kernel<N>), dim3((unsigned)groups), dim3(256), 0, stream(), a); break;
+	case N:                                                                                                               \
+		if (few) KMX_LAUNCH_KERNEL((select4_kernel<N, true>), dim3((unsigned)units), dim3(select_threads(N, true)), bytes, stream(), a, stride); \
+		else KMX_LAUNCH_KERNEL((select4_kernel<N, false>), dim3((unsigned)units), dim3(select_threads(N, false)), bytes, stream(), a, stride); \
+		break;
 			KMX_CASE(1) KMX_CASE(2) KMX_CASE(3) KMX_CASE(4) KMX_CASE(5) KMX_CASE(6) KMX_CASE(7) KMX_CASE(8)
 #undef KMX_CASE
 		}
-		KMX_LAUNCH_CHECK("score4_kernel");
+		KMX_LAUNCH_CHECK("select4_kernel");
+		return KMX_OK;
 	}
-	KMX_LAUNCH_KERNEL(choose4_kernel, dim3((unsigned)rows), dim3(256), 0, stream(), a);
+	/* parts of the pages: enough work-groups to fill the chip, of 128 pages at least */
+	const uint32_t tiles = (pages + 63) / 64; /* of 16 pages a wavefront */
+	uint64_t parts = (1024 + units - 1) / units;
+	if (parts > (tiles + 1) / 2) parts = (tiles + 1) / 2;
+	a.chunk = (uint32_t)((tiles + parts - 1) / parts);
+	a.chunks = (tiles + a.chunk - 1) / a.chunk;
+	if (units * a.chunks > 0x7FFFFFFFu) return fail(KMX_ERR_UNSUPPORTED, "kmx_cache4_select: too many queries for one call");
+	Workspace* ws = nullptr;
+	rc = workspace(&ws);
+	if (rc) return rc;
+	rc = reserve_cache4("kmx_cache4_select", ws, (size_t)batch->tokens * a.cache.heads * batch->table_stride);
+	if (rc) return rc;
+	a.keys = (uint32_t*)ws->partials;
+	switch (cache->dim / 32) {
+#define KMX_CASE(N)                                                                                                      \
+	case N: KMX_LAUNCH_KERNEL((score4_kernel<N>), dim3((unsigned)(units * a.chunks)), dim3(256), 0, stream(), a); break;
+		KMX_CASE(1) KMX_CASE(2) KMX_CASE(3) KMX_CASE(4) KMX_CASE(5) KMX_CASE(6) KMX_CASE(7) KMX_CASE(8)
+#undef KMX_CASE
+	}
+	KMX_LAUNCH_CHECK("score4_kernel");
+	KMX_LAUNCH_KERNEL(choose4_kernel, dim3((unsigned)rows), dim3(512), 0, stream(), a);
 	KMX_LAUNCH_CHECK("choose4_kernel");
 	return KMX_OK;
 }

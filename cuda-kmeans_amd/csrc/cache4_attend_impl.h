@@ -273,7 +273,7 @@ attend4_kernel(Attend4 a)
 				}
 				*(u32x4*)(scales + kg * SCALES + 256 * n + 16 * i16) = t.sc[n];
 			}
-		__builtin_amdgcn_wave_barrier();
+		wave_sync();
 		fetch_scales(t, next);
 		float sc[16];
 #pragma unroll
@@ -347,7 +347,7 @@ attend4_kernel(Attend4 a)
 		Tile4<J> t;
 		const uint32_t tile0 = begin + wave;
 		find_places(tile0, 0);
-		__builtin_amdgcn_wave_barrier();
+		wave_sync();
 		Where w = where(0);
 		fetch_scales(t, w);
 		fetch_keys(t, w);
@@ -355,7 +355,7 @@ attend4_kernel(Attend4 a)
 		for (uint32_t n = 0; n < count; ++n) {
 			const int32_t from = w.from;
 			if (n % 16 == 7 && n + 9 < count) find_places(tile0 + 4 * (n + 9), (n + 9) / 16 % 2);
-			__builtin_amdgcn_wave_barrier();
+			wave_sync();
 			w = where(min(n + 1, count - 1)); /* (the last tile is fetched twice: a fetch under a condition would make the compiler wait for everything) */
 			work(t, from, w);
 		}

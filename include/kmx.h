@@ -420,7 +420,7 @@ int kmx_probe_matrix_chain(int kind, const float* a, const float* b, const float
  * With levels from kmx_cache4_round_levels (6 significant bits) every such number is one of half precision.
  * Buffers are the caller's (kmx_cache4_sizes tells how large), 16-byte aligned. Pages that no token was written to may hold anything.
  * Bounds, where they are kept: for each page and head the largest and the smallest value of each channel of the keys, outwards in 127ths of
- * their largest magnitude (dim + dim bytes), behind all of them those largest magnitudes over 127 (floats).
+ * their largest magnitude m (dim + dim bytes: up(hi (1/m 127)), down(lo (1/m 127)) in floats), behind all of them those largest magnitudes over 127 (floats).
  * Places, pages and lengths on the device are not trusted: a place or page outside the cache is left out (reads as zeros, is not attended to).
  * kmx_cache4_select and kmx_cache4_attend use the library's work space (see kmx_cache4_reserve) under the rules of the updates.
  */
@@ -473,7 +473,7 @@ int kmx_cache4_bound(const kmx_cache4* cache, const int32_t* pages, const int32_
  * The pages that each query and head of the cache look at: chosen[token][head][top], numbers of pages inside the sequence (columns of the
  * table), ascending, -1 behind the last. Of the pages with a token the query sees: the `first` first and `last` last ones, then those of the
  * best score, the lower number of two as good. score = max over the query heads of the head of sum_c max(q_c hi_c, q_c lo_c), the bound on
- * q . k over the page, in 8 bits: q_c = rint(q 127 / its largest magnitude over these heads), hi and lo as kept; a whole number, times the page's
+ * q . k over the page, in 8 bits: q_c = rint(q (1/m 127)) in floats, m its largest magnitude over these heads, hi and lo as kept; a whole number, times the page's
  * scale in floats. Queries F16 or BF16, element (token, head, channel) as above.
  */
 int kmx_cache4_select(const kmx_cache4* cache, const kmx_cache4_batch* batch, int type, const void* q, size_t q_token_stride, size_t q_head_stride,
