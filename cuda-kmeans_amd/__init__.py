@@ -520,6 +520,24 @@ def cache4_round_levels(levels):
     return out
 
 
+def cache4_learn_levels(rows, iterations=12):
+    """The 8 levels that k-means (one dimension, 8 centroids) finds on the magnitudes of sample rows (any shape, the last axis a multiple of 32),
+    each over the largest of its 32 channels: one set for kmx_cache4, rounded. Rows of zeros say nothing and are left out."""
+    x = np.abs(np.asarray(rows, dtype=np.float32)).reshape(-1, 32)
+    largest = x.max(axis=1, keepdims=True)
+    x = np.ascontiguousarray((x / np.where(largest > 0, largest, 1))[largest[:, 0] > 0].reshape(-1))
+    if x.size < 8:
+        raise ValueError("no rows to learn from")
+    start = np.quantile(x, (np.arange(8) + 0.5) / 8).astype(np.float32)
+    alg = HipKMeansAlgorithm()
+    alg.initialize(1, 8, x.size, iterations, x, start)
+    alg.run()
+    means, sizes = alg.getMeans(), alg.getClusterSizes()
+    alg.cleanup()
+    levels = np.sort(np.where(sizes > 0, means, start))  # a centroid without members is zero: its start stands
+    return cache4_round_levels(np.clip(levels, 0, 1))
+
+
 class Cache4Batch:
     """Queries of some sequences (kmx_cache4_batch): `tokens` rows in all, starts, lengths and table in device memory."""
 

@@ -506,6 +506,7 @@ attend4_many_kernel(Attend4 a)
 {
 	constexpr uint32_t D = 32 * J, KROW = 2 * D + 16, VROW = 144, TILE = 64 * KROW + D * VROW;
 	extern __shared__ __attribute__((aligned(16))) uint8_t many[]; /* two tiles: keys [token][channel], values [channel][token] */
+	__shared__ uint32_t blocks_there[2][4];
 	const uint32_t wave = (uint32_t)__builtin_amdgcn_readfirstlane((int)(threadIdx.x / WAVE)), lane = threadIdx.x % WAVE, n32 = lane % 32, h = lane / 32;
 	const uint32_t units = gridDim.x / a.splits, part = blockIdx.x / units, whole = blockIdx.x % units;
 	const uint32_t row_tile = whole % a.row_tiles, head = whole / a.row_tiles % a.cache.heads, s = whole / a.row_tiles / a.cache.heads;
@@ -552,10 +553,11 @@ attend4_many_kernel(Attend4 a)
 	constexpr int VITEMS = (16 * J + WAVE - 1) / WAVE; /* pairs of channels a lane */
 	struct { uint32_t codes[values_words<J>()]; u32x4 scales[VITEMS][2]; uint32_t key_scales[(J + 1) / 2]; } in;
 	int32_t written = 0; /* tokens of the block that are there */
+	bool known = false;  /* it lies on a page of the cache */
 	auto fetch = [&](uint32_t tile) {
 		const uint32_t n = 4 * tile + b, entry = n >> sub_bits, sub = n & ((1u << sub_bits) - 1);
 		const uint32_t page = (uint32_t)table[min(entry, a.batch.table_stride - 1)];
-		const bool known = entry < a.batch.table_stride && page < a.cache.page_count;
+		known = entry < a.batch.table_stride && page < a.cache.page_count;
 		written = known ? (int32_t)seq.length - (int32_t)(16 * n) : 0;
 		const uint8_t* block = a.cache.blocks + block_offset<J>(a.cache, known ? page : 0, head, sub);
 		if (!values) {
@@ -572,8 +574,10 @@ attend4_many_kernel(Attend4 a)
 			}
 		}
 	};
-	auto unpack = [&](uint8_t* tile) {
+	auto unpack = [&](uint32_t buffer) {
+		uint8_t* const tile = many + buffer * TILE;
 		if (!values) {
+			if (lane == 0) blocks_there[buffer][b] = known ? 1 : 0;
 			uint8_t* row = tile + (16 * b + lane / 4) * KROW + 16 * (lane % 4);
 #pragma unroll
 			for (int j = 0; j < J; ++j) {
@@ -619,7 +623,11 @@ attend4_many_kernel(Attend4 a)
 	for (int j = 0; j < J; ++j)
 		for (int e = 0; e < 16; ++e) o[j][e] = 0.0f;
 
-	auto work = [&](const uint8_t* tile, int32_t from) {
+	auto work = [&](uint32_t buffer, int32_t from) {
+		const uint8_t* const tile = many + buffer * TILE;
+		uint32_t blocks = 0;
+		for (int n = 0; n < 4; ++n) blocks |= blocks_there[buffer][n] << n;
+		blocks = (uint32_t)__builtin_amdgcn_readfirstlane((int)blocks);
 		f32x16 sc[2];
 #pragma unroll
 		for (int t = 0; t < 2; ++t) {
@@ -628,11 +636,11 @@ attend4_many_kernel(Attend4 a)
 			for (int c = 0; c < 2 * J; ++c)
 				sc[t] = __builtin_amdgcn_mfma_f32_32x32x16_f16(*(const half8v*)(tile + (32 * t + n32) * KROW + 32 * c + 16 * h), q[c], sc[t], 0, 0, 0);
 		}
-		if (from + 64 > least) {
+		if (from + 64 > least || blocks != 15) {
 #pragma unroll
 			for (int e = 0; e < 32; ++e) {
 				const int32_t place = from + 32 * (e / 16) + 8 * (e % 16 / 4) + 4 * (int32_t)h + e % 4;
-				sc[e / 16][e % 16] = place < sees ? sc[e / 16][e % 16] : -__builtin_inff();
+				sc[e / 16][e % 16] = place < sees && (blocks >> (e / 8) & 1) ? sc[e / 16][e % 16] : -__builtin_inff();
 			}
 		}
 		float top = sc[0][0];
@@ -664,13 +672,12 @@ attend4_many_kernel(Attend4 a)
 
 	if (begin < end) {
 		fetch(begin);
-		unpack(many);
+		unpack(0);
 		fetch(min(begin + 1, end - 1));
 		__syncthreads();
 		for (uint32_t tile = begin; tile < end; ++tile) {
-			uint8_t* const now = many + (tile - begin) % 2 * TILE;
-			uint8_t* const next = many + (tile - begin + 1) % 2 * TILE;
-			if (tile + 1 < end) unpack(next);
+			const uint32_t now = (tile - begin) % 2;
+			if (tile + 1 < end) unpack(1 - now);
 			if (tile + 2 < end) fetch(tile + 2);
 			if ((int32_t)(64 * tile) < seen) work(now, (int32_t)(64 * tile));
 			__syncthreads();
