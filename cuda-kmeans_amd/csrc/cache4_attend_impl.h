@@ -505,6 +505,7 @@ __global__ void __launch_bounds__(512, 2)
 attend4_many_kernel(Attend4 a)
 {
 	constexpr uint32_t D = 32 * J, KROW = 2 * D + 16, VROW = 144, TILE = 64 * KROW + D * VROW;
+	constexpr int STEP = (J <= 5 ? 2 : 1); /* times 32 tokens of a tile: scores held at a time */
 	extern __shared__ __attribute__((aligned(16))) uint8_t many[]; /* two tiles: keys [token][channel], values [channel][token] */
 	__shared__ uint32_t blocks_there[2][4];
 	const uint32_t wave = (uint32_t)__builtin_amdgcn_readfirstlane((int)(threadIdx.x / WAVE)), lane = threadIdx.x % WAVE, n32 = lane % 32, h = lane / 32;
@@ -628,46 +629,49 @@ attend4_many_kernel(Attend4 a)
 		uint32_t blocks = 0;
 		for (int n = 0; n < 4; ++n) blocks |= blocks_there[buffer][n] << n;
 		blocks = (uint32_t)__builtin_amdgcn_readfirstlane((int)blocks);
-		f32x16 sc[2];
 #pragma unroll
-		for (int t = 0; t < 2; ++t) {
-			for (int e = 0; e < 16; ++e) sc[t][e] = 0.0f;
+		for (int t0 = 0; t0 < 2; t0 += STEP) {
+			f32x16 sc[STEP];
 #pragma unroll
-			for (int c = 0; c < 2 * J; ++c)
-				sc[t] = __builtin_amdgcn_mfma_f32_32x32x16_f16(*(const half8v*)(tile + (32 * t + n32) * KROW + 32 * c + 16 * h), q[c], sc[t], 0, 0, 0);
-		}
-		if (from + 64 > least || blocks != 15) {
+			for (int t = 0; t < STEP; ++t) {
+				for (int e = 0; e < 16; ++e) sc[t][e] = 0.0f;
 #pragma unroll
-			for (int e = 0; e < 32; ++e) {
-				const int32_t place = from + 32 * (e / 16) + 8 * (e % 16 / 4) + 4 * (int32_t)h + e % 4;
-				sc[e / 16][e % 16] = place < sees && (blocks >> (e / 8) & 1) ? sc[e / 16][e % 16] : -__builtin_inff();
+				for (int c = 0; c < 2 * J; ++c)
+					sc[t] = __builtin_amdgcn_mfma_f32_32x32x16_f16(*(const half8v*)(tile + (32 * (t0 + t) + n32) * KROW + 32 * c + 16 * h), q[c], sc[t], 0, 0, 0);
 			}
+			if (from + 64 > least || blocks != 15) {
+#pragma unroll
+				for (int e = 0; e < 16 * STEP; ++e) {
+					const int32_t place = from + 32 * (t0 + e / 16) + 8 * (e % 16 / 4) + 4 * (int32_t)h + e % 4;
+					sc[e / 16][e % 16] = place < sees && (blocks >> (2 * t0 + e / 8) & 1) ? sc[e / 16][e % 16] : -__builtin_inff();
+				}
+			}
+			float top = sc[0][0];
+#pragma unroll
+			for (int e = 1; e < 16 * STEP; ++e) top = fmaxf(top, sc[e / 16][e % 16]);
+			top = fmaxf(top, __shfl_xor(top, 32));
+			const float now = fmaxf(m, top);
+			if (__any(now > m)) {
+				const float less = m == now ? 1.0f : exp2_((m - now) * row_scale);
+				l *= less;
+#pragma unroll
+				for (int j = 0; j < J; ++j) o[j] *= less;
+				m = now;
+			}
+			const float base = m == -__builtin_inff() ? 0.0f : -m * row_scale;
+			half8v p[2 * STEP];
+#pragma unroll
+			for (int e = 0; e < 16 * STEP; ++e) {
+				const float v = exp2_(fmaf(sc[e / 16][e % 16], row_scale, base));
+				l += v;
+				p[e / 8][e % 8] = (_Float16)v;
+			}
+#pragma unroll
+			for (int j = 0; j < J; ++j)
+#pragma unroll
+				for (int c = 0; c < 2 * STEP; ++c)
+					o[j] = __builtin_amdgcn_mfma_f32_32x32x16_f16(*(const half8v*)(tile + 64 * KROW + (32 * j + n32) * VROW + 32 * (2 * t0 + c) + 16 * h), p[c], o[j], 0, 0, 0);
 		}
-		float top = sc[0][0];
-#pragma unroll
-		for (int e = 1; e < 32; ++e) top = fmaxf(top, sc[e / 16][e % 16]);
-		top = fmaxf(top, __shfl_xor(top, 32));
-		const float now = fmaxf(m, top);
-		if (__any(now > m)) {
-			const float less = m == now ? 1.0f : exp2_((m - now) * row_scale);
-			l *= less;
-#pragma unroll
-			for (int j = 0; j < J; ++j) o[j] *= less;
-			m = now;
-		}
-		const float base = m == -__builtin_inff() ? 0.0f : -m * row_scale;
-		half8v p[4];
-#pragma unroll
-		for (int e = 0; e < 32; ++e) {
-			const float v = exp2_(fmaf(sc[e / 16][e % 16], row_scale, base));
-			l += v;
-			p[e / 8][e % 8] = (_Float16)v;
-		}
-#pragma unroll
-		for (int j = 0; j < J; ++j)
-#pragma unroll
-			for (int c = 0; c < 4; ++c)
-				o[j] = __builtin_amdgcn_mfma_f32_32x32x16_f16(*(const half8v*)(tile + 64 * KROW + (32 * j + n32) * VROW + 32 * c + 16 * h), p[c], o[j], 0, 0, 0);
 	};
 
 	if (begin < end) {
