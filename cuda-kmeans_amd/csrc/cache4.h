@@ -141,14 +141,14 @@ __device__ __forceinline__ void store8(T* p, bool vec, const float x[8])
 {
 	if constexpr (sizeof(T) == 4) {
 		if (vec) {
-			*(f32x4*)p = f32x4{ x[0], x[1], x[2], x[3] };
-			*(f32x4*)(p + 4) = f32x4{ x[4], x[5], x[6], x[7] };
+			__builtin_nontemporal_store(f32x4{ x[0], x[1], x[2], x[3] }, (f32x4*)p);
+			__builtin_nontemporal_store(f32x4{ x[4], x[5], x[6], x[7] }, (f32x4*)(p + 4));
 		} else
 			for (int i = 0; i < 8; ++i) p[i] = x[i];
 	} else {
 		uint32_t b[8];
 		for (int i = 0; i < 8; ++i) b[i] = bits16<T>(x[i]);
-		if (vec) *(u32x4*)p = u32x4{ b[0] | b[1] << 16, b[2] | b[3] << 16, b[4] | b[5] << 16, b[6] | b[7] << 16 };
+		if (vec) __builtin_nontemporal_store(u32x4{ b[0] | b[1] << 16, b[2] | b[3] << 16, b[4] | b[5] << 16, b[6] | b[7] << 16 }, (u32x4*)p);
 		else
 			for (int i = 0; i < 8; ++i) ((uint16_t*)p)[i] = (uint16_t)b[i];
 	}

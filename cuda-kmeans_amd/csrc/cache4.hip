@@ -38,10 +38,11 @@ __device__ __forceinline__ uint32_t codes8(const float x[8], float scale, const 
 	for (int i = 0; i < 8; ++i) {
 		const float size = fabsf(x[i]);
 		const bool b2 = size > edge[3];
-		const bool b1 = size > (b2 ? edge[5] : edge[1]);
-		const float last = b2 ? (b1 ? edge[6] : edge[4]) : (b1 ? edge[2] : edge[0]);
-		const uint32_t code = (b2 ? 4u : 0u) | (b1 ? 2u : 0u) | (size > last ? 1u : 0u) | (x[i] < 0.0f ? 8u : 0u);
-		codes |= code << (4 * i);
+		const float low = b2 ? edge[4] : edge[0], half = b2 ? edge[5] : edge[1], high = b2 ? edge[6] : edge[2];
+		const bool b1 = size > half;
+		const bool b0 = size > (b1 ? high : low);
+		codes |= (b2 ? 4u << (4 * i) : 0u) | (b1 ? 2u << (4 * i) : 0u);
+		codes |= (b0 ? 1u << (4 * i) : 0u) | (x[i] < 0.0f ? 8u << (4 * i) : 0u);
 	}
 	return codes;
 }
@@ -52,10 +53,43 @@ __device__ __forceinline__ uint32_t nibbles_to_bytes(uint32_t w) /* four nibbles
 	return (w | w << 4) & 0x0F0F0F0Fu;
 }
 
+/* 8 elements of a row as they lie there, and in floats */
+template <typename T>
+struct Raw8 { u32x4 w[sizeof(T) / 2]; };
+template <typename T>
+__device__ __forceinline__ Raw8<T> fetch8(const T* p, bool vec)
+{
+	Raw8<T> r;
+	if (vec) {
+		for (uint32_t i = 0; i < sizeof(T) / 2; ++i) r.w[i] = __builtin_nontemporal_load((const u32x4*)p + i);
+	} else if constexpr (sizeof(T) == 4) {
+		for (int i = 0; i < 8; ++i) r.w[i / 4][i % 4] = ((const uint32_t*)p)[i];
+	} else {
+		for (int i = 0; i < 4; ++i) r.w[0][i] = ((const uint16_t*)p)[2 * i] | (uint32_t)((const uint16_t*)p)[2 * i + 1] << 16;
+	}
+	return r;
+}
+template <typename T>
+__device__ __forceinline__ void floats8(const Raw8<T>& r, float x[8])
+{
+	for (int i = 0; i < 8; ++i) {
+		if constexpr (sizeof(T) == 4) {
+			const uint32_t w = r.w[i / 4][i % 4];
+			x[i] = __builtin_bit_cast(float, w);
+		} else {
+			const uint32_t w = r.w[0][i / 2];
+			if constexpr (__is_same(T, __bf16)) x[i] = __builtin_bit_cast(float, i % 2 ? w & 0xFFFF0000u : w << 16);
+			else x[i] = (float)__builtin_bit_cast(half2v, w)[i % 2];
+		}
+	}
+}
+
 /*
- * A wavefront takes 16 tokens of one head; lane = 4 token + g holds channels 32 j + 8 g .. + 7 of each group j, so a group is four lanes and its
- * maximum two exchanges inside them. The keys' words go out as they stand (J side by side a lane); the values' bytes pass through LDS, 16
- * tokens of a pair side by side, and leave as 16 bytes a lane where the 16 tokens fill a block in order, else byte by byte.
+ * A wavefront takes 16 tokens of one head, 64 pieces of 8 channels at a time: piece n is channels 8 (n % 4 J) of token n / 4 J, so that a load of all
+ * lanes is whole rows side by side and a group of 32 channels four lanes, its maximum two exchanges inside them. The keys' words go where they
+ * belong (a token's lie together); the values' bytes pass through LDS, 16 tokens of a pair side by side, and leave as 16 bytes a lane where the 16
+ * tokens fill a block in order, else byte by byte. Bound by the rows that it reads, with some 18 instructions a number beside them: 16384 tokens of
+ * 8 heads of 128 in bf16, 86 MB.
  */
 template <int J, typename T>
 __global__ void __launch_bounds__(256)
@@ -63,21 +97,28 @@ write4_kernel(Rows4 a)
 {
 	constexpr uint32_t D = 32 * J;
 	__shared__ __attribute__((aligned(16))) uint8_t lds[4][16 * 16 * J];
-	const uint32_t wave = threadIdx.x / WAVE, lane = threadIdx.x % WAVE, t = lane / 4, g = lane % 4;
+	const uint32_t wave = (uint32_t)__builtin_amdgcn_readfirstlane((int)(threadIdx.x / WAVE)), lane = threadIdx.x % WAVE;
 	const uint64_t unit = (uint64_t)blockIdx.x * 4 + wave;
 	const uint32_t head = (uint32_t)(unit % a.cache.heads);
 	const uint64_t first = unit / a.cache.heads * 16;
 	if (first >= a.tokens) return; /* (no barriers below: a wavefront's LDS is its own) */
-	const uint64_t token = first + t;
-	const int32_t slot = token < a.tokens ? a.slots[token] : -1;
 	const uint64_t places = (uint64_t)a.cache.page_count << a.cache.page_shift;
-	const bool there = slot >= 0 && (uint64_t)slot < places;
-	const uint32_t page = (uint32_t)slot >> a.cache.page_shift, place = (uint32_t)slot & ((1u << a.cache.page_shift) - 1);
-	uint8_t* const block = a.cache.blocks + (there ? block_offset<J>(a.cache, page, head, place / 16) : 0);
-	const uint32_t at = place % 16;
+	const uint32_t page_mask = (1u << a.cache.page_shift) - 1;
+	const int32_t slot = first + lane % 16 < a.tokens ? a.slots[first + lane % 16] : -1; /* lane n: of token n % 16 */
 	uint8_t* const mine = lds[wave];
+	auto block_of = [&](int32_t s) { return a.cache.blocks + block_offset<J>(a.cache, (uint32_t)s >> a.cache.page_shift, head, ((uint32_t)s & page_mask) / 16); };
 
 	for (int which = 0; which < 2; ++which) {
+		Raw8<T> raw[J];
+		int32_t place[J];
+#pragma unroll
+		for (int n = 0; n < J; ++n) {
+			const uint32_t piece = WAVE * n + lane, t = piece / (4 * J), c = piece % (4 * J);
+			place[n] = __shfl(slot, (int)t);
+			if ((uint64_t)(int64_t)place[n] >= places) place[n] = -1; /* (negative ones too) */
+			const uint64_t token = min(first + t, (uint64_t)a.tokens - 1);
+			raw[n] = fetch8((const T*)(which ? a.values : a.keys) + token * a.token_stride + head * a.head_stride + 8 * c, a.vec);
+		}
 		float middle[7];
 		{
 			const uint16_t* l = a.cache.levels + ((size_t)head * 2 + which) * 8;
@@ -88,126 +129,130 @@ write4_kernel(Rows4 a)
 				below = above;
 			}
 		}
-		const T* row = (const T*)(which ? a.values : a.keys) + (there ? token * a.token_stride : 0) + head * a.head_stride + 8 * g;
-		float x[J][8];
 #pragma unroll
-		for (int j = 0; j < J; ++j) {
-			if (there) load8(row + 32 * j, a.vec, x[j]);
-			else
-				for (int i = 0; i < 8; ++i) x[j][i] = 0.0f;
-		}
-		uint32_t codes[J];
-		_Float16 scale[J];
-#pragma unroll
-		for (int j = 0; j < J; ++j) {
+		for (int n = 0; n < J; ++n) {
+			const uint32_t piece = WAVE * n + lane, t = piece / (4 * J), c = piece % (4 * J), j = c / 4, g = c % 4;
+			float x[8];
+			floats8<T>(raw[n], x);
 			float largest = 0.0f; /* fmaxf leaves NaN out */
-			for (int i = 0; i < 8; ++i) largest = fmaxf(largest, fabsf(x[j][i]));
+			for (int i = 0; i < 8; ++i) largest = fmaxf(largest, fabsf(x[i]));
 			largest = fmaxf(largest, dpp<DPP_XOR1>(largest));
 			largest = fmaxf(largest, dpp<DPP_XOR2>(largest));
-			scale[j] = group_scale(largest);
-			codes[j] = codes8(x[j], (float)scale[j], middle);
-		}
-		if (which == 0) {
-			if (there) {
-				uint32_t* out = (uint32_t*)(block + at * (D / 2) + g * 4 * J);
-#pragma unroll
-				for (int j = 0; j < J; ++j) out[j] = nibbles_to_bytes(codes[j] & 0xFFFFu) | nibbles_to_bytes(codes[j] >> 16) << 4;
-				if (g == 0)
-#pragma unroll
-					for (int j = 0; j < J; ++j) ((_Float16*)(block + 16 * D))[at * J + j] = scale[j];
-			}
-		} else {
-#pragma unroll
-			for (int j = 0; j < J; ++j) {
+			const _Float16 scale = group_scale(largest);
+			const uint32_t codes = codes8(x, (float)scale, middle);
+			const uint32_t at = (uint32_t)place[n] % 16;
+			if (which == 0) {
+				if (place[n] >= 0) {
+					uint8_t* const block = block_of(place[n]);
+					((uint32_t*)(block + at * (D / 2)))[g * J + j] = nibbles_to_bytes(codes & 0xFFFFu) | nibbles_to_bytes(codes >> 16) << 4;
+					if (g == 0) ((_Float16*)(block + 16 * D))[at * J + j] = scale;
+				}
+			} else {
 				/* lanes g and g + 2 hold the two channels of 8 pairs: each makes the bytes of four */
-				const uint32_t other = dpp<DPP_XOR2>(codes[j]), half = g / 2;
-				const uint32_t low = (half ? other : codes[j]) >> (16 * half), high = (half ? codes[j] : other) >> (16 * half);
+				const uint32_t other = dpp<DPP_XOR2>(codes), half = g / 2;
+				const uint32_t low = (half ? other : codes) >> (16 * half), high = (half ? codes : other) >> (16 * half);
 				const uint32_t bytes = nibbles_to_bytes(low & 0xFFFFu) | nibbles_to_bytes(high & 0xFFFFu) << 4;
 				const uint32_t pair = 16 * j + 8 * (g & 1) + 4 * half;
 				for (int b = 0; b < 4; ++b) mine[(pair + b) * 16 + t] = (uint8_t)(bytes >> (8 * b));
+				if (place[n] >= 0 && g == 0) ((_Float16*)(block_of(place[n]) + 17 * D))[16 * j + at] = scale;
 			}
-			if (there && g == 0)
+		}
+	}
+	wave_sync();
+	const int32_t slot0 = __builtin_amdgcn_readfirstlane(slot);
+	const bool in_order = (uint64_t)(int64_t)slot0 < places && slot0 % 16 == 0 && __ballot(slot != slot0 + (int32_t)(lane % 16)) == 0;
+	if (in_order) {
+		uint8_t* const block = block_of(slot0);
+		for (uint32_t p = lane; p < D / 2; p += WAVE) *(u32x4*)(block + 8 * D + p * 16) = *(const u32x4*)(mine + p * 16);
+	} else {
+		for (uint32_t p = lane; p < D / 2; p += WAVE) {
+			const u32x4 w = *(const u32x4*)(mine + p * 16);
 #pragma unroll
-				for (int j = 0; j < J; ++j) ((_Float16*)(block + 17 * D))[16 * j + at] = scale[j];
-			wave_sync();
-			const uint32_t slot0 = (uint32_t)__builtin_amdgcn_readfirstlane(slot);
-			if (__ballot(!there || (uint32_t)slot != slot0 + t) == 0 && slot0 % 16 == 0) {
-				for (uint32_t p = lane; p < D / 2; p += WAVE) *(u32x4*)(block + 8 * D + p * 16) = *(const u32x4*)(mine + p * 16);
-			} else {
-				for (uint32_t n = 0; n < 16; ++n) {
-					const int32_t s = __builtin_amdgcn_readlane(slot, 4 * n);
-					if (s < 0 || (uint64_t)s >= places) continue;
-					const uint32_t pl = (uint32_t)s & ((1u << a.cache.page_shift) - 1);
-					uint8_t* out = a.cache.blocks + block_offset<J>(a.cache, (uint32_t)s >> a.cache.page_shift, head, pl / 16) + 8 * D + pl % 16;
-					for (uint32_t p = lane; p < D / 2; p += WAVE) out[p * 16] = mine[p * 16 + n];
-				}
+			for (int n = 0; n < 16; ++n) {
+				const int32_t s = __builtin_amdgcn_readlane(slot, n);
+				if ((uint64_t)(int64_t)s < places) (block_of(s) + 8 * D + (uint32_t)s % 16)[p * 16] = (uint8_t)(w[n / 4] >> (8 * (n % 4)));
 			}
 		}
 	}
 }
 
-/* The same lanes backwards; a place outside the cache reads as zeros. */
+/* The same pieces backwards; a place outside the cache reads as zeros. */
 template <int J, typename T>
 __global__ void __launch_bounds__(256)
 read4_kernel(Rows4 a)
 {
 	constexpr uint32_t D = 32 * J, ROW = D / 2 + 8; /* LDS: the values' bytes token by token, rows 8 bytes apart in the banks */
 	__shared__ __attribute__((aligned(16))) uint8_t lds[4][16 * ROW];
-	const uint32_t wave = threadIdx.x / WAVE, lane = threadIdx.x % WAVE, t = lane / 4, g = lane % 4;
+	const uint32_t wave = (uint32_t)__builtin_amdgcn_readfirstlane((int)(threadIdx.x / WAVE)), lane = threadIdx.x % WAVE;
 	const uint64_t unit = (uint64_t)blockIdx.x * 4 + wave;
 	const uint32_t head = (uint32_t)(unit % a.cache.heads);
 	const uint64_t first = unit / a.cache.heads * 16;
 	if (first >= a.tokens) return;
-	const uint64_t token = first + t;
-	const int32_t slot = token < a.tokens ? a.slots[token] : -1;
 	const uint64_t places = (uint64_t)a.cache.page_count << a.cache.page_shift;
-	const bool there = slot >= 0 && (uint64_t)slot < places;
-	const uint32_t page = (uint32_t)slot >> a.cache.page_shift, place = (uint32_t)slot & ((1u << a.cache.page_shift) - 1);
-	const uint8_t* const block = a.cache.blocks + (there ? block_offset<J>(a.cache, page, head, place / 16) : 0);
-	const uint32_t at = place % 16;
+	const uint32_t page_mask = (1u << a.cache.page_shift) - 1;
+	const int32_t slot = first + lane % 16 < a.tokens ? a.slots[first + lane % 16] : -1;
 	uint8_t* const mine = lds[wave];
+	auto block_of = [&](int32_t s) { return a.cache.blocks + block_offset<J>(a.cache, (uint32_t)s >> a.cache.page_shift, head, ((uint32_t)s & page_mask) / 16); };
 
-	/* the values' bytes into LDS */
-	const uint32_t slot0 = (uint32_t)__builtin_amdgcn_readfirstlane(slot);
-	if (__ballot(!there || (uint32_t)slot != slot0 + t) == 0 && slot0 % 16 == 0) {
+	/* the keys' words and the scales under way, then the values' bytes into LDS */
+	uint32_t codes[J];
+	uint16_t scales[2][J];
+	int32_t place[J];
+#pragma unroll
+	for (int n = 0; n < J; ++n) {
+		const uint32_t piece = WAVE * n + lane, t = piece / (4 * J), c = piece % (4 * J), j = c / 4, g = c % 4;
+		place[n] = __shfl(slot, (int)t);
+		if ((uint64_t)(int64_t)place[n] >= places) place[n] = -1;
+		codes[n] = 0;
+		scales[0][n] = scales[1][n] = 0;
+		if (place[n] >= 0) {
+			const uint8_t* const block = block_of(place[n]);
+			const uint32_t at = (uint32_t)place[n] % 16;
+			codes[n] = ((const uint32_t*)(block + at * (D / 2)))[g * J + j];
+			scales[0][n] = ((const uint16_t*)(block + 16 * D))[at * J + j];
+			scales[1][n] = ((const uint16_t*)(block + 17 * D))[16 * j + at];
+		}
+	}
+	const int32_t slot0 = __builtin_amdgcn_readfirstlane(slot);
+	const bool in_order = (uint64_t)(int64_t)slot0 < places && slot0 % 16 == 0 && __ballot(slot != slot0 + (int32_t)(lane % 16)) == 0;
+	if (in_order) {
+		const uint8_t* const block = block_of(slot0);
 		for (uint32_t p = lane; p < D / 2; p += WAVE) {
 			const u32x4 w = *(const u32x4*)(block + 8 * D + p * 16);
 			for (int n = 0; n < 16; ++n) mine[n * ROW + p] = (uint8_t)(w[n / 4] >> (8 * (n % 4)));
 		}
 	} else {
-		for (uint32_t n = 0; n < 16; ++n) {
-			const int32_t s = __builtin_amdgcn_readlane(slot, 4 * n);
-			if (s < 0 || (uint64_t)s >= places) continue;
-			const uint32_t pl = (uint32_t)s & ((1u << a.cache.page_shift) - 1);
-			const uint8_t* in = a.cache.blocks + block_offset<J>(a.cache, (uint32_t)s >> a.cache.page_shift, head, pl / 16) + 8 * D + pl % 16;
-			for (uint32_t p = lane; p < D / 2; p += WAVE) mine[n * ROW + p] = in[p * 16];
+		for (uint32_t p = lane; p < D / 2; p += WAVE) {
+			uint8_t w[16]; /* all 16 under way before the first is waited for */
+#pragma unroll
+			for (int n = 0; n < 16; ++n) {
+				const int32_t s = __builtin_amdgcn_readlane(slot, n);
+				w[n] = (uint64_t)(int64_t)s < places ? (block_of(s) + 8 * D + (uint32_t)s % 16)[p * 16] : 0;
+			}
+#pragma unroll
+			for (int n = 0; n < 16; ++n) mine[n * ROW + p] = w[n];
 		}
 	}
 	wave_sync();
-	if (token >= a.tokens) return;
 	for (int which = 0; which < 2; ++which) {
 		const Magnitudes m = load_magnitudes(a.cache.levels, head, which);
-		T* row = (T*)(which ? a.values : a.keys) + token * a.token_stride + head * a.head_stride + 8 * g;
 #pragma unroll
-		for (int j = 0; j < J; ++j) {
-			uint32_t w[4] = { 0, 0, 0, 0 };
-			float scale = 0.0f;
-			if (there) {
-				if (which == 0) {
-					const uint32_t c = ((const uint32_t*)(block + at * (D / 2) + g * 4 * J))[j];
-					unpack4<false>(c, m, w[0], w[1]);
-					unpack4<true>(c, m, w[2], w[3]);
-					scale = (float)((const _Float16*)(block + 16 * D))[at * J + j];
-				} else {
-					const u32x2 c = *(const u32x2*)(mine + t * ROW + 16 * j + 8 * (g & 1));
-					unpack4<false>(c[0] >> (4 * (g / 2)), m, w[0], w[1]);
-					unpack4<false>(c[1] >> (4 * (g / 2)), m, w[2], w[3]);
-					scale = (float)((const _Float16*)(block + 17 * D))[16 * j + at];
-				}
+		for (int n = 0; n < J; ++n) {
+			const uint32_t piece = WAVE * n + lane, t = piece / (4 * J), c = piece % (4 * J), j = c / 4, g = c % 4;
+			if (first + t >= a.tokens) continue;
+			uint32_t w[4];
+			if (which == 0) {
+				unpack4<false>(codes[n], m, w[0], w[1]);
+				unpack4<true>(codes[n], m, w[2], w[3]);
+			} else {
+				const u32x2 b = *(const u32x2*)(mine + t * ROW + 16 * j + 8 * (g & 1));
+				unpack4<false>(b[0] >> (4 * (g / 2)), m, w[0], w[1]);
+				unpack4<false>(b[1] >> (4 * (g / 2)), m, w[2], w[3]);
 			}
+			const float scale = (float)__builtin_bit_cast(_Float16, scales[which][n]);
 			float x[8];
-			for (int i = 0; i < 8; ++i) x[i] = scale * (float)__builtin_bit_cast(half2v, w[i / 2])[i % 2];
-			store8(row + 32 * j, a.vec, x);
+			for (int i = 0; i < 8; ++i) x[i] = place[n] >= 0 ? scale * (float)__builtin_bit_cast(half2v, w[i / 2])[i % 2] : 0.0f;
+			store8((T*)(which ? a.values : a.keys) + (first + t) * a.token_stride + head * a.head_stride + 8 * c, a.vec, x);
 		}
 	}
 }
