@@ -651,3 +651,16 @@ def test_learned_levels_beat_even_ones(km, gpu):
     even = km.cache4_round_levels((np.arange(8) + 0.5) / 8)
     error = lambda lv: float(((held(rows, lv[None]) - rows) ** 2).mean())  # noqa: E731
     assert error(learned) < 0.9 * error(even)
+
+
+def test_the_example(km, gpu):
+    """The whole path: levels and layout learned by k-means, rows written, bounds, choice, attention. With the pages laid out by clusters the chosen
+    ones come closer to attention to all rows than with the prompt's order."""
+    import importlib.util
+    import os
+    spec = importlib.util.spec_from_file_location("cache4_decode", os.path.join(os.path.dirname(os.path.dirname(os.path.abspath(__file__))), "examples", "cache4_decode.py"))
+    example = importlib.util.module_from_spec(spec)
+    spec.loader.exec_module(example)
+    got = example.run(prompt=3000, steps=5, heads=2, group=4, dim=64, page=32, pages=16, say=lambda text: None)
+    assert got["by clusters"]["sparse"] < got["prompt's order"]["sparse"]
+    assert got["by clusters"]["whole"] < 0.2 and got["prompt's order"]["whole"] < 0.2
