@@ -122,6 +122,20 @@ __device__ __forceinline__ void load8(const T* p, bool vec, float x[8])
 	}
 }
 
+/* 8 elements as they are, two a word */
+__device__ __forceinline__ u32x4 load_raw8(const uint16_t* p, bool vec)
+{
+	if (vec) return *(const u32x4*)p;
+	u32x4 w;
+	for (int i = 0; i < 4; ++i) w[i] = p[2 * i] | (uint32_t)p[2 * i + 1] << 16;
+	return w;
+}
+__device__ __forceinline__ float raw_element(uint32_t w, bool upper, bool bf16)
+{
+	if (bf16) return __builtin_bit_cast(float, upper ? w & 0xFFFF0000u : w << 16);
+	return (float)__builtin_bit_cast(_Float16, (uint16_t)(upper ? w >> 16 : w));
+}
+
 /* rounded to the nearest, ties to even; NaN stays NaN */
 __device__ __forceinline__ uint32_t bf16_bits(float v)
 {

@@ -19,15 +19,20 @@ __device__ __forceinline__ float exp2_(float v) { return __builtin_amdgcn_exp2f(
 
 struct Row4 { uint32_t token, head; bool there; }; /* query number inside its sequence, query head inside its group */
 
+/* (divisions are some twenty instructions and come before the first load: none where a sequence has one query) */
 __device__ __forceinline__ Row4 row_of(const Attend4& a, const Sequence& seq, uint32_t row_tile, uint32_t r)
 {
 	Row4 row;
-	if (a.chosen) { /* the tokens' pages differ: a tile has rows of one token */
+	if (a.batch.max_queries == 1) {
+		row.token = 0;
+		row.head = row_tile * 16 + r;
+		row.there = seq.queries && row.head < a.batch.group;
+	} else if (a.chosen) { /* the tokens' pages differ: a tile has rows of one token */
 		const uint32_t tiles = (a.batch.group + 15) / 16;
 		row.token = row_tile / tiles;
 		row.head = row_tile % tiles * 16 + r;
 		row.there = row.token < seq.queries && row.head < a.batch.group;
-	} else {
+	} else { /* (at most MANY_ROWS of them) */
 		const uint32_t x = row_tile * 16 + r;
 		row.token = x / a.batch.group;
 		row.head = x % a.batch.group;
@@ -40,8 +45,15 @@ __device__ __forceinline__ Row4 row_of(const Attend4& a, const Sequence& seq, ui
 __device__ __forceinline__ uint32_t rows_of(const Attend4& a, const Sequence& seq, uint32_t row_tile)
 {
 	if (a.chosen) return min(16u, a.batch.group - row_tile % ((a.batch.group + 15) / 16) * 16);
-	const uint64_t rows = (uint64_t)seq.queries * a.batch.group, first = (uint64_t)row_tile * 16;
-	return first < rows ? (uint32_t)min((uint64_t)16, rows - first) : 0;
+	const uint32_t rows = seq.queries * a.batch.group, first = row_tile * 16;
+	return first < rows ? min(16u, rows - first) : 0;
+}
+
+/* the query of a tile's rows that sees the most */
+__device__ __forceinline__ uint32_t last_query_of(const Attend4& a, const Sequence& seq, uint32_t row_tile)
+{
+	if (a.batch.max_queries == 1) return 0;
+	return a.chosen ? row_tile / ((a.batch.group + 15) / 16) : min(seq.queries - 1, (row_tile * 16 + 15) / a.batch.group);
 }
 
 __device__ __forceinline__ uint64_t pair_of(float x, float y) { return (uint64_t)__builtin_bit_cast(uint32_t, y) << 32 | __builtin_bit_cast(uint32_t, x); }
@@ -49,17 +61,14 @@ __device__ __forceinline__ uint64_t pair_of(float x, float y) { return (uint64_t
 /* tiles of 64 tokens that a tile of rows looks at */
 __device__ __forceinline__ uint32_t tiles_of(const Attend4& a, const Sequence& seq, uint32_t row_tile)
 {
-	if (a.chosen) {
-		const uint32_t token = row_tile / ((a.batch.group + 15) / 16);
-		if (token >= seq.queries) return 0;
-		/* lists ascend: pages with a token that the query sees come first, and there are no more of them than the sequence has */
-		const uint32_t pages = (visible_to(a.batch, seq, token) + (1u << a.cache.page_shift) - 1) >> a.cache.page_shift;
-		return (uint32_t)((((uint64_t)min(a.top, pages) << (a.cache.page_shift - 4)) + 3) / 4);
-	}
-	const uint64_t x = (uint64_t)row_tile * 16;
-	if (x >= (uint64_t)seq.queries * a.batch.group) return 0;
-	const uint32_t last = (uint32_t)min((uint64_t)seq.queries - 1, (x + 15) / a.batch.group);
-	return (visible_to(a.batch, seq, last) + 63) / 64;
+	if (!a.chosen && row_tile * 16 >= seq.queries * a.batch.group) return 0;
+	const uint32_t query = last_query_of(a, seq, row_tile);
+	if (query >= seq.queries) return 0;
+	const uint32_t sees = visible_to(a.batch, seq, query);
+	if (!a.chosen) return (sees + 63) / 64;
+	/* lists ascend: pages with a token that the query sees come first, and there are no more of them than the sequence has */
+	const uint32_t pages = (sees + (1u << a.cache.page_shift) - 1) >> a.cache.page_shift;
+	return (uint32_t)((((uint64_t)min(a.top, pages) << (a.cache.page_shift - 4)) + 3) / 4);
 }
 
 template <int J>
@@ -95,18 +104,9 @@ __device__ __forceinline__ void load_halves(const uint8_t* p, uint32_t w[(J + 1)
 	}
 }
 
-/* 8 channels of every 32 of a row */
-template <int J, typename T>
-__device__ __forceinline__ void load_rows(const char* p, bool vec, float x[J][8])
-{
-	if (vec)
-		for (int j = 0; j < J; ++j) load8((const T*)p + 32 * j, true, x[j]);
-	else
-		for (int j = 0; j < J; ++j) load8((const T*)p + 32 * j, false, x[j]);
-}
-
+/* 8 channels of every 16 of a row */
 template <int N, typename T>
-__device__ __forceinline__ void load_steps(const char* p, bool vec, float x[N][8]) /* of every 16 */
+__device__ __forceinline__ void load_steps(const char* p, bool vec, float x[N][8])
 {
 	if (vec)
 		for (int c = 0; c < N; ++c) load8((const T*)p + 16 * c, true, x[c]);
@@ -175,42 +175,32 @@ attend4_kernel(Attend4 a)
 	__shared__ float most[4][16], total[4][16];
 	const uint32_t wave = (uint32_t)__builtin_amdgcn_readfirstlane((int)(threadIdx.x / WAVE)), lane = threadIdx.x % WAVE, i16 = lane % 16, kg = lane / 16;
 	/* first parts of all units before their second ones: the dies take work-groups in turn, and parts behind the end of a shorter sequence are empty */
-	const uint32_t units = gridDim.x / a.splits, part = blockIdx.x / units;
-	const uint32_t whole = blockIdx.x % units; /* sequence, head and tile of rows */
-	const uint32_t row_tile = whole % a.row_tiles, head = whole / a.row_tiles % a.cache.heads, s = whole / a.row_tiles / a.cache.heads;
+	const uint32_t head = blockIdx.x, s = blockIdx.y, part = a.row_tiles == 1 ? blockIdx.z : blockIdx.z / a.row_tiles, row_tile = blockIdx.z - part * a.row_tiles;
+	const uint32_t whole = (s * a.cache.heads + head) * a.row_tiles + row_tile; /* (counts work-groups: 31 bits) */
 	const Sequence seq = sequence_of(a.batch, s, a.cache.page_shift);
 	const uint32_t tiles = tiles_of(a, seq, row_tile);
 	const uint32_t begin = part * a.tiles_per_split, end = min(tiles, begin + a.tiles_per_split);
 	if (part > 0 && begin >= tiles) return;
 	const uint32_t parts = tiles > a.tiles_per_split ? (tiles + a.tiles_per_split - 1) / a.tiles_per_split : 1;
 	const Row4 row = row_of(a, seq, row_tile, i16);
+	if (seq.queries == 0) return; /* no rows */
 
-	/* queries: 8 channels a lane for each j */
-	half8v q[J];
-	float row_scale;
+	/* queries: 8 channels a lane for each j; on their way while the first tile's pages are looked up, put to use while that tile is on its way */
+	u32x4 raw[J];
 	{
-		float x[J][8];
-		const char* p = (const char*)a.q + 2 * ((size_t)(seq.first + (row.there ? row.token : 0)) * a.q_token + ((size_t)head * a.batch.group + (row.there ? row.head : 0)) * a.q_head + 8 * kg);
-		if (seq.queries == 0) {
-			for (int j = 0; j < J; ++j)
-				for (int e = 0; e < 8; ++e) x[j][e] = 0.0f;
-		} else if (a.bf16) load_rows<J, __bf16>(p, a.vec, x);
-		else load_rows<J, _Float16>(p, a.vec, x);
-		float largest = 0.0f;
+		const uint16_t* p = (const uint16_t*)a.q + (size_t)(seq.first + (row.there ? row.token : 0)) * a.q_token + ((size_t)head * a.batch.group + (row.there ? row.head : 0)) * a.q_head + 8 * kg;
+		if (a.vec) {
 #pragma unroll
-		for (int j = 0; j < J; ++j)
-			for (int e = 0; e < 8; ++e) largest = fmaxf(largest, fabsf(x[j][e]));
-		largest = fmaxf(largest, __shfl_xor(largest, 16));
-		largest = fmaxf(largest, __shfl_xor(largest, 32));
-		const float by = query_scale(a.scale, largest, &row_scale);
+			for (int j = 0; j < J; ++j) raw[j] = *(const u32x4*)(p + 32 * j);
+		} else {
 #pragma unroll
-		for (int j = 0; j < J; ++j)
-			for (int e = 0; e < 8; ++e) q[j][e] = (_Float16)(x[j][e] * by);
+			for (int j = 0; j < J; ++j) raw[j] = load_raw8(p + 32 * j, false);
+		}
 	}
 	const int32_t sees = row.there ? (int32_t)visible_to(a.batch, seq, row.token) : 0;
 	const Magnitudes mk = load_magnitudes(a.cache.levels, head, 0), mv = load_magnitudes(a.cache.levels, head, 1);
 	const bool listed = a.chosen != nullptr;
-	const int32_t* list = a.chosen + (listed ? ((size_t)(seq.first + row_tile / ((a.batch.group + 15) / 16)) * a.cache.heads + head) * a.top : 0);
+	const int32_t* list = a.chosen + (listed ? ((size_t)(seq.first + last_query_of(a, seq, row_tile)) * a.cache.heads + head) * a.top : 0);
 	const int32_t* table = a.batch.table + (size_t)s * a.batch.table_stride;
 	const uint32_t sub_bits = a.cache.page_shift - 4, last_entry = (listed ? a.top : a.batch.table_stride) - 1;
 
@@ -254,6 +244,30 @@ attend4_kernel(Attend4 a)
 	f32x4 o[2 * J];
 #pragma unroll
 	for (int c = 0; c < 2 * J; ++c) o[c] = f32x4{ 0.0f, 0.0f, 0.0f, 0.0f };
+
+	half8v q[J];
+	float row_scale = 1.0f;
+	auto take_queries = [&]() {
+		float x[J][8], largest = 0.0f;
+		if (a.bf16) {
+#pragma unroll
+			for (int j = 0; j < J; ++j)
+				for (int e = 0; e < 8; ++e) { const uint32_t w = raw[j][e / 2]; x[j][e] = raw_element(w, e % 2, true); }
+		} else {
+#pragma unroll
+			for (int j = 0; j < J; ++j)
+				for (int e = 0; e < 8; ++e) { const uint32_t w = raw[j][e / 2]; x[j][e] = raw_element(w, e % 2, false); }
+		}
+#pragma unroll
+		for (int j = 0; j < J; ++j)
+			for (int e = 0; e < 8; ++e) largest = fmaxf(largest, fabsf(x[j][e]));
+		largest = fmaxf(largest, __shfl_xor(largest, 16));
+		largest = fmaxf(largest, __shfl_xor(largest, 32));
+		const float by = query_scale(a.scale, largest, &row_scale);
+#pragma unroll
+		for (int j = 0; j < J; ++j)
+			for (int e = 0; e < 8; ++e) q[j][e] = (_Float16)(x[j][e] * by);
+	};
 
 	auto work = [&](Tile4<J>& t, int32_t from, const Where& next) { /* ... and leaves the next tile's loads under way */
 		const int32_t limit = from == INT32_MAX ? 0 : sees - from; /* tokens of the lane's block that its row sees */
@@ -352,6 +366,7 @@ attend4_kernel(Attend4 a)
 		fetch_scales(t, w);
 		fetch_keys(t, w);
 		fetch_values(t, w);
+		take_queries();
 		for (uint32_t n = 0; n < count; ++n) {
 			const int32_t from = w.from;
 			if (n % 16 == 7 && n + 9 < count) find_places(tile0 + 4 * (n + 9), (n + 9) / 16 % 2);
@@ -789,7 +804,9 @@ int launch_attend4(Attend4 a, uint32_t max_length, Workspace* ws, const DeviceIn
 		}
 		return KMX_OK;
 	}
-	KMX_LAUNCH_KERNEL((attend4_kernel<J>), dim3((unsigned)(units * a.splits)), dim3(256), 0, stream(), a);
+	if (a.batch.sequences > 65535 || (uint64_t)a.row_tiles * a.splits > 65535)
+		return fail(KMX_ERR_UNSUPPORTED, "kmx_cache4_attend: %u sequences of %u queries are too many for one call", a.batch.sequences, a.batch.max_queries);
+	KMX_LAUNCH_KERNEL((attend4_kernel<J>), dim3(a.cache.heads, a.batch.sequences, a.row_tiles * a.splits), dim3(256), 0, stream(), a);
 	KMX_LAUNCH_CHECK("attend4_kernel");
 	return KMX_OK;
 }
