@@ -376,7 +376,7 @@ struct Select4 {
 	uint32_t* keys;     /* [token][head][table_stride], larger for a better page */
 	int32_t* chosen;    /* [token][head][top] */
 	uint32_t top, first, last;
-	uint32_t span;      /* query heads of a token side by side: the power of two from `group` on, at most 16 */
+	uint32_t span, span_bits; /* query heads of a token side by side: the power of two from `group` on, at most 16 */
 	uint32_t per;       /* tokens of a tile of queries: a power of two, at most 16 / span and 8 */
 	uint32_t token_tiles, chunks, chunk; /* tiles of queries a sequence; parts of the pages and how many times 64 each */
 	bool bf16, vec;
@@ -409,15 +409,15 @@ struct Scorer4 {
 	i32x4 q8[J];
 
 	__device__ __forceinline__ Scorer4(const Select4& args, const Sequence& sequence, uint32_t cache_head, uint32_t tile_of_queries, uint32_t lane)
-	    : a(args), seq(sequence), head(cache_head), tile(tile_of_queries), col(lane % 16), kg(lane / 16), i(tile * args.per + lane % 16 / args.span)
+	    : a(args), seq(sequence), head(cache_head), tile(tile_of_queries), col(lane % 16), kg(lane / 16), i(tile * args.per + (lane % 16 >> args.span_bits))
 	{
-		token_there = lane % 16 / a.span < a.per && i < seq.queries;
+		token_there = (lane % 16 >> a.span_bits) < a.per && i < seq.queries;
 	}
 	/* 8 channels of a row of the 16 from query head g0 on; zeros where there is none */
 	__device__ __forceinline__ u32x4 load(uint32_t g0, uint32_t row, uint32_t channel) const
 	{
-		const uint32_t token = tile * a.per + row / a.span, h = g0 + row % a.span;
-		if (row / a.span >= a.per || token >= seq.queries || h >= a.batch.group) return u32x4{ 0, 0, 0, 0 };
+		const uint32_t token = tile * a.per + (row >> a.span_bits), h = g0 + (row & (a.span - 1));
+		if ((row >> a.span_bits) >= a.per || token >= seq.queries || h >= a.batch.group) return u32x4{ 0, 0, 0, 0 };
 		return load_raw8((const uint16_t*)a.q + (size_t)(seq.first + token) * a.q_token + (size_t)(head * a.batch.group + h) * a.q_head + channel, a.vec);
 	}
 	/* the largest magnitude of each token, over all its query heads; by all threads of the work-group */
@@ -433,7 +433,7 @@ struct Scorer4 {
 					const uint32_t w = raw[e / 2];
 					largest = fmaxf(largest, fabsf(raw_element(w, e % 2, a.bf16)));
 				}
-				atomicMax(&lds.largest[item / (D / 8) / a.span], __builtin_bit_cast(uint32_t, largest)); /* (not negative: in the order of their words) */
+				atomicMax(&lds.largest[item / (D / 8) >> a.span_bits], __builtin_bit_cast(uint32_t, largest)); /* (not negative: in the order of their words) */
 			}
 		__syncthreads();
 	}
@@ -442,7 +442,7 @@ struct Scorer4 {
 	{
 		for (uint32_t item = threadIdx.x; item < 16 * (D / 8); item += threads) {
 			const uint32_t row = item / (D / 8), channel = item % (D / 8) * 8;
-			const float largest = __builtin_bit_cast(float, lds.largest[min(row / a.span, 7u)]);
+			const float largest = __builtin_bit_cast(float, lds.largest[min((row >> a.span_bits), 7u)]);
 			const float by = largest > 0.0f ? 1.0f / largest * 127.0f : 0.0f;
 			const u32x4 raw = load(g0, row, channel);
 			u32x2 up{ 0, 0 }, down{ 0, 0 };
@@ -466,7 +466,7 @@ struct Scorer4 {
 		i32x4 dot{ 0, 0, 0, 0 };
 #pragma unroll
 		for (int c = 0; c < J; ++c) dot = __builtin_amdgcn_mfma_i32_16x16x64_i8(b[c], q8[c], dot, 0, 0, 0);
-		const bool there = token_there && g0 + col % a.span < a.batch.group;
+		const bool there = token_there && g0 + (col & (a.span - 1)) < a.batch.group;
 		for (int r = 0; r < 4; ++r) best[r] = there ? dot[r] : INT32_MIN;
 		for (uint32_t d = 1; d < a.span; d *= 2) /* the largest over the token's query heads */
 			for (int r = 0; r < 4; ++r) best[r] = max(best[r], __shfl_xor(best[r], (int)d));
@@ -474,7 +474,7 @@ struct Scorer4 {
 	/* pages of the sequence with a token that the lane's query sees */
 	__device__ __forceinline__ uint32_t seen() const { return token_there ? (visible_to(a.batch, seq, i) + (1u << a.cache.page_shift) - 1) >> a.cache.page_shift : 0; }
 	/* the lane that writes number r of its page: the lanes of a token share them out */
-	__device__ __forceinline__ bool writes(int r) const { return token_there && (col % a.span) < 4 && (uint32_t)r % min(a.span, 4u) == col % min(a.span, 4u); }
+	__device__ __forceinline__ bool writes(int r) const { return token_there && ((col & (a.span - 1))) < 4 && ((uint32_t)r & (a.span - 1) & 3) == (col & (a.span - 1) & 3); }
 	__device__ __forceinline__ uint32_t key(uint32_t page, uint32_t pages, int best, float scale, bool known) const
 	{
 		const bool forced = page < a.first || page + a.last >= pages;
@@ -558,12 +558,7 @@ score4_kernel(Select4 a)
 {
 	__shared__ typename Scorer4<J>::Lds lds;
 	const uint32_t wave = (uint32_t)__builtin_amdgcn_readfirstlane((int)(threadIdx.x / WAVE)), lane = threadIdx.x % WAVE;
-	uint32_t unit = blockIdx.x;
-	const uint32_t part = unit % a.chunks;
-	unit /= a.chunks;
-	const uint32_t head = unit % a.cache.heads;
-	unit /= a.cache.heads;
-	const uint32_t tile = unit % a.token_tiles, s = unit / a.token_tiles;
+	const uint32_t head = blockIdx.x, s = blockIdx.y, tile = a.token_tiles == 1 ? 0 : blockIdx.z % a.token_tiles, part = a.token_tiles == 1 ? blockIdx.z : blockIdx.z / a.token_tiles;
 	const Sequence seq = sequence_of(a.batch, s, a.cache.page_shift);
 	if (tile * a.per >= seq.queries) return;
 	const uint32_t page_tokens = 1u << a.cache.page_shift, last_i = min(seq.queries, (tile + 1) * a.per) - 1;
@@ -691,10 +686,7 @@ choose4_kernel(Select4 a)
 	constexpr uint32_t CACHED = 8192;
 	__shared__ uint32_t above[8], equal[8], cached[CACHED];
 	__shared__ ChooseLds lds;
-	uint32_t unit = blockIdx.x;
-	const uint32_t head = unit % a.cache.heads;
-	unit /= a.cache.heads;
-	const uint32_t i = unit % a.batch.max_queries, s = unit / a.batch.max_queries;
+	const uint32_t head = blockIdx.x, s = blockIdx.y, i = blockIdx.z;
 	const Sequence seq = sequence_of(a.batch, s, a.cache.page_shift);
 	if (i >= seq.queries) return;
 	const uint32_t n = (visible_to(a.batch, seq, i) + (1u << a.cache.page_shift) - 1) >> a.cache.page_shift;
@@ -726,17 +718,14 @@ select4_kernel(Select4 a, uint32_t stride)
 	__shared__ ChooseLds choose[8];
 	__shared__ uint32_t above[THREADS / WAVE], equal[THREADS / WAVE];
 	const uint32_t wave = (uint32_t)__builtin_amdgcn_readfirstlane((int)(threadIdx.x / WAVE)), lane = threadIdx.x % WAVE;
-	uint32_t unit = blockIdx.x;
-	const uint32_t head = unit % a.cache.heads;
-	unit /= a.cache.heads;
-	const uint32_t tile = unit % a.token_tiles, s = unit / a.token_tiles;
+	const uint32_t head = blockIdx.x, s = blockIdx.y, tile = blockIdx.z;
 	const Sequence seq = sequence_of(a.batch, s, a.cache.page_shift);
 	if (tile * a.per >= seq.queries) return;
 	const uint32_t page_tokens = 1u << a.cache.page_shift, last_i = min(seq.queries, (tile + 1) * a.per) - 1;
 	const uint32_t pages = (visible_to(a.batch, seq, last_i) + page_tokens - 1) >> a.cache.page_shift;
 	if (pages > a.top) {
 		Scorer4<J> scorer(a, seq, head, tile, lane);
-		uint32_t* const mine = keys + (scorer.token_there ? scorer.col / a.span : 0) * stride;
+		uint32_t* const mine = keys + (scorer.token_there ? (scorer.col >> a.span_bits) : 0) * stride;
 		constexpr int TILES = THREADS == 512 ? 2 : 1;
 		score_pages<J, TILES>(scorer, lds, a.batch.table + (size_t)s * a.batch.table_stride, 16 * TILES * wave, pages, pages, 16 * TILES * (THREADS / WAVE), THREADS,
 		                      [&](uint32_t p) { return mine[p]; }, [&](uint32_t p, uint32_t k) { mine[p] = k; });
@@ -970,22 +959,23 @@ int kmx_cache4_select(const kmx_cache4* cache, const kmx_cache4_batch* batch, in
 	a.bf16 = type == KMX_BF16;
 	a.vec = aligned_rows(q, q_token_stride, q_head_stride, 2);
 	a.span = 1;
-	while (a.span < a.batch.group && a.span < 16) a.span *= 2;
+	while (a.span < a.batch.group && a.span < 16) { a.span *= 2; ++a.span_bits; }
 	/* Scores and choice in one kernel where the pages are few, by 4 wavefronts or by 16 (64 sequences of 128 pages: 65 us by 16, 57 in two kernels; two
 	 * sequences of 625 pages, 128 queries: 37 us against 41); two kernels where one work-group would read for long (1 x 1024 pages: 29 us against 34) */
 	const bool one = pages <= SELECT_PAGES, few = pages <= SELECT_FEW;
 	a.per = 1;
 	while (a.per < batch->max_queries && a.per < (one && few ? 4 : 8) && a.per * a.span < 16) a.per *= 2;
 	a.token_tiles = (batch->max_queries + a.per - 1) / a.per;
-	const uint64_t units = (uint64_t)batch->sequences * a.token_tiles * a.cache.heads, rows = (uint64_t)batch->sequences * batch->max_queries * a.cache.heads;
-	if (units > 0x7FFFFFFFu || rows > 0x7FFFFFFFu) return fail(KMX_ERR_UNSUPPORTED, "kmx_cache4_select: too many queries for one call");
+	const uint64_t units = (uint64_t)batch->sequences * a.token_tiles * a.cache.heads;
+	if (batch->sequences > 65535 || batch->max_queries > 65535)
+		return fail(KMX_ERR_UNSUPPORTED, "kmx_cache4_select: %u sequences of %u queries are too many for one call", batch->sequences, batch->max_queries);
 	if (one) {
 		const uint32_t stride = pages | 1, bytes = 4 * a.per * stride; /* at most 24.6 KB */
 		switch (cache->dim / 32) {
 #define KMX_CASE(N)                                                                                                      \
 	case N:                                                                                                               \
-		if (few) KMX_LAUNCH_KERNEL((select4_kernel<N, true>), dim3((unsigned)units), dim3(select_threads(N, true)), bytes, stream(), a, stride); \
-		else KMX_LAUNCH_KERNEL((select4_kernel<N, false>), dim3((unsigned)units), dim3(select_threads(N, false)), bytes, stream(), a, stride); \
+		if (few) KMX_LAUNCH_KERNEL((select4_kernel<N, true>), dim3(a.cache.heads, batch->sequences, a.token_tiles), dim3(select_threads(N, true)), bytes, stream(), a, stride); \
+		else KMX_LAUNCH_KERNEL((select4_kernel<N, false>), dim3(a.cache.heads, batch->sequences, a.token_tiles), dim3(select_threads(N, false)), bytes, stream(), a, stride); \
 		break;
 			KMX_CASE(1) KMX_CASE(2) KMX_CASE(3) KMX_CASE(4) KMX_CASE(5) KMX_CASE(6) KMX_CASE(7) KMX_CASE(8)
 #undef KMX_CASE
@@ -999,7 +989,7 @@ int kmx_cache4_select(const kmx_cache4* cache, const kmx_cache4_batch* batch, in
 	if (parts > (tiles + 1) / 2) parts = (tiles + 1) / 2;
 	a.chunk = (uint32_t)((tiles + parts - 1) / parts);
 	a.chunks = (tiles + a.chunk - 1) / a.chunk;
-	if (units * a.chunks > 0x7FFFFFFFu) return fail(KMX_ERR_UNSUPPORTED, "kmx_cache4_select: too many queries for one call");
+	if ((uint64_t)a.token_tiles * a.chunks > 65535) return fail(KMX_ERR_UNSUPPORTED, "kmx_cache4_select: %u queries are too many for one call", batch->max_queries);
 	Workspace* ws = nullptr;
 	rc = workspace(&ws);
 	if (rc) return rc;
@@ -1008,12 +998,12 @@ int kmx_cache4_select(const kmx_cache4* cache, const kmx_cache4_batch* batch, in
 	a.keys = (uint32_t*)ws->partials;
 	switch (cache->dim / 32) {
 #define KMX_CASE(N)                                                                                                      \
-	case N: KMX_LAUNCH_KERNEL((score4_kernel<N>), dim3((unsigned)(units * a.chunks)), dim3(256), 0, stream(), a); break;
+	case N: KMX_LAUNCH_KERNEL((score4_kernel<N>), dim3(a.cache.heads, batch->sequences, a.token_tiles * a.chunks), dim3(256), 0, stream(), a); break;
 		KMX_CASE(1) KMX_CASE(2) KMX_CASE(3) KMX_CASE(4) KMX_CASE(5) KMX_CASE(6) KMX_CASE(7) KMX_CASE(8)
 #undef KMX_CASE
 	}
 	KMX_LAUNCH_CHECK("score4_kernel");
-	KMX_LAUNCH_KERNEL(choose4_kernel, dim3((unsigned)rows), dim3(512), 0, stream(), a);
+	KMX_LAUNCH_KERNEL(choose4_kernel, dim3(a.cache.heads, batch->sequences, batch->max_queries), dim3(512), 0, stream(), a);
 	KMX_LAUNCH_CHECK("choose4_kernel");
 	return KMX_OK;
 }
