@@ -741,29 +741,43 @@ select4_kernel(Select4 a, uint32_t stride)
 
 /* ---------------------------------------------------------------- launch shapes of the attention - */
 
-/* Tiles of 16 rows, or of 256 where there are many, and how many parts the tokens are taken in: enough work-groups to fill the chip, none below
- * one tile a wavefront */
-Plan4 plan_attend4(const Batch4& b, uint32_t heads, uint32_t max_length, uint32_t page_shift, uint32_t top, const DeviceInfo& dev)
+/*
+ * Tiles of 16 rows, or of 256 where there are many, and how many parts the tokens are taken in.
+ * 16 rows: two work-groups a compute unit in all, none below one tile a wavefront (64 sequences of 8192 tokens, 8 heads: 124 us in one part, 133 in
+ * four; one sequence of 131072: 32 us with one work-group a unit, 28.7 with two, 29.4 with four).
+ * 256 rows: as many parts as make the rounds of work-groups on the chip short, a part's own cost taken as that of MANY_COST tiles.
+ */
+Plan4 plan_attend4(uint32_t J, const Batch4& b, uint32_t heads, uint32_t max_length, uint32_t page_shift, uint32_t top, const DeviceInfo& dev)
 {
 	Plan4 plan;
 	const uint64_t rows = (uint64_t)b.max_queries * b.group;
-	plan.many = !top && rows > 64;
+	plan.many = !top && rows > MANY_ROWS;
 	plan.row_tiles = top ? b.max_queries * ((b.group + 15) / 16) : (uint32_t)(plan.many ? (rows + 255) / 256 : (rows + 15) / 16);
 	const uint64_t tokens = top ? (uint64_t)top << page_shift : max_length, units = (uint64_t)b.sequences * heads * plan.row_tiles;
-	const uint32_t tiles = (uint32_t)((tokens + 63) / 64), step = plan.many ? 1 : 4, least = plan.many ? 16 : 4;
-	uint64_t want = ((plan.many ? 1 : 2) * dev.compute_units + units - 1) / (units ? units : 1);
-	const uint64_t most = (tiles + least - 1) / least;
-	if (want > MOST_PARTS) want = MOST_PARTS;
-	if (units > TICKETS) want = 1;
-	const uint32_t splits = (uint32_t)(want < most ? want : most ? most : 1);
-	plan.tiles_per_split = tiles ? ((tiles + splits - 1) / splits + step - 1) / step * step : step;
+	const uint32_t tiles = (uint32_t)((tokens + 63) / 64);
+	uint64_t parts = 1;
+	if (plan.many) {
+		const uint64_t slots = (J <= 2 ? 2 : 1) * (uint64_t)dev.compute_units; /* work-groups on the chip at a time */
+		uint64_t best = ~0ull;
+		for (uint64_t p = 1; p <= 16 && (p == 1 || p * MANY_LEAST <= tiles); ++p) {
+			const uint64_t time = (units * p + slots - 1) / slots * ((tiles + p - 1) / p + MANY_COST);
+			if (time < best) { best = time; parts = p; }
+		}
+	} else {
+		parts = (2 * dev.compute_units + units - 1) / (units ? units : 1);
+		if (parts > (tiles + 3) / 4) parts = (tiles + 3) / 4;
+		if (parts > MOST_PARTS) parts = MOST_PARTS;
+		if (parts == 0 || units > TICKETS) parts = 1;
+	}
+	const uint32_t step = plan.many ? 1 : 4; /* a tile for each wavefront */
+	plan.tiles_per_split = tiles ? (uint32_t)(((tiles + parts - 1) / parts + step - 1) / step * step) : step;
 	plan.splits = tiles ? (tiles + plan.tiles_per_split - 1) / plan.tiles_per_split : 1;
 	return plan;
 }
 
 size_t attend4_partial_floats(uint32_t J, const Batch4& b, uint32_t heads, uint32_t max_length, uint32_t page_shift, uint32_t top, const DeviceInfo& dev)
 {
-	const Plan4 plan = plan_attend4(b, heads, max_length, page_shift, top, dev);
+	const Plan4 plan = plan_attend4(J, b, heads, max_length, page_shift, top, dev);
 	return plan.splits > 1 ? (size_t)b.sequences * heads * plan.row_tiles * plan.splits * ((plan.many ? 256 : 16) * (32 * J + 2)) : 0;
 }
 

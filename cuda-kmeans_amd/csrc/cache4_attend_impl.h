@@ -516,7 +516,7 @@ typedef float f32x16 __attribute__((ext_vector_type(16)));
  * LDS are 16 bytes longer than their contents: 8 lanes one below the other read 8 different groups of banks.
  */
 template <int J>
-__global__ void __launch_bounds__(512, 2)
+__global__ void __launch_bounds__(512, J <= 2 ? 4 : 2)
 attend4_many_kernel(Attend4 a)
 {
 	constexpr uint32_t D = 32 * J, KROW = 2 * D + 16, VROW = 144, TILE = 64 * KROW + D * VROW;
@@ -781,7 +781,7 @@ join4_kernel(Attend4 a)
 template <int J>
 int launch_attend4(Attend4 a, uint32_t max_length, Workspace* ws, const DeviceInfo& dev)
 {
-	const Plan4 plan = plan_attend4(a.batch, a.cache.heads, max_length, a.cache.page_shift, a.top, dev);
+	const Plan4 plan = plan_attend4(J, a.batch, a.cache.heads, max_length, a.cache.page_shift, a.top, dev);
 	a.row_tiles = plan.row_tiles;
 	a.splits = plan.splits;
 	a.tiles_per_split = plan.tiles_per_split;
