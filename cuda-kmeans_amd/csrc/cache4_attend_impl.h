@@ -149,12 +149,15 @@ struct Tile4 {
 /*
  * A work-group of four wavefronts takes 16 rows of one head of the cache (the query heads of a token side by side, then the next token's) and
  * a part of the tokens; a wavefront takes every fourth tile of 64 tokens. The registers of a tile's keys are loaded with the next tile's as soon as
- * the scores are there, those of its values as soon as the sums are: each load has the other half of a tile's work to arrive in, and three or four
- * wavefronts fit a SIMD. Both products
- * have the cache as their first operand (v_mfma_f32_16x16x32_f16): scores come out as [token][row], so a lane has all its 16 scores in one row
- * -- maxima and sums are its own but for two exchanges -- and its probabilities are, as they stand, its piece of the second operand of
- * [channel][row] = values . p. Tokens go to the rows of the first product such that a lane's 16 are those of one block: its values are 16 bytes
- * side by side.
+ * the scores are there, those of its values as soon as the sums are: each load has the other half of a tile's work to arrive in, and three
+ * wavefronts fit a SIMD (two above 128 channels). Both products have the cache as their first operand (v_mfma_f32_16x16x32_f16): scores come out as
+ * [token][row], so a lane has all its 16 scores in one row -- maxima and sums are its own but for two exchanges -- and its probabilities are, as they
+ * stand, its piece of the second operand of [channel][row] = values . p. Tokens go to the rows of the first product such that a lane's 16 are those
+ * of one block: its values are 16 bytes side by side.
+ * Bound by unpacking: some 760 instructions a tile of 64 tokens at 128 channels, 1.4 us a tile and SIMD, about what the memory takes for it. 64
+ * sequences of 8192 tokens, 8 heads of 128: 124 us, 4.8 TB/s of packed bytes; the same of 1 to 8192 tokens 102 to 107 us, where the longest ones
+ * end last. Short sequences: 7 to 9 us, of which 4.5 are a launch with its first load and last store, the rest loads that wait for each other
+ * (length, table, codes).
  */
 template <int J>
 __global__ void __launch_bounds__(256, J <= 4 ? 3 : 2)
@@ -514,6 +517,10 @@ typedef float f32x16 __attribute__((ext_vector_type(16)));
  * into one of two buffers while everybody works on the other. Scores are [token][row] as above (v_mfma_f32_32x32x16_f16, 16 tokens a lane and
  * half of the tile), so that probabilities stay in their registers: the values' tokens lie in LDS in the order in which a lane has them. Rows of
  * LDS are 16 bytes longer than their contents: 8 lanes one below the other read 8 different groups of banks.
+ * Bound by the matrix instructions with the softmax between them: 2 x 1024 queries, 32 heads on 8 of 128, 16384 tokens each: 590 us, 900 TFLOP/s of
+ * the 1150 that a large matrix product reaches; lengths that differ 570 us at 0.77 of the work: the longer sequence ends last. Heads of 32 and 64
+ * channels have two work-groups on a compute unit (2 x 1024 of up to 16384 tokens: 319 and 373 us against 376 and 405 with one). 256 channels: a
+ * wavefront's sums and queries are more than the registers hold, 68 of them go to memory, 507 TFLOP/s.
  */
 template <int J>
 __global__ void __launch_bounds__(512, J <= 2 ? 4 : 2)
