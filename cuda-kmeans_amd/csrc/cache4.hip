@@ -748,7 +748,10 @@ select4_kernel(Select4 a, uint32_t stride)
  * Tiles of 16 rows, or of 256 where there are many, and how many parts the tokens are taken in.
  * 16 rows: two work-groups a compute unit in all, none below one tile a wavefront (64 sequences of 8192 tokens, 8 heads: 124 us in one part, 133 in
  * four; one sequence of 131072: 32 us with one work-group a unit, 28.7 with two, 29.4 with four).
- * 256 rows: as many parts as make the rounds of work-groups on the chip short, a part's own cost taken as that of MANY_COST tiles.
+ * 256 rows: lengths are known on the device only. Several sequences whose lengths may differ by much are divided in equal shares there, one for each
+ * work-group that the chip holds (2 x 1024 queries over 16384 and fewer tokens, 8 heads: of 128 channels 568 -> 521 us, 64: 375 -> 325, 256: 1598 ->
+ * 1475; 5 x 700 over up to 9000: 505 -> 463; but equal lengths 588 -> 622). Not one sequence (323 -> 347), nor where units are many and fill the chip
+ * as they come (1024 units: 477 -> 534), nor short ones: there as many parts as make the rounds of work-groups short.
  */
 Plan4 plan_attend4(uint32_t J, const Batch4& b, uint32_t heads, uint32_t max_length, uint32_t page_shift, uint32_t top, const DeviceInfo& dev)
 {
@@ -758,22 +761,30 @@ Plan4 plan_attend4(uint32_t J, const Batch4& b, uint32_t heads, uint32_t max_len
 	plan.row_tiles = top ? b.max_queries * ((b.group + 15) / 16) : (uint32_t)(plan.many ? (rows + 255) / 256 : (rows + 15) / 16);
 	const uint64_t tokens = top ? (uint64_t)top << page_shift : max_length, units = (uint64_t)b.sequences * heads * plan.row_tiles;
 	const uint32_t tiles = (uint32_t)((tokens + 63) / 64);
-	uint64_t parts = 1;
+	plan.joined = false;
 	if (plan.many) {
 		const uint64_t slots = (J <= 2 ? 2 : 1) * (uint64_t)dev.compute_units; /* work-groups on the chip at a time */
-		uint64_t best = ~0ull;
+		if (b.sequences > 1 && units <= 2 * slots && units * tiles >= SHARE_LEAST * slots && rows <= 0x7FFFFF00u && units * tiles <= 0x7FFFFFFFu) {
+			plan.splits = (uint32_t)slots;
+			plan.tiles_per_split = 0;
+			plan.joined = true;
+			return plan;
+		}
+		uint64_t best = ~0ull, parts = 1;
 		for (uint64_t p = 1; p <= 16 && (p == 1 || p * MANY_LEAST <= tiles); ++p) {
 			const uint64_t time = (units * p + slots - 1) / slots * ((tiles + p - 1) / p + MANY_COST);
 			if (time < best) { best = time; parts = p; }
 		}
-	} else {
-		parts = (2 * dev.compute_units + units - 1) / (units ? units : 1);
-		if (parts > (tiles + 3) / 4) parts = (tiles + 3) / 4;
-		if (parts > MOST_PARTS) parts = MOST_PARTS;
-		if (parts == 0 || units > TICKETS) parts = 1;
+		plan.tiles_per_split = tiles ? (uint32_t)((tiles + parts - 1) / parts) : 1;
+		plan.splits = (uint32_t)(units * parts);
+		plan.joined = parts > 1;
+		return plan;
 	}
-	const uint32_t step = plan.many ? 1 : 4; /* a tile for each wavefront */
-	plan.tiles_per_split = tiles ? (uint32_t)(((tiles + parts - 1) / parts + step - 1) / step * step) : step;
+	uint64_t parts = (2 * dev.compute_units + units - 1) / (units ? units : 1);
+	if (parts > (tiles + 3) / 4) parts = (tiles + 3) / 4;
+	if (parts > MOST_PARTS) parts = MOST_PARTS;
+	if (parts == 0 || units > TICKETS) parts = 1;
+	plan.tiles_per_split = tiles ? (uint32_t)(((tiles + parts - 1) / parts + 3) / 4 * 4) : 4; /* a tile for each wavefront */
 	plan.splits = tiles ? (tiles + plan.tiles_per_split - 1) / plan.tiles_per_split : 1;
 	return plan;
 }
@@ -781,7 +792,9 @@ Plan4 plan_attend4(uint32_t J, const Batch4& b, uint32_t heads, uint32_t max_len
 size_t attend4_partial_floats(uint32_t J, const Batch4& b, uint32_t heads, uint32_t max_length, uint32_t page_shift, uint32_t top, const DeviceInfo& dev)
 {
 	const Plan4 plan = plan_attend4(J, b, heads, max_length, page_shift, top, dev);
-	return plan.splits > 1 ? (size_t)b.sequences * heads * plan.row_tiles * plan.splits * ((plan.many ? 256 : 16) * (32 * J + 2)) : 0;
+	const size_t units = (size_t)b.sequences * heads * plan.row_tiles;
+	if (plan.many) return plan.joined ? 2 * (size_t)plan.splits * (256 * (32 * J + 2)) + 2 * units : 0; /* two parts a work-group, two words a unit */
+	return plan.splits > 1 ? units * plan.splits * (16 * (32 * J + 2)) : 0;
 }
 
 } // namespace kmx

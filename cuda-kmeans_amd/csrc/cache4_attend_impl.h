@@ -511,36 +511,116 @@ attend4_kernel(Attend4 a)
 
 typedef float f32x16 __attribute__((ext_vector_type(16)));
 
+/* tiles of 64 tokens that 256 rows of a sequence look at; 0: no such rows, and at least 1 (of nothing) where there are. (Rows, and tiles of all units,
+ * are counted in 31 bits where a call is divided in shares.) */
+__device__ __forceinline__ uint32_t many_tiles(const Attend4& a, uint32_t s, uint32_t row_tile)
+{
+	const Sequence seq = sequence_of(a.batch, s, a.cache.page_shift);
+	const uint64_t all_rows = (uint64_t)seq.queries * a.batch.group, first_row = (uint64_t)row_tile * 256;
+	if (first_row >= all_rows) return 0;
+	const uint64_t last = min(first_row + 255, all_rows - 1);
+	const uint32_t query = !a.batch.causal ? 0 : a.joined ? (uint32_t)last / a.batch.group : (uint32_t)(last / a.batch.group);
+	return max(1u, (visible_to(a.batch, seq, query) + 63) / 64);
+}
+
+__device__ __forceinline__ uint32_t scan4(uint32_t v) /* sums up to and with each lane */
+{
+	for (uint32_t d = 1; d < WAVE; d *= 2) {
+		const uint32_t below = (uint32_t)__shfl_up((int)v, d);
+		if (threadIdx.x % WAVE >= d) v += below;
+	}
+	return v;
+}
+
+/* What a work-group of the many-rows kernel takes: the tiles [from, to) of all units (a unit is a head of an entry, an entry 256 rows of a
+ * sequence; entries in order, their heads side by side), which begin in a place of unit (entry, head); or whole units. Each wavefront finds it. */
+struct Share4 { uint32_t from, to, entry, head, at, shares, total; };
+__device__ __forceinline__ uint32_t share_begin(uint32_t total, uint32_t g, uint32_t shares)
+{
+	const uint32_t each = total / shares, more = total - each * shares; /* the first ones take one more */
+	return each * g + min(g, more);
+}
+__device__ __forceinline__ uint32_t share_with(uint32_t total, uint32_t tile, uint32_t shares)
+{
+	const uint32_t each = total / shares, more = total - each * shares, large = more * (each + 1);
+	return tile < large ? tile / (each + 1) : more + (tile - large) / each;
+}
+__device__ __forceinline__ Share4 share_of(const Attend4& a, uint32_t g)
+{
+	const uint32_t lane = threadIdx.x % WAVE, entries = a.batch.sequences * a.row_tiles, heads = a.cache.heads;
+	Share4 share{};
+	uint32_t total = 0, most = 0, units = 0, w = 0, upto = 0;
+	for (uint32_t base = 0; base < entries; base += WAVE) {
+		const uint32_t e = base + lane;
+		w = e < entries ? many_tiles(a, e / a.row_tiles, e % a.row_tiles) : 0;
+		upto = scan4(w);
+		total += (uint32_t)__builtin_amdgcn_readlane((int)upto, WAVE - 1);
+		units += (uint32_t)__popcll(__ballot(w != 0));
+		uint32_t largest = w;
+		for (int d = 1; d < WAVE; d *= 2) largest = max(largest, (uint32_t)__shfl_xor((int)largest, d));
+		most = max(most, (uint32_t)__builtin_amdgcn_readfirstlane((int)largest));
+	}
+	total *= heads;
+	units *= heads;
+	share.total = total;
+	if (total == 0) return share;
+	share.shares = min(a.splits, max(total / MANY_LEAST, units));
+	/* whole units, a round of them at a time, where that takes no longer than equal shares and what joining them costs */
+	if ((uint64_t)((entries * heads + a.splits - 1) / a.splits) * most <= total / share.shares + MANY_COST) {
+		share.shares = 0;
+		return share;
+	}
+	if (g >= share.shares) return share;
+	share.from = share_begin(total, g, share.shares);
+	share.to = share_begin(total, g + 1, share.shares);
+	uint32_t before = 0;
+	for (uint32_t base = 0; base < entries; base += WAVE) {
+		if (entries > WAVE) {
+			const uint32_t e = base + lane;
+			w = e < entries ? many_tiles(a, e / a.row_tiles, e % a.row_tiles) : 0;
+			upto = scan4(w);
+		}
+		const uint64_t behind = __ballot(before + upto * heads > share.from);
+		if (behind) {
+			const int e = __ffsll((unsigned long long)behind) - 1;
+			const uint32_t tiles = (uint32_t)__builtin_amdgcn_readlane((int)w, e);
+			const uint32_t into = share.from - (before + ((uint32_t)__builtin_amdgcn_readlane((int)upto, e) - tiles) * heads);
+			share.entry = base + (uint32_t)e;
+			share.head = into / tiles;
+			share.at = into - share.head * tiles;
+			break;
+		}
+		before += (uint32_t)__builtin_amdgcn_readlane((int)upto, WAVE - 1) * heads;
+	}
+	return share;
+}
+
 /*
  * Many rows (pieces of prompts): a work-group of eight wavefronts takes 256 rows of one head, 32 a wavefront, and a part of the tokens. Tiles of 64
  * tokens become half-precision numbers once for all of them: wavefront w < 4 unpacks the keys of block w, wavefront 4 + w its values, into LDS,
  * into one of two buffers while everybody works on the other. Scores are [token][row] as above (v_mfma_f32_32x32x16_f16, 16 tokens a lane and
  * half of the tile), so that probabilities stay in their registers: the values' tokens lie in LDS in the order in which a lane has them. Rows of
  * LDS are 16 bytes longer than their contents: 8 lanes one below the other read 8 different groups of banks.
- * Bound by the matrix instructions with the softmax between them: 2 x 1024 queries, 32 heads on 8 of 128, 16384 tokens each: 590 us, 900 TFLOP/s of
- * the 1150 that a large matrix product reaches; lengths that differ 570 us at 0.77 of the work: the longer sequence ends last. Heads of 32 and 64
- * channels have two work-groups on a compute unit (2 x 1024 of up to 16384 tokens: 319 and 373 us against 376 and 405 with one). 256 channels: a
- * wavefront's sums and queries are more than the registers hold, 68 of them go to memory, 507 TFLOP/s.
+ * Bound by the matrix instructions with the softmax between them: 2 x 1024 queries, 32 heads on 8 of 128, 16384 and fewer tokens: 521 us, 777 TFLOP/s
+ * of the 1150 that a large matrix product reaches; one sequence of 16384, in two parts: 323 us, 824. A work-group takes a part of a unit (256 rows of a
+ * head), or its share of all units' tiles, from inside of one to inside of another. Heads of 32 and 64 channels have two work-groups on a compute
+ * unit (376 and 405 us with one, 321 and 375 with two, before the shares). 256 channels: a wavefront's sums and queries are more than the registers
+ * hold, and go to memory in part, 549 TFLOP/s.
  */
 template <int J>
-__global__ void __launch_bounds__(512, J <= 2 ? 4 : 2)
-attend4_many_kernel(Attend4 a)
+__device__ __forceinline__ void many_unit(const Attend4& a, uint8_t* many, uint32_t (*blocks_there)[4], uint32_t entry, uint32_t head, uint32_t begin, uint32_t until,
+                                          bool whole, uint32_t parts)
 {
 	constexpr uint32_t D = 32 * J, KROW = 2 * D + 16, VROW = 144, TILE = 64 * KROW + D * VROW;
 	constexpr int STEP = (J <= 5 ? 2 : 1); /* times 32 tokens of a tile: scores held at a time */
-	extern __shared__ __attribute__((aligned(16))) uint8_t many[]; /* two tiles: keys [token][channel], values [channel][token] */
-	__shared__ uint32_t blocks_there[2][4];
-	const uint32_t wave = (uint32_t)__builtin_amdgcn_readfirstlane((int)(threadIdx.x / WAVE)), lane = threadIdx.x % WAVE, n32 = lane % 32, h = lane / 32;
-	const uint32_t units = gridDim.x / a.splits, part = blockIdx.x / units, whole = blockIdx.x % units;
-	const uint32_t row_tile = whole % a.row_tiles, head = whole / a.row_tiles % a.cache.heads, s = whole / a.row_tiles / a.cache.heads;
+	uint32_t thread = threadIdx.x;
+	asm volatile("" : "+v"(thread)); /* addresses that follow from it are made anew for each unit, not kept from one to the next */
+	const uint32_t wave = (uint32_t)__builtin_amdgcn_readfirstlane((int)(thread / WAVE)), lane = thread % WAVE, n32 = lane % 32, h = lane / 32;
+	const uint32_t s = entry / a.row_tiles;
 	const Sequence seq = sequence_of(a.batch, s, a.cache.page_shift);
-	const uint64_t all_rows = (uint64_t)seq.queries * a.batch.group, first_row = (uint64_t)row_tile * 256;
-	if (first_row >= all_rows) return;
+	const uint64_t all_rows = (uint64_t)seq.queries * a.batch.group, first_row = (uint64_t)(entry % a.row_tiles) * 256;
 	const uint32_t rows = (uint32_t)min((uint64_t)256, all_rows - first_row);
-	const uint32_t tiles = (visible_to(a.batch, seq, (uint32_t)((first_row + rows - 1) / a.batch.group)) + 63) / 64;
-	const uint32_t begin = part * a.tiles_per_split, end = min(tiles, begin + a.tiles_per_split);
-	if (part > 0 && begin >= tiles) return;
-	const uint32_t parts = tiles > a.tiles_per_split ? (tiles + a.tiles_per_split - 1) / a.tiles_per_split : 1;
+	const uint32_t end = min(until, (visible_to(a.batch, seq, (uint32_t)((first_row + rows - 1) / a.batch.group)) + 63) / 64);
 
 	/* the lane's row, and what the rows of its wavefront see at least and at most */
 	const uint32_t wave_rows = rows > 32 * wave ? min(32u, rows - 32 * wave) : 0;
@@ -572,7 +652,7 @@ attend4_many_kernel(Attend4 a)
 	const uint32_t b = wave % 4, sub_bits = a.cache.page_shift - 4; /* the block of a tile that this wavefront unpacks */
 	const bool values = wave >= 4;
 	const Magnitudes mag = load_magnitudes(a.cache.levels, head, values ? 1 : 0);
-	const int32_t* table = a.batch.table + (size_t)s * a.batch.table_stride;
+	const Constant4 table = constant4(a.batch.table) + (size_t)s * a.batch.table_stride;
 	constexpr int VITEMS = (16 * J + WAVE - 1) / WAVE; /* pairs of channels a lane */
 	struct { uint32_t codes[values_words<J>()]; u32x4 scales[VITEMS][2]; uint32_t key_scales[(J + 1) / 2]; } in;
 	int32_t written = 0; /* tokens of the block that are there */
@@ -711,8 +791,10 @@ attend4_many_kernel(Attend4 a)
 	}
 	l += __shfl_xor(l, 32);
 
-	if (parts == 1) {
-		if (!there) return;
+	if (a.joined && begin == 0 && threadIdx.x == 0) /* for the join: the unit's first share, and how many it lies in */
+		((uint2*)(a.partial + (size_t)2 * a.splits * (256 * (D + 2))))[entry * a.cache.heads + head] = uint2{ blockIdx.x, parts };
+	if (!there) return;
+	if (whole) {
 		const float by = l > 0.0f ? 1.0f / l : l == l ? 0.0f : l;
 		char* to = (char*)a.out + 2 * ((size_t)(seq.first + token) * a.out_token + (size_t)query_head * a.out_head);
 #pragma unroll
@@ -727,8 +809,7 @@ attend4_many_kernel(Attend4 a)
 	}
 
 	/* a part of the tokens: [256][D] sums, then [256] pairs of maximum and sum, for join4_kernel */
-	float* const to = a.partial + ((size_t)whole * a.splits + part) * (256 * (D + 2));
-	if (!there) return;
+	float* const to = a.partial + (size_t)(2 * blockIdx.x + (begin == 0)) * (256 * (D + 2));
 	const uint32_t r = 32 * wave + n32;
 #pragma unroll
 	for (int j = 0; j < J; ++j)
@@ -736,8 +817,57 @@ attend4_many_kernel(Attend4 a)
 	if (h == 0) *(float2*)(to + 256 * D + 2 * r) = float2{ m * row_scale, l };
 }
 
+template <int J, bool SHARES>
+__global__ void __launch_bounds__(512, J <= 2 ? 4 : 2)
+attend4_many_kernel(Attend4 a)
+{
+	extern __shared__ __attribute__((aligned(16))) uint8_t many[]; /* two tiles: keys [token][channel], values [channel][token] */
+	__shared__ uint32_t blocks_there[2][4];
+	const uint32_t heads = a.cache.heads, entries = a.batch.sequences * a.row_tiles;
+	if constexpr (!SHARES) {
+		const uint32_t units = entries * heads, part = blockIdx.x / units, unit = blockIdx.x % units, entry = unit / heads;
+		const uint32_t weight = many_tiles(a, entry / a.row_tiles, entry % a.row_tiles), begin = part * a.tiles_per_split;
+		if (begin >= weight) return;
+		const uint32_t parts = (weight + a.tiles_per_split - 1) / a.tiles_per_split;
+		many_unit<J>(a, many, blocks_there, entry, unit % heads, begin, min(weight, begin + a.tiles_per_split), parts == 1, parts);
+	} else {
+		__shared__ Share4 share; /* (in registers it would be there through all the work) */
+		const Share4 mine = share_of(a, blockIdx.x);
+		if (mine.total == 0 || (mine.shares && blockIdx.x >= mine.shares)) return;
+		if (threadIdx.x == 0) share = mine;
+		__syncthreads();
+		const bool shared = __builtin_amdgcn_readfirstlane((int)mine.shares) != 0;
+		uint32_t entry = (uint32_t)__builtin_amdgcn_readfirstlane((int)(shared ? mine.entry : blockIdx.x / heads));
+		uint32_t head = (uint32_t)__builtin_amdgcn_readfirstlane((int)(shared ? mine.head : blockIdx.x % heads));
+		uint32_t at = (uint32_t)__builtin_amdgcn_readfirstlane((int)mine.at);
+		uint32_t left = (uint32_t)__builtin_amdgcn_readfirstlane((int)(mine.to - mine.from)); /* tiles of the share */
+		while (entry < entries) { /* a unit, or a part of one, after the other */
+			const uint32_t weight = many_tiles(a, entry / a.row_tiles, entry % a.row_tiles);
+			const uint32_t begin = at, until = shared ? min(weight, at + left) : weight;
+			const bool whole = begin == 0 && until == weight;
+			uint32_t parts = 1;
+			if (!whole && begin == 0) parts = share_with(share.total, share.to - left + weight - 1, share.shares) - blockIdx.x + 1;
+			if (weight) many_unit<J>(a, many, blocks_there, entry, head, begin, until, whole, parts);
+			if (!shared) {
+				const uint32_t next = entry * heads + head + gridDim.x;
+				entry = next / heads;
+				head = next % heads;
+				continue;
+			}
+			left -= until - begin;
+			if (left == 0) return;
+			at = 0;
+			if (++head == heads || weight == 0) {
+				head = 0;
+				++entry;
+			}
+		}
+	}
+}
+
 /* Joins the parts of many rows: 256 rows of sums are more than one work-group should read alone, so they have a kernel. A wavefront takes a row, 8 J
  * lanes 4 channels each of every (64 / 8 J)-th part. */
+constexpr uint32_t JOIN_GROUPS = 64; /* work-groups a unit */
 template <int J>
 __global__ void __launch_bounds__(256)
 join4_kernel(Attend4 a)
@@ -745,44 +875,47 @@ join4_kernel(Attend4 a)
 	constexpr uint32_t D = 32 * J, LANES = 8 * J, GROUPS = WAVE / LANES;
 	constexpr size_t PART = 256 * (D + 2);
 	const uint32_t wave = (uint32_t)__builtin_amdgcn_readfirstlane((int)(threadIdx.x / WAVE)), lane = threadIdx.x % WAVE;
-	const uint32_t whole = blockIdx.x / 64, r = blockIdx.x % 64 * 4 + wave;
-	const uint32_t row_tile = whole % a.row_tiles, head = whole / a.row_tiles % a.cache.heads, s = whole / a.row_tiles / a.cache.heads;
-	const Sequence seq = sequence_of(a.batch, s, a.cache.page_shift);
-	const uint64_t all_rows = (uint64_t)seq.queries * a.batch.group, first_row = (uint64_t)row_tile * 256;
-	if (first_row + r >= all_rows) return;
+	const uint32_t unit = blockIdx.x / JOIN_GROUPS, entry = unit / a.cache.heads, head = unit % a.cache.heads;
+	const Sequence seq = sequence_of(a.batch, entry / a.row_tiles, a.cache.page_shift);
+	const uint64_t all_rows = (uint64_t)seq.queries * a.batch.group, first_row = (uint64_t)(entry % a.row_tiles) * 256;
+	if (first_row >= all_rows) return;
 	const uint32_t rows = (uint32_t)min((uint64_t)256, all_rows - first_row);
-	const uint32_t tiles = (visible_to(a.batch, seq, (uint32_t)((first_row + rows - 1) / a.batch.group)) + 63) / 64;
-	if (tiles <= a.tiles_per_split) return; /* one part: written where it belongs */
-	const uint32_t parts = (tiles + a.tiles_per_split - 1) / a.tiles_per_split, group = lane / LANES, at = lane % LANES;
-	const float* left = a.partial + (size_t)whole * a.splits * PART;
-	float top = -__builtin_inff();
-	for (uint32_t p = lane; p < parts; p += WAVE) top = fmaxf(top, left[p * PART + 256 * D + 2 * r]);
-	for (int d = 1; d < WAVE; d *= 2) top = fmaxf(top, __shfl_xor(top, d));
-	const float lowest = top == -__builtin_inff() ? 0.0f : top;
-	float sum = 0.0f;
-	f32x4 mine{ 0.0f, 0.0f, 0.0f, 0.0f };
-	if (group < GROUPS)
+	const uint2 record = ((const uint2*)(a.partial + 2 * (size_t)a.splits * PART))[unit];
+	const uint32_t parts = record.y, group = lane / LANES, at = lane % LANES;
+	if (parts <= 1) return; /* written where it belongs */
+	const float* left = a.partial + 2 * (size_t)record.x * PART; /* the first part is the second one of its work-group, the others are first ones */
+	const size_t step = (a.tiles_per_split ? 2 * (size_t)a.batch.sequences * a.row_tiles * a.cache.heads : 2) * PART; /* from a part's work-group to the next one's */
+	for (uint32_t r = blockIdx.x % JOIN_GROUPS * 4 + wave; r < rows; r += 4 * JOIN_GROUPS) {
+		float top = -__builtin_inff();
+		for (uint32_t p = lane; p < parts; p += WAVE) top = fmaxf(top, left[(p ? p * step : PART) + 256 * D + 2 * r]);
+		for (int d = 1; d < WAVE; d *= 2) top = fmaxf(top, __shfl_xor(top, d));
+		const float lowest = top == -__builtin_inff() ? 0.0f : top;
+		float sum = 0.0f;
+		f32x4 mine{ 0.0f, 0.0f, 0.0f, 0.0f };
+		if (group < GROUPS)
 #pragma unroll 4
-		for (uint32_t p = group; p < parts; p += GROUPS) {
-			const float2 ml = *(const float2*)(left + p * PART + 256 * D + 2 * r);
-			const float weight = exp2_(ml.x - lowest);
-			sum += ml.y * weight;
-			mine += *(const f32x4*)(left + p * PART + (size_t)r * D + 4 * at) * weight;
+			for (uint32_t p = group; p < parts; p += GROUPS) {
+				const float* part = left + (p ? p * step : PART);
+				const float2 ml = *(const float2*)(part + 256 * D + 2 * r);
+				const float weight = exp2_(ml.x - lowest);
+				sum += ml.y * weight;
+				mine += *(const f32x4*)(part + (size_t)r * D + 4 * at) * weight;
+			}
+		for (uint32_t g = 1; g < GROUPS; ++g) { /* the groups' sums, in their order */
+			const int other = (int)(at + g * LANES);
+			const f32x4 more{ __shfl(mine[0], other), __shfl(mine[1], other), __shfl(mine[2], other), __shfl(mine[3], other) };
+			const float more_sum = __shfl(sum, other);
+			if (group == 0) { mine += more; sum += more_sum; }
 		}
-	for (uint32_t g = 1; g < GROUPS; ++g) { /* the groups' sums, in their order */
-		const int other = (int)(at + g * LANES);
-		const f32x4 more{ __shfl(mine[0], other), __shfl(mine[1], other), __shfl(mine[2], other), __shfl(mine[3], other) };
-		const float more_sum = __shfl(sum, other);
-		if (group == 0) { mine += more; sum += more_sum; }
+		if (group != 0) continue;
+		const float by = sum > 0.0f ? 1.0f / sum : sum == sum ? 0.0f : sum;
+		const uint64_t x = first_row + r;
+		const size_t to_token = seq.first + x / a.batch.group, to_head = (size_t)head * a.batch.group + x % a.batch.group;
+		float v[4];
+		for (int e = 0; e < 4; ++e) v[e] = mine[e] * by;
+		store_out4(a, (char*)a.out + 2 * (to_token * a.out_token + to_head * a.out_head), 4 * at, v);
+		if (at == 0 && a.lse) a.lse[to_token * a.batch.query_heads + to_head] = sum == 0.0f ? -__builtin_inff() : (top + log2f(sum)) * 0.693147180559945309f;
 	}
-	if (group != 0) return;
-	const float by = sum > 0.0f ? 1.0f / sum : sum == sum ? 0.0f : sum;
-	const uint64_t x = first_row + r;
-	const size_t to_token = seq.first + x / a.batch.group, to_head = (size_t)head * a.batch.group + x % a.batch.group;
-	float v[4];
-	for (int e = 0; e < 4; ++e) v[e] = mine[e] * by;
-	store_out4(a, (char*)a.out + 2 * (to_token * a.out_token + to_head * a.out_head), 4 * at, v);
-	if (at == 0 && a.lse) a.lse[to_token * a.batch.query_heads + to_head] = sum == 0.0f ? -__builtin_inff() : (top + log2f(sum)) * 0.693147180559945309f;
 }
 
 template <int J>
@@ -792,21 +925,24 @@ int launch_attend4(Attend4 a, uint32_t max_length, Workspace* ws, const DeviceIn
 	a.row_tiles = plan.row_tiles;
 	a.splits = plan.splits;
 	a.tiles_per_split = plan.tiles_per_split;
+	a.joined = plan.joined;
 	a.partial = ws->partials;
 	a.tickets = ws->tickets;
 	const uint64_t units = (uint64_t)a.batch.sequences * a.cache.heads * a.row_tiles;
-	if (units * (a.splits < 64 ? 64 : a.splits) > 0x7FFFFFFFu) return fail(KMX_ERR_UNSUPPORTED, "kmx_cache4_attend: too many queries for one call");
+	if (units >= 1u << 23) return fail(KMX_ERR_UNSUPPORTED, "kmx_cache4_attend: too many queries for one call");
 	if (plan.many) {
 		constexpr uint32_t bytes = 2 * (64 * (64 * J + 16) + 32 * J * 144);
 		static bool allowed = false; /* more LDS than a launch may ask for unannounced */
 		if (!allowed && bytes > 65536) {
-			KMX_HIP(hipFuncSetAttribute((const void*)attend4_many_kernel<J>, hipFuncAttributeMaxDynamicSharedMemorySize, (int)bytes));
+			KMX_HIP(hipFuncSetAttribute((const void*)attend4_many_kernel<J, false>, hipFuncAttributeMaxDynamicSharedMemorySize, (int)bytes));
+			KMX_HIP(hipFuncSetAttribute((const void*)attend4_many_kernel<J, true>, hipFuncAttributeMaxDynamicSharedMemorySize, (int)bytes));
 			allowed = true;
 		}
-		KMX_LAUNCH_KERNEL((attend4_many_kernel<J>), dim3((unsigned)(units * a.splits)), dim3(512), bytes, stream(), a);
+		if (a.tiles_per_split == 0) KMX_LAUNCH_KERNEL((attend4_many_kernel<J, true>), dim3(a.splits), dim3(512), bytes, stream(), a);
+		else KMX_LAUNCH_KERNEL((attend4_many_kernel<J, false>), dim3(a.splits), dim3(512), bytes, stream(), a);
 		KMX_LAUNCH_CHECK("attend4_many_kernel");
-		if (a.splits > 1) {
-			KMX_LAUNCH_KERNEL((join4_kernel<J>), dim3((unsigned)(units * 64)), dim3(256), 0, stream(), a);
+		if (a.joined) {
+			KMX_LAUNCH_KERNEL((join4_kernel<J>), dim3((unsigned)(units * JOIN_GROUPS)), dim3(256), 0, stream(), a);
 			KMX_LAUNCH_CHECK("join4_kernel");
 		}
 		return KMX_OK;

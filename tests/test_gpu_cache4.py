@@ -357,6 +357,27 @@ def test_tokens_in_parts(km, gpu, group, counts):
         assert np.array_equal(first[0], again[0]) and np.array_equal(first[1], again[1])
 
 
+SEVENTY = [2500 if s == 67 else 5 + s for s in range(70)]
+
+
+@pytest.mark.parametrize("heads,group,dim,page,lengths,counts", [
+    (2, 3, 96, 64, [3000, 500, 0, 64, 1], [30, 90, 5, 1, 3]),                              # a sequence much longer than the others
+    (1, 4, 128, 16, [700, 1500], [300, 20]), (2, 1, 64, 32, [2000, 30, 900], [70, 2, 270]),  # some 256 rows of one, none of the other
+    (2, 1, 32, 64, SEVENTY, [1 + s % 3 if s else 80 for s in range(70)]),                  # more than 64 sequences
+    (3, 2, 256, 128, [500, 400], [40, 33]),                                                # all short: whole units
+    (4, 1, 96, 16, [20 + s for s in range(70)], [66 if s == 9 else 1 for s in range(70)])])  # and more of them than work-groups
+def test_lengths_far_below_what_the_batch_allows(km, gpu, heads, group, dim, page, lengths, counts):
+    """The host knows the longest length that may come; what there is is divided on the device."""
+    rng = np.random.default_rng(dim + len(lengths))
+    c = Cache(km, rng, heads, dim, page, sum(-(-n // page) for n in lengths) + 2)
+    tiles = -(-65536 // (heads * len(lengths)))
+    s = Queries(km, rng, c, lengths, counts, group, BF16, extra=64 * tiles // page).fill(rng)
+    s.batch = km.Cache4Batch(len(lengths), heads * group, s.tokens, max(counts), 64 * tiles, device(km, s.starts), device(km, np.int32(lengths)), device(km, s.table), s.table.shape[1])
+    first = s.check()
+    again = s.attend()
+    assert np.array_equal(first[0], again[0]) and np.array_equal(first[1], again[1])
+
+
 @pytest.mark.parametrize("counts", [[4, 9, 2], [70, 90, 80]])
 def test_more_queries_than_tokens_and_empty_sequences(km, gpu, counts):
     """The first queries of a sequence that holds fewer tokens than it has queries see nothing: zeros and minus infinity."""
