@@ -3,6 +3,7 @@
  * C entry points of all of it (include/kmx.h, kmx_cache4_*). The attention that reads it is in cache4_attend_impl.h.
  */
 #include "cache4.h"
+#include "cache4_keys.h"
 
 #include <cmath>
 #include <cstring>
@@ -384,13 +385,6 @@ struct Select4 {
 	bool bf16, vec;
 };
 
-/* floats in the order of unsigned words */
-__device__ __forceinline__ uint32_t ordered(float v)
-{
-	const uint32_t u = __builtin_bit_cast(uint32_t, v);
-	return u & 0x80000000u ? ~u : u | 0x80000000u;
-}
-
 /*
  * The scores of pages: the bound on q . k over a page, in 8 bits. 16 rows of queries (tokens of one head of the cache, their query heads side by
  * side) are 8-bit columns of v_mfma_i32_16x16x64_i8: the positive parts against the largest values, the negative ones against the smallest.
@@ -479,8 +473,7 @@ struct Scorer4 {
 	__device__ __forceinline__ bool writes(int r) const { return token_there && ((col & (a.span - 1))) < 4 && ((uint32_t)r & (a.span - 1) & 3) == (col & (a.span - 1) & 3); }
 	__device__ __forceinline__ uint32_t key(uint32_t page, uint32_t pages, int best, float scale, bool known) const
 	{
-		const bool forced = page < a.first || page + a.last >= pages;
-		return ordered(forced ? __builtin_inff() : known ? (float)best * scale + 0.0f : -__builtin_inff()); /* (+ 0: one zero) */
+		return page_key(page < a.first || page + a.last >= pages, known, best, scale);
 	}
 };
 
@@ -577,9 +570,9 @@ score4_kernel(Select4 a)
  * The `top` best of n keys, ascending. The keys' range is cut into 512 steps, whose numbers of keys tell the step with the threshold, that step again
  * into 512, until all of a step is wanted or its keys are equal (four passes over 8 bits each, whatever the keys, took 9 us for 1024 keys; this
  * mostly ends after one). Then one pass in the order of the pages keeps what lies above the threshold and as many at it as are left, the lowest
- * first. All threads of the work-group come here, `threads` of them (whole wavefronts, thread `tid` of them) to each list.
+ * first. All threads of the work-group come here, `threads` of them (whole wavefronts, thread `tid` of them) to each list. Pages that are always taken
+ * are no more than `top` (page_key gives their key to no score); nothing is written behind the list whatever the keys.
  */
-constexpr uint32_t FORCED_KEY = 0xFF800000u; /* ordered(infinity) */
 struct ChooseLds { uint32_t histogram[512], low, high, forced, step[3]; }; /* of a list */
 template <typename KEY>
 __device__ __forceinline__ void choose_top(const KEY& key, uint32_t n, uint32_t top, int32_t* out, uint32_t tid, uint32_t threads, ChooseLds& lds, uint32_t* above, uint32_t* equal)
@@ -608,7 +601,7 @@ __device__ __forceinline__ void choose_top(const KEY& key, uint32_t n, uint32_t 
 	}
 	__syncthreads();
 	/* kept: the keys above `threshold`, and the first `rest` of those equal to it */
-	uint32_t low = lds.low, width = 0xFFFFFFFFu, rest = top - (all ? top : lds.forced), threshold = lds.high; /* the threshold lies in [low, low + width) */
+	uint32_t low = lds.low, width = 0xFFFFFFFFu, rest = top - (all ? top : min(lds.forced, top)), threshold = lds.high; /* the threshold lies in [low, low + width) */
 	int shift = all || lds.high <= low ? 0 : 32 - __clz(lds.high - low);
 	shift = shift > 9 ? shift - 9 : 0;
 	bool done = all || rest == 0;
@@ -677,7 +670,8 @@ __device__ __forceinline__ void choose_top(const KEY& key, uint32_t n, uint32_t 
 		const bool is_above = p < to && k > threshold, is_equal = p < to && k == threshold;
 		const uint64_t ballot_above = __ballot(is_above), ballot_equal = __ballot(is_equal);
 		const uint32_t my_eq = ties + __popcll(ballot_equal & below), my_gt = written + __popcll(ballot_above & below);
-		if (is_above || (is_equal && my_eq < rest)) out[my_gt + min(my_eq, rest)] = (int32_t)p;
+		const uint32_t at = my_gt + min(my_eq, rest);
+		if ((is_above || (is_equal && my_eq < rest)) && at < top) out[at] = (int32_t)p;
 		written += __popcll(ballot_above);
 		ties += __popcll(ballot_equal);
 	}

@@ -474,7 +474,7 @@ int kmx_cache4_bound(const kmx_cache4* cache, const int32_t* pages, const int32_
  * table), ascending, -1 behind the last. Of the pages with a token the query sees: the `first` first and `last` last ones, then those of the
  * best score, the lower number of two as good. score = max over the query heads of the head of sum_c max(q_c hi_c, q_c lo_c), the bound on
  * q . k over the page, in 8 bits: q_c = rint(q (1/m 127)) in floats, m its largest magnitude over these heads, hi and lo as kept; a whole number, times the page's
- * scale in floats. Queries F16 or BF16, element (token, head, channel) as above.
+ * scale in floats, held to the finite numbers (NaN, from bounds that nobody made: the lowest of them). Queries F16 or BF16, element (token, head, channel) as above.
  */
 int kmx_cache4_select(const kmx_cache4* cache, const kmx_cache4_batch* batch, int type, const void* q, size_t q_token_stride, size_t q_head_stride,
                       int32_t* chosen, uint32_t top, uint32_t first, uint32_t last, int causal);
