@@ -118,14 +118,27 @@ template <int J>
 constexpr int values_words() { return J > 4 * ((J + 3) / 4) ? J : 4 * ((J + 3) / 4); } /* words of codes a lane holds: J of keys, or 4 for each of its pairs of channels */
 
 /* What queries of that largest magnitude are multiplied with to become halves of at most 2 in magnitude (bf16 has more exponents), with the sign
- * of the scale; *row_scale takes a score of theirs to the exponent of 2 */
+ * of the scale; *row_scale takes a score of theirs, below 2^26, to the exponent of 2, which stays a number: at most 2^100, where any two scores that
+ * differ do so by far more than a softmax tells from infinity */
 __device__ __forceinline__ float query_scale(float scale, float largest, float* row_scale)
 {
 	int power = (int)(__builtin_bit_cast(uint32_t, largest) >> 23) - 127;
 	power = power < -126 ? 0 : power > 126 ? 126 : power;
 	const float by = __builtin_bit_cast(float, (uint32_t)(127 - power) << 23);
-	*row_scale = fmaxf(fabsf(scale) * 1.44269504088896341f * __builtin_bit_cast(float, (uint32_t)(127 + power) << 23), 1.2e-38f);
+	*row_scale = fminf(fmaxf(fabsf(scale) * 1.44269504088896341f * __builtin_bit_cast(float, (uint32_t)(127 + power) << 23), 1.2e-38f), 0x1p100f);
 	return scale > 0.0f ? by : scale < 0.0f ? -by : 0.0f;
+}
+
+/* What is added to row_scale times the scores so that the largest, m, becomes 0. One fused operation a score, whose error is that of m row_scale,
+ * 2^-24 of it: where that is no longer small, the scores of the row give m up themselves, exactly at the largest. */
+constexpr float FAR_SCORE = 1024.0f;
+template <typename LOWER>
+__device__ __forceinline__ float below_most(float m, float row_scale, const LOWER& lower)
+{
+	const float most = m == -__builtin_inff() ? 0.0f : m, base = -most * row_scale; /* (-inf: nothing seen yet) */
+	const bool far = fabsf(base) > FAR_SCORE;
+	if (__any(far)) lower(far ? most : 0.0f);
+	return far ? 0.0f : base;
 }
 
 /* 4 channels of an output row */
@@ -328,7 +341,10 @@ attend4_kernel(Attend4 a)
 			for (int c = 0; c < 2 * J; ++c) o[c] *= less;
 			m = now;
 		}
-		const float base = m == -__builtin_inff() ? 0.0f : -m * row_scale;
+		const float base = below_most(m, row_scale, [&](float most) {
+#pragma unroll
+			for (int e = 0; e < 16; ++e) sc[e] -= most;
+		});
 		half8v p[2];
 #pragma unroll
 		for (int e = 0; e < 16; ++e) {
@@ -760,7 +776,10 @@ __device__ __forceinline__ void many_unit(const Attend4& a, uint8_t* many, uint3
 				for (int j = 0; j < J; ++j) o[j] *= less;
 				m = now;
 			}
-			const float base = m == -__builtin_inff() ? 0.0f : -m * row_scale;
+			const float base = below_most(m, row_scale, [&](float most) {
+#pragma unroll
+				for (int t = 0; t < STEP; ++t) sc[t] -= most;
+			});
 			half8v p[2 * STEP];
 #pragma unroll
 			for (int e = 0; e < 16 * STEP; ++e) {

@@ -482,7 +482,8 @@ int kmx_cache4_select(const kmx_cache4* cache, const kmx_cache4_batch* batch, in
 /*
  * out[token][head] = sum_t p_t v_t, p = softmax over the tokens t that the query sees of scale * q . k_t; lse (may be null): the logarithm of the
  * softmax's sum, tokens x query_heads. A query that sees nothing gets zeros and minus infinity. chosen (may be null): only tokens of these pages,
- * lists as kmx_cache4_select writes them (distinct). Queries and outputs F16 or BF16; products of numbers of half precision, sums in floats.
+ * lists as kmx_cache4_select writes them (distinct). Queries and outputs F16 or BF16; products of numbers of half precision, sums in floats. Scores are
+ * floats, whatever their size (where they may come near 2^127, lse is only known to be large).
  */
 int kmx_cache4_attend(const kmx_cache4* cache, const kmx_cache4_batch* batch, int type, const void* q, size_t q_token_stride, size_t q_head_stride,
                       void* out, size_t out_token_stride, size_t out_head_stride, float* lse, float scale, int causal,
