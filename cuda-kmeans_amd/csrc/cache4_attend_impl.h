@@ -3,7 +3,7 @@
  *
  * For a row r (a query head of a token) that sees the tokens t < vis:  o_r = sum_t p_rt v_t / l_r,  p_rt = 2^(s_rt - m_r),
  * s_rt = scale log2(e) q_r . k_t,  m_r = max_t s_rt,  l_r = sum_t p_rt;  lse_r = ln 2 (m_r + log2 l_r). One pass over the cache with the running
- * maximum and sum; parts of the tokens (wavefronts, and work-groups where there are few rows) are joined at the end.
+ * maximum and sum; parts of the tokens (wavefronts, and work-groups where there are few rows) are joined at the end. (The kernels keep p and l times 2^15.)
  */
 #ifndef KMX_CACHE4_ATTEND_IMPL_H
 #define KMX_CACHE4_ATTEND_IMPL_H
@@ -129,16 +129,30 @@ __device__ __forceinline__ float query_scale(float scale, float largest, float* 
 	return scale > 0.0f ? by : scale < 0.0f ? -by : 0.0f;
 }
 
-/* What is added to row_scale times the scores so that the largest, m, becomes 0. One fused operation a score, whose error is that of m row_scale,
- * 2^-24 of it: where that is no longer small, the scores of the row give m up themselves, exactly at the largest. */
+/*
+ * Probabilities are rounded to half precision for their product with the values: 11 bits from 2^-14 on, none below 2^-25. They are taken times 2^15, so
+ * that the largest is as large as half precision allows for: then 11 bits reach down to 2^-29 of it and the last one to 2^-39, and what all
+ * tokens of a long row add up to below one that stands far out is there. Sums are of the same size; only lse takes the factor off.
+ */
+constexpr float RAISE = 15.0f, LOWERED = 0x1p-15f;
+
+/*
+ * What is added to row_scale times the scores so that the largest, m, becomes RAISE. One fused operation a score, whose error is that of m row_scale,
+ * 2^-24 of it: in rows where that is no longer small the scores give m up themselves, exactly at the largest. Whether a row of the wavefront is
+ * such a one is found where a maximum rises (found for each tile: 533 us of the many-rows kernel in place of 524).
+ */
 constexpr float FAR_SCORE = 1024.0f;
+__device__ __forceinline__ bool far_score(float m, float row_scale) { return m != -__builtin_inff() && fabsf(m * row_scale) > FAR_SCORE; } /* (-inf: nothing seen yet) */
 template <typename LOWER>
-__device__ __forceinline__ float below_most(float m, float row_scale, const LOWER& lower)
+__device__ __forceinline__ float below_most(float m, float row_scale, bool any_far, const LOWER& lower)
 {
-	const float most = m == -__builtin_inff() ? 0.0f : m, base = -most * row_scale; /* (-inf: nothing seen yet) */
-	const bool far = fabsf(base) > FAR_SCORE;
-	if (__any(far)) lower(far ? most : 0.0f);
-	return far ? 0.0f : base;
+	float base = m == -__builtin_inff() ? RAISE : fmaf(-m, row_scale, RAISE);
+	if (any_far) {
+		const bool far = far_score(m, row_scale);
+		lower(far ? m : 0.0f);
+		base = far ? RAISE : base;
+	}
+	return base;
 }
 
 /* 4 channels of an output row */
@@ -257,6 +271,7 @@ attend4_kernel(Attend4 a)
 	};
 
 	float m = -__builtin_inff(), l = 0.0f; /* of the lane's row: the maximum of all its lanes, the sum of the lane's own tokens */
+	bool any_far = false; /* rows of the wavefront with scores far from zero */
 	f32x4 o[2 * J];
 #pragma unroll
 	for (int c = 0; c < 2 * J; ++c) o[c] = f32x4{ 0.0f, 0.0f, 0.0f, 0.0f };
@@ -340,8 +355,9 @@ attend4_kernel(Attend4 a)
 #pragma unroll
 			for (int c = 0; c < 2 * J; ++c) o[c] *= less;
 			m = now;
+			any_far = __any(far_score(m, row_scale));
 		}
-		const float base = below_most(m, row_scale, [&](float most) {
+		const float base = below_most(m, row_scale, any_far, [&](float most) {
 #pragma unroll
 			for (int e = 0; e < 16; ++e) sc[e] -= most;
 		});
@@ -350,7 +366,7 @@ attend4_kernel(Attend4 a)
 		for (int e = 0; e < 16; ++e) {
 			const float v = exp2_(fmaf(sc[e], row_scale, base));
 			l += v;
-			p[e / 8][e % 8] = (_Float16)v; /* 11 bits: the error of a probability is below that of the result's type, and sums of them are kept in 32 */
+			p[e / 8][e % 8] = (_Float16)v; /* (the sum is that of the floats: see RAISE) */
 		}
 #pragma unroll
 		for (int j = 0; j < J; ++j) {
@@ -435,7 +451,7 @@ attend4_kernel(Attend4 a)
 			for (int r = 0; r < 4; ++r) v[r] = o[c][r] * by;
 			store_out4(a, to, 16 * c + 4 * kg, v);
 		}
-		if (kg == 0 && a.lse) a.lse[token * a.batch.query_heads + query_head] = sum == 0.0f ? -__builtin_inff() : (all * row_scale + log2f(sum)) * 0.693147180559945309f;
+		if (kg == 0 && a.lse) a.lse[token * a.batch.query_heads + query_head] = sum == 0.0f ? -__builtin_inff() : (all * row_scale + log2f(sum * LOWERED)) * 0.693147180559945309f;
 		return;
 	}
 
@@ -519,7 +535,7 @@ attend4_kernel(Attend4 a)
 		float v[4];
 		for (int i = 0; i < 4; ++i) v[i] = mine[i] * by;
 		store_out4(a, (char*)a.out + 2 * (token * a.out_token + query_head * a.out_head), 4 * (e % (D / 4)), v);
-		if (e % (D / 4) == 0 && a.lse) a.lse[token * a.batch.query_heads + query_head] = s1 == 0.0f ? -__builtin_inff() : (most[0][r] + log2f(s1)) * 0.693147180559945309f;
+		if (e % (D / 4) == 0 && a.lse) a.lse[token * a.batch.query_heads + query_head] = s1 == 0.0f ? -__builtin_inff() : (most[0][r] + log2f(s1 * LOWERED)) * 0.693147180559945309f;
 	}
 }
 
@@ -737,6 +753,7 @@ __device__ __forceinline__ void many_unit(const Attend4& a, uint8_t* many, uint3
 	};
 
 	float m = -__builtin_inff(), l = 0.0f;
+	bool any_far = false; /* rows of the wavefront with scores far from zero */
 	f32x16 o[J];
 #pragma unroll
 	for (int j = 0; j < J; ++j)
@@ -775,8 +792,9 @@ __device__ __forceinline__ void many_unit(const Attend4& a, uint8_t* many, uint3
 #pragma unroll
 				for (int j = 0; j < J; ++j) o[j] *= less;
 				m = now;
+				any_far = __any(far_score(m, row_scale));
 			}
-			const float base = below_most(m, row_scale, [&](float most) {
+			const float base = below_most(m, row_scale, any_far, [&](float most) {
 #pragma unroll
 				for (int t = 0; t < STEP; ++t) sc[t] -= most;
 			});
@@ -823,7 +841,7 @@ __device__ __forceinline__ void many_unit(const Attend4& a, uint8_t* many, uint3
 				for (int r = 0; r < 4; ++r) v[r] = o[j][4 * e + r] * by;
 				store_out4(a, to, 32 * j + 8 * e + 4 * h, v);
 			}
-		if (h == 0 && a.lse) a.lse[(size_t)(seq.first + token) * a.batch.query_heads + query_head] = l == 0.0f ? -__builtin_inff() : (m * row_scale + log2f(l)) * 0.693147180559945309f;
+		if (h == 0 && a.lse) a.lse[(size_t)(seq.first + token) * a.batch.query_heads + query_head] = l == 0.0f ? -__builtin_inff() : (m * row_scale + log2f(l * LOWERED)) * 0.693147180559945309f;
 		return;
 	}
 
@@ -933,7 +951,7 @@ join4_kernel(Attend4 a)
 		float v[4];
 		for (int e = 0; e < 4; ++e) v[e] = mine[e] * by;
 		store_out4(a, (char*)a.out + 2 * (to_token * a.out_token + to_head * a.out_head), 4 * at, v);
-		if (at == 0 && a.lse) a.lse[to_token * a.batch.query_heads + to_head] = sum == 0.0f ? -__builtin_inff() : (top + log2f(sum)) * 0.693147180559945309f;
+		if (at == 0 && a.lse) a.lse[to_token * a.batch.query_heads + to_head] = sum == 0.0f ? -__builtin_inff() : (top + log2f(sum * LOWERED)) * 0.693147180559945309f;
 	}
 }
 

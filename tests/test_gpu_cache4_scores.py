@@ -1,8 +1,8 @@
-"""Attention over the 4-bit cache where scores are far from zero, against its definition in 64 bits (-m gpu)."""
+"""Attention over the 4-bit cache where scores are far from zero or far apart, against its definition in 64 bits (-m gpu)."""
 import numpy as np
 import pytest
 
-from test_gpu_cache4 import BF16, F16, UNIT, Cache, Queries
+from test_gpu_cache4 import BF16, F16, UNIT, Cache, Queries, device
 
 pytestmark = pytest.mark.gpu
 
@@ -39,3 +39,49 @@ def test_scores_far_from_zero(km, gpu, length, counts, kind, loud, scale):
             else:
                 assert lse[i, 0, g] > 1e29
     assert clear >= counts  # half of the rows at least
+
+
+SEQUENCES, TOKENS = 128, 65536
+
+
+@pytest.mark.parametrize("kind", [F16, BF16])
+@pytest.mark.parametrize("queries", [1, 17])  # 16 rows and 256 a work-group, all tokens in one part
+@pytest.mark.parametrize("behind", [12.0, 15.0, 17.4])
+def test_one_token_far_above_the_others(km, gpu, kind, queries, behind):
+    """One token holds nearly all of the softmax and has a value of zero: what all the others add up to is the result. Off by the roundings of the type, of a
+    probability (2^-11 of it, 2^-40 at least), of scores and of sums in 24 bits."""
+    rng = np.random.default_rng(queries)
+    heads, group, dim, page = 4, 4, 32, 256
+    c = Cache(km, rng, heads, dim, page, TOKENS // page)
+    along = np.where(rng.random(dim) < 0.5, -1.0, 1.0)
+    scale = 1 / np.sqrt(dim)
+    keys, values = 0.3 * rng.normal(size=(TOKENS, heads, dim)), 1 + 0.3 * rng.normal(size=(TOKENS, heads, dim))
+    sink = 1000
+    keys[sink], values[sink] = along * behind / (scale * dim), 0
+    c.write(F16, np.float32(keys), np.float32(values), np.arange(TOKENS))
+    one = Queries(km, rng, c, [TOKENS], [queries], group, kind)  # (its table is replaced: all sequences look at the same pages in order)
+    one.table = np.arange(TOKENS // page, dtype=np.int32)[None]
+    q = np.float32(along + 0.1 * rng.normal(size=(queries, heads, group, dim)))
+    s = Queries(km, rng, c, [0] * SEQUENCES, [queries] * SEQUENCES, group, kind)
+    s.q = np.tile(q.astype(np.float16).astype(np.float32) if kind == F16 else (q.view(np.uint32) & 0xFFFF0000).view(np.float32), (SEQUENCES, 1, 1, 1))
+    table = np.tile(one.table, (SEQUENCES, 1))
+    s.batch = km.Cache4Batch(SEQUENCES, heads * group, SEQUENCES * queries, queries, TOKENS, device(km, s.starts), device(km, np.full(SEQUENCES, TOKENS, np.int32)),
+                             device(km, table), table.shape[1])
+    got, lse = s.attend()
+    assert np.array_equal(got, np.tile(got[:queries], (SEQUENCES, 1, 1, 1))) and np.array_equal(lse, np.tile(lse[:queries], (SEQUENCES, 1, 1)))
+    for i in range(queries):
+        n = TOKENS - queries + i + 1
+        for h in range(heads):
+            k, v = c.k[:n, h].astype(np.float64), c.v[:n, h].astype(np.float64)
+            x = s.q[i, h].astype(np.float64)
+            score = scale * x @ k.T
+            top = score.max(-1, keepdims=True)
+            p = np.exp(score - top)
+            assert np.all(p.argmax(-1) == sink)
+            total = p.sum(-1, keepdims=True)
+            want = p @ v / total
+            delta = ((dim + 16) * 2.0 ** -23 * (scale * np.abs(x) @ np.abs(k).T).max(-1) + 2.0 ** -22 * np.abs(score).max(-1))[:, None]
+            terms = (n + 64) * 2.0 ** -24
+            off = UNIT[kind] * np.abs(want) + (2.0 ** -11 + 2 * delta + 2 * terms) * (p @ np.abs(v) / total) + n * 2.0 ** -40 * np.abs(v).max() / total
+            assert np.all(np.abs(got[i, h] - want) <= off), (np.abs(got[i, h] - want) / off).max()
+            assert np.all(np.abs(lse[i, h] - (top + np.log(total))[:, 0]) <= delta[:, 0] + terms + 2.0 ** -21 * (1 + np.abs(lse[i, h])))
