@@ -139,7 +139,7 @@ constexpr float RAISE = 15.0f, LOWERED = 0x1p-15f;
 /*
  * What is added to row_scale times the scores so that the largest, m, becomes RAISE. One fused operation a score, whose error is that of m row_scale,
  * 2^-24 of it: in rows where that is no longer small the scores give m up themselves, exactly at the largest. Whether a row of the wavefront is
- * such a one is found where a maximum rises (found for each tile: 533 us of the many-rows kernel in place of 524).
+ * such a one is found where a maximum rises (found for each tile: 533 us of the many-rows kernel in place of 524; see also EXACT there).
  */
 constexpr float FAR_SCORE = 1024.0f;
 __device__ __forceinline__ bool far_score(float m, float row_scale) { return m != -__builtin_inff() && fabsf(m * row_scale) > FAR_SCORE; } /* (-inf: nothing seen yet) */
@@ -645,6 +645,9 @@ __device__ __forceinline__ void many_unit(const Attend4& a, uint8_t* many, uint3
 {
 	constexpr uint32_t D = 32 * J, KROW = 2 * D + 16, VROW = 144, TILE = 64 * KROW + D * VROW;
 	constexpr int STEP = (J <= 5 ? 2 : 1); /* times 32 tokens of a tile: scores held at a time */
+	/* scores always give the maximum up themselves (see below_most) where registers go to memory anyway, and a branch costs more of them (2 x 1024 queries, 256
+	 * channels: 1328 us, 1475 with the branch; 224: 947 and 954; 192: 762 and 747, 128: 550 and 540) */
+	constexpr bool EXACT = J > 6;
 	uint32_t thread = threadIdx.x;
 	asm volatile("" : "+v"(thread)); /* addresses that follow from it are made anew for each unit, not kept from one to the next */
 	const uint32_t wave = (uint32_t)__builtin_amdgcn_readfirstlane((int)(thread / WAVE)), lane = thread % WAVE, n32 = lane % 32, h = lane / 32;
@@ -752,7 +755,7 @@ __device__ __forceinline__ void many_unit(const Attend4& a, uint8_t* many, uint3
 		}
 	};
 
-	float m = -__builtin_inff(), l = 0.0f;
+	float m = -__builtin_inff(), l = 0.0f, base = RAISE;
 	bool any_far = false; /* rows of the wavefront with scores far from zero */
 	f32x16 o[J];
 #pragma unroll
@@ -786,18 +789,25 @@ __device__ __forceinline__ void many_unit(const Attend4& a, uint8_t* many, uint3
 			for (int e = 1; e < 16 * STEP; ++e) top = fmaxf(top, sc[e / 16][e % 16]);
 			top = fmaxf(top, __shfl_xor(top, 32));
 			const float now = fmaxf(m, top);
-			if (__any(now > m)) {
+			if (any_far || __any(now > m)) {
 				const float less = m == now ? 1.0f : exp2_((m - now) * row_scale);
 				l *= less;
 #pragma unroll
 				for (int j = 0; j < J; ++j) o[j] *= less;
 				m = now;
-				any_far = __any(far_score(m, row_scale));
+				if constexpr (!EXACT) {
+					any_far = __any(far_score(m, row_scale));
+					base = below_most(m, row_scale, any_far, [&](float most) {
+#pragma unroll
+						for (int t = 0; t < STEP; ++t) sc[t] -= most;
+					});
+				}
 			}
-			const float base = below_most(m, row_scale, any_far, [&](float most) {
+			if constexpr (EXACT) {
+				const float most = m == -__builtin_inff() ? 0.0f : m;
 #pragma unroll
 				for (int t = 0; t < STEP; ++t) sc[t] -= most;
-			});
+			}
 			half8v p[2 * STEP];
 #pragma unroll
 			for (int e = 0; e < 16 * STEP; ++e) {
