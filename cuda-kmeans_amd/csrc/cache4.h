@@ -15,6 +15,7 @@
 #define KMX_CACHE4_H
 
 #include "kmx_internal.h"
+#include "cache4_plan.h"
 
 namespace kmx {
 
@@ -221,16 +222,7 @@ struct Attend4 {
 	bool joined; /* parts of many rows are left to the kernel that joins them */
 	float* partial; uint32_t* tickets;
 };
-constexpr uint32_t MOST_PARTS = 128; /* of the tokens of a row */
-constexpr uint32_t TICKETS = 8192;   /* units (sequence, head, tile of rows) of a call that takes its tokens in parts */
-/* launch shape: tiles of 16 rows, parts of the tokens, tiles of 64 tokens a part (cache4.hip) */
-struct Plan4 { uint32_t row_tiles, splits, tiles_per_split; bool many, joined; }; /* many: splits is the number of work-groups; tiles_per_split 0: shares */
-constexpr uint32_t MANY_ROWS = 64;    /* rows of a head: above it 256 a work-group (2 sequences of up to 16384 tokens, 8 heads, 64 rows: 39 us by 16, 41 by 256; 128 rows: 62 and 44) */
-constexpr uint32_t MANY_LEAST = 4, MANY_COST = 8; /* tiles of a part at least; tiles that a part costs beside its own (2, 4, 8: 128.7, 128.4, 123.6 us for 54 units of 178 tiles) */
-constexpr uint32_t SHARE_LEAST = 64; /* tiles for each work-group of a call divided in shares (16 tiles: 57 us in parts, 62 in shares; 128 and more: see plan_attend4) */
-Plan4 plan_attend4(uint32_t J, const Batch4& b, uint32_t heads, uint32_t max_length, uint32_t page_shift, uint32_t top, const DeviceInfo& dev);
-template <int J> int launch_attend4(Attend4 a, uint32_t max_length, Workspace* ws, const DeviceInfo& dev);
-size_t attend4_partial_floats(uint32_t J, const Batch4& b, uint32_t heads, uint32_t max_length, uint32_t page_shift, uint32_t top, const DeviceInfo& dev);
+template <int J> int launch_attend4(Attend4 a, const Plan4& plan, Workspace* ws);
 
 } // namespace kmx
 

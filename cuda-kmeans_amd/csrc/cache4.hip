@@ -736,61 +736,6 @@ select4_kernel(Select4 a, uint32_t stride)
 	choose_top([&](uint32_t p) { return from[p]; }, n, a.top, out, tid, threads, choose[list], above + list * (threads / WAVE), equal + list * (threads / WAVE));
 }
 
-/* ---------------------------------------------------------------- launch shapes of the attention - */
-
-/*
- * Tiles of 16 rows, or of 256 where there are many, and how many parts the tokens are taken in.
- * 16 rows: two work-groups a compute unit in all, none below one tile a wavefront (64 sequences of 8192 tokens, 8 heads: 124 us in one part, 133 in
- * four; one sequence of 131072: 32 us with one work-group a unit, 28.7 with two, 29.4 with four).
- * 256 rows: lengths are known on the device only. Several sequences whose lengths may differ by much are divided in equal shares there, one for each
- * work-group that the chip holds (2 x 1024 queries over 16384 and fewer tokens, 8 heads: of 128 channels 568 -> 521 us, 64: 375 -> 325, 256: 1598 ->
- * 1475; 5 x 700 over up to 9000: 505 -> 463; but equal lengths 588 -> 622). Not one sequence (323 -> 347), nor where units are many and fill the chip
- * as they come (1024 units: 477 -> 534), nor short ones: there as many parts as make the rounds of work-groups short.
- */
-Plan4 plan_attend4(uint32_t J, const Batch4& b, uint32_t heads, uint32_t max_length, uint32_t page_shift, uint32_t top, const DeviceInfo& dev)
-{
-	Plan4 plan;
-	const uint64_t rows = (uint64_t)b.max_queries * b.group;
-	plan.many = !top && rows > MANY_ROWS;
-	plan.row_tiles = top ? b.max_queries * ((b.group + 15) / 16) : (uint32_t)(plan.many ? (rows + 255) / 256 : (rows + 15) / 16);
-	const uint64_t tokens = top ? (uint64_t)top << page_shift : max_length, units = (uint64_t)b.sequences * heads * plan.row_tiles;
-	const uint32_t tiles = (uint32_t)((tokens + 63) / 64);
-	plan.joined = false;
-	if (plan.many) {
-		const uint64_t slots = (J <= 2 ? 2 : 1) * (uint64_t)dev.compute_units; /* work-groups on the chip at a time */
-		if (b.sequences > 1 && units <= 2 * slots && units * tiles >= SHARE_LEAST * slots && rows <= 0x7FFFFF00u && units * tiles <= 0x7FFFFFFFu) {
-			plan.splits = (uint32_t)slots;
-			plan.tiles_per_split = 0;
-			plan.joined = true;
-			return plan;
-		}
-		uint64_t best = ~0ull, parts = 1;
-		for (uint64_t p = 1; p <= 16 && (p == 1 || p * MANY_LEAST <= tiles); ++p) {
-			const uint64_t time = (units * p + slots - 1) / slots * ((tiles + p - 1) / p + MANY_COST);
-			if (time < best) { best = time; parts = p; }
-		}
-		plan.tiles_per_split = tiles ? (uint32_t)((tiles + parts - 1) / parts) : 1;
-		plan.splits = (uint32_t)(units * parts);
-		plan.joined = parts > 1;
-		return plan;
-	}
-	uint64_t parts = (2 * dev.compute_units + units - 1) / (units ? units : 1);
-	if (parts > (tiles + 3) / 4) parts = (tiles + 3) / 4;
-	if (parts > MOST_PARTS) parts = MOST_PARTS;
-	if (parts == 0 || units > TICKETS) parts = 1;
-	plan.tiles_per_split = tiles ? (uint32_t)(((tiles + parts - 1) / parts + 3) / 4 * 4) : 4; /* a tile for each wavefront */
-	plan.splits = tiles ? (tiles + plan.tiles_per_split - 1) / plan.tiles_per_split : 1;
-	return plan;
-}
-
-size_t attend4_partial_floats(uint32_t J, const Batch4& b, uint32_t heads, uint32_t max_length, uint32_t page_shift, uint32_t top, const DeviceInfo& dev)
-{
-	const Plan4 plan = plan_attend4(J, b, heads, max_length, page_shift, top, dev);
-	const size_t units = (size_t)b.sequences * heads * plan.row_tiles;
-	if (plan.many) return plan.joined ? 2 * (size_t)plan.splits * (256 * (32 * J + 2)) + 2 * units : 0; /* two parts a work-group, two words a unit */
-	return plan.splits > 1 ? units * plan.splits * (16 * (32 * J + 2)) : 0;
-}
-
 } // namespace kmx
 
 using namespace kmx;
@@ -879,6 +824,15 @@ static int reserve_cache4(const char* who, Workspace* ws, size_t floats)
 	if (recording_graph()) scratch_recorded();
 	const int rc = reserve_tickets(ws, TICKETS);
 	return rc ? rc : reserve_partials(ws, floats);
+}
+
+/* the numbers of a call that decide how it is launched */
+static Shape4 shape_of(const kmx_cache4* cache, const kmx_cache4_batch* b, uint32_t table_stride, uint32_t top, const DeviceInfo& dev)
+{
+	uint32_t shift = 4;
+	while ((1u << shift) < cache->page_tokens) ++shift;
+	const uint64_t most = (uint64_t)table_stride << shift;
+	return Shape4{ cache->dim / 32, cache->heads, b->query_heads / cache->heads, b->sequences, b->max_queries, b->max_length < most ? b->max_length : (uint32_t)most, shift, top, dev.compute_units };
 }
 
 static uint32_t table_pages(const kmx_cache4_batch* b, uint32_t page_tokens)
@@ -1062,28 +1016,28 @@ int kmx_cache4_attend(const kmx_cache4* cache, const kmx_cache4_batch* batch, in
 	a.scale = scale;
 	a.bf16 = type == KMX_BF16;
 	a.vec = aligned_rows(q, q_token_stride, q_head_stride, 2) && aligned_rows(out, out_token_stride, out_head_stride, 2);
-	const uint64_t most = (uint64_t)batch->table_stride << a.cache.page_shift;
-	const uint32_t max_length = batch->max_length < most ? batch->max_length : (uint32_t)most;
 	const DeviceInfo* dev = nullptr;
 	rc = device_info(&dev);
 	if (rc) return rc;
+	const Plan4 plan = plan_attend4(shape_of(cache, batch, a.batch.table_stride, a.top, *dev));
+	if (plan.units >= MOST_UNITS) return fail(KMX_ERR_UNSUPPORTED, "kmx_cache4_attend: too many queries for one call");
 	Workspace* ws = nullptr;
 	rc = workspace(&ws);
 	if (rc) return rc;
-	const size_t floats = attend4_partial_floats(cache->dim / 32, a.batch, a.cache.heads, max_length, a.cache.page_shift, a.top, *dev);
+	const size_t floats = plan_floats(plan, cache->dim / 32);
 	if (floats) {
 		rc = reserve_cache4("kmx_cache4_attend", ws, floats);
 		if (rc) return rc;
 	}
 	switch (cache->dim / 32) {
-	case 1: return launch_attend4<1>(a, max_length, ws, *dev);
-	case 2: return launch_attend4<2>(a, max_length, ws, *dev);
-	case 3: return launch_attend4<3>(a, max_length, ws, *dev);
-	case 4: return launch_attend4<4>(a, max_length, ws, *dev);
-	case 5: return launch_attend4<5>(a, max_length, ws, *dev);
-	case 6: return launch_attend4<6>(a, max_length, ws, *dev);
-	case 7: return launch_attend4<7>(a, max_length, ws, *dev);
-	default: return launch_attend4<8>(a, max_length, ws, *dev);
+	case 1: return launch_attend4<1>(a, plan, ws);
+	case 2: return launch_attend4<2>(a, plan, ws);
+	case 3: return launch_attend4<3>(a, plan, ws);
+	case 4: return launch_attend4<4>(a, plan, ws);
+	case 5: return launch_attend4<5>(a, plan, ws);
+	case 6: return launch_attend4<6>(a, plan, ws);
+	case 7: return launch_attend4<7>(a, plan, ws);
+	default: return launch_attend4<8>(a, plan, ws);
 	}
 }
 
@@ -1102,14 +1056,10 @@ int kmx_cache4_reserve(const kmx_cache4* cache, const kmx_cache4_batch* batch, u
 	Workspace* ws = nullptr;
 	rc = workspace(&ws);
 	if (rc) return rc;
-	uint32_t shift = 4;
-	while ((1u << shift) < cache->page_tokens) ++shift;
-	const Batch4 b{ nullptr, nullptr, nullptr, batch->sequences, batch->tokens, batch->max_queries, batch->table_stride, batch->max_length, batch->query_heads / cache->heads, batch->query_heads, true };
-	const uint64_t most = (uint64_t)batch->table_stride << shift;
-	const uint32_t max_length = batch->max_length < most ? batch->max_length : (uint32_t)most;
-	size_t floats = attend4_partial_floats(cache->dim / 32, b, cache->heads, max_length, shift, 0, *dev);
+	const uint32_t J = cache->dim / 32;
+	size_t floats = plan_floats(plan_attend4(shape_of(cache, batch, batch->table_stride, 0, *dev)), J);
 	if (top) {
-		const size_t sparse = attend4_partial_floats(cache->dim / 32, b, cache->heads, max_length, shift, top, *dev);
+		const size_t sparse = plan_floats(plan_attend4(shape_of(cache, batch, batch->table_stride, top, *dev)), J);
 		const size_t keys = (size_t)batch->tokens * cache->heads * batch->table_stride;
 		if (sparse > floats) floats = sparse;
 		if (keys > floats) floats = keys;

@@ -641,7 +641,7 @@ __device__ __forceinline__ Share4 share_of(const Attend4& a, uint32_t g)
  */
 template <int J>
 __device__ __forceinline__ void many_unit(const Attend4& a, uint8_t* many, uint32_t (*blocks_there)[4], uint32_t entry, uint32_t head, uint32_t begin, uint32_t until,
-                                          bool whole, uint32_t parts)
+                                          bool whole, uint32_t parts, uint32_t slot)
 {
 	constexpr uint32_t D = 32 * J, KROW = 2 * D + 16, VROW = 144, TILE = 64 * KROW + D * VROW;
 	constexpr int STEP = (J <= 5 ? 2 : 1); /* times 32 tokens of a tile: scores held at a time */
@@ -839,7 +839,7 @@ __device__ __forceinline__ void many_unit(const Attend4& a, uint8_t* many, uint3
 	l += __shfl_xor(l, 32);
 
 	if (a.joined && begin == 0 && threadIdx.x == 0) /* for the join: the unit's first share, and how many it lies in */
-		((uint2*)(a.partial + (size_t)2 * a.splits * (256 * (D + 2))))[entry * a.cache.heads + head] = uint2{ blockIdx.x, parts };
+		((uint2*)(a.partial + (size_t)(a.tiles_per_split ? 1 : 2) * a.splits * (256 * (D + 2))))[entry * a.cache.heads + head] = uint2{ blockIdx.x, parts };
 	if (!there) return;
 	if (whole) {
 		const float by = l > 0.0f ? 1.0f / l : l == l ? 0.0f : l;
@@ -856,7 +856,7 @@ __device__ __forceinline__ void many_unit(const Attend4& a, uint8_t* many, uint3
 	}
 
 	/* a part of the tokens: [256][D] sums, then [256] pairs of maximum and sum, for join4_kernel */
-	float* const to = a.partial + (size_t)(2 * blockIdx.x + (begin == 0)) * (256 * (D + 2));
+	float* const to = a.partial + (size_t)slot * (256 * (D + 2));
 	const uint32_t r = 32 * wave + n32;
 #pragma unroll
 	for (int j = 0; j < J; ++j)
@@ -876,7 +876,7 @@ attend4_many_kernel(Attend4 a)
 		const uint32_t weight = many_tiles(a, entry / a.row_tiles, entry % a.row_tiles), begin = part * a.tiles_per_split;
 		if (begin >= weight) return;
 		const uint32_t parts = (weight + a.tiles_per_split - 1) / a.tiles_per_split;
-		many_unit<J>(a, many, blocks_there, entry, unit % heads, begin, min(weight, begin + a.tiles_per_split), parts == 1, parts);
+		many_unit<J>(a, many, blocks_there, entry, unit % heads, begin, min(weight, begin + a.tiles_per_split), parts == 1, parts, blockIdx.x);
 	} else {
 		__shared__ Share4 share; /* (in registers it would be there through all the work) */
 		const Share4 mine = share_of(a, blockIdx.x);
@@ -894,7 +894,7 @@ attend4_many_kernel(Attend4 a)
 			const bool whole = begin == 0 && until == weight;
 			uint32_t parts = 1;
 			if (!whole && begin == 0) parts = share_with(share.total, share.to - left + weight - 1, share.shares) - blockIdx.x + 1;
-			if (weight) many_unit<J>(a, many, blocks_there, entry, head, begin, until, whole, parts);
+			if (weight) many_unit<J>(a, many, blocks_there, entry, head, begin, until, whole, parts, 2 * blockIdx.x + (begin == 0));
 			if (!shared) {
 				const uint32_t next = entry * heads + head + gridDim.x;
 				entry = next / heads;
@@ -927,14 +927,16 @@ join4_kernel(Attend4 a)
 	const uint64_t all_rows = (uint64_t)seq.queries * a.batch.group, first_row = (uint64_t)(entry % a.row_tiles) * 256;
 	if (first_row >= all_rows) return;
 	const uint32_t rows = (uint32_t)min((uint64_t)256, all_rows - first_row);
-	const uint2 record = ((const uint2*)(a.partial + 2 * (size_t)a.splits * PART))[unit];
+	const uint32_t each = a.tiles_per_split ? 1 : 2; /* slots a work-group */
+	const uint2 record = ((const uint2*)(a.partial + each * (size_t)a.splits * PART))[unit];
 	const uint32_t parts = record.y, group = lane / LANES, at = lane % LANES;
 	if (parts <= 1) return; /* written where it belongs */
-	const float* left = a.partial + 2 * (size_t)record.x * PART; /* the first part is the second one of its work-group, the others are first ones */
-	const size_t step = (a.tiles_per_split ? 2 * (size_t)a.batch.sequences * a.row_tiles * a.cache.heads : 2) * PART; /* from a part's work-group to the next one's */
+	/* of shares the first part is the second one of its work-group, the others are first ones */
+	const float* left = a.partial + each * (size_t)record.x * PART;
+	const size_t first = (each - 1) * PART, step = (a.tiles_per_split ? (size_t)a.batch.sequences * a.row_tiles * a.cache.heads : 2) * PART; /* from a part's work-group to the next one's */
 	for (uint32_t r = blockIdx.x % JOIN_GROUPS * 4 + wave; r < rows; r += 4 * JOIN_GROUPS) {
 		float top = -__builtin_inff();
-		for (uint32_t p = lane; p < parts; p += WAVE) top = fmaxf(top, left[(p ? p * step : PART) + 256 * D + 2 * r]);
+		for (uint32_t p = lane; p < parts; p += WAVE) top = fmaxf(top, left[(p ? p * step : first) + 256 * D + 2 * r]);
 		for (int d = 1; d < WAVE; d *= 2) top = fmaxf(top, __shfl_xor(top, d));
 		const float lowest = top == -__builtin_inff() ? 0.0f : top;
 		float sum = 0.0f;
@@ -942,7 +944,7 @@ join4_kernel(Attend4 a)
 		if (group < GROUPS)
 #pragma unroll 4
 			for (uint32_t p = group; p < parts; p += GROUPS) {
-				const float* part = left + (p ? p * step : PART);
+				const float* part = left + (p ? p * step : first);
 				const float2 ml = *(const float2*)(part + 256 * D + 2 * r);
 				const float weight = exp2_(ml.x - lowest);
 				sum += ml.y * weight;
@@ -966,17 +968,14 @@ join4_kernel(Attend4 a)
 }
 
 template <int J>
-int launch_attend4(Attend4 a, uint32_t max_length, Workspace* ws, const DeviceInfo& dev)
+int launch_attend4(Attend4 a, const Plan4& plan, Workspace* ws)
 {
-	const Plan4 plan = plan_attend4(J, a.batch, a.cache.heads, max_length, a.cache.page_shift, a.top, dev);
 	a.row_tiles = plan.row_tiles;
 	a.splits = plan.splits;
 	a.tiles_per_split = plan.tiles_per_split;
 	a.joined = plan.joined;
 	a.partial = ws->partials;
 	a.tickets = ws->tickets;
-	const uint64_t units = (uint64_t)a.batch.sequences * a.cache.heads * a.row_tiles;
-	if (units >= 1u << 23) return fail(KMX_ERR_UNSUPPORTED, "kmx_cache4_attend: too many queries for one call");
 	if (plan.many) {
 		constexpr uint32_t bytes = 2 * (64 * (64 * J + 16) + 32 * J * 144);
 		static bool allowed = false; /* more LDS than a launch may ask for unannounced */
@@ -989,7 +988,7 @@ int launch_attend4(Attend4 a, uint32_t max_length, Workspace* ws, const DeviceIn
 		else KMX_LAUNCH_KERNEL((attend4_many_kernel<J, false>), dim3(a.splits), dim3(512), bytes, stream(), a);
 		KMX_LAUNCH_CHECK("attend4_many_kernel");
 		if (a.joined) {
-			KMX_LAUNCH_KERNEL((join4_kernel<J>), dim3((unsigned)(units * JOIN_GROUPS)), dim3(256), 0, stream(), a);
+			KMX_LAUNCH_KERNEL((join4_kernel<J>), dim3((unsigned)(plan.units * JOIN_GROUPS)), dim3(256), 0, stream(), a);
 			KMX_LAUNCH_CHECK("join4_kernel");
 		}
 		return KMX_OK;
