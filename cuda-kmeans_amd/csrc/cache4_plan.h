@@ -52,7 +52,8 @@ inline Plan4 plan_attend4(const Shape4& s)
 	plan.row_tiles = (uint32_t)row_tiles;
 	plan.splits = 1;
 	if (units >= MOST_UNITS) return plan; /* (refused) */
-	const uint64_t tokens = s.top ? (uint64_t)s.top << s.page_shift : s.max_length;
+	/* of a list no more pages are looked at than a sequence has (tiles_of) */
+	const uint64_t pages = ((uint64_t)s.max_length + (1u << s.page_shift) - 1) >> s.page_shift, tokens = s.top ? (s.top < pages ? s.top : pages) << s.page_shift : s.max_length;
 	const uint32_t tiles = (uint32_t)((tokens + 63) / 64);
 	if (plan.many) {
 		const uint64_t slots = (s.J <= 2 ? 2 : 1) * (uint64_t)s.compute_units; /* work-groups on the chip at a time */

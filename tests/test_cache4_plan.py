@@ -74,7 +74,7 @@ def test_parts_cover_all_tokens(plan):
             rows = b["queries"] * b["group"]
             want = b["queries"] * -(-b["group"] // 16) if top else -(-rows // 256) if rows > 64 else -(-rows // 16)
             assert p["row_tiles"] == want and p["units"] == b["sequences"] * b["heads"] * want and p["many"] == (not top and rows > 64)
-            tiles = -(-(top * b["page"] if top else b["length"]) // 64)
+            tiles = -(-(min(top, -(-b["length"] // b["page"])) * b["page"] if top else b["length"]) // 64)
             if p["many"] and p["tiles_per_split"] == 0:
                 assert p["splits"] in (UNITS, 2 * UNITS) and p["joined"]
                 assert p["floats"] == 2 * p["splits"] * 256 * (b["dim"] + 2) + 2 * p["units"]
@@ -87,3 +87,14 @@ def test_parts_cover_all_tokens(plan):
             else:
                 assert p["tiles_per_split"] * (parts - 1) < tiles and p["tiles_per_split"] % 4 == 0 and parts <= 128
                 assert p["floats"] == (p["units"] * parts * 16 * (b["dim"] + 2) if parts > 1 else 0)
+
+
+def test_lists_longer_than_any_sequence(plan):
+    """As many tokens as 32 bits do not count if the lists were full: what a sequence can have decides, in as many parts as there are work-groups for."""
+    for page in (16, 64, 256):
+        for top in ((1 << 30) - 1, 1 << 30, (1 << 30) + 1, (1 << 32) - 1):
+            for length in (1, 9000, 2 ** 31 - 1):
+                p, pages = plan(64, 1, 2, 1, 1, length, page, top), -(-length // page)
+                assert p["splits"] * p["tiles_per_split"] >= -(-pages * page // 64)
+                assert p == plan(64, 1, 2, 1, 1, length, page, pages)
+                assert (p["floats"] > 0) == (p["splits"] > 1) == (length > 1000)
