@@ -801,6 +801,9 @@ static int rows4(const char* who, bool write, const kmx_cache4* cache, int type,
 	return launch_rows4<__bf16>(write, a, J);
 }
 
+/* a bound may be as loose as it likes: no sequence has more queries than there are */
+static uint32_t most_queries(const kmx_cache4_batch* b) { return b->max_queries < b->tokens ? b->max_queries : b->tokens; }
+
 static int check_batch4(const char* who, const kmx_cache4* cache, const kmx_cache4_batch* batch, int causal, Batch4* out)
 {
 	if (!batch) return fail(KMX_ERR_INVALID_ARGUMENT, "%s: null batch", who);
@@ -811,7 +814,7 @@ static int check_batch4(const char* who, const kmx_cache4* cache, const kmx_cach
 		if (!batch->starts || !batch->lengths || (batch->table_stride && !batch->table)) return fail(KMX_ERR_INVALID_ARGUMENT, "%s: null device pointer in the batch", who);
 		if (batch->max_length > 0x7FFFFFFFu || batch->tokens > 0x7FFFFFFFu) return fail(KMX_ERR_UNSUPPORTED, "%s: lengths and tokens are counted in 31 bits", who);
 	}
-	*out = Batch4{ batch->starts, batch->lengths, batch->table, batch->sequences, batch->tokens, batch->max_queries, batch->table_stride,
+	*out = Batch4{ batch->starts, batch->lengths, batch->table, batch->sequences, batch->tokens, most_queries(batch), batch->table_stride,
 		       batch->max_length, batch->query_heads / cache->heads, batch->query_heads, causal != 0 };
 	if (cache->page_count == 0) out->table_stride = 0; /* nothing is cached */
 	return KMX_OK;
@@ -832,7 +835,7 @@ static Shape4 shape_of(const kmx_cache4* cache, const kmx_cache4_batch* b, uint3
 	uint32_t shift = 4;
 	while ((1u << shift) < cache->page_tokens) ++shift;
 	const uint64_t most = (uint64_t)table_stride << shift;
-	return Shape4{ cache->dim / 32, cache->heads, b->query_heads / cache->heads, b->sequences, b->max_queries, b->max_length < most ? b->max_length : (uint32_t)most, shift, top, dev.compute_units };
+	return Shape4{ cache->dim / 32, cache->heads, b->query_heads / cache->heads, b->sequences, most_queries(b), b->max_length < most ? b->max_length : (uint32_t)most, shift, top, dev.compute_units };
 }
 
 static uint32_t table_pages(const kmx_cache4_batch* b, uint32_t page_tokens)
@@ -942,11 +945,11 @@ int kmx_cache4_select(const kmx_cache4* cache, const kmx_cache4_batch* batch, in
 	 * sequences of 625 pages, 128 queries: 37 us against 41); two kernels where one work-group would read for long (1 x 1024 pages: 29 us against 34) */
 	const bool one = pages <= SELECT_PAGES, few = pages <= SELECT_FEW;
 	a.per = 1;
-	while (a.per < batch->max_queries && a.per < (one && few ? 4 : 8) && a.per * a.span < 16) a.per *= 2;
-	a.token_tiles = (batch->max_queries + a.per - 1) / a.per;
+	while (a.per < a.batch.max_queries && a.per < (one && few ? 4 : 8) && a.per * a.span < 16) a.per *= 2;
+	a.token_tiles = (a.batch.max_queries + a.per - 1) / a.per;
 	const uint64_t units = (uint64_t)batch->sequences * a.token_tiles * a.cache.heads;
-	if (batch->sequences > 65535 || batch->max_queries > 65535)
-		return fail(KMX_ERR_UNSUPPORTED, "kmx_cache4_select: %u sequences of %u queries are too many for one call", batch->sequences, batch->max_queries);
+	if (batch->sequences > 65535 || a.batch.max_queries > 65535)
+		return fail(KMX_ERR_UNSUPPORTED, "kmx_cache4_select: %u sequences of %u queries are too many for one call", batch->sequences, a.batch.max_queries);
 	if (one) {
 		const uint32_t stride = pages | 1, bytes = 4 * a.per * stride; /* at most 24.6 KB */
 		switch (cache->dim / 32) {
@@ -967,7 +970,7 @@ int kmx_cache4_select(const kmx_cache4* cache, const kmx_cache4_batch* batch, in
 	if (parts > (tiles + 1) / 2) parts = (tiles + 1) / 2;
 	a.chunk = (uint32_t)((tiles + parts - 1) / parts);
 	a.chunks = (tiles + a.chunk - 1) / a.chunk;
-	if ((uint64_t)a.token_tiles * a.chunks > 65535) return fail(KMX_ERR_UNSUPPORTED, "kmx_cache4_select: %u queries are too many for one call", batch->max_queries);
+	if ((uint64_t)a.token_tiles * a.chunks > 65535) return fail(KMX_ERR_UNSUPPORTED, "kmx_cache4_select: %u queries are too many for one call", a.batch.max_queries);
 	Workspace* ws = nullptr;
 	rc = workspace(&ws);
 	if (rc) return rc;
@@ -981,7 +984,7 @@ int kmx_cache4_select(const kmx_cache4* cache, const kmx_cache4_batch* batch, in
 #undef KMX_CASE
 	}
 	KMX_LAUNCH_CHECK("score4_kernel");
-	KMX_LAUNCH_KERNEL(choose4_kernel, dim3(a.cache.heads, batch->sequences, batch->max_queries), dim3(512), 0, stream(), a);
+	KMX_LAUNCH_KERNEL(choose4_kernel, dim3(a.cache.heads, batch->sequences, a.batch.max_queries), dim3(512), 0, stream(), a);
 	KMX_LAUNCH_CHECK("choose4_kernel");
 	return KMX_OK;
 }
