@@ -220,9 +220,9 @@ struct Attend4 {
 	bool bf16, vec;
 	uint32_t row_tiles, splits, tiles_per_split; /* (filled in by the launcher) */
 	bool joined; /* parts of many rows are left to the kernel that joins them */
-	float* partial; uint32_t* tickets;
+	float* partial; /* sums of parts, where there are any */
 };
-template <int J> int launch_attend4(Attend4 a, const Plan4& plan, Workspace* ws);
+template <int J> int launch_attend4(Attend4 a, const Plan4& plan);
 
 } // namespace kmx
 

@@ -820,13 +820,17 @@ static int check_batch4(const char* who, const kmx_cache4* cache, const kmx_cach
 	return KMX_OK;
 }
 
-static int reserve_cache4(const char* who, Workspace* ws, size_t floats)
+static int reserve_cache4(const char* who, size_t floats, float** partials)
 {
-	if ((floats > ws->partials_cap || !ws->tickets) && launches_recorded())
+	Workspace* ws = nullptr;
+	int rc = workspace(&ws);
+	if (rc) return rc;
+	if (floats > ws->partials_cap && launches_recorded())
 		return fail(KMX_ERR_INVALID_ARGUMENT, "%s: the call needs a larger work space, which cannot be allocated while it is recorded: kmx_cache4_reserve, or the same call once before", who);
 	if (recording_graph()) scratch_recorded();
-	const int rc = reserve_tickets(ws, TICKETS);
-	return rc ? rc : reserve_partials(ws, floats);
+	rc = reserve_partials(ws, floats);
+	*partials = ws->partials;
+	return rc;
 }
 
 /* the numbers of a call that decide how it is launched */
@@ -971,12 +975,10 @@ int kmx_cache4_select(const kmx_cache4* cache, const kmx_cache4_batch* batch, in
 	a.chunk = (uint32_t)((tiles + parts - 1) / parts);
 	a.chunks = (tiles + a.chunk - 1) / a.chunk;
 	if ((uint64_t)a.token_tiles * a.chunks > 65535) return fail(KMX_ERR_UNSUPPORTED, "kmx_cache4_select: %u queries are too many for one call", a.batch.max_queries);
-	Workspace* ws = nullptr;
-	rc = workspace(&ws);
+	float* keys = nullptr;
+	rc = reserve_cache4("kmx_cache4_select", (size_t)batch->tokens * a.cache.heads * batch->table_stride, &keys);
 	if (rc) return rc;
-	rc = reserve_cache4("kmx_cache4_select", ws, (size_t)batch->tokens * a.cache.heads * batch->table_stride);
-	if (rc) return rc;
-	a.keys = (uint32_t*)ws->partials;
+	a.keys = (uint32_t*)keys;
 	switch (cache->dim / 32) {
 #define KMX_CASE(N)                                                                                                      \
 	case N: KMX_LAUNCH_KERNEL((score4_kernel<N>), dim3(a.cache.heads, batch->sequences, a.token_tiles * a.chunks), dim3(256), 0, stream(), a); break;
@@ -1024,23 +1026,20 @@ int kmx_cache4_attend(const kmx_cache4* cache, const kmx_cache4_batch* batch, in
 	if (rc) return rc;
 	const Plan4 plan = plan_attend4(shape_of(cache, batch, a.batch.table_stride, a.top, *dev));
 	if (plan.units >= MOST_UNITS) return fail(KMX_ERR_UNSUPPORTED, "kmx_cache4_attend: too many queries for one call");
-	Workspace* ws = nullptr;
-	rc = workspace(&ws);
-	if (rc) return rc;
 	const size_t floats = plan_floats(plan, cache->dim / 32);
 	if (floats) {
-		rc = reserve_cache4("kmx_cache4_attend", ws, floats);
+		rc = reserve_cache4("kmx_cache4_attend", floats, &a.partial);
 		if (rc) return rc;
 	}
 	switch (cache->dim / 32) {
-	case 1: return launch_attend4<1>(a, plan, ws);
-	case 2: return launch_attend4<2>(a, plan, ws);
-	case 3: return launch_attend4<3>(a, plan, ws);
-	case 4: return launch_attend4<4>(a, plan, ws);
-	case 5: return launch_attend4<5>(a, plan, ws);
-	case 6: return launch_attend4<6>(a, plan, ws);
-	case 7: return launch_attend4<7>(a, plan, ws);
-	default: return launch_attend4<8>(a, plan, ws);
+	case 1: return launch_attend4<1>(a, plan);
+	case 2: return launch_attend4<2>(a, plan);
+	case 3: return launch_attend4<3>(a, plan);
+	case 4: return launch_attend4<4>(a, plan);
+	case 5: return launch_attend4<5>(a, plan);
+	case 6: return launch_attend4<6>(a, plan);
+	case 7: return launch_attend4<7>(a, plan);
+	default: return launch_attend4<8>(a, plan);
 	}
 }
 
@@ -1056,18 +1055,13 @@ int kmx_cache4_reserve(const kmx_cache4* cache, const kmx_cache4_batch* batch, u
 	const DeviceInfo* dev = nullptr;
 	rc = device_info(&dev);
 	if (rc) return rc;
-	Workspace* ws = nullptr;
-	rc = workspace(&ws);
-	if (rc) return rc;
-	const uint32_t J = cache->dim / 32;
-	size_t floats = plan_floats(plan_attend4(shape_of(cache, batch, batch->table_stride, 0, *dev)), J);
-	if (top) {
-		const size_t sparse = plan_floats(plan_attend4(shape_of(cache, batch, batch->table_stride, top, *dev)), J);
+	size_t floats = most_floats(shape_of(cache, batch, batch->table_stride, top, *dev));
+	if (top && table_pages(batch, cache->page_tokens) > SELECT_PAGES) { /* scores of the choice in two kernels */
 		const size_t keys = (size_t)batch->tokens * cache->heads * batch->table_stride;
-		if (sparse > floats) floats = sparse;
 		if (keys > floats) floats = keys;
 	}
-	return floats ? reserve_cache4("kmx_cache4_reserve", ws, floats) : KMX_OK;
+	float* partials = nullptr;
+	return floats ? reserve_cache4("kmx_cache4_reserve", floats, &partials) : KMX_OK;
 }
 
 } // extern "C"

@@ -17,6 +17,9 @@ namespace kmx {
 /* 2^v by the instruction: results below 2^-126 are 0, which no sum here notices */
 __device__ __forceinline__ float exp2_(float v) { return __builtin_amdgcn_exp2f(v); }
 
+/* parts done of each unit of a call, zero between calls: in the code's own memory, so that no call allocates or clears it */
+static __device__ uint32_t tickets[TICKETS];
+
 struct Row4 { uint32_t token, head; bool there; }; /* query number inside its sequence, query head inside its group */
 
 /* (divisions are some twenty instructions and come before the first load: none where a sequence has one query) */
@@ -472,11 +475,11 @@ attend4_kernel(Attend4 a)
 	asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
 	__syncthreads();
 	const uint32_t tid = threadIdx.x;
-	if (tid == 0) last = atomicAdd(&a.tickets[whole], 1u) == parts - 1;
+	if (tid == 0) last = atomicAdd(&tickets[whole], 1u) == parts - 1;
 	__syncthreads();
 	if (!last) return;
 	__builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "agent"); /* (nothing below is read ahead of the ticket, nor from a cache that was filled before it) */
-	if (tid == 0) __hip_atomic_store(&a.tickets[whole], 0u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT); /* for the next call */
+	if (tid == 0) __hip_atomic_store(&tickets[whole], 0u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT); /* for the next call */
 	const float* const left = (const float*)all_parts;
 	constexpr size_t PART = 2 * 16 * (D / 2 + 1);
 	{ /* weights: 16 lanes a row, all their parts under way at once */
@@ -968,14 +971,12 @@ join4_kernel(Attend4 a)
 }
 
 template <int J>
-int launch_attend4(Attend4 a, const Plan4& plan, Workspace* ws)
+int launch_attend4(Attend4 a, const Plan4& plan)
 {
 	a.row_tiles = plan.row_tiles;
 	a.splits = plan.splits;
 	a.tiles_per_split = plan.tiles_per_split;
 	a.joined = plan.joined;
-	a.partial = ws->partials;
-	a.tickets = ws->tickets;
 	if (plan.many) {
 		constexpr uint32_t bytes = 2 * (64 * (64 * J + 16) + 32 * J * 144);
 		static bool allowed = false; /* more LDS than a launch may ask for unannounced */

@@ -7,6 +7,6 @@
 
 namespace kmx {
 
-template int launch_attend4<KMX_J>(Attend4 a, const Plan4& plan, Workspace* ws);
+template int launch_attend4<KMX_J>(Attend4 a, const Plan4& plan);
 
 } // namespace kmx

@@ -92,6 +92,30 @@ inline size_t plan_floats(const Plan4& plan, uint32_t J)
 	return plan.splits > 1 ? plan.units * plan.splits * part_floats(J, false) : 0;
 }
 
+/*
+ * The most that this takes for any batch that is no larger: fewer units are taken in more parts. Of few rows units with parts are fewer than 2 compute_units, and
+ * there are at most 2 compute_units / units + 1 parts of each; of many rows MANY_ROUNDS rounds of parts, or shares, one for each work-group that the chip holds.
+ */
+inline size_t most_floats(const Shape4& s)
+{
+	constexpr uint64_t PLENTY = (uint64_t)1 << 40;
+	const auto times = [](uint64_t a, uint64_t b) { return a == 0 || b == 0 ? 0 : a > PLENTY / b ? PLENTY : a * b; };
+	const auto least = [](uint64_t a, uint64_t b) { return a < b ? a : b; };
+	const uint64_t pages = ((uint64_t)s.max_length + (1u << s.page_shift) - 1) >> s.page_shift;
+	const uint64_t tiles = ((pages << s.page_shift) + 63) / 64; /* (of lists, whose last page counts as a whole) */
+	const uint64_t rows = (uint64_t)s.max_queries * s.group, heads = times(s.sequences, s.heads), slots = (s.J <= 2 ? 2 : 1) * (uint64_t)s.compute_units;
+	const uint64_t listed = s.top ? times(s.max_queries, ((uint64_t)s.group + 15) / 16) : 0, few = (least(rows, MANY_ROWS) + 15) / 16;
+	size_t most = tiles > 4 ? least(4 * (uint64_t)s.compute_units, times(times(heads, listed > few ? listed : few), (tiles + 3) / 4)) * part_floats(s.J, false) : 0;
+	if (rows > MANY_ROWS) {
+		const uint64_t units = times(heads, (rows + 255) / 256), parts = least(16, tiles / MANY_LEAST);
+		const size_t floats = parts > 1 ? least(MANY_ROUNDS * slots, times(units, parts)) * (part_floats(s.J, true) + 1) : 0; /* (two words a unit, of two parts at least) */
+		const size_t shared = s.sequences > 1 && times(units, tiles) >= SHARE_LEAST * slots ? slots * (2 * part_floats(s.J, true) + 4) : 0;
+		if (floats > most) most = floats;
+		if (shared > most) most = shared;
+	}
+	return most;
+}
+
 } // namespace kmx
 
 #endif

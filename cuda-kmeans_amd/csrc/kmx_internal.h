@@ -68,7 +68,6 @@ struct Workspace {
 	uint32_t* queued_index = nullptr;     size_t queued_index_cap = 0;  /* words: per row 2 (queue) + 2 (assignment or 64-bit key), then the screen's pair counters and pairs */
 	uint32_t* carried = nullptr;          size_t carried_cap = 0;       /* words: per point the leader and the two smallest ranking values over the slices of centroids swept so far */
 	uint32_t* listed = nullptr;           size_t listed_cap = 0;        /* words: two per point the half-precision sweep could not settle (its length: counters[LISTED_COUNTER]) */
-	uint32_t* tickets = nullptr;          /* words, zero between calls: parts done of each unit of the attention over the 4-bit cache */
 	const float* exact_norms = nullptr; /* |c|^2 of the centroids as given, in the layout of `norms`, for the exact pass of a sweep that moved its frame (points into `norms`; null: `norms` holds them) */
 	bool fixed = false; /* the work space of the entry point that allocates nothing: its buffers never grow, a call that needs more is refused */
 };
@@ -84,7 +83,6 @@ int reserve_rows_copy(Workspace* ws, size_t floats);
 int reserve_queued_rows(Workspace* ws, size_t rows, size_t dim, size_t extra_words);
 int reserve_carried(Workspace* ws, size_t words);
 int reserve_listed(Workspace* ws, size_t words);
-int reserve_tickets(Workspace* ws, size_t words); /* (the same number every time) */
 int two_level_mode(); /* kmx_set_two_level_sweep */
 constexpr uint32_t CELLS_COUNTER = 5;  /* word of Workspace::counters that counts the list units handed out by build_cells_kernel */
 constexpr uint32_t FINISH_COUNTER = 6; /* and the one that counts the work-groups fused_finish_kernel has behind it */

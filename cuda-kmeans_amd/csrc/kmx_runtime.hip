@@ -176,16 +176,6 @@ int reserve_queued_rows(Workspace* ws, size_t rows, size_t dim, size_t extra_wor
 
 int reserve_carried(Workspace* ws, size_t words) { return grow(&ws->carried, &ws->carried_cap, words); }
 int reserve_listed(Workspace* ws, size_t words) { return grow(&ws->listed, &ws->listed_cap, words); }
-int reserve_tickets(Workspace* ws, size_t words)
-{
-	if (ws->tickets) return KMX_OK;
-	size_t none = 0;
-	const int rc = grow(&ws->tickets, &none, words);
-	if (rc) return rc;
-	KMX_HIP(hipMemset(ws->tickets, 0, words * sizeof(uint32_t)));
-	KMX_HIP(hipDeviceSynchronize()); /* (the caller's stream may be one that waits for no other) */
-	return KMX_OK;
-}
 static int g_two_level_mode = 1;
 int two_level_mode() { return g_two_level_mode; }
 
@@ -207,7 +197,6 @@ static int release_workspace()
 	if (g_ws.queued_index) KMX_HIP(hipFree(g_ws.queued_index));
 	if (g_ws.carried) KMX_HIP(hipFree(g_ws.carried));
 	if (g_ws.listed) KMX_HIP(hipFree(g_ws.listed));
-	if (g_ws.tickets) KMX_HIP(hipFree(g_ws.tickets));
 	g_ws = Workspace();
 	return release_f64_workspace();
 }

@@ -490,7 +490,8 @@ int kmx_cache4_attend(const kmx_cache4* cache, const kmx_cache4_batch* batch, in
                       const int32_t* chosen, uint32_t top);
 
 /* Sizes the work space for kmx_cache4_attend on such a batch, and for kmx_cache4_select and attention to `top` chosen pages (0: neither), so that
- * they allocate nothing afterwards (recordings, serving loops). Of the batch it looks at the numbers only. */
+ * they allocate nothing afterwards (recordings, serving loops): neither on this batch nor on one that is no larger in any of its numbers, nor with fewer chosen
+ * pages. Of the batch it looks at the numbers only. */
 int kmx_cache4_reserve(const kmx_cache4* cache, const kmx_cache4_batch* batch, uint32_t top);
 
 /* Message of the last failed call on this thread ("" if none). */

@@ -23,14 +23,18 @@ def plan(tmp_path_factory):
                    'using namespace kmx;\n'
                    'extern "C" void plan(const uint32_t* s, uint64_t* out)\n'
                    "{ const Plan4 p = plan_attend4(Shape4{ s[0], s[1], s[2], s[3], s[4], s[5], s[6], s[7], s[8] });\n"
-                   "  out[0] = p.units; out[1] = p.row_tiles; out[2] = p.splits; out[3] = p.tiles_per_split; out[4] = p.many; out[5] = p.joined; out[6] = plan_floats(p, s[0]); }\n")
+                   "  out[0] = p.units; out[1] = p.row_tiles; out[2] = p.splits; out[3] = p.tiles_per_split; out[4] = p.many; out[5] = p.joined; out[6] = plan_floats(p, s[0]); }\n"
+                   'extern "C" uint64_t most(const uint32_t* s) { return most_floats(Shape4{ s[0], s[1], s[2], s[3], s[4], s[5], s[6], s[7], s[8] }); }\n')
     subprocess.check_call(["g++", "-std=c++17", "-Wall", "-Werror", "-shared", "-fPIC", "-I", os.path.join(ROOT, "cuda-kmeans_amd", "csrc"), str(src), "-o", str(lib)])
-    fn = ctypes.CDLL(str(lib)).plan
+    lib = ctypes.CDLL(str(lib))
+    lib.most.restype = ctypes.c_uint64
 
-    def call(dim, heads, group, sequences, queries, length, page=64, top=0):
+    def call(dim, heads, group, sequences, queries, length, page=64, top=0, most=False):
         out = np.zeros(7, np.uint64)
         numbers = np.array([dim // 32, heads, group, sequences, queries, length, page.bit_length() - 1, top, UNITS], np.uint32)
-        fn(numbers.ctypes.data_as(ctypes.c_void_p), out.ctypes.data_as(ctypes.c_void_p))
+        if most:
+            return lib.most(numbers.ctypes.data_as(ctypes.c_void_p))
+        lib.plan(numbers.ctypes.data_as(ctypes.c_void_p), out.ctypes.data_as(ctypes.c_void_p))
         return dict(zip(("units", "row_tiles", "splits", "tiles_per_split", "many", "joined", "floats"), (int(v) for v in out)))
     return call
 
@@ -98,3 +102,24 @@ def test_lists_longer_than_any_sequence(plan):
                 assert p["splits"] * p["tiles_per_split"] >= -(-pages * page // 64)
                 assert p == plan(64, 1, 2, 1, 1, length, page, pages)
                 assert (p["floats"] > 0) == (p["splits"] > 1) == (length > 1000)
+
+
+def test_room_for_a_batch_is_room_for_smaller_ones(plan):
+    """Fewer units have more parts: 64 sequences of 8 heads need nothing, 63 do. What is reserved for a batch holds for all that are no larger, and is not
+    more than the largest of them could take by far: 1024 parts of 16 rows, eight rounds of parts of 256."""
+    full, fewer = (plan(128, 8, 4, n, 1, 8192) for n in (64, 63))
+    assert full["floats"] == 0 and fewer["floats"] > 0 and plan(128, 8, 4, 64, 1, 8192, most=True) >= fewer["floats"]
+    rng = np.random.default_rng(4)
+    for b in batches(3, 20000):
+        top = int(rng.integers(1, 200)) if rng.random() < 0.5 else 0
+        most = plan(**b, top=top, most=True)
+        assert most <= max(4 * UNITS * 16 * (b["dim"] + 2), 8 * UNITS * (2 if b["dim"] <= 64 else 1) * (256 * (b["dim"] + 2) + 1))
+        for _ in range(8):
+            less = dict(b, **{name: int(np.ceil(b[name] * rng.random() ** rng.integers(0, 4))) or 1 for name in ("sequences", "queries", "length")})
+            assert plan(**less)["floats"] <= most, (b, less)
+            if top:
+                assert plan(**less, top=int(rng.integers(1, top + 1)))["floats"] <= most, (b, less, top)
+    for sequences in range(1, 70):
+        for queries in (1, 5, 17, 64, 300, 1056):
+            for length in (1, 300, 5000, 131072):
+                assert plan(128, 8, 4, sequences, queries, length)["floats"] <= plan(128, 8, 4, 70, 1056, 131072, most=True)

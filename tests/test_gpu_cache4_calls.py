@@ -2,7 +2,8 @@
 import numpy as np
 import pytest
 
-from test_gpu_cache4 import BF16, Cache, Queries, bound_all, choice, device, select
+from test_gpu_cache4 import BF16, Cache, Queries, bound_all, choice, device, select, to_bits
+from test_zz_no_alloc import device_memory_in_use
 
 pytestmark = pytest.mark.gpu
 
@@ -22,3 +23,51 @@ def test_bounds_on_queries_that_say_nothing(km, gpu, group, counts):
         chosen = select(s, 6, 1, 1)
         assert np.array_equal(chosen, choice(s, want, 6, 1, 1, True))
         s.check(chosen=chosen)
+
+
+def test_reserved_for_a_batch_and_smaller_ones(km, gpu):
+    """A serving loop whose sequences end one after the other: reserved for the full batch, no smaller one allocates, and each can be recorded. (The full batch itself
+    needs nothing: fewer units are taken in more parts.)"""
+    rng = np.random.default_rng(3)
+    heads, group, dim, page = 8, 2, 64, 16
+    c = Cache(km, rng, heads, dim, page, 64 * 125 + 2, garbage=0x2B)  # (some numbers everywhere)
+    kept = []
+    for sequences, queries, length in ((64, 1, 2000), (63, 1, 2000), (40, 1, 1999), (7, 1, 2000), (1, 1, 600), (2, 40, 2000), (1, 64, 700), (5, 33, 1200)):
+        s = Queries(km, rng, c, [length] * sequences, [queries] * sequences, group, BF16)
+        s.bits, s.out = device(km, to_bits(s.q, BF16)), km.DeviceBuffer(2 * s.tokens * heads * group * dim)
+        s.chosen, s.sparse = km.DeviceBuffer(4 * s.tokens * heads * 9), km.DeviceBuffer(2 * s.tokens * heads * group * dim)
+        kept.append(s)
+    bound_pages = np.arange(c.pages, dtype=np.int32)
+    c.dev.bound(device(km, bound_pages), device(km, np.full(c.pages, page, np.int32)), c.pages)
+
+    def step(s):
+        c.dev.attend(s.batch, BF16, s.bits, s.out, s.scale)
+        c.dev.select(s.batch, BF16, s.bits, s.chosen, 9)
+        c.dev.attend(s.batch, BF16, s.bits, s.sparse, s.scale, chosen=s.chosen, top=9)
+
+    def results(s):
+        km.sync()
+        return [b.read(np.uint16, b.nbytes // 2) for b in (s.out, s.sparse)]
+
+    for s in kept:
+        step(s)  # (the code is on the device)
+    want = [results(s) for s in kept]
+    km.check(km.hip_lib().kmx_shutdown())  # and the work space is not
+    large = km.Cache4Batch(64, heads * group, 80 * 2, 64, 2000, device(km, np.int32([0])), device(km, np.int32([0])), device(km, np.int32([0])), kept[0].table.shape[1])
+    c.dev.reserve(large, 9)
+    km.sync()
+    before = device_memory_in_use()
+    for s, w in zip(kept, want):
+        step(s)
+        assert all(np.array_equal(a, b) for a, b in zip(results(s), w))
+    assert device_memory_in_use() == before
+    for s, w in zip(kept, want):
+        with km.Graph() as g:
+            step(s)
+        for _ in range(3):
+            for b in (s.out, s.sparse):
+                b.zero()
+            g.launch()
+            assert all(np.array_equal(a, b) for a, b in zip(results(s), w))
+            step(s)
+        g.destroy()
