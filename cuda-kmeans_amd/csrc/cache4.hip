@@ -820,14 +820,25 @@ static int check_batch4(const char* who, const kmx_cache4* cache, const kmx_cach
 	return KMX_OK;
 }
 
-static int reserve_cache4(const char* who, size_t floats, float** partials)
+/*
+ * Work space of a call. A recording keeps the addresses of its moment, and the work space moves when a later call needs more of it: recorded calls take the static
+ * scratch array of recorded updates where it has room (64 MB: all attention of few rows, and choices of 16M scores), else the work space.
+ */
+static int place_cache4(const char* who, size_t floats, float** partials)
 {
+	const bool recorded = launches_recorded();
+	const Workspace* fixed = recorded ? fixed_scratch() : nullptr;
+	if (fixed && floats <= fixed->partials_cap) {
+		*partials = fixed->partials;
+		scratch_recorded();
+		return KMX_OK;
+	}
 	Workspace* ws = nullptr;
 	int rc = workspace(&ws);
 	if (rc) return rc;
-	if (floats > ws->partials_cap && launches_recorded())
+	if (recorded && floats > ws->partials_cap)
 		return fail(KMX_ERR_INVALID_ARGUMENT, "%s: the call needs a larger work space, which cannot be allocated while it is recorded: kmx_cache4_reserve, or the same call once before", who);
-	if (recording_graph()) scratch_recorded();
+	if (recorded) scratch_recorded();
 	rc = reserve_partials(ws, floats);
 	*partials = ws->partials;
 	return rc;
@@ -976,7 +987,7 @@ int kmx_cache4_select(const kmx_cache4* cache, const kmx_cache4_batch* batch, in
 	a.chunks = (tiles + a.chunk - 1) / a.chunk;
 	if ((uint64_t)a.token_tiles * a.chunks > 65535) return fail(KMX_ERR_UNSUPPORTED, "kmx_cache4_select: %u queries are too many for one call", a.batch.max_queries);
 	float* keys = nullptr;
-	rc = reserve_cache4("kmx_cache4_select", (size_t)batch->tokens * a.cache.heads * batch->table_stride, &keys);
+	rc = place_cache4("kmx_cache4_select", (size_t)batch->tokens * a.cache.heads * batch->table_stride, &keys);
 	if (rc) return rc;
 	a.keys = (uint32_t*)keys;
 	switch (cache->dim / 32) {
@@ -1028,7 +1039,7 @@ int kmx_cache4_attend(const kmx_cache4* cache, const kmx_cache4_batch* batch, in
 	if (plan.units >= MOST_UNITS) return fail(KMX_ERR_UNSUPPORTED, "kmx_cache4_attend: too many queries for one call");
 	const size_t floats = plan_floats(plan, cache->dim / 32);
 	if (floats) {
-		rc = reserve_cache4("kmx_cache4_attend", floats, &a.partial);
+		rc = place_cache4("kmx_cache4_attend", floats, &a.partial);
 		if (rc) return rc;
 	}
 	switch (cache->dim / 32) {
@@ -1060,8 +1071,10 @@ int kmx_cache4_reserve(const kmx_cache4* cache, const kmx_cache4_batch* batch, u
 		const size_t keys = (size_t)batch->tokens * cache->heads * batch->table_stride;
 		if (keys > floats) floats = keys;
 	}
+	Workspace* scratch = nullptr;
+	if (noalloc_workspace(&scratch)) clear_error(); /* the address of the scratch array that recorded calls use (they do without if it has none) */
 	float* partials = nullptr;
-	return floats ? reserve_cache4("kmx_cache4_reserve", floats, &partials) : KMX_OK;
+	return floats ? place_cache4("kmx_cache4_reserve", floats, &partials) : KMX_OK;
 }
 
 } // extern "C"

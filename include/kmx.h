@@ -191,7 +191,7 @@ int kmx_update_f32(int variant,
  * work space that kmx_update_f32 grows with hipMalloc. The call allocates and frees nothing; a shape whose partial
  * sums do not fit is refused with KMX_ERR_UNSUPPORTED (the message names both sizes). SoA points skip the AoS copy
  * kmx_update_f32 makes of them and run the element-wise kernels (slower, same results). Per-kernel profiling
- * (kmx_set_profiling) does not cover this call. All calls on one GPU share that GPU's array, also with recorded updates (see
+ * (kmx_set_profiling) does not cover this call. All calls on one GPU share that GPU's array, also with recorded updates, choices of pages and attention (see
  * kmx_graph_begin): calls and replays that overlap in
  * time on one GPU (different streams, different threads) race; calls on the library's one stream do not.
  * The address of a device's array is looked up once per device: by kmx_set_device, by kmx_reserve_f32, or else by the
@@ -316,17 +316,18 @@ int kmx_event_elapsed_ms(void* start, void* stop, float* ms); /* waits for `stop
 /*
  * ---- recorded iterations (no counterpart in the reference, whose loop launches kernel by kernel,
  *      cuda.hpp:70-88) ----
- * Between kmx_graph_begin and kmx_graph_end the launching calls (kmx_assign_f32, kmx_update_f32, kmx_fused_f32,
- * kmx_bucket_sum_f32, kmx_fill_zero_u32) run nothing: their kernels, with the arguments of that moment, are recorded into
+ * Between kmx_graph_begin and kmx_graph_end the launching calls (kmx_assign_f32, kmx_update_f32, kmx_fused_f32, kmx_iteration_f32,
+ * kmx_bucket_sum_f32, kmx_fill_zero_u32, kmx_cache4_write, _read, _bound, _select and _attend) run nothing: their kernels, with the arguments of that moment, are recorded into
  * a HIP graph. kmx_graph_launch enqueues the whole recording on the library's stream as one unit, any number of times
  * (the host driver records two ping-pong iterations once and replays them). Everything that allocates, copies or
  * waits is refused while recording; a call whose work space would have to grow is refused too -- make the same
  * calls once before recording. Per-kernel profiling events are not recorded.
  * A recording holds the addresses of its moment: those of its buffers, and of the work space where a call uses it, which a later call that needs more
  * of it, and kmx_shutdown, release. It is not launched after that; kmx_reserve_f32 for the largest shape beforehand keeps the work space where it is.
- * Updates with KMX_UPDATE_ATOMIC_SHM (kmx_update_f32, kmx_update_f64) whose sums fit LDS take their scratch memory from the static array of kmx_update_f32_noalloc instead, so
+ * Updates with KMX_UPDATE_ATOMIC_SHM (kmx_update_f32, kmx_update_f64) whose sums fit LDS take their scratch memory from the static array of kmx_update_f32_noalloc instead, as do
+ * kmx_cache4_select and kmx_cache4_attend where it has room (attention with up to 64 rows of a head, or to chosen pages, always), so
  * recordings of nothing else stay valid. The same holds where the caller records the stream of kmx_set_stream with the runtime's own means, except that kmx_set_device,
- * kmx_reserve_f32 or kmx_graph_begin has to come first (the array's address) and that replays are the caller's to keep from overlapping with other users of the array.
+ * kmx_reserve_f32, kmx_cache4_reserve or kmx_graph_begin has to come first (the array's address) and that replays are the caller's to keep from overlapping with other users of the array.
  */
 int kmx_graph_begin(void);
 int kmx_graph_end(void** graph);
@@ -422,7 +423,8 @@ int kmx_probe_matrix_chain(int kind, const float* a, const float* b, const float
  * Bounds, where they are kept: for each page and head the largest and the smallest value of each channel of the keys, outwards in 127ths of
  * their largest magnitude m (dim + dim bytes: up(hi (1/m 127)), down(lo (1/m 127)) in floats), behind all of them those largest magnitudes over 127 (floats).
  * Places, pages and lengths on the device are not trusted: a place or page outside the cache is left out (reads as zeros, is not attended to).
- * kmx_cache4_select and kmx_cache4_attend use the library's work space (see kmx_cache4_reserve) under the rules of the updates.
+ * kmx_cache4_select and kmx_cache4_attend use the library's work space (see kmx_cache4_reserve), recorded ones the static scratch array (see kmx_graph_begin), under the
+ * rules of the updates.
  */
 typedef enum kmx_type { KMX_F32 = 0, KMX_F16 = 1, KMX_BF16 = 2 } kmx_type;
 

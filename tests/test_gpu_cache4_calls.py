@@ -71,3 +71,61 @@ def test_reserved_for_a_batch_and_smaller_ones(km, gpu):
             assert all(np.array_equal(a, b) for a, b in zip(results(s), w))
             step(s)
         g.destroy()
+
+
+def test_recordings_outlive_the_work_space(km, gpu):
+    """Recorded attention, in parts of 16 rows and of 256, and the choice in two kernels: then the work space moves (a larger call) and goes (kmx_shutdown), and the
+    replays are still the calls themselves."""
+    rng = np.random.default_rng(5)
+    c = Cache(km, rng, 1, 64, 16, 2500, garbage=0x2B)  # (some numbers everywhere)
+    few = Queries(km, rng, c, [14000, 9000], [1, 2], 4, BF16)
+    many = Queries(km, rng, c, [9000], [40], 2, BF16)
+    large = Queries(km, rng, c, [15000], [600], 2, BF16)
+    pages = np.arange(c.pages, dtype=np.int32)
+    c.dev.bound(device(km, pages), device(km, np.full(c.pages, 16, np.int32)), c.pages)
+    for s in (few, many, large):
+        s.bits, s.out = device(km, to_bits(s.q, BF16)), km.DeviceBuffer(2 * s.tokens * s.group * 64)
+    chosen, sparse = km.DeviceBuffer(4 * few.tokens * 12), km.DeviceBuffer(2 * few.tokens * 4 * 64)
+
+    def step():
+        c.dev.attend(few.batch, BF16, few.bits, few.out, few.scale)
+        c.dev.attend(many.batch, BF16, many.bits, many.out, many.scale)
+        c.dev.select(few.batch, BF16, few.bits, chosen, 12)
+        c.dev.attend(few.batch, BF16, few.bits, sparse, few.scale, chosen=chosen, top=12)
+
+    buffers = (few.out, many.out, chosen, sparse)
+
+    def results():
+        km.sync()
+        return [b.read(np.uint16, b.nbytes // 2) for b in buffers]
+
+    step()
+    want = results()
+    with km.Graph() as g:
+        step()
+
+    def replay():
+        for b in buffers:
+            b.zero()
+        g.launch()
+        assert all(np.array_equal(a, b) for a, b in zip(results(), want))
+
+    replay()
+    c.dev.attend(large.batch, BF16, large.bits, large.out, large.scale)  # more work space
+    step()
+    assert all(np.array_equal(a, b) for a, b in zip(results(), want))
+    for _ in range(2):
+        replay()
+    km.check(km.hip_lib().kmx_shutdown())
+    filler = [km.DeviceBuffer(1 << 22) for _ in range(4)]  # (where the work space was, for all one knows)
+    for b in filler:
+        b.write(np.full(1 << 20, 0x7FC00001, np.uint32))
+    replay()
+    km.sync()
+    for b in filler:
+        assert (b.read(np.uint32, 1 << 20) == 0x7FC00001).all()
+    c.dev.attend(large.batch, BF16, large.bits, large.out, large.scale)
+    replay()
+    step()
+    assert all(np.array_equal(a, b) for a, b in zip(results(), want))
+    g.destroy()
