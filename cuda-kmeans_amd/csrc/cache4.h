@@ -8,8 +8,8 @@
  *   [8 dim, 16 dim)   codes of the values, pair by pair: pair 16 j + i holds channels 32 j + i (low) and 32 j + 16 + i (high), one byte a
  *                     token. A lane of the second product wants tokens of one channel, and a token that is written touches no byte of another.
  *   [16 dim, 17 dim)  scales of the keys, half precision, [token][j];  [17 dim, 18 dim) scales of the values, [j][token]
- * A scale has 5 significant bits and a magnitude 6, so that their product is a number of half precision: the matrix cores take the very
- * values that the cache stands for.
+ * A scale has 5 significant bits and a magnitude 6, so that their product is a number of half precision from 2^-14 on: the matrix cores take the very
+ * values that the cache stands for, smaller ones to the nearest multiple of 2^-24.
  */
 #ifndef KMX_CACHE4_H
 #define KMX_CACHE4_H
@@ -208,7 +208,7 @@ __device__ __forceinline__ uint32_t visible_to(const Batch4& b, const Sequence& 
 	return n > 0 ? (uint32_t)n : 0;
 }
 
-/* cache4_attend.hip, one object per J: see there */
+/* cache4_attend_impl.h, one object per J: see there */
 struct Attend4 {
 	Cache4 cache;
 	Batch4 batch;

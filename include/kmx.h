@@ -418,7 +418,8 @@ int kmx_probe_matrix_chain(int kind, const float* a, const float* b, const float
  *     most 63488; below 2^-14 it has the bits that half precision has there.
  *   code: the number of j < 7 with |x| > scale (L_j + L_j+1) / 2, in floats -- the nearest level, the lower one of two as near; NaN: 0 --
  *     and the sign (x < 0). It stands for +- scale L_code. Infinities stand for the largest number their group can hold.
- * With levels from kmx_cache4_round_levels (6 significant bits) every such number is one of half precision.
+ * With levels from kmx_cache4_round_levels (6 significant bits) every such number from 2^-14 on is one of half precision. Smaller ones may have places below 2^-24:
+ * kmx_cache4_read and kmx_cache4_bound take them as they are, kmx_cache4_attend rounded to half precision (2^-25 off at most).
  * Buffers are the caller's (kmx_cache4_sizes tells how large), 16-byte aligned. Pages that no token was written to may hold anything.
  * Bounds, where they are kept: for each page and head the largest and the smallest value of each channel of the keys, outwards in 127ths of
  * their largest magnitude m (dim + dim bytes: up(hi (1/m 127)), down(lo (1/m 127)) in floats), behind all of them those largest magnitudes over 127 (floats).

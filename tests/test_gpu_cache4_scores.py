@@ -1,8 +1,8 @@
-"""Attention over the 4-bit cache where scores are far from zero or far apart, against its definition in 64 bits (-m gpu)."""
+"""Attention over the 4-bit cache where scores are far from zero or far apart and where rows are small, against its definition in 64 bits (-m gpu)."""
 import numpy as np
 import pytest
 
-from test_gpu_cache4 import BF16, F16, UNIT, Cache, Queries, device
+from test_gpu_cache4 import BF16, F16, F32, UNIT, Cache, Queries, device
 
 pytestmark = pytest.mark.gpu
 
@@ -85,3 +85,31 @@ def test_one_token_far_above_the_others(km, gpu, kind, queries, behind):
             off = UNIT[kind] * np.abs(want) + (2.0 ** -11 + 2 * delta + 2 * terms) * (p @ np.abs(v) / total) + n * 2.0 ** -40 * np.abs(v).max() / total
             assert np.all(np.abs(got[i, h] - want) <= off), (np.abs(got[i, h] - want) / off).max()
             assert np.all(np.abs(lse[i, h] - (top + np.log(total))[:, 0]) <= delta[:, 0] + terms + 2.0 ** -21 * (1 + np.abs(lse[i, h])))
+
+
+@pytest.mark.parametrize("kind", [F16, BF16])
+@pytest.mark.parametrize("dim,counts", [(64, [1, 1]), (64, [70, 33]), (256, [1, 3])])
+@pytest.mark.parametrize("size", [1e-3, 1e-4, 1e-6])
+def test_small_rows(km, gpu, kind, dim, counts, size):
+    """Numbers of the cache below 2^-14 are held in more places than half precision has: attention takes them rounded to it, which is what read returns as F16."""
+    rng = np.random.default_rng(dim)
+    c = Cache(km, rng, 1, dim, 32, 14)
+    s = Queries(km, rng, c, [300, 90], counts, 2, kind)
+    for b, n in enumerate(s.lengths):
+        at = np.arange(n)
+        c.write(F32, *(np.float32(size * rng.normal(size=(n, 1, dim))) for _ in range(2)), s.table[b, at // 32] * 32 + at % 32)
+    everywhere = np.arange(14 * 32)
+    k, v = (x.astype(np.float32) for x in c.read(F16, everywhere))
+    written = np.zeros(14 * 32, bool)
+    for b, n in enumerate(s.lengths):
+        at = np.arange(n)
+        written[s.table[b, at // 32] * 32 + at % 32] = True
+    assert np.array_equal(k[written], c.k[written].astype(np.float16).astype(np.float32))
+    assert np.array_equal(k[written], c.k[written]) == (size == 1e-3)  # (products of these levels and scales still fit there)
+    c.k[written], c.v[written] = k[written], v[written]
+    got, lse = s.attend(scale=1 / (size * np.sqrt(dim)))
+    want, want_lse, off, lse_off = s.expected(scale=1 / (size * np.sqrt(dim)))
+    if kind == F16:
+        off = off + 2.0 ** -25  # results below 2^-14 have no more places either
+    assert np.all(np.abs(got - want) <= off), (np.abs(got - want) / off).max()
+    assert np.all(np.abs(lse - want_lse) <= lse_off)
