@@ -236,6 +236,7 @@ attend4_kernel(Attend4 a)
 	const int32_t* list = a.chosen + (listed ? ((size_t)(seq.first + last_query_of(a, seq, row_tile)) * a.cache.heads + head) * a.top : 0);
 	const int32_t* table = a.batch.table + (size_t)s * a.batch.table_stride;
 	const uint32_t sub_bits = a.cache.page_shift - 4, last_entry = (listed ? a.top : a.batch.table_stride) - 1;
+	const uint32_t last_page = (seq.length - 1) >> a.cache.page_shift; /* (looked at where there is a token) places on pages behind it may not fit 32 bits */
 
 	/*
 	 * Where the blocks of the wavefront's tiles lie, 16 tiles at a time, one block a lane (4 n + b: block b of the n-th tile), and their places in
@@ -246,7 +247,7 @@ attend4_kernel(Attend4 a)
 		uint32_t logical = min(entry, last_entry);
 		if (listed) logical = (uint32_t)list[logical];
 		const uint32_t page = (uint32_t)table[min(logical, a.batch.table_stride - 1)];
-		const bool there = entry <= last_entry && logical < a.batch.table_stride && page < a.cache.page_count;
+		const bool there = entry <= last_entry && logical <= last_page && page < a.cache.page_count;
 		lds.places[wave][half][lane] = block_offset<J>(a.cache, there ? page : 0, head, sub);
 		lds.from[wave][half][lane] = there ? (int32_t)((logical << a.cache.page_shift) + 16 * sub) : INT32_MAX;
 	};

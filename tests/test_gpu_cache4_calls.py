@@ -129,3 +129,18 @@ def test_recordings_outlive_the_work_space(km, gpu):
     step()
     assert all(np.array_equal(a, b) for a, b in zip(results(), want))
     g.destroy()
+
+
+def test_chosen_pages_behind_the_sequence(km, gpu):
+    """Columns of the table behind a sequence's last page are left out wherever they are, also where their tokens' places would pass 32 bits."""
+    rng = np.random.default_rng(6)
+    c = Cache(km, rng, 1, 32, 256, 4)
+    s = Queries(km, rng, c, [1000], [1], 2, BF16).fill(rng)
+    pages, width = s.table[0, :4], (1 << 24) + 8
+    table = np.full(width, -1, np.int32)
+    table[:4] = pages
+    table[[4, 5, 1 << 22, 1 << 23, (1 << 23) + 1, 1 << 24, (1 << 24) + 3]] = pages[0]
+    s.table = table[None]
+    s.batch = km.Cache4Batch(1, 2, 1, 1, 1000, device(km, s.starts), device(km, np.int32([1000])), device(km, table), width)
+    for chosen in ([1, 4, 5, 1 << 22], [2, 1 << 23, (1 << 23) + 1, 1 << 24], [1 << 24, (1 << 24) + 3, -1, -1], [0, 1, 3, (1 << 24) + 7]):
+        s.check(chosen=np.array(chosen)[None, None])
