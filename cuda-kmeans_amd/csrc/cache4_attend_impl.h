@@ -980,11 +980,16 @@ int launch_attend4(Attend4 a, const Plan4& plan)
 	a.joined = plan.joined;
 	if (plan.many) {
 		constexpr uint32_t bytes = 2 * (64 * (64 * J + 16) + 32 * J * 144);
-		static bool allowed = false; /* more LDS than a launch may ask for unannounced */
-		if (!allowed && bytes > 65536) {
-			KMX_HIP(hipFuncSetAttribute((const void*)attend4_many_kernel<J, false>, hipFuncAttributeMaxDynamicSharedMemorySize, (int)bytes));
-			KMX_HIP(hipFuncSetAttribute((const void*)attend4_many_kernel<J, true>, hipFuncAttributeMaxDynamicSharedMemorySize, (int)bytes));
-			allowed = true;
+		if (bytes > 65536) { /* more LDS than a launch may ask for unannounced, on this device */
+			static int allowed = -1;
+			const DeviceInfo* dev = nullptr;
+			const int rc = device_info(&dev);
+			if (rc) return rc;
+			if (allowed != dev->device) {
+				KMX_HIP(hipFuncSetAttribute((const void*)attend4_many_kernel<J, false>, hipFuncAttributeMaxDynamicSharedMemorySize, (int)bytes));
+				KMX_HIP(hipFuncSetAttribute((const void*)attend4_many_kernel<J, true>, hipFuncAttributeMaxDynamicSharedMemorySize, (int)bytes));
+				allowed = dev->device;
+			}
 		}
 		if (a.tiles_per_split == 0) KMX_LAUNCH_KERNEL((attend4_many_kernel<J, true>), dim3(a.splits), dim3(512), bytes, stream(), a);
 		else KMX_LAUNCH_KERNEL((attend4_many_kernel<J, false>), dim3(a.splits), dim3(512), bytes, stream(), a);
