@@ -522,10 +522,12 @@ def cache4_round_levels(levels):
 
 def cache4_learn_levels(rows, iterations=12):
     """The 8 levels that k-means (one dimension, 8 centroids) finds on the magnitudes of sample rows (any shape, the last axis a multiple of 32),
-    each over the largest of its 32 channels: one set for kmx_cache4, rounded. Rows of zeros say nothing and are left out."""
+    each over the largest of its 32 channels: one set for kmx_cache4, rounded. Groups of zeros say nothing and are left out, as are those that hold
+    infinities or NaN."""
     x = np.abs(np.asarray(rows, dtype=np.float32)).reshape(-1, 32)
-    largest = x.max(axis=1, keepdims=True)
-    x = np.ascontiguousarray((x / np.where(largest > 0, largest, 1))[largest[:, 0] > 0].reshape(-1))
+    largest = x.max(axis=1, keepdims=True)  # (NaN where one is among them)
+    some = (largest > 0) & (largest < np.inf)
+    x = np.ascontiguousarray((x[some[:, 0]] / largest[some[:, 0]]).reshape(-1))
     if x.size < 8:
         raise ValueError("no rows to learn from")
     start = np.quantile(x, (np.arange(8) + 0.5) / 8).astype(np.float32)

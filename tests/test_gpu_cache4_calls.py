@@ -144,3 +144,17 @@ def test_chosen_pages_behind_the_sequence(km, gpu):
     s.batch = km.Cache4Batch(1, 2, 1, 1, 1000, device(km, s.starts), device(km, np.int32([1000])), device(km, table), width)
     for chosen in ([1, 4, 5, 1 << 22], [2, 1 << 23, (1 << 23) + 1, 1 << 24], [1 << 24, (1 << 24) + 3, -1, -1], [0, 1, 3, (1 << 24) + 7]):
         s.check(chosen=np.array(chosen)[None, None])
+
+
+def test_levels_learned_from_rows_with_unusual_numbers(km, gpu):
+    """Groups of 32 with infinities, NaN or nothing but zeros teach nothing: the levels are those of the other groups."""
+    rng = np.random.default_rng(7)
+    rows = rng.standard_t(6, size=(2000, 64)).astype(np.float32)
+    want = km.cache4_learn_levels(rows)
+    worse = np.concatenate([rows, rows[:300]])
+    worse[2000:2100, [3, 40]], worse[2100:2200, [5, 63]], worse[2200:2300] = np.inf, np.nan, 0
+    worse[2050, 7] = -np.inf
+    assert np.array_equal(km.cache4_learn_levels(worse), want)
+    for nothing in (np.full((4, 32), np.inf), np.full((4, 32), np.nan), np.zeros((4, 32))):
+        with pytest.raises(ValueError):
+            km.cache4_learn_levels(nothing)
