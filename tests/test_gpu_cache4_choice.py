@@ -2,7 +2,7 @@
 import numpy as np
 import pytest
 
-from test_gpu_cache4 import BF16, F16, Cache, Queries, bound_all, choice, device, kept_bounds, ordinary, select
+from test_gpu_cache4 import BF16, F16, Cache, Queries, bound_all, choice, kept_bounds, select
 
 pytestmark = pytest.mark.gpu
 
@@ -71,3 +71,21 @@ def test_bounds_that_nobody_made(km, gpu, heads, group, dim, page, lengths, coun
             seen = -(-s.sees(b, i) // page)
             for h in range(heads):
                 assert set(range(min(first, seen))) | set(range(max(0, seen - last), seen)) <= set(chosen[s.starts[b] + i, h].tolist())
+
+
+@pytest.mark.parametrize("heads,group,dim,page,lengths,counts,top,first,last", [
+    (1, 4, 160, 16, [9700], [3], 9, 1, 1), (1, 2, 256, 16, [12200, 8300], [2, 1], 12, 1, 1), (1, 20, 192, 16, [10000], [1], 6, 0, 1),  # one kernel of 8 wavefronts, two tiles of pages each
+    (1, 4, 128, 16, [13000, 12400], [20, 7], 10, 1, 1), (2, 2, 64, 16, [12500], [17], 5, 1, 0), (1, 16, 256, 16, [12900], [3], 8, 1, 1),  # two kernels, several tiles of queries
+    (1, 1, 32, 16, [140000], [2], 700, 1, 1)])                                                                                          # keys from memory
+def test_choice_in_kernels_that_few_sizes_reach(km, gpu, heads, group, dim, page, lengths, counts, top, first, last):
+    rng = np.random.default_rng(dim + heads)
+    c = Cache(km, rng, heads, dim, page, sum(-(-n // page) for n in lengths) + 2)
+    s = Queries(km, rng, c, lengths, counts, group, F16).fill(rng)
+    want = bound_all(s)
+    chosen = select(s, top, first, last)
+    assert np.array_equal(chosen, choice_by_kept_bounds(s, top, first, last))
+    if max(lengths) < 20000:  # (the definition page by page takes long)
+        assert np.array_equal(chosen, choice(s, want, top, first, last, True))
+    s.check(chosen=chosen)
+    apart = select(s, top, first, last, causal=False)
+    assert np.array_equal(apart, choice_by_kept_bounds(s, top, first, last, causal=False))
