@@ -781,7 +781,7 @@ __device__ __forceinline__ void many_unit(const Attend4& a, uint8_t* many, uint3
 				for (int c = 0; c < 2 * J; ++c)
 					sc[t] = __builtin_amdgcn_mfma_f32_32x32x16_f16(*(const half8v*)(tile + (32 * (t0 + t) + n32) * KROW + 32 * c + 16 * h), q[c], sc[t], 0, 0, 0);
 			}
-			if (from + 64 > least || blocks != 15) {
+			if (least - from < 64 || blocks != 15) { /* (neither is negative: no sum that may pass 31 bits) */
 #pragma unroll
 				for (int e = 0; e < 16 * STEP; ++e) {
 					const int32_t place = from + 32 * (t0 + e / 16) + 8 * (e % 16 / 4) + 4 * (int32_t)h + e % 4;

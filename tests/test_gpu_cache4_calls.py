@@ -2,7 +2,7 @@
 import numpy as np
 import pytest
 
-from test_gpu_cache4 import BF16, Cache, Queries, bound_all, choice, device, select, to_bits
+from test_gpu_cache4 import BF16, F16, Cache, Queries, bound_all, choice, device, select, to_bits
 from test_zz_no_alloc import device_memory_in_use
 
 pytestmark = pytest.mark.gpu
@@ -158,3 +158,29 @@ def test_levels_learned_from_rows_with_unusual_numbers(km, gpu):
     for nothing in (np.full((4, 32), np.inf), np.full((4, 32), np.nan), np.zeros((4, 32))):
         with pytest.raises(ValueError):
             km.cache4_learn_levels(nothing)
+
+
+def test_the_last_tile_that_31_bits_count(km, gpu):
+    """A sequence of 2^31 - 1 tokens, all pages but the last the same: its last tokens hold all of the softmax, and queries before them do not see them."""
+    rng = np.random.default_rng(8)
+    c = Cache(km, rng, 1, 32, 256, 2)
+    along = np.ones(32, np.float32)
+    values = rng.normal(size=(512, 1, 32)).astype(np.float32)
+    keys = np.zeros((512, 1, 32), np.float32)
+    keys[256:] = 2 * np.arange(1, 257)[:, None, None] * along  # (held in 5 bits: some tokens in a row are alike, the next ones far above them)
+    c.write(F16, keys, values, np.arange(512))
+    length, counts, width = 2 ** 31 - 1, 100, 1 << 23
+    table = np.zeros(width, np.int32)
+    table[-1] = 1
+    s = Queries(km, rng, c, [256], [counts], 1, F16)
+    s.q = np.ones((counts, 1, 1, 32), np.float32)
+    s.batch = km.Cache4Batch(1, 1, counts, counts, length, device(km, s.starts), device(km, np.int32([length])), device(km, table), width)
+    got, lse = s.attend(scale=1.0)
+    for i in range(counts):
+        seen = slice(256, 256 + 256 - counts + i)  # of the last page, whose last token is not there
+        k, v = c.k[seen, 0].astype(np.float64), c.v[seen, 0].astype(np.float64)
+        score = k.sum(-1)
+        p = np.exp(score - score.max())  # (e^-64 at most of what is not alike)
+        want = p @ v / p.sum()
+        assert np.all(np.abs(got[i, 0, 0] - want) <= 2.0 ** -11 * np.abs(want) + 2.0 ** -11 * (p @ np.abs(v)) / p.sum()), i
+        assert abs(lse[i, 0, 0] - score.max() - np.log(p.sum())) <= 2.0 ** -20 * lse[i, 0, 0]
