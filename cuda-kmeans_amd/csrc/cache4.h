@@ -89,41 +89,9 @@ __device__ __forceinline__ uint32_t dpp(uint32_t v)
 {
 	return (uint32_t)__builtin_amdgcn_mov_dpp((int)v, CTRL, 0xF, 0xF, false);
 }
-constexpr int DPP_XOR1 = 0xB1, DPP_XOR2 = 0x4E, DPP_ROR4 = 0x124, DPP_ROR8 = 0x128; /* inside groups of 4 lanes, rotations inside 16 */
+constexpr int DPP_XOR1 = 0xB1, DPP_XOR2 = 0x4E; /* inside groups of 4 lanes */
 
-/* Elements of the caller's rows */
-__device__ __forceinline__ float element(const float* p) { return *p; }
-__device__ __forceinline__ float element(const _Float16* p) { return (float)*p; }
-__device__ __forceinline__ float element(const __bf16* p) { return __builtin_bit_cast(float, (uint32_t)*(const uint16_t*)p << 16); }
-
-/* 8 elements side by side; vec: 16-byte aligned */
-template <typename T>
-__device__ __forceinline__ void load8(const T* p, bool vec, float x[8])
-{
-	if (vec) {
-		if constexpr (sizeof(T) == 4) {
-			const f32x4 a = *(const f32x4*)p, b = *(const f32x4*)(p + 4);
-			for (int i = 0; i < 4; ++i) { x[i] = a[i]; x[4 + i] = b[i]; }
-		} else {
-			const u32x4 w = *(const u32x4*)p;
-			for (int i = 0; i < 4; ++i) {
-				if constexpr (__is_same(T, __bf16)) {
-					x[2 * i] = __builtin_bit_cast(float, w[i] << 16);
-					x[2 * i + 1] = __builtin_bit_cast(float, w[i] & 0xFFFF0000u);
-				} else {
-					const uint32_t pair = w[i]; /* (a bit cast of a vector's element itself takes the first one) */
-					const half2v h = __builtin_bit_cast(half2v, pair);
-					x[2 * i] = (float)h[0];
-					x[2 * i + 1] = (float)h[1];
-				}
-			}
-		}
-	} else {
-		for (int i = 0; i < 8; ++i) x[i] = element(p + i);
-	}
-}
-
-/* 8 elements as they are, two a word */
+/* 8 elements of a caller's row of 16 bits each as they are, two a word; vec: 16-byte aligned */
 __device__ __forceinline__ u32x4 load_raw8(const uint16_t* p, bool vec)
 {
 	if (vec) return *(const u32x4*)p;

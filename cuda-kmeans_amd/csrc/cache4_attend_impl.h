@@ -107,14 +107,30 @@ __device__ __forceinline__ void load_halves(const uint8_t* p, uint32_t w[(J + 1)
 	}
 }
 
-/* 8 channels of every 16 of a row */
-template <int N, typename T>
-__device__ __forceinline__ void load_steps(const char* p, bool vec, float x[N][8])
+/* N pieces of 8 channels of a row, `apart` channels from one to the next */
+template <int N>
+__device__ __forceinline__ void load_pieces(const uint16_t* p, uint32_t apart, bool vec, u32x4 raw[N])
 {
-	if (vec)
-		for (int c = 0; c < N; ++c) load8((const T*)p + 16 * c, true, x[c]);
-	else
-		for (int c = 0; c < N; ++c) load8((const T*)p + 16 * c, false, x[c]);
+	if (vec) {
+#pragma unroll
+		for (int n = 0; n < N; ++n) raw[n] = load_raw8(p + apart * n, true);
+	} else {
+#pragma unroll
+		for (int n = 0; n < N; ++n) raw[n] = load_raw8(p + apart * n, false);
+	}
+}
+template <int N>
+__device__ __forceinline__ void floats_of(const u32x4 raw[N], bool bf16, float x[N][8])
+{
+	if (bf16) {
+#pragma unroll
+		for (int n = 0; n < N; ++n)
+			for (int e = 0; e < 8; ++e) { const uint32_t w = raw[n][e / 2]; x[n][e] = raw_element(w, e % 2, true); }
+	} else {
+#pragma unroll
+		for (int n = 0; n < N; ++n)
+			for (int e = 0; e < 8; ++e) { const uint32_t w = raw[n][e / 2]; x[n][e] = raw_element(w, e % 2, false); }
+	}
 }
 
 template <int J>
@@ -222,13 +238,7 @@ attend4_kernel(Attend4 a)
 	u32x4 raw[J];
 	{
 		const uint16_t* p = (const uint16_t*)a.q + (size_t)(seq.first + (row.there ? row.token : 0)) * a.q_token + ((size_t)head * a.batch.group + (row.there ? row.head : 0)) * a.q_head + 8 * kg;
-		if (a.vec) {
-#pragma unroll
-			for (int j = 0; j < J; ++j) raw[j] = *(const u32x4*)(p + 32 * j);
-		} else {
-#pragma unroll
-			for (int j = 0; j < J; ++j) raw[j] = load_raw8(p + 32 * j, false);
-		}
+		load_pieces<J>(p, 32, a.vec, raw);
 	}
 	const int32_t sees = row.there ? (int32_t)visible_to(a.batch, seq, row.token) : 0;
 	const Magnitudes mk = load_magnitudes(a.cache.levels, head, 0), mv = load_magnitudes(a.cache.levels, head, 1);
@@ -284,15 +294,7 @@ attend4_kernel(Attend4 a)
 	float row_scale = 1.0f;
 	auto take_queries = [&]() {
 		float x[J][8], largest = 0.0f;
-		if (a.bf16) {
-#pragma unroll
-			for (int j = 0; j < J; ++j)
-				for (int e = 0; e < 8; ++e) { const uint32_t w = raw[j][e / 2]; x[j][e] = raw_element(w, e % 2, true); }
-		} else {
-#pragma unroll
-			for (int j = 0; j < J; ++j)
-				for (int e = 0; e < 8; ++e) { const uint32_t w = raw[j][e / 2]; x[j][e] = raw_element(w, e % 2, false); }
-		}
+		floats_of<J>(raw, a.bf16, x);
 #pragma unroll
 		for (int j = 0; j < J; ++j)
 			for (int e = 0; e < 8; ++e) largest = fmaxf(largest, fabsf(x[j][e]));
@@ -674,9 +676,9 @@ __device__ __forceinline__ void many_unit(const Attend4& a, uint8_t* many, uint3
 	float row_scale;
 	{
 		float x[2 * J][8];
-		const char* p = (const char*)a.q + 2 * ((size_t)(seq.first + token) * a.q_token + (size_t)query_head * a.q_head + 8 * h);
-		if (a.bf16) load_steps<2 * J, __bf16>(p, a.vec, x);
-		else load_steps<2 * J, _Float16>(p, a.vec, x);
+		u32x4 raw[2 * J];
+		load_pieces<2 * J>((const uint16_t*)a.q + (size_t)(seq.first + token) * a.q_token + (size_t)query_head * a.q_head + 8 * h, 16, a.vec, raw);
+		floats_of<2 * J>(raw, a.bf16, x);
 		float largest = 0.0f;
 #pragma unroll
 		for (int c = 0; c < 2 * J; ++c)
