@@ -142,7 +142,7 @@ constexpr int values_words() { return J > 4 * ((J + 3) / 4) ? J : 4 * ((J + 3) /
 __device__ __forceinline__ float query_scale(float scale, float largest, float* row_scale)
 {
 	int power = (int)(__builtin_bit_cast(uint32_t, largest) >> 23) - 127;
-	power = power < -126 ? 0 : power > 126 ? 126 : power;
+	power = power < -126 ? -126 : power > 126 ? 126 : power; /* (queries below 2^-126 too) */
 	const float by = __builtin_bit_cast(float, (uint32_t)(127 - power) << 23);
 	*row_scale = fminf(fmaxf(fabsf(scale) * 1.44269504088896341f * __builtin_bit_cast(float, (uint32_t)(127 + power) << 23), 1.2e-38f), 0x1p100f);
 	return scale > 0.0f ? by : scale < 0.0f ? -by : 0.0f;

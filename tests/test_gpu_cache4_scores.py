@@ -2,7 +2,7 @@
 import numpy as np
 import pytest
 
-from test_gpu_cache4 import BF16, F16, F32, UNIT, Cache, Queries, device
+from test_gpu_cache4 import BF16, F16, F32, UNIT, Cache, Queries, device, from_bits, to_bits
 
 pytestmark = pytest.mark.gpu
 
@@ -113,3 +113,14 @@ def test_small_rows(km, gpu, kind, dim, counts, size):
         off = off + 2.0 ** -25  # results below 2^-14 have no more places either
     assert np.all(np.abs(got - want) <= off), (np.abs(got - want) / off).max()
     assert np.all(np.abs(lse - want_lse) <= lse_off)
+
+
+@pytest.mark.parametrize("counts", [[1], [70]])
+def test_queries_below_the_normal_numbers(km, gpu, counts):
+    rng = np.random.default_rng(9)
+    c = Cache(km, rng, 1, 64, 64, 5)
+    s = Queries(km, rng, c, [150], counts, 2, BF16, loud=2.0 ** -126).fill(rng)
+    small = from_bits(to_bits(s.q / 64, BF16), BF16)
+    s.q = small
+    assert np.abs(small).max() < 2.0 ** -126 and np.abs(small).max() > 0
+    s.check(scale=2.0 ** 126)
