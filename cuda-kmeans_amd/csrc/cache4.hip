@@ -89,8 +89,8 @@ __device__ __forceinline__ void floats8(const Raw8<T>& r, float x[8])
  * A wavefront takes 16 tokens of one head, 64 pieces of 8 channels at a time: piece n is channels 8 (n % 4 J) of token n / 4 J, so that a load of all
  * lanes is whole rows side by side and a group of 32 channels four lanes, its maximum two exchanges inside them. The keys' words go where they
  * belong (a token's lie together); the values' bytes pass through LDS, 16 tokens of a pair side by side, and leave as 16 bytes a lane where the 16
- * tokens fill a block in order, else byte by byte. Rows go past the caches: nobody comes back to them. Some 18 instructions a number
- * stand beside the loads, and both take about as long: 16384 tokens of 8 heads of 128 in bf16 (86 MB) 27 us, 3.2 TB/s.
+ * tokens fill a block in order, else byte by byte. Rows go past the caches: nobody comes back to them. Bound by the vector units: 26 instructions a number,
+ * 99 % of their time: 16384 tokens of 8 heads of 128 in bf16 (86 MB) 27 us, 3.2 TB/s.
  */
 template <int J, typename T>
 __global__ void __launch_bounds__(256)

@@ -200,7 +200,8 @@ struct Tile4 {
  * [token][row], so a lane has all its 16 scores in one row -- maxima and sums are its own but for two exchanges -- and its probabilities are, as they
  * stand, its piece of the second operand of [channel][row] = values . p. Tokens go to the rows of the first product such that a lane's 16 are those
  * of one block: its values are 16 bytes side by side.
- * Bound by unpacking: some 760 instructions a tile of 64 tokens at 128 channels, 1.4 us a tile and SIMD, about what the memory takes for it. 64
+ * Bound by unpacking: some 760 vector instructions a tile of 64 tokens at 128 channels, 1.4 us a tile and SIMD, about what the memory takes for it (72 % of the
+ * vector units' time in all, where lengths differ and the longest sequences end alone; matrix cores 12 %). 64
  * sequences of 8192 tokens, 8 heads of 128: 124 us, 4.8 TB/s of packed bytes; the same of 1 to 8192 tokens 102 to 107 us, where the longest ones
  * end last. Short sequences: 7 to 9 us, of which 4.5 are a launch with its first load and last store, the rest loads that wait for each other
  * (length, table, codes).
@@ -639,11 +640,12 @@ __device__ __forceinline__ Share4 share_of(const Attend4& a, uint32_t g)
  * into one of two buffers while everybody works on the other. Scores are [token][row] as above (v_mfma_f32_32x32x16_f16, 16 tokens a lane and
  * half of the tile), so that probabilities stay in their registers: the values' tokens lie in LDS in the order in which a lane has them. Rows of
  * LDS are 16 bytes longer than their contents: 8 lanes one below the other read 8 different groups of banks.
- * Bound by the matrix instructions with the softmax between them: 2 x 1024 queries, 32 heads on 8 of 128, 16384 and fewer tokens: 521 us, 777 TFLOP/s
- * of the 1150 that a large matrix product reaches; one sequence of 16384, in two parts: 323 us, 824. A work-group takes a part of a unit (256 rows of a
- * head), or its share of all units' tiles, from inside of one to inside of another. Heads of 32 and 64 channels have two work-groups on a compute
- * unit (376 and 405 us with one, 321 and 375 with two, before the shares). 256 channels: a wavefront's sums and queries are more than the registers
- * hold, and go to memory in part, 549 TFLOP/s.
+ * Bound by the sum of its phases: 2 x 1024 queries, 32 heads on 8 of 128, 16384 and fewer tokens take 530 us (570 on another card), 764 TFLOP/s of the 1150 that a large matrix
+ * product reaches; one sequence of 16384, in two parts, 328, 812. Matrix cores are busy 34 % of that time, vector units 49 % (265 instructions a wavefront and
+ * tile, 36 %, and 32 exponentials among them that take four times as long), LDS some 40 %: all wavefronts pass one barrier a tile and are in the same phase
+ * at the same time. A work-group takes a part of a unit (256 rows of a head), or its share of all units' tiles, from inside of one to inside of another. Heads of
+ * 32 and 64 channels have two work-groups on a compute unit (376 and 405 us with one, 321 and 375 with two, before the shares), for which 64 channels keep 4 to 12
+ * registers in memory. So do wide heads, whose sums and queries are more than the registers hold: 192 channels 2, 224 19 to 33, 256 50 to 72 (1277 us, 635 TFLOP/s).
  */
 template <int J>
 __device__ __forceinline__ void many_unit(const Attend4& a, uint8_t* many, uint32_t (*blocks_there)[4], uint32_t entry, uint32_t head, uint32_t begin, uint32_t until,
