@@ -27,7 +27,7 @@ UPDATE_ATOMIC_SHM2, UPDATE_FAKE, UPDATE_FAKE_SHM = 5, 6, 7  # the remaining kern
 UPDATE_SERIAL_ORDER = 8  # the sums of the serial loop (ascending point number inside a cluster), bit for bit, in O(n dim)
 UPDATE_EMULATED_ATOMICS = 0x100  # flag for the point, fine and wavefront variants: compare-and-swap loops
 
-TYPE_F32, TYPE_F16, TYPE_BF16 = 0, 1, 2  # element types of the rows of the 4-bit cache
+TYPE_F32, TYPE_F16, TYPE_BF16 = 0, 1, 2  # element types of rows: of the 4-bit cache, and what stands around it
 
 KMX_OK, KMX_ERR_INVALID_ARGUMENT, KMX_ERR_UNSUPPORTED, KMX_ERR_DEVICE, KMX_ERR_NO_DEVICE = 0, 1, 2, 3, 4
 
@@ -40,6 +40,7 @@ ABI_SYMBOLS = [
     "kmx_event_elapsed_ms", "kmx_set_profiling", "kmx_last_kernel_ms", "kmx_last_error", "kmx_certificate_tau", "kmx_certificate_unmoved_threshold",
     "kmx_update_f32_noalloc", "kmx_reserve_f32", "kmx_prepare_points_f64", "kmx_forget_points_f64", "kmx_probe_matrix_chain", "kmx_set_two_level_sweep", "kmx_iteration_f32", "kmx_iteration_last_passes",
     "kmx_cache4_sizes", "kmx_cache4_round_levels", "kmx_cache4_write", "kmx_cache4_read", "kmx_cache4_bound", "kmx_cache4_select", "kmx_cache4_attend", "kmx_cache4_reserve",
+    "kmx_cache4_attend_shared", "kmx_cache4_reserve_shared", "kmx_cache4_weigh", "kmx_cache4_evict", "kmx_rotary_turns", "kmx_rotary", "kmx_prompt_attend",
 ]
 
 
@@ -86,6 +87,18 @@ class Cache4BatchStruct(ctypes.Structure):
     _fields_ = [("sequences", ctypes.c_uint32), ("query_heads", ctypes.c_uint32), ("tokens", ctypes.c_uint32), ("max_queries", ctypes.c_uint32),
                 ("max_length", ctypes.c_uint32), ("table_stride", ctypes.c_uint32), ("starts", ctypes.c_void_p), ("lengths", ctypes.c_void_p),
                 ("table", ctypes.c_void_p)]
+
+
+class RotaryRowsStruct(ctypes.Structure):
+    """= kmx_rotary_rows."""
+    _fields_ = [("in_", ctypes.c_void_p), ("out", ctypes.c_void_p), ("in_token_stride", ctypes.c_size_t), ("in_head_stride", ctypes.c_size_t),
+                ("out_token_stride", ctypes.c_size_t), ("out_head_stride", ctypes.c_size_t), ("heads", ctypes.c_uint32)]
+
+
+class PromptStruct(ctypes.Structure):
+    """= kmx_prompt."""
+    _fields_ = [("sequences", ctypes.c_uint32), ("query_heads", ctypes.c_uint32), ("heads", ctypes.c_uint32), ("dim", ctypes.c_uint32), ("queries", ctypes.c_uint32),
+                ("tokens", ctypes.c_uint32), ("max_queries", ctypes.c_uint32), ("max_tokens", ctypes.c_uint32), ("query_starts", ctypes.c_void_p), ("token_starts", ctypes.c_void_p)]
 
 
 def build(force=True):
@@ -164,6 +177,14 @@ def hip_lib():
         lib.kmx_cache4_select.argtypes = [cache, batch, ctypes.c_int, vp, sz, sz, vp, u32, u32, u32, ctypes.c_int]
         lib.kmx_cache4_attend.argtypes = [cache, batch, ctypes.c_int, vp, sz, sz, vp, sz, sz, vp, ctypes.c_float, ctypes.c_int, vp, u32]
         lib.kmx_cache4_reserve.argtypes = [cache, batch, u32]
+        lib.kmx_cache4_attend_shared.argtypes = [cache, batch, batch, ctypes.c_int, vp, sz, sz, vp, sz, sz, vp, ctypes.c_float, ctypes.c_int]
+        lib.kmx_cache4_reserve_shared.argtypes = [cache, batch, batch]
+        lib.kmx_cache4_weigh.argtypes = [cache, batch, ctypes.c_int, vp, sz, sz, vp, ctypes.c_float, ctypes.c_int, vp]
+        lib.kmx_cache4_evict.argtypes = [cache, batch, vp, u32, u32, u32, vp, vp]
+        f64 = ctypes.c_double
+        lib.kmx_rotary_turns.argtypes = [u32, f64, f64, f64, f64, f64, vp]
+        lib.kmx_rotary.argtypes = [ctypes.c_int, ctypes.POINTER(RotaryRowsStruct), u32, u32, u32, u32, vp, vp, ctypes.c_int, ctypes.c_int, ctypes.c_float]
+        lib.kmx_prompt_attend.argtypes = [ctypes.POINTER(PromptStruct), ctypes.c_int, vp, sz, sz, vp, vp, sz, sz, vp, sz, sz, vp, ctypes.c_float, ctypes.c_int]
         _hip = lib
     return _hip
 
@@ -602,6 +623,78 @@ class Cache4:
     def reserve(self, batch, top=0):
         """Sizes the work space for attention on such a batch, and to `top` chosen pages (kmx_cache4_reserve)."""
         check(hip_lib().kmx_cache4_reserve(self.ref, batch.ref, top))
+
+    def attend_shared(self, prefix, batch, element_type, q, out, scale, causal=True, lse=None, q_token_stride=None, q_head_stride=None,
+                      out_token_stride=None, out_head_stride=None):
+        """Attention of sequences to prefixes that they share and to their own tokens (kmx_cache4_attend_shared)."""
+        strides = self._strides(batch.query_heads, q_token_stride, q_head_stride)
+        out_strides = self._strides(batch.query_heads, out_token_stride, out_head_stride)
+        check(hip_lib().kmx_cache4_attend_shared(self.ref, prefix.ref, batch.ref, element_type, q.ptr, *strides, out.ptr, *out_strides,
+                                                 lse.ptr if lse is not None else None, scale, int(causal)))
+
+    def reserve_shared(self, prefix, batch):
+        """Sizes the work space for attention to shared prefixes on such batches (kmx_cache4_reserve_shared)."""
+        check(hip_lib().kmx_cache4_reserve_shared(self.ref, prefix.ref, batch.ref))
+
+    def weigh(self, batch, element_type, q, lse, weights, scale, causal=True, q_token_stride=None, q_head_stride=None):
+        """Adds the attention that the tokens got from the queries to their weights (kmx_cache4_weigh)."""
+        strides = self._strides(batch.query_heads, q_token_stride, q_head_stride)
+        check(hip_lib().kmx_cache4_weigh(self.ref, batch.ref, element_type, q.ptr, *strides, lse.ptr, scale, int(causal), weights.ptr))
+
+    def evict(self, batch, weights, keep, first, recent, kept, left):
+        """Sequences back to `keep` tokens of each head: the first, the recent and the heaviest ones (kmx_cache4_evict)."""
+        check(hip_lib().kmx_cache4_evict(self.ref, batch.ref, weights.ptr, keep, first, recent, kept.ptr, left.ptr))
+
+
+# ---------------------------------------------------------------- around the cache ---------------
+
+def rotary_turns(channels, base=10000.0, stretch=1.0, length=0.0, slow=1.0, fast=32.0):
+    """Frequencies of the pairs of `channels` channels in 2^-64 of a turn a position, uint64, stretched for contexts longer than `length` (kmx_rotary_turns)."""
+    out = np.empty(channels // 2, dtype=np.uint64)
+    check(hip_lib().kmx_rotary_turns(channels, base, stretch, length, slow, fast, out.ctypes.data))
+    return out
+
+
+class RotaryRows:
+    """Rows of `heads` heads for rotary(): where they are, and where they go (None: where they are). Element strides default to rows without gaps."""
+
+    def __init__(self, rows, heads, out=None, token_stride=None, head_stride=None, out_token_stride=None, out_head_stride=None):
+        self.rows, self.heads, self.out = rows, heads, rows if out is None else out
+        self._strides = (token_stride, head_stride) + ((token_stride, head_stride) if out is None else (out_token_stride, out_head_stride))
+
+    def struct(self, dim):
+        token, head, out_token, out_head = self._strides
+        head, out_head = dim if head is None else head, dim if out_head is None else out_head
+        return RotaryRowsStruct(self.rows.ptr, self.out.ptr, self.heads * head if token is None else token, head, self.heads * out_head if out_token is None else out_token, out_head, self.heads)
+
+
+def rotary(element_type, sets, tokens, dim, turns, positions, channels=None, halves=True, inverse=False, gain=1.0):
+    """Rotates the first `channels` channels (None: all) of the rows of up to 4 sets to the tokens' positions, or back (kmx_rotary)."""
+    rows = (RotaryRowsStruct * max(1, len(sets)))(*[s.struct(dim) for s in sets])
+    check(hip_lib().kmx_rotary(element_type, rows, len(sets), tokens, dim, dim if channels is None else channels, turns.ptr, positions.ptr, int(halves), int(inverse), gain))
+
+
+class Prompt:
+    """Prompts side by side (kmx_prompt): `queries` rows of queries and `tokens` rows of keys and values in all, where each sequence's start in device memory."""
+
+    def __init__(self, sequences, query_heads, heads, dim, queries, tokens, max_queries, max_tokens, query_starts, token_starts):
+        self.query_heads, self.heads, self.dim = query_heads, heads, dim
+        self._buffers = (query_starts, token_starts)  # kept alive
+        self._prompt = PromptStruct(sequences, query_heads, heads, dim, queries, tokens, max_queries, max_tokens, query_starts.ptr, token_starts.ptr)
+        self.ref = ctypes.byref(self._prompt)
+
+    def _strides(self, heads, token_stride, head_stride):
+        head_stride = self.dim if head_stride is None else head_stride
+        return heads * head_stride if token_stride is None else token_stride, head_stride
+
+    def attend(self, element_type, q, keys, values, out, scale, causal=True, lse=None, q_token_stride=None, q_head_stride=None, token_stride=None, head_stride=None,
+               out_token_stride=None, out_head_stride=None):
+        """Attention of the queries to their prompts' tokens (kmx_prompt_attend)."""
+        strides = self._strides(self.query_heads, q_token_stride, q_head_stride)
+        key_strides = self._strides(self.heads, token_stride, head_stride)
+        out_strides = self._strides(self.query_heads, out_token_stride, out_head_stride)
+        check(hip_lib().kmx_prompt_attend(self.ref, element_type, q.ptr, *strides, keys.ptr, values.ptr, *key_strides, out.ptr, *out_strides,
+                                          lse.ptr if lse is not None else None, scale, int(causal)))
 
 
 # ---------------------------------------------------------------- algorithm objects --------------

@@ -176,6 +176,25 @@ __device__ __forceinline__ uint32_t visible_to(const Batch4& b, const Sequence& 
 	return n > 0 ? (uint32_t)n : 0;
 }
 
+/* What queries of that largest magnitude are multiplied with to become halves of at most 2 in magnitude (bf16 has more exponents), with the sign
+ * of the scale; *row_scale takes a score of theirs, below 2^26, to the exponent of 2, which stays a number: at most 2^100, where any two scores that
+ * differ do so by far more than a softmax tells from infinity */
+__device__ __forceinline__ float query_scale(float scale, float largest, float* row_scale)
+{
+	int power = (int)(__builtin_bit_cast(uint32_t, largest) >> 23) - 127;
+	power = power < -126 ? -126 : power > 126 ? 126 : power; /* (queries below 2^-126 too) */
+	const float by = __builtin_bit_cast(float, (uint32_t)(127 - power) << 23);
+	*row_scale = fminf(fmaxf(fabsf(scale) * 1.44269504088896341f * __builtin_bit_cast(float, (uint32_t)(127 + power) << 23), 1.2e-38f), 0x1p100f);
+	return scale > 0.0f ? by : scale < 0.0f ? -by : 0.0f;
+}
+
+/* cache4.hip: the checks of the entry points, and the work space of a call */
+int check_cache4(const char* who, const kmx_cache4* cache, Cache4* out);
+int check_batch4(const char* who, const kmx_cache4* cache, const kmx_cache4_batch* batch, int causal, Batch4* out);
+int check_type(const char* who, int type, bool floats);
+bool aligned_rows(const void* p, size_t token_stride, size_t head_stride, size_t size);
+int place_cache4(const char* who, size_t floats, float** partials);
+
 /* cache4_attend_impl.h, one object per J: see there */
 struct Attend4 {
 	Cache4 cache;
@@ -189,6 +208,9 @@ struct Attend4 {
 	uint32_t row_tiles, splits, tiles_per_split; /* (filled in by the launcher) */
 	bool joined; /* parts of many rows are left to the kernel that joins them */
 	float* partial; /* sums of parts, where there are any */
+	/* prefixes that sequences share: what their attention leaves (no prefix_starts), and what that of the sequences' own tokens is joined with */
+	float* rows; float* row_sums; /* [token][query head][channel], and of each row the largest score (to the base of 2) and the sum; null: no prefix */
+	const int32_t* prefix_starts; uint32_t prefixes, prefix_queries;
 };
 template <int J> int launch_attend4(Attend4 a, const Plan4& plan);
 

@@ -742,7 +742,7 @@ using namespace kmx;
 
 /* ---------------------------------------------------------------- entry points ------------------- */
 
-static int check_cache4(const char* who, const kmx_cache4* cache, Cache4* out)
+int kmx::check_cache4(const char* who, const kmx_cache4* cache, Cache4* out)
 {
 	if (!cache) return fail(KMX_ERR_INVALID_ARGUMENT, "%s: null cache", who);
 	if (cache->heads == 0) return fail(KMX_ERR_INVALID_ARGUMENT, "%s: heads must be positive", who);
@@ -762,14 +762,14 @@ static int check_cache4(const char* who, const kmx_cache4* cache, Cache4* out)
 	return KMX_OK;
 }
 
-static int check_type(const char* who, int type, bool floats)
+int kmx::check_type(const char* who, int type, bool floats)
 {
 	if (type == KMX_F16 || type == KMX_BF16 || (floats && type == KMX_F32)) return KMX_OK;
 	if (type == KMX_F32) return fail(KMX_ERR_UNSUPPORTED, "%s: queries are KMX_F16 or KMX_BF16", who);
 	return fail(KMX_ERR_INVALID_ARGUMENT, "%s: unknown element type %d", who, type);
 }
 
-static bool aligned_rows(const void* p, size_t token_stride, size_t head_stride, size_t size)
+bool kmx::aligned_rows(const void* p, size_t token_stride, size_t head_stride, size_t size)
 {
 	return (uintptr_t)p % 16 == 0 && token_stride * size % 16 == 0 && head_stride * size % 16 == 0;
 }
@@ -804,7 +804,7 @@ static int rows4(const char* who, bool write, const kmx_cache4* cache, int type,
 /* a bound may be as loose as it likes: no sequence has more queries than there are */
 static uint32_t most_queries(const kmx_cache4_batch* b) { return b->max_queries < b->tokens ? b->max_queries : b->tokens; }
 
-static int check_batch4(const char* who, const kmx_cache4* cache, const kmx_cache4_batch* batch, int causal, Batch4* out)
+int kmx::check_batch4(const char* who, const kmx_cache4* cache, const kmx_cache4_batch* batch, int causal, Batch4* out)
 {
 	if (!batch) return fail(KMX_ERR_INVALID_ARGUMENT, "%s: null batch", who);
 	if (batch->query_heads == 0 || batch->query_heads % cache->heads)
@@ -824,7 +824,7 @@ static int check_batch4(const char* who, const kmx_cache4* cache, const kmx_cach
  * Work space of a call. A recording keeps the addresses of its moment, and the work space moves when a later call needs more of it: recorded calls take the static
  * scratch array of recorded updates where it has room (64 MB: all attention of few rows, and choices of 16M scores), else the work space.
  */
-static int place_cache4(const char* who, size_t floats, float** partials)
+int kmx::place_cache4(const char* who, size_t floats, float** partials)
 {
 	const bool recorded = launches_recorded();
 	const Workspace* fixed = recorded ? fixed_scratch() : nullptr;
@@ -857,6 +857,52 @@ static uint32_t table_pages(const kmx_cache4_batch* b, uint32_t page_tokens)
 {
 	const uint32_t need = b->max_length / page_tokens + (b->max_length % page_tokens ? 1 : 0);
 	return need < b->table_stride ? need : b->table_stride;
+}
+
+/* queries and outputs of an attention; *nothing: there are none */
+static int take_rows(const char* who, const kmx_cache4* cache, const kmx_cache4_batch* batch, int type, const void* q, size_t q_token_stride, size_t q_head_stride,
+                     void* out, size_t out_token_stride, size_t out_head_stride, float* lse, float scale, Attend4* a, bool* nothing)
+{
+	const int rc = check_type(who, type, false);
+	if (rc) return rc;
+	if (!(std::fabs(scale) <= 3.4e38f)) return fail(KMX_ERR_INVALID_ARGUMENT, "%s: the scale is not finite", who);
+	*nothing = batch->sequences == 0 || batch->tokens == 0 || batch->max_queries == 0;
+	if (*nothing) return KMX_OK;
+	if (!q || !out) return fail(KMX_ERR_INVALID_ARGUMENT, "%s: null device pointer", who);
+	if ((uintptr_t)q % 2 || (uintptr_t)out % 2) return fail(KMX_ERR_INVALID_ARGUMENT, "%s: rows start at multiples of 2 bytes", who);
+	if (batch->query_heads > 1 && out_head_stride < cache->dim) return fail(KMX_ERR_INVALID_ARGUMENT, "%s: head stride of the output %zu < dim %u", who, out_head_stride, cache->dim);
+	if (batch->tokens > 1 && out_token_stride < cache->dim) return fail(KMX_ERR_INVALID_ARGUMENT, "%s: token stride of the output %zu < dim %u", who, out_token_stride, cache->dim);
+	a->q = q;
+	a->q_token = q_token_stride;
+	a->q_head = q_head_stride;
+	a->out = out;
+	a->out_token = out_token_stride;
+	a->out_head = out_head_stride;
+	a->lse = lse;
+	a->scale = scale;
+	a->bf16 = type == KMX_BF16;
+	a->vec = aligned_rows(q, q_token_stride, q_head_stride, 2) && aligned_rows(out, out_token_stride, out_head_stride, 2);
+	return KMX_OK;
+}
+
+static int launch_attend(const Attend4& a, const Plan4& plan, uint32_t J)
+{
+	switch (J) {
+	case 1: return launch_attend4<1>(a, plan);
+	case 2: return launch_attend4<2>(a, plan);
+	case 3: return launch_attend4<3>(a, plan);
+	case 4: return launch_attend4<4>(a, plan);
+	case 5: return launch_attend4<5>(a, plan);
+	case 6: return launch_attend4<6>(a, plan);
+	case 7: return launch_attend4<7>(a, plan);
+	default: return launch_attend4<8>(a, plan);
+	}
+}
+
+/* what the attention to shared prefixes leaves for that to the sequences' own tokens: a row of floats and two more for each query and head (whole 64s) */
+static size_t shared_floats(const kmx_cache4_batch* b, uint32_t dim)
+{
+	return ((size_t)b->tokens * b->query_heads * (dim + 2) + 63) / 64 * 64;
 }
 
 extern "C" {
@@ -1011,27 +1057,12 @@ int kmx_cache4_attend(const kmx_cache4* cache, const kmx_cache4_batch* batch, in
 	if (rc) return rc;
 	rc = check_batch4("kmx_cache4_attend", cache, batch, causal, &a.batch);
 	if (rc) return rc;
-	rc = check_type("kmx_cache4_attend", type, false);
-	if (rc) return rc;
 	if (chosen && top == 0) return fail(KMX_ERR_INVALID_ARGUMENT, "kmx_cache4_attend: chosen pages, but top is 0");
-	if (!(std::fabs(scale) <= 3.4e38f)) return fail(KMX_ERR_INVALID_ARGUMENT, "kmx_cache4_attend: the scale is not finite");
-	if (batch->sequences == 0 || batch->tokens == 0 || batch->max_queries == 0) return KMX_OK;
-	if (!q || !out) return fail(KMX_ERR_INVALID_ARGUMENT, "kmx_cache4_attend: null device pointer");
-	if ((uintptr_t)q % 2 || (uintptr_t)out % 2) return fail(KMX_ERR_INVALID_ARGUMENT, "kmx_cache4_attend: rows start at multiples of 2 bytes");
-	if (batch->query_heads > 1 && out_head_stride < cache->dim) return fail(KMX_ERR_INVALID_ARGUMENT, "kmx_cache4_attend: head stride of the output %zu < dim %u", out_head_stride, cache->dim);
-	if (batch->tokens > 1 && out_token_stride < cache->dim) return fail(KMX_ERR_INVALID_ARGUMENT, "kmx_cache4_attend: token stride of the output %zu < dim %u", out_token_stride, cache->dim);
-	a.q = q;
-	a.q_token = q_token_stride;
-	a.q_head = q_head_stride;
-	a.out = out;
-	a.out_token = out_token_stride;
-	a.out_head = out_head_stride;
-	a.lse = lse;
+	bool nothing = false;
+	rc = take_rows("kmx_cache4_attend", cache, batch, type, q, q_token_stride, q_head_stride, out, out_token_stride, out_head_stride, lse, scale, &a, &nothing);
+	if (rc || nothing) return rc;
 	a.chosen = chosen;
 	a.top = chosen ? top : 0;
-	a.scale = scale;
-	a.bf16 = type == KMX_BF16;
-	a.vec = aligned_rows(q, q_token_stride, q_head_stride, 2) && aligned_rows(out, out_token_stride, out_head_stride, 2);
 	const DeviceInfo* dev = nullptr;
 	rc = device_info(&dev);
 	if (rc) return rc;
@@ -1042,16 +1073,53 @@ int kmx_cache4_attend(const kmx_cache4* cache, const kmx_cache4_batch* batch, in
 		rc = place_cache4("kmx_cache4_attend", floats, &a.partial);
 		if (rc) return rc;
 	}
-	switch (cache->dim / 32) {
-	case 1: return launch_attend4<1>(a, plan);
-	case 2: return launch_attend4<2>(a, plan);
-	case 3: return launch_attend4<3>(a, plan);
-	case 4: return launch_attend4<4>(a, plan);
-	case 5: return launch_attend4<5>(a, plan);
-	case 6: return launch_attend4<6>(a, plan);
-	case 7: return launch_attend4<7>(a, plan);
-	default: return launch_attend4<8>(a, plan);
+	return launch_attend(a, plan, cache->dim / 32);
+}
+
+int kmx_cache4_attend_shared(const kmx_cache4* cache, const kmx_cache4_batch* prefix, const kmx_cache4_batch* batch, int type, const void* q, size_t q_token_stride,
+                             size_t q_head_stride, void* out, size_t out_token_stride, size_t out_head_stride, float* lse, float scale, int causal)
+{
+	clear_error();
+	Attend4 a{}, front{};
+	int rc = check_cache4("kmx_cache4_attend_shared", cache, &a.cache);
+	if (rc) return rc;
+	rc = check_batch4("kmx_cache4_attend_shared", cache, batch, causal, &a.batch);
+	if (rc) return rc;
+	rc = check_batch4("kmx_cache4_attend_shared", cache, prefix, 0, &front.batch);
+	if (rc) return rc;
+	if (prefix->tokens != batch->tokens || prefix->query_heads != batch->query_heads)
+		return fail(KMX_ERR_INVALID_ARGUMENT, "kmx_cache4_attend_shared: the prefixes have %u rows of %u query heads, the sequences %u of %u", prefix->tokens, prefix->query_heads, batch->tokens, batch->query_heads);
+	bool nothing = false;
+	rc = take_rows("kmx_cache4_attend_shared", cache, batch, type, q, q_token_stride, q_head_stride, out, out_token_stride, out_head_stride, lse, scale, &a, &nothing);
+	if (rc || nothing) return rc;
+	const DeviceInfo* dev = nullptr;
+	rc = device_info(&dev);
+	if (rc) return rc;
+	const uint32_t J = cache->dim / 32;
+	const bool any = prefix->sequences && prefix->max_queries;
+	const Plan4 plan = plan_attend4(shape_of(cache, batch, a.batch.table_stride, 0, *dev));
+	const Plan4 ahead = plan_attend4(shape_of(cache, prefix, front.batch.table_stride, 0, *dev));
+	if (plan.units >= MOST_UNITS || (any && ahead.units >= MOST_UNITS)) return fail(KMX_ERR_UNSUPPORTED, "kmx_cache4_attend_shared: too many queries for one call");
+	const size_t rows = any ? shared_floats(batch, cache->dim) : 0, mine = plan_floats(plan, J), theirs = any ? plan_floats(ahead, J) : 0;
+	float* space = nullptr;
+	if (rows + mine + theirs) {
+		rc = place_cache4("kmx_cache4_attend_shared", rows + (mine > theirs ? mine : theirs), &space);
+		if (rc) return rc;
 	}
+	a.partial = space + rows;
+	if (any) {
+		const Batch4 queries = front.batch;
+		front = a;
+		front.batch = queries;
+		front.rows = a.rows = space;
+		front.row_sums = a.row_sums = space + (size_t)batch->tokens * batch->query_heads * cache->dim;
+		rc = launch_attend(front, ahead, J);
+		if (rc) return rc;
+		a.prefix_starts = prefix->starts;
+		a.prefixes = prefix->sequences;
+		a.prefix_queries = front.batch.max_queries;
+	}
+	return launch_attend(a, plan, J);
 }
 
 int kmx_cache4_reserve(const kmx_cache4* cache, const kmx_cache4_batch* batch, uint32_t top)
@@ -1075,6 +1143,28 @@ int kmx_cache4_reserve(const kmx_cache4* cache, const kmx_cache4_batch* batch, u
 	if (noalloc_workspace(&scratch)) clear_error(); /* the address of the scratch array that recorded calls use (they do without if it has none) */
 	float* partials = nullptr;
 	return floats ? place_cache4("kmx_cache4_reserve", floats, &partials) : KMX_OK;
+}
+
+int kmx_cache4_reserve_shared(const kmx_cache4* cache, const kmx_cache4_batch* prefix, const kmx_cache4_batch* batch)
+{
+	clear_error();
+	if (recording_graph()) return fail(KMX_ERR_INVALID_ARGUMENT, "kmx_cache4_reserve_shared: not allowed between kmx_graph_begin and kmx_graph_end");
+	int rc = check_cache4("kmx_cache4_reserve_shared", cache, nullptr);
+	if (rc) return rc;
+	if (!prefix || !batch) return fail(KMX_ERR_INVALID_ARGUMENT, "kmx_cache4_reserve_shared: null batch");
+	if (batch->query_heads == 0 || batch->query_heads % cache->heads)
+		return fail(KMX_ERR_INVALID_ARGUMENT, "kmx_cache4_reserve_shared: %u query heads are no multiple of the cache's %u", batch->query_heads, cache->heads);
+	if (prefix->tokens != batch->tokens || prefix->query_heads != batch->query_heads)
+		return fail(KMX_ERR_INVALID_ARGUMENT, "kmx_cache4_reserve_shared: the prefixes have %u rows of %u query heads, the sequences %u of %u", prefix->tokens, prefix->query_heads, batch->tokens, batch->query_heads);
+	const DeviceInfo* dev = nullptr;
+	rc = device_info(&dev);
+	if (rc) return rc;
+	const size_t mine = most_floats(shape_of(cache, batch, batch->table_stride, 0, *dev)), theirs = most_floats(shape_of(cache, prefix, prefix->table_stride, 0, *dev));
+	const size_t floats = shared_floats(batch, cache->dim) + (mine > theirs ? mine : theirs);
+	Workspace* scratch = nullptr;
+	if (noalloc_workspace(&scratch)) clear_error(); /* the address of the scratch array that recorded calls use (they do without if it has none) */
+	float* partials = nullptr;
+	return floats ? place_cache4("kmx_cache4_reserve_shared", floats, &partials) : KMX_OK;
 }
 
 } // extern "C"

@@ -136,18 +136,6 @@ __device__ __forceinline__ void floats_of(const u32x4 raw[N], bool bf16, float x
 template <int J>
 constexpr int values_words() { return J > 4 * ((J + 3) / 4) ? J : 4 * ((J + 3) / 4); } /* words of codes a lane holds: J of keys, or 4 for each of its pairs of channels */
 
-/* What queries of that largest magnitude are multiplied with to become halves of at most 2 in magnitude (bf16 has more exponents), with the sign
- * of the scale; *row_scale takes a score of theirs, below 2^26, to the exponent of 2, which stays a number: at most 2^100, where any two scores that
- * differ do so by far more than a softmax tells from infinity */
-__device__ __forceinline__ float query_scale(float scale, float largest, float* row_scale)
-{
-	int power = (int)(__builtin_bit_cast(uint32_t, largest) >> 23) - 127;
-	power = power < -126 ? -126 : power > 126 ? 126 : power; /* (queries below 2^-126 too) */
-	const float by = __builtin_bit_cast(float, (uint32_t)(127 - power) << 23);
-	*row_scale = fminf(fmaxf(fabsf(scale) * 1.44269504088896341f * __builtin_bit_cast(float, (uint32_t)(127 + power) << 23), 1.2e-38f), 0x1p100f);
-	return scale > 0.0f ? by : scale < 0.0f ? -by : 0.0f;
-}
-
 /*
  * Probabilities are rounded to half precision for their product with the values: 11 bits from 2^-14 on, none below 2^-25. They are taken times 2^15, so
  * that the largest is as large as half precision allows for: then 11 bits reach down to 2^-29 of it and the last one to 2^-39, and what all
@@ -182,6 +170,66 @@ __device__ __forceinline__ void store_out4(const Attend4& a, char* row, uint32_t
 	if (a.vec) *(u32x2*)(row + 2 * channel) = u32x2{ b[0] | b[1] << 16, b[2] | b[3] << 16 };
 	else
 		for (int i = 0; i < 4; ++i) ((uint16_t*)row)[channel + i] = (uint16_t)b[i];
+}
+
+/* Whether a prefix answers for that row of queries (starts ascend) */
+__device__ __forceinline__ bool has_prefix(const Attend4& a, size_t token)
+{
+	uint32_t low = 0, high = a.prefixes;
+	while (low < high) { /* the last one that starts at it or before */
+		const uint32_t middle = (low + high) / 2;
+		if ((int64_t)a.prefix_starts[middle] <= (int64_t)token) low = middle + 1;
+		else high = middle;
+	}
+	if (low == 0) return false;
+	const int64_t from = a.prefix_starts[low - 1], to = a.prefix_starts[low];
+	return from >= 0 && to <= (int64_t)a.batch.tokens && (int64_t)token < to && (int64_t)token - from < (int64_t)a.prefix_queries;
+}
+
+/*
+ * The end of a row: its sums over `l`, the largest score m scale (to the base of 2); with a prefix these are joined with what the prefix has left, of a prefix they
+ * are left as they are. `by` is what sums are multiplied with, `theirs` the prefix's sums at `from`.
+ */
+struct End4 { float by, theirs; float* from; };
+template <uint32_t D>
+__device__ __forceinline__ End4 end_of(const Attend4& a, size_t token, size_t query_head, float m, float scale, float l, bool says)
+{
+	const size_t row = token * a.batch.query_heads + query_head;
+	End4 e{ 1.0f, 0.0f, nullptr };
+	if (a.rows && !a.prefix_starts) {
+		e.from = a.rows + row * D;
+		if (says) *(float2*)(a.row_sums + 2 * row) = float2{ m * scale, l };
+		return e;
+	}
+	if (a.rows && has_prefix(a, token)) {
+		const float2 p = *(const float2*)(a.row_sums + 2 * row);
+		const float mine = m * scale, top = fmaxf(mine, p.x), lowest = top == -__builtin_inff() ? 0.0f : top;
+		e.by = exp2_(mine - lowest);
+		e.theirs = exp2_(p.x - lowest);
+		e.from = a.rows + row * D;
+		l = l * e.by + p.y * e.theirs;
+		m = top;
+		scale = 1.0f;
+	}
+	const float by = l > 0.0f ? 1.0f / l : l == l ? 0.0f : l; /* a row that sees nothing is zero; NaN stays */
+	e.by *= by;
+	e.theirs *= by;
+	if (says && a.lse) a.lse[row] = l == 0.0f ? -__builtin_inff() : (m * scale + log2f(l * LOWERED)) * 0.693147180559945309f;
+	return e;
+}
+__device__ __forceinline__ void put4(const Attend4& a, const End4& e, char* to, uint32_t channel, const f32x4& sums)
+{
+	if (a.rows && !a.prefix_starts) {
+		*(f32x4*)(e.from + channel) = sums;
+		return;
+	}
+	float v[4];
+	for (int i = 0; i < 4; ++i) v[i] = sums[i] * e.by;
+	if (e.from) {
+		const f32x4 p = *(const f32x4*)(e.from + channel);
+		for (int i = 0; i < 4; ++i) v[i] += p[i] * e.theirs;
+	}
+	store_out4(a, to, channel, v);
 }
 
 /* What a wavefront loads for 64 tokens. A lane is row i = lane % 16 of the operands and holds their piece kg = lane / 16. */
@@ -449,16 +497,11 @@ attend4_kernel(Attend4 a)
 	}
 	if (parts == 1) {
 		if (wave != 0 || !row.there) return;
-		const float by = sum > 0.0f ? 1.0f / sum : sum == sum ? 0.0f : sum; /* a row that sees nothing is zero; NaN stays */
 		const size_t token = seq.first + row.token, query_head = (size_t)head * a.batch.group + row.head;
+		const End4 e = end_of<D>(a, token, query_head, all, row_scale, sum, kg == 0);
 		char* to = (char*)a.out + 2 * (token * a.out_token + query_head * a.out_head);
 #pragma unroll
-		for (int c = 0; c < 2 * J; ++c) {
-			float v[4];
-			for (int r = 0; r < 4; ++r) v[r] = o[c][r] * by;
-			store_out4(a, to, 16 * c + 4 * kg, v);
-		}
-		if (kg == 0 && a.lse) a.lse[token * a.batch.query_heads + query_head] = sum == 0.0f ? -__builtin_inff() : (all * row_scale + log2f(sum * LOWERED)) * 0.693147180559945309f;
+		for (int c = 0; c < 2 * J; ++c) put4(a, e, to, 16 * c + 4 * kg, o[c]);
 		return;
 	}
 
@@ -536,13 +579,10 @@ attend4_kernel(Attend4 a)
 				for (uint32_t g = 1; g < groups; ++g) mine += shares[g * across + tid];
 		}
 		if (group != 0 || e >= quads) continue;
-		const float s1 = total[0][r], by = s1 > 0.0f ? 1.0f / s1 : s1 == s1 ? 0.0f : s1;
 		const Row4 to_row = row_of(a, seq, row_tile, r);
 		const size_t token = seq.first + to_row.token, query_head = (size_t)head * a.batch.group + to_row.head;
-		float v[4];
-		for (int i = 0; i < 4; ++i) v[i] = mine[i] * by;
-		store_out4(a, (char*)a.out + 2 * (token * a.out_token + query_head * a.out_head), 4 * (e % (D / 4)), v);
-		if (e % (D / 4) == 0 && a.lse) a.lse[token * a.batch.query_heads + query_head] = s1 == 0.0f ? -__builtin_inff() : (most[0][r] + log2f(s1 * LOWERED)) * 0.693147180559945309f;
+		const End4 end_row = end_of<D>(a, token, query_head, most[0][r], 1.0f, total[0][r], e % (D / 4) == 0);
+		put4(a, end_row, (char*)a.out + 2 * (token * a.out_token + query_head * a.out_head), 4 * (e % (D / 4)), mine);
 	}
 }
 
@@ -850,16 +890,11 @@ __device__ __forceinline__ void many_unit(const Attend4& a, uint8_t* many, uint3
 		((uint2*)(a.partial + (size_t)(a.tiles_per_split ? 1 : 2) * a.splits * (256 * (D + 2))))[entry * a.cache.heads + head] = uint2{ blockIdx.x, parts };
 	if (!there) return;
 	if (whole) {
-		const float by = l > 0.0f ? 1.0f / l : l == l ? 0.0f : l;
+		const End4 end_row = end_of<D>(a, seq.first + token, query_head, m, row_scale, l, h == 0);
 		char* to = (char*)a.out + 2 * ((size_t)(seq.first + token) * a.out_token + (size_t)query_head * a.out_head);
 #pragma unroll
 		for (int j = 0; j < J; ++j)
-			for (int e = 0; e < 4; ++e) {
-				float v[4];
-				for (int r = 0; r < 4; ++r) v[r] = o[j][4 * e + r] * by;
-				store_out4(a, to, 32 * j + 8 * e + 4 * h, v);
-			}
-		if (h == 0 && a.lse) a.lse[(size_t)(seq.first + token) * a.batch.query_heads + query_head] = l == 0.0f ? -__builtin_inff() : (m * row_scale + log2f(l * LOWERED)) * 0.693147180559945309f;
+			for (int e = 0; e < 4; ++e) put4(a, end_row, to, 32 * j + 8 * e + 4 * h, f32x4{ o[j][4 * e], o[j][4 * e + 1], o[j][4 * e + 2], o[j][4 * e + 3] });
 		return;
 	}
 
@@ -965,13 +1000,10 @@ join4_kernel(Attend4 a)
 			if (group == 0) { mine += more; sum += more_sum; }
 		}
 		if (group != 0) continue;
-		const float by = sum > 0.0f ? 1.0f / sum : sum == sum ? 0.0f : sum;
 		const uint64_t x = first_row + r;
 		const size_t to_token = seq.first + x / a.batch.group, to_head = (size_t)head * a.batch.group + x % a.batch.group;
-		float v[4];
-		for (int e = 0; e < 4; ++e) v[e] = mine[e] * by;
-		store_out4(a, (char*)a.out + 2 * (to_token * a.out_token + to_head * a.out_head), 4 * at, v);
-		if (at == 0 && a.lse) a.lse[to_token * a.batch.query_heads + to_head] = sum == 0.0f ? -__builtin_inff() : (top + log2f(sum * LOWERED)) * 0.693147180559945309f;
+		const End4 end_row = end_of<D>(a, to_token, to_head, top, 1.0f, sum, at == 0);
+		put4(a, end_row, (char*)a.out + 2 * (to_token * a.out_token + to_head * a.out_head), 4 * at, mine);
 	}
 }
 

@@ -1,0 +1,558 @@
+/*
+ * What of the 4-bit cache is kept (kmx_cache4_weigh, kmx_cache4_evict of include/kmx.h): attention weights added up token by token, and the choice and the moves by
+ * which a sequence gets back to its budget.
+ */
+#include "cache4.h"
+
+#include <cmath>
+
+namespace kmx {
+
+/* ---------------------------------------------------------------- weights ------------------------ */
+
+struct Weigh4 {
+	Cache4 cache;
+	Batch4 batch;
+	const void* q; size_t q_token, q_head;
+	const float* lse;
+	float* weights; /* [page][head][token of the page] */
+	float scale;
+	bool bf16, vec;
+};
+
+constexpr uint32_t WEIGH_TOKENS = 256; /* of a work-group, 64 a wavefront */
+
+/*
+ * A work-group takes 256 tokens of one head of a sequence, whose keys its wavefronts unpack once and keep, four blocks each; the rows (query heads of the head, of all queries)
+ * come by 64 at a time through LDS, a tile of 16 from each wavefront. The keys are the second operand (v_mfma_f32_16x16x32_f16): scores come out as [row][token], so that
+ * the weights of a token, 2^(c s - log2(e) lse), are added up in the lane that has it, and four lanes at the end.
+ */
+template <int J>
+__global__ void __launch_bounds__(256)
+weigh4_kernel(Weigh4 a)
+{
+	constexpr uint32_t D = 32 * J;
+	__shared__ half8v queries[4][J][WAVE];
+	__shared__ float factors[4][16], sums[4][16];
+	__shared__ int32_t looks[4][16];
+	const uint32_t wave = (uint32_t)__builtin_amdgcn_readfirstlane((int)(threadIdx.x / WAVE)), lane = threadIdx.x % WAVE, i16 = lane % 16, kg = lane / 16;
+	const uint32_t head = blockIdx.x, s = blockIdx.y, from = blockIdx.z * WEIGH_TOKENS;
+	const Sequence seq = sequence_of(a.batch, s, a.cache.page_shift);
+	if (seq.queries == 0 || from >= visible_to(a.batch, seq, seq.queries - 1)) return;
+	const int32_t least = (int32_t)visible_to(a.batch, seq, 0);
+
+	/* the wavefront's blocks */
+	const Constant4 table = constant4(a.batch.table) + (size_t)s * a.batch.table_stride;
+	const uint32_t sub_bits = a.cache.page_shift - 4, begin = from + 64 * wave;
+	const Magnitudes mag = load_magnitudes(a.cache.levels, head, 0);
+	half8v keys[4][J];
+	bool known[4];
+	size_t to[4];
+	const bool some = begin < seq.length;
+	if (some) {
+#pragma unroll
+		for (int b = 0; b < 4; ++b) {
+			const uint32_t n = begin / 16 + b, entry = n >> sub_bits, sub = n & ((1u << sub_bits) - 1);
+			const uint32_t page = entry < a.batch.table_stride ? (uint32_t)table[entry] : ~0u;
+			known[b] = 16 * n < seq.length && page < a.cache.page_count;
+			const uint8_t* block = a.cache.blocks + block_offset<J>(a.cache, known[b] ? page : 0, head, known[b] ? sub : 0);
+			to[b] = (((size_t)(known[b] ? page : 0) * a.cache.heads + head) << a.cache.page_shift) + 16 * sub;
+			uint32_t codes[J];
+			if constexpr (J % 4 == 0) {
+				for (int i = 0; i < J / 4; ++i) { const u32x4 v = ((const u32x4*)(block + i16 * (D / 2) + kg * 4 * J))[i]; for (int e = 0; e < 4; ++e) codes[4 * i + e] = v[e]; }
+			} else {
+				for (int j = 0; j < J; ++j) codes[j] = ((const uint32_t*)(block + i16 * (D / 2) + kg * 4 * J))[j];
+			}
+			const uint16_t* scales = (const uint16_t*)(block + 16 * D) + i16 * J;
+#pragma unroll
+			for (int j = 0; j < J; ++j) {
+				uint32_t p[4];
+				unpack4<false>(codes[j], mag, p[0], p[1]);
+				unpack4<true>(codes[j], mag, p[2], p[3]);
+				const uint32_t scale = scales[j] | (uint32_t)scales[j] << 16;
+				keys[b][j] = __builtin_bit_cast(half8v, u32x4{ times(p[0], scale), times(p[1], scale), times(p[2], scale), times(p[3], scale) });
+			}
+		}
+	}
+	float w[4] = { 0.0f, 0.0f, 0.0f, 0.0f };
+	const bool cut = (int32_t)(begin + 64) > least; /* not all queries see all of the wavefront's tokens */
+	const uint64_t rows = (uint64_t)seq.queries * a.batch.group;
+	for (uint64_t first = 0; first < rows; first += 64) {
+		__syncthreads(); /* (the rows before are done with) */
+		if (first + 16 * wave < rows) {
+			const uint64_t row = first + 16 * wave + i16;
+			const bool there = row < rows;
+			const uint32_t token = there ? (uint32_t)(row / a.batch.group) : 0, query_head = head * a.batch.group + (there ? (uint32_t)(row % a.batch.group) : 0);
+			const uint16_t* p = (const uint16_t*)a.q + (size_t)(seq.first + token) * a.q_token + (size_t)query_head * a.q_head + 8 * kg;
+			float x[J][8], largest = 0.0f;
+#pragma unroll
+			for (int j = 0; j < J; ++j) {
+				const u32x4 raw = a.vec ? load_raw8(p + 32 * j, true) : load_raw8(p + 32 * j, false);
+				for (int e = 0; e < 8; ++e) {
+					x[j][e] = there ? raw_element(raw[e / 2], e % 2, a.bf16) : 0.0f;
+					largest = fmaxf(largest, fabsf(x[j][e]));
+				}
+			}
+			largest = fmaxf(largest, __shfl_xor(largest, 16));
+			largest = fmaxf(largest, __shfl_xor(largest, 32));
+			float factor;
+			const float by = query_scale(a.scale, largest, &factor);
+#pragma unroll
+			for (int j = 0; j < J; ++j) {
+				half8v v;
+				for (int e = 0; e < 8; ++e) v[e] = (_Float16)(x[j][e] * by);
+				queries[wave][j][lane] = v;
+			}
+			if (kg == 0) {
+				factors[wave][i16] = factor;
+				sums[wave][i16] = there ? -1.44269504088896341f * a.lse[(size_t)(seq.first + token) * a.batch.query_heads + query_head] : -__builtin_inff(); /* no such row: no weight */
+				looks[wave][i16] = there ? (int32_t)visible_to(a.batch, seq, token) : 0;
+			}
+		}
+		__syncthreads();
+		if (!some) continue;
+		const uint32_t tiles = (uint32_t)min((uint64_t)4, (rows - first + 15) / 16);
+		for (uint32_t n = 0; n < tiles; ++n) {
+			f32x4 sc[4];
+#pragma unroll
+			for (int b = 0; b < 4; ++b) sc[b] = f32x4{ 0.0f, 0.0f, 0.0f, 0.0f };
+#pragma unroll
+			for (int j = 0; j < J; ++j) {
+				const half8v v = queries[n][j][lane];
+#pragma unroll
+				for (int b = 0; b < 4; ++b) sc[b] = __builtin_amdgcn_mfma_f32_16x16x32_f16(v, keys[b][j], sc[b], 0, 0, 0);
+			}
+			const f32x4 factor = *(const f32x4*)&factors[n][4 * kg], less = *(const f32x4*)&sums[n][4 * kg];
+			if (cut) {
+				const i32x4 look = *(const i32x4*)&looks[n][4 * kg];
+#pragma unroll
+				for (int b = 0; b < 4; ++b)
+					for (int r = 0; r < 4; ++r) {
+						const float p = __builtin_amdgcn_exp2f(fmaf(sc[b][r], factor[r], less[r]));
+						w[b] += (int32_t)(begin + 16 * b + i16) < look[r] ? p : 0.0f;
+					}
+			} else {
+#pragma unroll
+				for (int b = 0; b < 4; ++b)
+					for (int r = 0; r < 4; ++r) w[b] += __builtin_amdgcn_exp2f(fmaf(sc[b][r], factor[r], less[r]));
+			}
+		}
+	}
+	if (!some) return;
+	float mine = 0.0f;
+	size_t at = 0;
+	bool store = false;
+#pragma unroll
+	for (int b = 0; b < 4; ++b) {
+		w[b] += __shfl_xor(w[b], 16);
+		w[b] += __shfl_xor(w[b], 32);
+		if ((int)kg == b) { mine = w[b]; at = to[b]; store = known[b] && begin + 16 * b + i16 < seq.length; }
+	}
+	/* one addition to a token of a sequence; of a page that several sequences have, each adds its own */
+	if (store) unsafeAtomicAdd(a.weights + at + i16, mine);
+}
+
+/* ---------------------------------------------------------------- choice ------------------------- */
+
+struct Evict4 {
+	Cache4 cache;
+	const int32_t* lengths;
+	const int32_t* table;
+	float* weights;
+	int32_t* kept; /* [sequence][head][keep] */
+	int32_t* left; /* [sequence] */
+	uint32_t sequences, table_stride, max_length, keep, first, recent;
+	uint32_t cached; /* tokens whose keys LDS holds */
+};
+
+constexpr uint32_t EVICT_THREADS = 1024, EVICT_WAVES = EVICT_THREADS / WAVE, EVICT_BINS = 2048;
+constexpr uint32_t EVICT_CACHED = 24576;   /* keys of a sequence that LDS holds: 96 KB */
+constexpr uint32_t EVICT_TOKENS = 1 << 18; /* of a sequence: a bit for each place, and a count for each 64 */
+
+__device__ __forceinline__ uint32_t evict_length(const Evict4& e, uint32_t s)
+{
+	const int32_t n = constant4(e.lengths)[s];
+	const uint64_t room = min((uint64_t)e.table_stride << e.cache.page_shift, (uint64_t)e.max_length);
+	return n > 0 ? (uint32_t)min((uint64_t)n, room) : 0;
+}
+/* where place t of a sequence's tokens has its weight; false: its page is not there */
+__device__ __forceinline__ bool weight_of(const Evict4& e, const int32_t* table, uint32_t head, uint32_t t, size_t* at)
+{
+	const uint32_t page = (uint32_t)table[t >> e.cache.page_shift];
+	*at = (((size_t)page * e.cache.heads + head) << e.cache.page_shift) + (t & ((1u << e.cache.page_shift) - 1));
+	return page < e.cache.page_count;
+}
+/* whole numbers in the order of the weights; NaN, and pages that are not there: the lowest */
+__device__ __forceinline__ uint32_t key_of(float w)
+{
+	const uint32_t u = __builtin_bit_cast(uint32_t, w + 0.0f); /* (one zero) */
+	return w != w ? 0 : u >> 31 ? ~u : u | 0x80000000u;
+}
+__device__ __forceinline__ uint32_t sum_below(const uint32_t* counts, uint32_t wave)
+{
+	uint32_t sum = 0;
+	for (uint32_t w = 0; w < wave; ++w) sum += counts[w];
+	return sum;
+}
+__device__ __forceinline__ uint64_t lanes_below(uint32_t lane) { return ((uint64_t)1 << lane) - 1; }
+
+/*
+ * One work-group a sequence and head. The threshold of the weights by counting them in 2048 equal shares of the range of their keys, then of the share that it lies in:
+ * three rounds at most. Then all places in order, each wavefront a run of them: which stay (of those at the threshold the first ones), which of the places below the
+ * edge become free, which tokens from the edge on have to move. The moving ones are listed at the begin of `kept` and go from there to the free places, the
+ * highest first: none of them lies below where it is listed.
+ */
+__global__ void __launch_bounds__(EVICT_THREADS)
+evict4_choose_kernel(Evict4 e)
+{
+	extern __shared__ __attribute__((aligned(16))) uint32_t lds[]; /* bits of the places that stay, free places before each 64, keys */
+	__shared__ uint32_t bins[EVICT_BINS], counts[3][EVICT_WAVES], found[3];
+	const uint32_t tid = threadIdx.x, wave = (uint32_t)__builtin_amdgcn_readfirstlane((int)(tid / WAVE)), lane = tid % WAVE;
+	const uint32_t head = blockIdx.x, s = blockIdx.y, n = evict_length(e, s);
+	int32_t* const kept = e.kept + ((size_t)s * e.cache.heads + head) * e.keep;
+	if (head == 0 && tid == 0) e.left[s] = (int32_t)min(n, e.keep);
+	if (n <= e.keep) {
+		for (uint32_t i = tid; i < e.keep; i += EVICT_THREADS) kept[i] = i < n ? (int32_t)i : -1;
+		return;
+	}
+	const int32_t* table = e.table + (size_t)s * e.table_stride;
+	const uint32_t edge = e.keep - e.recent, places = edge - e.first, rest = n - e.first - e.recent; /* `places` of the `rest` tokens stay: fewer */
+	const uint32_t words = (places + 63) / 64;
+	uint64_t* const bits = (uint64_t*)lds;
+	uint32_t* const before = lds + 2 * words;
+	uint32_t* const cache = before + words + words % 2;
+	const bool cached = rest <= e.cached;
+	auto key_at = [&](uint32_t x) {
+		size_t at;
+		return weight_of(e, table, head, e.first + x, &at) ? key_of(e.weights[at]) : 0u;
+	};
+	auto key = [&](uint32_t x) { return cached ? cache[x] : key_at(x); };
+
+	/* the range of the keys */
+	if (tid < 2) found[tid] = tid ? 0u : ~0u;
+	__syncthreads();
+	uint32_t low = ~0u, high = 0;
+	for (uint32_t x = tid; x < rest; x += EVICT_THREADS) {
+		const uint32_t k = key_at(x);
+		if (cached) cache[x] = k;
+		low = min(low, k);
+		high = max(high, k);
+	}
+	for (int d = 1; d < WAVE; d *= 2) {
+		low = min(low, (uint32_t)__shfl_xor((int)low, d));
+		high = max(high, (uint32_t)__shfl_xor((int)high, d));
+	}
+	if (lane == 0) {
+		atomicMin(&found[0], low);
+		atomicMax(&found[1], high);
+	}
+	__syncthreads();
+	low = found[0];
+	high = found[1];
+	uint32_t need = places; /* of the tokens between low and high */
+	while (need && low != high) {
+		uint32_t shift = 0;
+		while ((high - low) >> shift >= EVICT_BINS) ++shift;
+		for (uint32_t i = tid; i < EVICT_BINS; i += EVICT_THREADS) bins[i] = 0;
+		__syncthreads();
+		for (uint32_t x = tid; x < rest; x += EVICT_THREADS) {
+			const uint32_t k = key(x);
+			if (k >= low && k <= high) atomicAdd(&bins[(k - low) >> shift], 1u);
+		}
+		__syncthreads();
+		/* the share that holds the need-th largest: thread t has shares 2047 - 2 t and the one below */
+		const uint32_t upper = bins[EVICT_BINS - 1 - 2 * tid], lower = bins[EVICT_BINS - 2 - 2 * tid];
+		uint32_t upto = upper + lower;
+		for (uint32_t d = 1; d < WAVE; d *= 2) {
+			const uint32_t v = (uint32_t)__shfl_up((int)upto, d);
+			if (lane >= d) upto += v;
+		}
+		if (lane == WAVE - 1) counts[0][wave] = upto;
+		__syncthreads();
+		const uint32_t above = sum_below(counts[0], wave) + upto - upper - lower;
+		if (above < need && above + upper + lower >= need) {
+			const bool first = above + upper >= need;
+			found[0] = EVICT_BINS - (first ? 1 : 2) - 2 * tid;
+			found[1] = need - above - (first ? 0 : upper);
+		}
+		__syncthreads();
+		low += found[0] << shift;
+		high = min(high, low + ((1u << shift) - 1));
+		need = found[1];
+	}
+	const uint32_t threshold = need ? low : ~0u; /* above it all stay, at it the first `need` (without places: none) */
+
+	/* runs of places, whole 64s, a wavefront each */
+	const uint32_t run = ((rest + EVICT_WAVES - 1) / EVICT_WAVES + 63) / 64 * 64, begin = min(rest, wave * run), end = min(rest, begin + run);
+	uint32_t equal = 0;
+	for (uint32_t x0 = begin; x0 < end; x0 += WAVE) equal += (uint32_t)__popcll(__ballot(x0 + lane < end && key(x0 + lane) == threshold));
+	if (lane == 0) counts[0][wave] = equal;
+	__syncthreads();
+	const uint32_t equal_before = sum_below(counts[0], wave);
+	auto stays = [&](uint32_t x, uint32_t& seen) { /* bits of 64 places; seen: those at the threshold so far */
+		const uint32_t k = x < end ? key(x) : 0;
+		const uint64_t at = __ballot(x < end && k == threshold);
+		const uint64_t bit = __ballot(x < end && (k > threshold || (k == threshold && seen + (uint32_t)__popcll(at & lanes_below(lane)) < need)));
+		seen += (uint32_t)__popcll(at);
+		return bit;
+	};
+	uint32_t seen = equal_before, freed = 0, moved = 0;
+	for (uint32_t x0 = begin; x0 < end; x0 += WAVE) {
+		const uint64_t bit = stays(x0 + lane, seen), below = x0 >= places ? 0 : places - x0 >= 64 ? ~(uint64_t)0 : lanes_below(places - x0);
+		if (x0 < places && lane == 0) {
+			bits[x0 / 64] = bit;
+			before[x0 / 64] = freed;
+		}
+		freed += (uint32_t)__popcll(~bit & below);
+		moved += (uint32_t)__popcll(bit & ~below);
+	}
+	if (lane == 0) {
+		counts[1][wave] = freed;
+		counts[2][wave] = moved;
+	}
+	__syncthreads();
+	const uint32_t freed_before = sum_below(counts[1], wave);
+	moved = sum_below(counts[2], wave);
+	seen = equal_before;
+	for (uint32_t x0 = begin; x0 < end; x0 += WAVE) {
+		if (x0 < places && lane == 0) before[x0 / 64] += freed_before;
+		const uint64_t bit = stays(x0 + lane, seen), beyond = bit & (x0 >= places ? ~(uint64_t)0 : places - x0 >= 64 ? 0 : ~lanes_below(places - x0));
+		if (beyond >> lane & 1) kept[e.first + moved + (uint32_t)__popcll(beyond & lanes_below(lane))] = (int32_t)(e.first + x0 + lane);
+		moved += (uint32_t)__popcll(beyond);
+	}
+	__syncthreads();
+	for (uint32_t top = (places + EVICT_THREADS - 1) / EVICT_THREADS; top-- > 0;) {
+		const uint32_t x = top * EVICT_THREADS + tid;
+		int32_t from = (int32_t)(e.first + x);
+		bool free = false;
+		if (x < places) {
+			free = !(bits[x / 64] >> lane & 1);
+			if (free) from = kept[e.first + before[x / 64] + (uint32_t)__popcll(~bits[x / 64] & lanes_below(lane))];
+		}
+		__syncthreads();
+		if (x < places) {
+			kept[e.first + x] = from;
+			size_t a, b;
+			if (free && weight_of(e, table, head, e.first + x, &b)) e.weights[b] = weight_of(e, table, head, (uint32_t)from, &a) ? e.weights[a] : 0.0f;
+		}
+	}
+	for (uint32_t i = tid; i < e.first; i += EVICT_THREADS) kept[i] = (int32_t)i;
+	for (uint32_t i = tid; i < e.recent; i += EVICT_THREADS) kept[edge + i] = (int32_t)(n - e.recent + i);
+	__syncthreads();
+	/* the recent ones move down in their order, later ones from places that earlier ones do not go to */
+	for (uint32_t i0 = 0; i0 < e.recent; i0 += EVICT_THREADS) {
+		const uint32_t i = i0 + tid;
+		float w = 0.0f;
+		size_t at;
+		if (i < e.recent && weight_of(e, table, head, n - e.recent + i, &at)) w = e.weights[at];
+		__syncthreads();
+		if (i < e.recent && weight_of(e, table, head, edge + i, &at)) e.weights[at] = w;
+	}
+	__syncthreads();
+	for (uint32_t t = e.keep + tid; t < n; t += EVICT_THREADS) {
+		size_t at;
+		if (weight_of(e, table, head, t, &at)) e.weights[at] = 0.0f;
+	}
+}
+
+/* ---------------------------------------------------------------- moves -------------------------- */
+
+/* what a lane holds of a row: a word of the keys' codes, a byte of one or two pairs of the values' channels, half a word of the scales */
+template <int J> struct Row16 { uint32_t key; uint8_t value[J > 4 ? 2 : 1]; uint16_t scale; };
+
+template <int J>
+__device__ __forceinline__ Row16<J> take_row(const uint8_t* block, uint32_t t, uint32_t lane)
+{
+	constexpr uint32_t D = 32 * J;
+	Row16<J> r{};
+	if (lane < 4 * J) r.key = *(const uint32_t*)(block + t * (D / 2) + 4 * lane);
+#pragma unroll
+	for (int i = 0; i < (J > 4 ? 2 : 1); ++i)
+		if (lane + WAVE * i < 16 * J) r.value[i] = block[8 * D + 16 * (lane + WAVE * i) + t];
+	if (lane < 2 * J) r.scale = ((const uint16_t*)(block + 16 * D))[lane < J ? t * J + lane : 16 * J + 16 * (lane - J) + t];
+	return r;
+}
+template <int J>
+__device__ __forceinline__ void put_row(uint8_t* block, uint32_t t, uint32_t lane, const Row16<J>& r)
+{
+	constexpr uint32_t D = 32 * J;
+	if (lane < 4 * J) *(uint32_t*)(block + t * (D / 2) + 4 * lane) = r.key;
+#pragma unroll
+	for (int i = 0; i < (J > 4 ? 2 : 1); ++i)
+		if (lane + WAVE * i < 16 * J) block[8 * D + 16 * (lane + WAVE * i) + t] = r.value[i];
+	if (lane < 2 * J) ((uint16_t*)(block + 16 * D))[lane < J ? t * J + lane : 16 * J + 16 * (lane - J) + t] = r.scale;
+}
+
+/*
+ * Rows to their new places, a wavefront a row. Of a sequence and head the first work-group moves those that come from the places which the recent ones are about to
+ * take, and then these, in their order; the others share the rest, which come from behind all new places.
+ */
+template <int J>
+__global__ void __launch_bounds__(256)
+evict4_move_kernel(Evict4 e)
+{
+	const uint32_t wave = (uint32_t)__builtin_amdgcn_readfirstlane((int)(threadIdx.x / WAVE)), lane = threadIdx.x % WAVE;
+	const uint32_t head = blockIdx.x, s = blockIdx.y, n = evict_length(e, s);
+	if (n <= e.keep) return;
+	const int32_t* table = e.table + (size_t)s * e.table_stride;
+	const int32_t* kept = e.kept + ((size_t)s * e.cache.heads + head) * e.keep;
+	const uint32_t edge = e.keep - e.recent, page_mask = (1u << e.cache.page_shift) - 1;
+	auto block_of = [&](uint32_t t, bool* there) { /* t: the same in all lanes */
+		const uint32_t page = (uint32_t)__builtin_amdgcn_readfirstlane(table[t >> e.cache.page_shift]);
+		*there = page < e.cache.page_count;
+		return e.cache.blocks + block_offset<J>(e.cache, *there ? page : 0, head, (t & page_mask) / 16);
+	};
+	const bool begins = blockIdx.z == 0;
+	const uint32_t waves = begins ? 4 : 4 * (gridDim.z - 1), number = begins ? wave : 4 * (blockIdx.z - 1) + wave;
+	for (uint32_t i0 = e.first + 64 * number; i0 < edge; i0 += 64 * waves) {
+		const uint32_t from = i0 + lane < edge ? (uint32_t)kept[i0 + lane] : 0;
+		uint64_t moves = __ballot(i0 + lane < edge && (begins ? from >= edge && from < e.keep : from >= e.keep));
+		while (moves) {
+			constexpr int AT_ONCE = 4;
+			Row16<J> row[AT_ONCE];
+			uint32_t to[AT_ONCE];
+			bool good[AT_ONCE];
+#pragma unroll
+			for (int k = 0; k < AT_ONCE; ++k) {
+				good[k] = moves != 0;
+				if (!good[k]) continue;
+				const int bit = __ffsll((unsigned long long)moves) - 1;
+				moves &= moves - 1;
+				to[k] = i0 + (uint32_t)bit;
+				const uint32_t t = (uint32_t)__builtin_amdgcn_readlane((int)from, bit);
+				const uint8_t* block = block_of(t, &good[k]);
+				if (good[k]) row[k] = take_row<J>(block, t % 16, lane);
+			}
+#pragma unroll
+			for (int k = 0; k < AT_ONCE; ++k) {
+				if (!good[k]) continue;
+				bool there;
+				uint8_t* block = block_of(to[k], &there);
+				if (there) put_row<J>(block, to[k] % 16, lane, row[k]);
+			}
+		}
+	}
+	if (!begins) return;
+	for (uint32_t i0 = 0; i0 < e.recent; i0 += 32) {
+		__syncthreads(); /* what lay there has been read */
+		Row16<J> row[8];
+		bool good[8];
+#pragma unroll
+		for (int k = 0; k < 8; ++k) {
+			const uint32_t i = i0 + 8 * wave + k, t = n - e.recent + i;
+			good[k] = i < e.recent;
+			if (!good[k]) continue;
+			const uint8_t* block = block_of(t, &good[k]);
+			if (good[k]) row[k] = take_row<J>(block, t % 16, lane);
+		}
+		__syncthreads();
+#pragma unroll
+		for (int k = 0; k < 8; ++k) {
+			if (!good[k]) continue;
+			const uint32_t t = edge + i0 + 8 * wave + k;
+			bool there;
+			uint8_t* block = block_of(t, &there);
+			if (there) put_row<J>(block, t % 16, lane, row[k]);
+		}
+	}
+}
+
+} // namespace kmx
+
+using namespace kmx;
+
+extern "C" {
+
+int kmx_cache4_weigh(const kmx_cache4* cache, const kmx_cache4_batch* batch, int type, const void* q, size_t q_token_stride, size_t q_head_stride,
+                     const float* lse, float scale, int causal, float* weights)
+{
+	clear_error();
+	Weigh4 a{};
+	int rc = check_cache4("kmx_cache4_weigh", cache, &a.cache);
+	if (rc) return rc;
+	rc = check_batch4("kmx_cache4_weigh", cache, batch, causal, &a.batch);
+	if (rc) return rc;
+	rc = check_type("kmx_cache4_weigh", type, false);
+	if (rc) return rc;
+	if (!(std::fabs(scale) <= 3.4e38f)) return fail(KMX_ERR_INVALID_ARGUMENT, "kmx_cache4_weigh: the scale is not finite");
+	const uint64_t most = (uint64_t)a.batch.table_stride * cache->page_tokens;
+	const uint32_t longest = a.batch.max_length < most ? a.batch.max_length : (uint32_t)most;
+	if (batch->sequences == 0 || batch->tokens == 0 || batch->max_queries == 0 || longest == 0) return KMX_OK;
+	if (!q || !lse || !weights) return fail(KMX_ERR_INVALID_ARGUMENT, "kmx_cache4_weigh: null device pointer");
+	if ((uintptr_t)q % 2 || (uintptr_t)lse % 4 || (uintptr_t)weights % 4) return fail(KMX_ERR_INVALID_ARGUMENT, "kmx_cache4_weigh: rows start at multiples of their element's size");
+	a.q = q;
+	a.q_token = q_token_stride;
+	a.q_head = q_head_stride;
+	a.lse = lse;
+	a.weights = weights;
+	a.scale = scale;
+	a.bf16 = type == KMX_BF16;
+	a.vec = aligned_rows(q, q_token_stride, q_head_stride, 2);
+	const uint32_t chunks = (longest - 1) / WEIGH_TOKENS + 1;
+	if (batch->sequences > 65535 || chunks > 65535) return fail(KMX_ERR_UNSUPPORTED, "kmx_cache4_weigh: %u sequences of up to %u tokens are too many for one call", batch->sequences, longest);
+	switch (cache->dim / 32) {
+#define KMX_CASE(N) case N: KMX_LAUNCH_KERNEL((weigh4_kernel<N>), dim3(cache->heads, batch->sequences, chunks), dim3(256), 0, stream(), a); break;
+		KMX_CASE(1) KMX_CASE(2) KMX_CASE(3) KMX_CASE(4) KMX_CASE(5) KMX_CASE(6) KMX_CASE(7) KMX_CASE(8)
+#undef KMX_CASE
+	}
+	KMX_LAUNCH_CHECK("weigh4_kernel");
+	return KMX_OK;
+}
+
+int kmx_cache4_evict(const kmx_cache4* cache, const kmx_cache4_batch* batch, float* weights, uint32_t keep, uint32_t first, uint32_t recent, int32_t* kept, int32_t* left)
+{
+	clear_error();
+	Evict4 e{};
+	int rc = check_cache4("kmx_cache4_evict", cache, &e.cache);
+	if (rc) return rc;
+	if (!batch) return fail(KMX_ERR_INVALID_ARGUMENT, "kmx_cache4_evict: null batch");
+	if ((uint64_t)first + recent > keep) return fail(KMX_ERR_INVALID_ARGUMENT, "kmx_cache4_evict: %u tokens have no room for the %u first and %u recent ones", keep, first, recent);
+	if (batch->max_length > EVICT_TOKENS) return fail(KMX_ERR_UNSUPPORTED, "kmx_cache4_evict: sequences of up to %u tokens, at most %u", batch->max_length, EVICT_TOKENS);
+	if (batch->sequences == 0) return KMX_OK;
+	if (!batch->lengths || (batch->table_stride && !batch->table) || !weights || (keep && !kept) || !left) return fail(KMX_ERR_INVALID_ARGUMENT, "kmx_cache4_evict: null device pointer");
+	if ((uintptr_t)weights % 4 || (uintptr_t)kept % 4 || (uintptr_t)left % 4) return fail(KMX_ERR_INVALID_ARGUMENT, "kmx_cache4_evict: arrays start at multiples of their element's size");
+	if (left == batch->lengths) return fail(KMX_ERR_INVALID_ARGUMENT, "kmx_cache4_evict: lengths and what is left of them are two arrays");
+	if (batch->sequences > 65535) return fail(KMX_ERR_UNSUPPORTED, "kmx_cache4_evict: %u sequences are too many for one call", batch->sequences);
+	const uint32_t table_stride = cache->page_count ? batch->table_stride : 0;
+	const uint64_t most = (uint64_t)table_stride * cache->page_tokens;
+	const uint32_t longest = batch->max_length < most ? batch->max_length : (uint32_t)most;
+	e.lengths = batch->lengths;
+	e.table = batch->table;
+	e.weights = weights;
+	e.kept = kept;
+	e.left = left;
+	e.sequences = batch->sequences;
+	e.table_stride = table_stride;
+	e.max_length = batch->max_length;
+	e.keep = keep;
+	e.first = first;
+	e.recent = recent;
+	const uint32_t places = keep < longest ? keep - recent - first : 0, words = (places + 63) / 64;
+	e.cached = longest < EVICT_CACHED ? longest : EVICT_CACHED;
+	const uint32_t bytes = 4 * (2 * words + words + words % 2 + e.cached);
+	static int allowed = -1;
+	const DeviceInfo* dev = nullptr;
+	rc = device_info(&dev);
+	if (rc) return rc;
+	if (bytes > 32768 && allowed != dev->device) { /* more LDS than a launch may ask for unannounced, on this device */
+		KMX_HIP(hipFuncSetAttribute((const void*)evict4_choose_kernel, hipFuncAttributeMaxDynamicSharedMemorySize, (int)(4 * (EVICT_TOKENS / 64 * 3 + 2 + EVICT_CACHED))));
+		allowed = dev->device;
+	}
+	KMX_LAUNCH_KERNEL(evict4_choose_kernel, dim3(cache->heads, batch->sequences), dim3(EVICT_THREADS), bytes, stream(), e);
+	KMX_LAUNCH_CHECK("evict4_choose_kernel");
+	if (longest <= keep) return KMX_OK; /* nothing moves */
+	/* work-groups for the moves of a head: about 16 rows each, and two that do all where they are many anyway */
+	uint64_t parts = 1 + (places < longest - keep ? places : longest - keep) / 16;
+	const uint64_t units = (uint64_t)cache->heads * batch->sequences, enough = 8 * (uint64_t)dev->compute_units / units + 1;
+	if (parts > enough) parts = enough;
+	if (parts > 65534) parts = 65534;
+	switch (cache->dim / 32) {
+#define KMX_CASE(N) case N: KMX_LAUNCH_KERNEL((evict4_move_kernel<N>), dim3(cache->heads, batch->sequences, (unsigned)parts + 1), dim3(256), 0, stream(), e); break;
+		KMX_CASE(1) KMX_CASE(2) KMX_CASE(3) KMX_CASE(4) KMX_CASE(5) KMX_CASE(6) KMX_CASE(7) KMX_CASE(8)
+#undef KMX_CASE
+	}
+	KMX_LAUNCH_CHECK("evict4_move_kernel");
+	return KMX_OK;
+}
+
+} // extern "C"

@@ -1,0 +1,368 @@
+/*
+ * Attention over prompts (kmx_prompt_attend of include/kmx.h), kernels for J groups of 32 channels (one object per J: prompt_attend_inst.hip).
+ *
+ * For a row r (a query head of a query) that sees the tokens t < vis: o_r = sum_t p_rt v_t / l_r, p_rt = 2^(c s_rt - m_r), s_rt = +- q_r . k_t, c = |scale| log2(e),
+ * l_r = sum_t p_rt; lse_r = ln 2 (m_r + log2 l_r). m_r is any number near the largest c s_rt: it is raised when one passes it by more than 2^RISE, and what
+ * was added up before is lowered by as much.
+ */
+#ifndef KMX_PROMPT_ATTEND_IMPL_H
+#define KMX_PROMPT_ATTEND_IMPL_H
+
+#include "prompt_attend.h"
+
+namespace kmx {
+
+typedef float f32x16 __attribute__((ext_vector_type(16)));
+typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
+typedef short i16x4 __attribute__((ext_vector_type(4)));
+
+/*
+ * Probabilities are rounded to the type of the values for their product with them, sums are those of the floats. They are taken times 2^LIFT, and may pass the
+ * reference by 2^RISE: half precision holds them up to 2^15, with 11 bits down to 2^-21 of the reference and none below 2^-32; bfloat16 has 8 bits of all of them.
+ */
+constexpr float LIFT = 7.0f, RISE = 8.0f;
+
+__device__ __forceinline__ f32x16 product(const u32x4& a, const u32x4& b, const f32x16& c, __bf16)
+{
+	return __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8, a), __builtin_bit_cast(bf16x8, b), c, 0, 0, 0);
+}
+__device__ __forceinline__ f32x16 product(const u32x4& a, const u32x4& b, const f32x16& c, _Float16)
+{
+	return __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(half8v, a), __builtin_bit_cast(half8v, b), c, 0, 0, 0);
+}
+/* two numbers that are no NaN, or both whatever they are, rounded to the nearest */
+__device__ __forceinline__ uint32_t rounded_pair(float x, float y, __bf16)
+{
+	typedef __bf16 bf16x2 __attribute__((ext_vector_type(2)));
+	return __builtin_bit_cast(uint32_t, bf16x2{ (__bf16)x, (__bf16)y });
+}
+__device__ __forceinline__ uint32_t rounded_pair(float x, float y, _Float16)
+{
+	return __builtin_bit_cast(uint32_t, half2v{ (_Float16)x, (_Float16)y });
+}
+/* the larger one of a lane's and of that 32 lanes on (of the two results of the exchange the compiler would drop the second: it is hidden from it that they are) */
+__device__ __forceinline__ float both_halves_most(float v)
+{
+	const auto r = __builtin_amdgcn_permlane32_swap(__builtin_bit_cast(uint32_t, v), __builtin_bit_cast(uint32_t, v), false, false);
+	uint32_t low = r[0], high = r[1];
+	asm volatile("" : "+v"(low), "+v"(high));
+	return fmaxf(__builtin_bit_cast(float, low), __builtin_bit_cast(float, high));
+}
+/* 4 rows (tokens) x 16 columns of LDS: the lanes of each group of 16 hand in 8 bytes of a row, 4 lanes a row, and get 4 tokens of their column */
+__device__ __forceinline__ u32x2 read_turned(const uint8_t* p)
+{
+	return __builtin_bit_cast(u32x2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) i16x4*)(p)));
+}
+
+/* whether one of the 8 numbers is an infinity or NaN; those as zeros */
+template <typename T>
+__device__ __forceinline__ bool without_strange(u32x4& w)
+{
+	constexpr uint32_t EXPONENT = __is_same(T, __bf16) ? 0x7F80u : 0x7C00u;
+	bool found = false;
+#pragma unroll
+	for (int i = 0; i < 4; ++i) {
+		const bool low = (w[i] & EXPONENT) == EXPONENT, high = (w[i] >> 16 & EXPONENT) == EXPONENT;
+		w[i] &= (low ? 0u : 0xFFFFu) | (high ? 0u : 0xFFFF0000u);
+		found = found || low || high;
+	}
+	return found;
+}
+
+struct Prompt4 { uint32_t query_first, queries, token_first, tokens; };
+/* queries and tokens of sequence s, held to what there is */
+__device__ __forceinline__ Prompt4 prompt_of(const PromptAttend& a, uint32_t s)
+{
+	const int32_t from = constant4(a.query_starts)[s], to = constant4(a.query_starts)[s + 1], begin = constant4(a.token_starts)[s], end = constant4(a.token_starts)[s + 1];
+	Prompt4 p{ 0, 0, 0, 0 };
+	if (from >= 0 && to > from && (uint32_t)to <= a.queries) {
+		p.query_first = (uint32_t)from;
+		p.queries = min((uint32_t)(to - from), a.max_queries);
+	}
+	if (begin >= 0 && end > begin && (uint32_t)end <= a.tokens) {
+		p.token_first = (uint32_t)begin;
+		p.tokens = min((uint32_t)(end - begin), a.max_tokens);
+	}
+	return p;
+}
+__device__ __forceinline__ int32_t sees_of(const PromptAttend& a, const Prompt4& p, uint32_t query)
+{
+	if (!a.causal) return (int32_t)p.tokens;
+	const int64_t n = (int64_t)p.tokens - p.queries + query + 1;
+	return n > 0 ? (int32_t)n : 0;
+}
+
+template <int J> constexpr uint32_t key_row() { return 64 * J + 16; }                       /* bytes: 8 tokens one below the other read 8 groups of banks */
+template <int J> constexpr uint32_t value_row() { return 64 * J + (J % 2 ? 0 : 64); }       /* 64 or 192 bytes on in the banks: 4 tokens side by side */
+template <int J> constexpr uint32_t prompt_lds() { return 2 * 32 * (key_row<J>() + value_row<J>()); }
+
+/*
+ * A work-group of four wavefronts takes 128 B rows of one head of the keys (the query heads of a query side by side, then the next query's), 32 B a wavefront. Tiles of
+ * 32 tokens pass through LDS as they are, two of keys and two of values. Both products have the cache's side as their first operand
+ * (v_mfma_f32_32x32x16): scores come out as [token][row], a lane has 16 scores of its row, and its probabilities are, as they stand, its piece of the second
+ * operand of [channel][row] = values . p; the values' columns are turned on the way from LDS (ds_read_b64_tr_b16).
+ */
+template <typename T, int J, int B>
+__global__ void __launch_bounds__(256, J <= 2 ? 2 : 1)
+prompt_attend_kernel(PromptAttend a)
+{
+	constexpr uint32_t KROW = key_row<J>(), VROW = value_row<J>(), KTILE = 32 * KROW, VTILE = 32 * VROW;
+	constexpr int PIECES = (4 * J * 32 + 255) / 256; /* of 16 bytes that a lane brings of a tile */
+	extern __shared__ __attribute__((aligned(16))) uint8_t lds[];
+	__shared__ uint32_t strange; /* values that are no numbers, where not all rows see them */
+	uint8_t* const keys = lds;
+	uint8_t* const values = lds + 2 * KTILE;
+	const uint32_t tid = threadIdx.x, wave = (uint32_t)__builtin_amdgcn_readfirstlane((int)(tid / WAVE)), lane = tid % WAVE, n32 = lane % 32, h = lane / 32;
+	/* heads take turns over the dies, and the rows that see the most come first */
+	const uint32_t head = blockIdx.x % a.heads, rest = blockIdx.x / a.heads, s = rest % a.sequences, row_tile = a.row_tiles - 1 - rest / a.sequences;
+	const Prompt4 p = prompt_of(a, s);
+	const uint64_t all_rows = (uint64_t)p.queries * a.group, first_row = (uint64_t)row_tile * (128 * B);
+	if (first_row >= all_rows) return;
+	const uint32_t rows = (uint32_t)min((uint64_t)(128 * B), all_rows - first_row);
+	const uint32_t first_query = (uint32_t)(first_row / a.group), last_query = (uint32_t)((first_row + rows - 1) / a.group);
+	const uint32_t end = ((uint32_t)sees_of(a, p, last_query) + 31) / 32; /* tiles */
+	const int32_t all_see = sees_of(a, p, first_query);
+
+	/* the rows of the lane, what those of its wavefront see at least and at most */
+	const uint32_t wave_first = 32 * B * wave, wave_rows = rows > wave_first ? min(32u * B, rows - wave_first) : 0;
+	uint32_t query[B], query_head[B];
+	int32_t sees[B];
+	bool there[B];
+#pragma unroll
+	for (int b = 0; b < B; ++b) {
+		there[b] = 32 * b + n32 < wave_rows;
+		const uint64_t x = first_row + (there[b] ? wave_first + 32 * b + n32 : 0);
+		query[b] = (uint32_t)(x / a.group);
+		query_head[b] = head * a.group + (uint32_t)(x - (uint64_t)query[b] * a.group);
+		sees[b] = there[b] ? sees_of(a, p, query[b]) : 0;
+	}
+	const int32_t least = wave_rows ? sees_of(a, p, (uint32_t)((first_row + wave_first) / a.group)) : 0;
+	const int32_t seen = wave_rows ? sees_of(a, p, (uint32_t)((first_row + wave_first + wave_rows - 1) / a.group)) : 0;
+
+	u32x4 q[B][2 * J]; /* channels 16 c + 8 h .. + 7 */
+#pragma unroll
+	for (int b = 0; b < B; ++b) {
+		const uint16_t* from = (const uint16_t*)a.q + (size_t)(p.query_first + query[b]) * a.q_token + (size_t)query_head[b] * a.q_head + 8 * h;
+		if (a.vec) {
+#pragma unroll
+			for (int c = 0; c < 2 * J; ++c) q[b][c] = load_raw8(from + 16 * c, true);
+		} else {
+#pragma unroll
+			for (int c = 0; c < 2 * J; ++c) q[b][c] = load_raw8(from + 16 * c, false);
+		}
+#pragma unroll
+		for (int c = 0; c < 2 * J; ++c)
+			for (int e = 0; e < 4; ++e) q[b][c][e] = (q[b][c][e] & a.q_keep) ^ a.q_turn; /* the sign of the scale; nothing of them where it is 0 */
+	}
+
+	const uint16_t* const key_rows = (const uint16_t*)a.k + (size_t)p.token_first * a.token_stride + (size_t)head * a.head_stride;
+	const uint16_t* const value_rows = (const uint16_t*)a.v + (size_t)p.token_first * a.token_stride + (size_t)head * a.head_stride;
+	struct Staged { u32x4 w[PIECES]; };
+	auto fetch = [&](Staged& g, const uint16_t* from, uint32_t tile) {
+#pragma unroll
+		for (int i = 0; i < PIECES; ++i) {
+			const uint32_t piece = tid + 256 * i, token = 32 * tile + piece / (4 * J), part = piece % (4 * J);
+			if (4 * J * 32 % 256 && piece >= 4 * J * 32) continue;
+			const uint16_t* at = from + (size_t)min(token, p.tokens - 1) * a.token_stride + 8 * part;
+			g.w[i] = a.vec ? load_raw8(at, true) : load_raw8(at, false);
+			if (token >= p.tokens) g.w[i] = u32x4{ 0, 0, 0, 0 };
+		}
+	};
+	auto store_keys = [&](const Staged& g, uint32_t tile) {
+#pragma unroll
+		for (int i = 0; i < PIECES; ++i) {
+			const uint32_t piece = tid + 256 * i;
+			if (4 * J * 32 % 256 && piece >= 4 * J * 32) continue;
+			*(u32x4*)(keys + tile % 2 * KTILE + piece / (4 * J) * KROW + 16 * (piece % (4 * J))) = g.w[i];
+		}
+	};
+	auto store_values = [&](Staged& g, uint32_t tile) {
+		if ((int32_t)(32 * tile + 32) > all_see) { /* not all rows see all of the tile: 0 times an infinity must not come in */
+			bool found = false;
+#pragma unroll
+			for (int i = 0; i < PIECES; ++i) {
+				if (4 * J * 32 % 256 && tid + 256 * i >= 4 * J * 32) continue;
+				found = without_strange<T>(g.w[i]) || found;
+			}
+			if (found) strange = 1;
+		}
+#pragma unroll
+		for (int i = 0; i < PIECES; ++i) {
+			const uint32_t piece = tid + 256 * i;
+			if (4 * J * 32 % 256 && piece >= 4 * J * 32) continue;
+			*(u32x4*)(values + tile % 2 * VTILE + piece / (4 * J) * VROW + 16 * (piece % (4 * J))) = g.w[i];
+		}
+	};
+
+	float reference[B], base[B], l[B];
+	f32x16 o[B][J];
+#pragma unroll
+	for (int b = 0; b < B; ++b) {
+		reference[b] = -__builtin_inff();
+		base[b] = LIFT;
+		l[b] = 0.0f;
+#pragma unroll
+		for (int j = 0; j < J; ++j)
+			for (int e = 0; e < 16; ++e) o[b][j][e] = 0.0f;
+	}
+
+	const uint8_t* const key_at = keys + n32 * KROW + 16 * h;
+	const uint8_t* const value_at = values + (4 * h + lane % 16 / 4) * VROW + 32 * (lane / 16 % 2) + 8 * (lane % 4);
+	auto work = [&](uint32_t tile) {
+		const uint8_t* const k = key_at + tile % 2 * KTILE;
+		const uint8_t* const v = value_at + tile % 2 * VTILE;
+		f32x16 sc[B];
+#pragma unroll
+		for (int b = 0; b < B; ++b)
+			for (int e = 0; e < 16; ++e) sc[b][e] = 0.0f;
+#pragma unroll
+		for (int c = 0; c < 2 * J; ++c) {
+			const u32x4 w = *(const u32x4*)(k + 32 * c);
+#pragma unroll
+			for (int b = 0; b < B; ++b) sc[b] = product(w, q[b][c], sc[b], T{});
+		}
+		const int32_t from = (int32_t)(32 * tile);
+		if (least - from < 32) {
+#pragma unroll
+			for (int b = 0; b < B; ++b)
+#pragma unroll
+				for (int e = 0; e < 16; ++e) sc[b][e] = 8 * (e / 4) + 4 * (int32_t)h + e % 4 < sees[b] - from ? sc[b][e] : -__builtin_inff();
+		}
+		u32x4 pr[B][2];
+		float top[B];
+		bool rises = false;
+#pragma unroll
+		for (int b = 0; b < B; ++b) {
+			float t = sc[b][0];
+#pragma unroll
+			for (int e = 1; e < 16; ++e) t = fmaxf(t, sc[b][e]);
+			top[b] = both_halves_most(t) * a.factor;
+			rises = rises || top[b] > reference[b] + RISE;
+		}
+		if (__any(rises)) {
+#pragma unroll
+			for (int b = 0; b < B; ++b) {
+				const float now = fmaxf(reference[b], top[b]), less = now == reference[b] ? 1.0f : __builtin_amdgcn_exp2f(reference[b] - now);
+				reference[b] = now;
+				base[b] = now == -__builtin_inff() ? LIFT : LIFT - now;
+				l[b] *= less;
+#pragma unroll
+				for (int j = 0; j < J; ++j) o[b][j] *= less;
+			}
+		}
+#pragma unroll
+		for (int b = 0; b < B; ++b) {
+#pragma unroll
+			for (int e = 0; e < 16; e += 2) {
+				const float x = __builtin_amdgcn_exp2f(fmaf(sc[b][e], a.factor, base[b])), y = __builtin_amdgcn_exp2f(fmaf(sc[b][e + 1], a.factor, base[b]));
+				l[b] += x;
+				l[b] += y;
+				pr[b][e / 8][e % 8 / 2] = rounded_pair(x, y, T{});
+			}
+		}
+#pragma unroll
+		for (int j = 0; j < J; ++j)
+#pragma unroll
+			for (int c = 0; c < 2; ++c) {
+				const u32x2 low = read_turned(v + 16 * c * VROW + 64 * j), high = read_turned(v + (16 * c + 8) * VROW + 64 * j);
+				const u32x4 w{ low[0], low[1], high[0], high[1] };
+#pragma unroll
+				for (int b = 0; b < B; ++b) o[b][j] = product(w, pr[b][c], o[b][j], T{});
+			}
+	};
+
+	if (tid == 0) strange = 0;
+	__syncthreads();
+	if (end) {
+		Staged gk, gv;
+		fetch(gk, key_rows, 0);
+		fetch(gv, value_rows, 0);
+		store_keys(gk, 0);
+		store_values(gv, 0);
+		fetch(gk, key_rows, min(1u, end - 1));
+		fetch(gv, value_rows, min(1u, end - 1));
+		__syncthreads();
+		for (uint32_t tile = 0; tile < end; ++tile) {
+			if (tile + 1 < end) {
+				store_keys(gk, tile + 1);
+				store_values(gv, tile + 1);
+			}
+			if (tile + 2 < end) {
+				fetch(gk, key_rows, tile + 2);
+				fetch(gv, value_rows, tile + 2);
+			}
+			if ((int32_t)(32 * tile) < seen) work(tile);
+			__syncthreads();
+		}
+	}
+
+	if (strange) { /* infinities and NaN come to the rows that see them (their weights are above 0, however small) */
+#pragma unroll 1
+		for (uint32_t t = (uint32_t)all_see / 32 * 32; t < p.tokens && t < 32 * end; ++t) {
+			const uint16_t* from = value_rows + (size_t)t * a.token_stride;
+#pragma unroll
+			for (int j = 0; j < J; ++j)
+#pragma unroll
+				for (int e = 0; e < 16; ++e) {
+					const float x = raw_element(from[32 * j + 8 * (e / 4) + 4 * h + e % 4], false, __is_same(T, __bf16));
+					const bool number = fabsf(x) <= 3.4028235e38f;
+#pragma unroll
+					for (int b = 0; b < B; ++b) o[b][j][e] += !number && (int32_t)t < sees[b] ? x : 0.0f;
+				}
+		}
+	}
+
+#pragma unroll
+	for (int b = 0; b < B; ++b) {
+		l[b] += __shfl_xor(l[b], 32);
+		if (!there[b]) continue;
+		const float by = l[b] > 0.0f ? 1.0f / l[b] : l[b] == l[b] ? 0.0f : l[b]; /* a row that sees nothing is zero; NaN stays */
+		uint16_t* to = (uint16_t*)a.out + (size_t)(p.query_first + query[b]) * a.out_token + (size_t)query_head[b] * a.out_head;
+#pragma unroll
+		for (int j = 0; j < J; ++j)
+			for (int e = 0; e < 4; ++e) {
+				uint32_t w[4];
+				for (int r = 0; r < 4; ++r) w[r] = bits16<T>(o[b][j][4 * e + r] * by);
+				uint16_t* at = to + 32 * j + 8 * e + 4 * h;
+				if (a.vec) *(u32x2*)at = u32x2{ w[0] | w[1] << 16, w[2] | w[3] << 16 };
+				else
+					for (int r = 0; r < 4; ++r) at[r] = (uint16_t)w[r];
+			}
+		if (h == 0 && a.lse)
+			a.lse[(size_t)(p.query_first + query[b]) * a.query_heads + query_head[b]] = l[b] == 0.0f ? -__builtin_inff() : (reference[b] + log2f(l[b]) - LIFT) * 0.693147180559945309f;
+	}
+}
+
+template <typename T, int J>
+static int launch_prompt_of(PromptAttend a)
+{
+	constexpr int B = J <= 4 ? 2 : 1;
+	const uint64_t rows = (uint64_t)a.max_queries * a.group;
+	const uint64_t row_tiles = (rows + 128 * B - 1) / (128 * B), units = row_tiles < 0x80000000u ? row_tiles * a.heads * a.sequences : ~0ull;
+	if ((uint64_t)a.heads * a.sequences > 0x7FFFFFFFu || units > 0x7FFFFFFFu) return fail(KMX_ERR_UNSUPPORTED, "kmx_prompt_attend: too many queries for one call");
+	a.row_tiles = (uint32_t)row_tiles;
+	constexpr uint32_t bytes = prompt_lds<J>();
+	if (bytes > 65536 - 64) { /* more LDS than a launch may ask for unannounced, on this device */
+		static int allowed = -1;
+		const DeviceInfo* dev = nullptr;
+		const int rc = device_info(&dev);
+		if (rc) return rc;
+		if (allowed != dev->device) {
+			KMX_HIP(hipFuncSetAttribute((const void*)prompt_attend_kernel<T, J, B>, hipFuncAttributeMaxDynamicSharedMemorySize, (int)bytes));
+			allowed = dev->device;
+		}
+	}
+	KMX_LAUNCH_KERNEL((prompt_attend_kernel<T, J, B>), dim3((unsigned)units), dim3(256), bytes, stream(), a);
+	KMX_LAUNCH_CHECK("prompt_attend_kernel");
+	return KMX_OK;
+}
+
+template <int J>
+int launch_prompt_attend(const PromptAttend& a, bool bf16)
+{
+	return bf16 ? launch_prompt_of<__bf16, J>(a) : launch_prompt_of<_Float16, J>(a);
+}
+
+} // namespace kmx
+
+#endif

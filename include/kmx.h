@@ -497,6 +497,84 @@ int kmx_cache4_attend(const kmx_cache4* cache, const kmx_cache4_batch* batch, in
  * pages. Of the batch it looks at the numbers only. */
 int kmx_cache4_reserve(const kmx_cache4* cache, const kmx_cache4_batch* batch, uint32_t top);
 
+/*
+ * Attention for sequences that share prefixes (the same instructions, the same document): what is common to them is looked at once for all their queries. Sequence p of
+ * `prefix` is a prefix, with the cached tokens that its table says, all of which the rows starts[p] .. starts[p + 1] - 1 see -- those of all its sequences, side by side;
+ * `batch` has the sequences' own tokens, which come behind the prefix. tokens and query_heads are the same in both. out and lse are those of one softmax over both, causal
+ * in the own tokens. A row that no prefix has sees its own tokens only; rows that no sequence of `batch` has are left as they were. Everything else as for kmx_cache4_attend.
+ * The work space is that of the attention to each, and dim + 2 floats for each row and query head: kmx_cache4_reserve_shared.
+ */
+int kmx_cache4_attend_shared(const kmx_cache4* cache, const kmx_cache4_batch* prefix, const kmx_cache4_batch* batch, int type, const void* q, size_t q_token_stride,
+                             size_t q_head_stride, void* out, size_t out_token_stride, size_t out_head_stride, float* lse, float scale, int causal);
+int kmx_cache4_reserve_shared(const kmx_cache4* cache, const kmx_cache4_batch* prefix, const kmx_cache4_batch* batch);
+
+/*
+ * Attention weights added up: weights[page][head][token of the page] += sum over the queries that see the token, and the query heads of the head, of
+ * exp(scale q . k - lse), lse as kmx_cache4_attend (or _attend_shared, for prefix and own tokens each) has written it for the same queries. Tokens of a page that several
+ * sequences have get all of their weights. Floats; nothing is added for pages that are not there.
+ */
+int kmx_cache4_weigh(const kmx_cache4* cache, const kmx_cache4_batch* batch, int type, const void* q, size_t q_token_stride, size_t q_head_stride,
+                     const float* lse, float scale, int causal, float* weights);
+
+/*
+ * Sequences of more than `keep` tokens back to that many, for each head its own. Of the batch sequences, max_length (at most 262144), lengths and table are looked at; its pages
+ * belong to one sequence each. The `first` first and `recent` last tokens stay, and of the others those of the largest weights, the lower place of two as heavy (NaN
+ * are the lightest). The recent ones become the last ones, in their order; of the others those below keep - recent stay where they are, and what has to leave there makes room for
+ * the others, the lowest place for the lowest: no more rows move than have to, and a sequence's tokens are not in their order any more but for the recent ones. Weights
+ * move with their rows, and are zero at the places behind. kept[sequence][head][i] is the place that the token of place i had, -1 behind the last; left[sequence] what is left of
+ * its length (an array of its own). Shorter sequences stay as they are. Bounds of pages are not kept up: kmx_cache4_bound, before the next kmx_cache4_select.
+ */
+int kmx_cache4_evict(const kmx_cache4* cache, const kmx_cache4_batch* batch, float* weights, uint32_t keep, uint32_t first, uint32_t recent, int32_t* kept, int32_t* left);
+
+/*
+ * ---- around the cache (no counterpart in the reference) ----
+ * Rotary positions: of each row the first `channels` channels are pairs (a, b) -- i and i + channels / 2 with `halves`, else 2 i and 2 i + 1 -- that become
+ * gain (a cos x - b sin x), gain (a sin x + b cos x), x = 2 pi positions[token] turns[i] / 2^64, with `inverse` -x (times gain^2 that is the way back, and for a gradient the
+ * transpose). The other channels stay. In floats, rounded to the type once. Up to 4 sets of rows (queries, keys) with the positions of the same tokens in one call; out is in, with its
+ * strides, or apart from it. F32, F16, BF16; element (token, head, channel) as for kmx_cache4_write. positions may be negative.
+ */
+typedef struct kmx_rotary_rows {
+	const void* in;
+	void* out;
+	size_t in_token_stride;
+	size_t in_head_stride;
+	size_t out_token_stride;
+	size_t out_head_stride;
+	uint32_t heads;
+} kmx_rotary_rows;
+
+/* turns[channels / 2] as kmx_rotary takes them, host arrays: the frequency of pair i, f = base^(-2 i / channels) radians a position, in 2^-64 of a turn. Stretched for contexts
+ * longer than the `length` that was trained on: f (share + (1 - share) / stretch), where share goes from 0, at `slow` turns over that length and less, to 1, at `fast` and more
+ * (length 0: share is 0, all frequencies are divided; stretch 1: none). Host only. */
+int kmx_rotary_turns(uint32_t channels, double base, double stretch, double length, double slow, double fast, uint64_t* turns);
+
+int kmx_rotary(int type, const kmx_rotary_rows* rows, uint32_t sets, uint32_t tokens, uint32_t dim, uint32_t channels, const uint64_t* turns, const int32_t* positions,
+               int halves, int inverse, float gain);
+
+/*
+ * Attention over prompts, on their rows as they are before they go to the cache. Sequence s has the queries query_starts[s] .. query_starts[s + 1] - 1 and the keys and values
+ * token_starts[s] .. token_starts[s + 1] - 1 of the rows handed over; its queries are those of its last tokens: with `causal` query i of n sees the first tokens - n + i + 1 of
+ * them, else all. out and lse as for kmx_cache4_attend; nothing that a query does not see, infinities and NaN among it, comes into its row. dim: a multiple of 32 up to 256.
+ * F16 or BF16, products of numbers as they are, probabilities rounded to the type before the second product, sums in floats. Starts on the device are not trusted: a sequence whose
+ * starts are not within the rows has none. max_queries and max_tokens bound queries and tokens of a sequence (more is cut off).
+ */
+typedef struct kmx_prompt {
+	uint32_t sequences;
+	uint32_t query_heads; /* a multiple of heads: the query heads h g .. h g + g - 1 look at head h */
+	uint32_t heads;
+	uint32_t dim;
+	uint32_t queries;     /* rows of queries in all */
+	uint32_t tokens;      /* rows of keys and values in all */
+	uint32_t max_queries;
+	uint32_t max_tokens;
+	const int32_t* query_starts; /* sequences + 1, ascending from 0 */
+	const int32_t* token_starts;
+} kmx_prompt;
+
+int kmx_prompt_attend(const kmx_prompt* prompt, int type, const void* q, size_t q_token_stride, size_t q_head_stride,
+                      const void* keys, const void* values, size_t token_stride, size_t head_stride,
+                      void* out, size_t out_token_stride, size_t out_head_stride, float* lse, float scale, int causal);
+
 /* Message of the last failed call on this thread ("" if none). */
 const char* kmx_last_error(void);
 
