@@ -98,16 +98,19 @@ template <int J> constexpr uint32_t prompt_lds() { return 2 * 32 * (key_row<J>()
 
 /*
  * A work-group of four wavefronts takes 128 B rows of one head of the keys (the query heads of a query side by side, then the next query's), 32 B a wavefront. Tiles of
- * 32 tokens pass through LDS as they are, two of keys and two of values. Both products have the cache's side as their first operand
- * (v_mfma_f32_32x32x16): scores come out as [token][row], a lane has 16 scores of its row, and its probabilities are, as they stand, its piece of the second
- * operand of [channel][row] = values . p; the values' columns are turned on the way from LDS (ds_read_b64_tr_b16).
+ * 32 tokens pass through LDS as they are, two of keys and two of values, from registers that were loaded two tiles before. Both products have the cache's side as
+ * their first operand (v_mfma_f32_32x32x16): scores come out as [token][row], a lane has 16 scores of its row, and its probabilities are, as they stand, its piece of the
+ * second operand of [channel][row] = values . p; the values' columns are turned on the way from LDS (ds_read_b64_tr_b16).
+ * While the vector units make a tile's probabilities, the matrix cores have the scores of the next one and the sums of the one before: nothing of these three waits for
+ * another. The probabilities are made against the reference as it was; where a score passes it by too much they are made again.
  */
-template <typename T, int J, int B>
+template <typename T, int J, int B, bool VEC>
 __global__ void __launch_bounds__(256, J <= 2 ? 2 : 1)
 prompt_attend_kernel(PromptAttend a)
 {
 	constexpr uint32_t KROW = key_row<J>(), VROW = value_row<J>(), KTILE = 32 * KROW, VTILE = 32 * VROW;
 	constexpr int PIECES = (4 * J * 32 + 255) / 256; /* of 16 bytes that a lane brings of a tile */
+	constexpr bool UNEVEN = 4 * J * 32 % 256 != 0;
 	extern __shared__ __attribute__((aligned(16))) uint8_t lds[];
 	__shared__ uint32_t strange; /* values that are no numbers, where not all rows see them */
 	uint8_t* const keys = lds;
@@ -116,14 +119,13 @@ prompt_attend_kernel(PromptAttend a)
 	/* heads take turns over the dies, and the rows that see the most come first */
 	const uint32_t head = blockIdx.x % a.heads, rest = blockIdx.x / a.heads, s = rest % a.sequences, row_tile = a.row_tiles - 1 - rest / a.sequences;
 	const Prompt4 p = prompt_of(a, s);
-	const uint64_t all_rows = (uint64_t)p.queries * a.group, first_row = (uint64_t)row_tile * (128 * B);
+	const uint32_t all_rows = p.queries * a.group, first_row = row_tile * (128 * B); /* (31 bits) */
 	if (first_row >= all_rows) return;
-	const uint32_t rows = (uint32_t)min((uint64_t)(128 * B), all_rows - first_row);
-	const uint32_t first_query = (uint32_t)(first_row / a.group), last_query = (uint32_t)((first_row + rows - 1) / a.group);
-	const uint32_t end = ((uint32_t)sees_of(a, p, last_query) + 31) / 32; /* tiles */
-	const int32_t all_see = sees_of(a, p, first_query);
+	const uint32_t rows = min(128u * B, all_rows - first_row);
+	const uint32_t end = ((uint32_t)sees_of(a, p, (first_row + rows - 1) / a.group) + 31) / 32; /* tiles */
+	const int32_t all_see = sees_of(a, p, first_row / a.group);
 
-	/* the rows of the lane, what those of its wavefront see at least and at most */
+	/* the rows of the lane, what those of its wavefront see at least, and the tiles they look at */
 	const uint32_t wave_first = 32 * B * wave, wave_rows = rows > wave_first ? min(32u * B, rows - wave_first) : 0;
 	uint32_t query[B], query_head[B];
 	int32_t sees[B];
@@ -131,67 +133,49 @@ prompt_attend_kernel(PromptAttend a)
 #pragma unroll
 	for (int b = 0; b < B; ++b) {
 		there[b] = 32 * b + n32 < wave_rows;
-		const uint64_t x = first_row + (there[b] ? wave_first + 32 * b + n32 : 0);
-		query[b] = (uint32_t)(x / a.group);
-		query_head[b] = head * a.group + (uint32_t)(x - (uint64_t)query[b] * a.group);
+		const uint32_t x = first_row + (there[b] ? wave_first + 32 * b + n32 : 0);
+		query[b] = x / a.group;
+		query_head[b] = head * a.group + (x - query[b] * a.group);
 		sees[b] = there[b] ? sees_of(a, p, query[b]) : 0;
 	}
-	const int32_t least = wave_rows ? sees_of(a, p, (uint32_t)((first_row + wave_first) / a.group)) : 0;
-	const int32_t seen = wave_rows ? sees_of(a, p, (uint32_t)((first_row + wave_first + wave_rows - 1) / a.group)) : 0;
+	const int32_t least = wave_rows ? sees_of(a, p, (first_row + wave_first) / a.group) : 0;
+	const uint32_t mine = wave_rows ? ((uint32_t)sees_of(a, p, (first_row + wave_first + wave_rows - 1) / a.group) + 31) / 32 : 0;
 
 	u32x4 q[B][2 * J]; /* channels 16 c + 8 h .. + 7 */
 #pragma unroll
 	for (int b = 0; b < B; ++b) {
 		const uint16_t* from = (const uint16_t*)a.q + (size_t)(p.query_first + query[b]) * a.q_token + (size_t)query_head[b] * a.q_head + 8 * h;
-		if (a.vec) {
 #pragma unroll
-			for (int c = 0; c < 2 * J; ++c) q[b][c] = load_raw8(from + 16 * c, true);
-		} else {
-#pragma unroll
-			for (int c = 0; c < 2 * J; ++c) q[b][c] = load_raw8(from + 16 * c, false);
-		}
-#pragma unroll
-		for (int c = 0; c < 2 * J; ++c)
+		for (int c = 0; c < 2 * J; ++c) {
+			q[b][c] = load_raw8(from + 16 * c, VEC);
 			for (int e = 0; e < 4; ++e) q[b][c][e] = (q[b][c][e] & a.q_keep) ^ a.q_turn; /* the sign of the scale; nothing of them where it is 0 */
+		}
 	}
 
+	/* what lies behind the last token is the last token again: no row sees it */
 	const uint16_t* const key_rows = (const uint16_t*)a.k + (size_t)p.token_first * a.token_stride + (size_t)head * a.head_stride;
 	const uint16_t* const value_rows = (const uint16_t*)a.v + (size_t)p.token_first * a.token_stride + (size_t)head * a.head_stride;
-	struct Staged { u32x4 w[PIECES]; };
-	auto fetch = [&](Staged& g, const uint16_t* from, uint32_t tile) {
+	struct Staged { u32x4 k[PIECES], v[PIECES]; };
+	auto fetch = [&](u32x4 (&w)[PIECES], const uint16_t* from, uint32_t tile) {
 #pragma unroll
 		for (int i = 0; i < PIECES; ++i) {
-			const uint32_t piece = tid + 256 * i, token = 32 * tile + piece / (4 * J), part = piece % (4 * J);
-			if (4 * J * 32 % 256 && piece >= 4 * J * 32) continue;
-			const uint16_t* at = from + (size_t)min(token, p.tokens - 1) * a.token_stride + 8 * part;
-			g.w[i] = a.vec ? load_raw8(at, true) : load_raw8(at, false);
-			if (token >= p.tokens) g.w[i] = u32x4{ 0, 0, 0, 0 };
+			const uint32_t piece = min(tid + 256 * i, 4u * J * 32 - 1), token = min(32 * tile + piece / (4 * J), p.tokens - 1);
+			w[i] = load_raw8(from + (size_t)token * a.token_stride + 8 * (piece % (4 * J)), VEC);
 		}
 	};
-	auto store_keys = [&](const Staged& g, uint32_t tile) {
+	auto store = [&](uint8_t* to, uint32_t row, const u32x4 (&w)[PIECES]) {
 #pragma unroll
 		for (int i = 0; i < PIECES; ++i) {
 			const uint32_t piece = tid + 256 * i;
-			if (4 * J * 32 % 256 && piece >= 4 * J * 32) continue;
-			*(u32x4*)(keys + tile % 2 * KTILE + piece / (4 * J) * KROW + 16 * (piece % (4 * J))) = g.w[i];
+			if (!UNEVEN || piece < 4 * J * 32) *(u32x4*)(to + piece / (4 * J) * row + 16 * (piece % (4 * J))) = w[i];
 		}
 	};
-	auto store_values = [&](Staged& g, uint32_t tile) {
-		if ((int32_t)(32 * tile + 32) > all_see) { /* not all rows see all of the tile: 0 times an infinity must not come in */
-			bool found = false;
+	auto check = [&](u32x4 (&w)[PIECES], uint32_t tile) { /* 0 times an infinity must not come into rows that do not see it */
+		if ((int32_t)(32 * tile + 32) <= all_see) return;
+		bool found = false;
 #pragma unroll
-			for (int i = 0; i < PIECES; ++i) {
-				if (4 * J * 32 % 256 && tid + 256 * i >= 4 * J * 32) continue;
-				found = without_strange<T>(g.w[i]) || found;
-			}
-			if (found) strange = 1;
-		}
-#pragma unroll
-		for (int i = 0; i < PIECES; ++i) {
-			const uint32_t piece = tid + 256 * i;
-			if (4 * J * 32 % 256 && piece >= 4 * J * 32) continue;
-			*(u32x4*)(values + tile % 2 * VTILE + piece / (4 * J) * VROW + 16 * (piece % (4 * J))) = g.w[i];
-		}
+		for (int i = 0; i < PIECES; ++i) found = without_strange<T>(w[i]) || found;
+		if (found) strange = 1;
 	};
 
 	float reference[B], base[B], l[B];
@@ -206,60 +190,24 @@ prompt_attend_kernel(PromptAttend a)
 			for (int e = 0; e < 16; ++e) o[b][j][e] = 0.0f;
 	}
 
+	struct Scores { f32x16 s[B]; };
+	struct Weights { u32x4 w[B][2]; float sum[B]; };
 	const uint8_t* const key_at = keys + n32 * KROW + 16 * h;
 	const uint8_t* const value_at = values + (4 * h + lane % 16 / 4) * VROW + 32 * (lane / 16 % 2) + 8 * (lane % 4);
-	auto work = [&](uint32_t tile) {
+	auto score = [&](Scores& sc, uint32_t tile) {
 		const uint8_t* const k = key_at + tile % 2 * KTILE;
-		const uint8_t* const v = value_at + tile % 2 * VTILE;
-		f32x16 sc[B];
 #pragma unroll
 		for (int b = 0; b < B; ++b)
-			for (int e = 0; e < 16; ++e) sc[b][e] = 0.0f;
+			for (int e = 0; e < 16; ++e) sc.s[b][e] = 0.0f;
 #pragma unroll
 		for (int c = 0; c < 2 * J; ++c) {
 			const u32x4 w = *(const u32x4*)(k + 32 * c);
 #pragma unroll
-			for (int b = 0; b < B; ++b) sc[b] = product(w, q[b][c], sc[b], T{});
+			for (int b = 0; b < B; ++b) sc.s[b] = product(w, q[b][c], sc.s[b], T{});
 		}
-		const int32_t from = (int32_t)(32 * tile);
-		if (least - from < 32) {
-#pragma unroll
-			for (int b = 0; b < B; ++b)
-#pragma unroll
-				for (int e = 0; e < 16; ++e) sc[b][e] = 8 * (e / 4) + 4 * (int32_t)h + e % 4 < sees[b] - from ? sc[b][e] : -__builtin_inff();
-		}
-		u32x4 pr[B][2];
-		float top[B];
-		bool rises = false;
-#pragma unroll
-		for (int b = 0; b < B; ++b) {
-			float t = sc[b][0];
-#pragma unroll
-			for (int e = 1; e < 16; ++e) t = fmaxf(t, sc[b][e]);
-			top[b] = both_halves_most(t) * a.factor;
-			rises = rises || top[b] > reference[b] + RISE;
-		}
-		if (__any(rises)) {
-#pragma unroll
-			for (int b = 0; b < B; ++b) {
-				const float now = fmaxf(reference[b], top[b]), less = now == reference[b] ? 1.0f : __builtin_amdgcn_exp2f(reference[b] - now);
-				reference[b] = now;
-				base[b] = now == -__builtin_inff() ? LIFT : LIFT - now;
-				l[b] *= less;
-#pragma unroll
-				for (int j = 0; j < J; ++j) o[b][j] *= less;
-			}
-		}
-#pragma unroll
-		for (int b = 0; b < B; ++b) {
-#pragma unroll
-			for (int e = 0; e < 16; e += 2) {
-				const float x = __builtin_amdgcn_exp2f(fmaf(sc[b][e], a.factor, base[b])), y = __builtin_amdgcn_exp2f(fmaf(sc[b][e + 1], a.factor, base[b]));
-				l[b] += x;
-				l[b] += y;
-				pr[b][e / 8][e % 8 / 2] = rounded_pair(x, y, T{});
-			}
-		}
+	};
+	auto add = [&](const Weights& p, uint32_t tile) {
+		const uint8_t* const v = value_at + tile % 2 * VTILE;
 #pragma unroll
 		for (int j = 0; j < J; ++j)
 #pragma unroll
@@ -267,31 +215,110 @@ prompt_attend_kernel(PromptAttend a)
 				const u32x2 low = read_turned(v + 16 * c * VROW + 64 * j), high = read_turned(v + (16 * c + 8) * VROW + 64 * j);
 				const u32x4 w{ low[0], low[1], high[0], high[1] };
 #pragma unroll
-				for (int b = 0; b < B; ++b) o[b][j] = product(w, pr[b][c], o[b][j], T{});
+				for (int b = 0; b < B; ++b) o[b][j] = product(w, p.w[b][c], o[b][j], T{});
 			}
+	};
+	auto weigh = [&](Weights& p, const Scores& sc) {
+#pragma unroll
+		for (int b = 0; b < B; ++b) {
+			float sum[2] = { 0.0f, 0.0f };
+#pragma unroll
+			for (int e = 0; e < 16; e += 2) {
+				const float x = __builtin_amdgcn_exp2f(fmaf(sc.s[b][e], a.factor, base[b])), y = __builtin_amdgcn_exp2f(fmaf(sc.s[b][e + 1], a.factor, base[b]));
+				sum[0] += x;
+				sum[1] += y;
+				p.w[b][e / 8][e % 8 / 2] = rounded_pair(x, y, T{});
+			}
+			p.sum[b] = sum[0] + sum[1];
+		}
+	};
+	auto work = [&](uint32_t tile, Scores& now, Scores& next, const Weights& before, Weights& weights) {
+		const int32_t from = (int32_t)(32 * tile);
+		if (least - from < 32) {
+#pragma unroll
+			for (int b = 0; b < B; ++b)
+#pragma unroll
+				for (int e = 0; e < 16; ++e) now.s[b][e] = 8 * (e / 4) + 4 * (int32_t)h + e % 4 < sees[b] - from ? now.s[b][e] : -__builtin_inff();
+		}
+		float top[B];
+#pragma unroll
+		for (int b = 0; b < B; ++b) {
+			top[b] = now.s[b][0];
+#pragma unroll
+			for (int e = 1; e < 16; ++e) top[b] = fmaxf(top[b], now.s[b][e]);
+		}
+		score(next, tile + 1);
+		add(before, tile + 1);
+		weigh(weights, now);
+		bool rises = false;
+#pragma unroll
+		for (int b = 0; b < B; ++b) {
+			top[b] = both_halves_most(top[b]) * a.factor;
+			rises = rises || top[b] > reference[b] + RISE;
+		}
+		if (__any(rises)) {
+#pragma unroll
+			for (int b = 0; b < B; ++b) {
+				const float higher = fmaxf(reference[b], top[b]), less = higher == reference[b] ? 1.0f : __builtin_amdgcn_exp2f(reference[b] - higher);
+				reference[b] = higher;
+				base[b] = higher == -__builtin_inff() ? LIFT : LIFT - higher;
+				l[b] *= less;
+#pragma unroll
+				for (int j = 0; j < J; ++j) o[b][j] *= less;
+			}
+			weigh(weights, now);
+		}
+#pragma unroll
+		for (int b = 0; b < B; ++b) l[b] += weights.sum[b];
 	};
 
 	if (tid == 0) strange = 0;
 	__syncthreads();
 	if (end) {
-		Staged gk, gv;
-		fetch(gk, key_rows, 0);
-		fetch(gv, value_rows, 0);
-		store_keys(gk, 0);
-		store_values(gv, 0);
-		fetch(gk, key_rows, min(1u, end - 1));
-		fetch(gv, value_rows, min(1u, end - 1));
+		Staged g0, g1; /* keys two tiles ahead of the one that is worked on, its own values; then those of the next tile */
+		Scores s0, s1;
+		Weights w0, w1;
+		const uint32_t last = end - 1;
+#pragma unroll
+		for (int b = 0; b < B; ++b)
+			for (int c = 0; c < 2; ++c) w1.w[b][c] = u32x4{ 0, 0, 0, 0 };
+		fetch(g0.k, key_rows, 0);
+		fetch(g1.k, key_rows, min(1u, last));
+		fetch(g0.v, value_rows, 0);
+		store(keys, KROW, g0.k);
+		store(keys + KTILE, KROW, g1.k);
+#pragma unroll
+		for (int i = 0; i < PIECES; ++i) g1.v[i] = u32x4{ 0, 0, 0, 0 };
+		store(values + VTILE, VROW, g1.v); /* (nothing before the first tile) */
+		fetch(g0.k, key_rows, min(2u, last));
+		fetch(g1.k, key_rows, min(3u, last));
+		fetch(g1.v, value_rows, min(1u, last));
 		__syncthreads();
-		for (uint32_t tile = 0; tile < end; ++tile) {
-			if (tile + 1 < end) {
-				store_keys(gk, tile + 1);
-				store_values(gv, tile + 1);
-			}
-			if (tile + 2 < end) {
-				fetch(gk, key_rows, tile + 2);
-				fetch(gv, value_rows, tile + 2);
-			}
-			if ((int32_t)(32 * tile) < seen) work(tile);
+		if (mine) score(s0, 0);
+		__syncthreads();
+		/* a step stages the keys of two tiles on and the tile's own values, and works on the tile; the last one of a wavefront adds up the sums of its last tile (and sees no
+		 * tokens). All wavefronts make as many steps, an even number; those with fewer tiles only bring theirs. */
+		auto bring = [&](uint32_t tile, Staged& g) {
+			check(g.v, tile);
+			store(keys + tile % 2 * KTILE, KROW, g.k);
+			store(values + tile % 2 * VTILE, VROW, g.v);
+			fetch(g.k, key_rows, min(tile + 4, last));
+			fetch(g.v, value_rows, min(tile + 2, last));
+		};
+		const uint32_t steps = (end + 2) / 2 * 2, my_steps = mine ? (mine + 2) / 2 * 2 : 0;
+		uint32_t tile = 0;
+		for (; tile < my_steps; tile += 2) {
+			bring(tile, g0);
+			work(tile, s0, s1, w1, w0);
+			__syncthreads();
+			bring(tile + 1, g1);
+			work(tile + 1, s1, s0, w0, w1);
+			__syncthreads();
+		}
+		for (; tile < steps; tile += 2) {
+			bring(tile, g0);
+			__syncthreads();
+			bring(tile + 1, g1);
 			__syncthreads();
 		}
 	}
@@ -321,26 +348,24 @@ prompt_attend_kernel(PromptAttend a)
 #pragma unroll
 		for (int j = 0; j < J; ++j)
 			for (int e = 0; e < 4; ++e) {
-				uint32_t w[4];
-				for (int r = 0; r < 4; ++r) w[r] = bits16<T>(o[b][j][4 * e + r] * by);
+				const uint32_t low = rounded_pair(o[b][j][4 * e] * by, o[b][j][4 * e + 1] * by, T{}), high = rounded_pair(o[b][j][4 * e + 2] * by, o[b][j][4 * e + 3] * by, T{});
 				uint16_t* at = to + 32 * j + 8 * e + 4 * h;
-				if (a.vec) *(u32x2*)at = u32x2{ w[0] | w[1] << 16, w[2] | w[3] << 16 };
-				else
-					for (int r = 0; r < 4; ++r) at[r] = (uint16_t)w[r];
+				if constexpr (VEC) *(u32x2*)at = u32x2{ low, high };
+				else {
+					at[0] = (uint16_t)low;
+					at[1] = (uint16_t)(low >> 16);
+					at[2] = (uint16_t)high;
+					at[3] = (uint16_t)(high >> 16);
+				}
 			}
 		if (h == 0 && a.lse)
 			a.lse[(size_t)(p.query_first + query[b]) * a.query_heads + query_head[b]] = l[b] == 0.0f ? -__builtin_inff() : (reference[b] + log2f(l[b]) - LIFT) * 0.693147180559945309f;
 	}
 }
 
-template <typename T, int J>
-static int launch_prompt_of(PromptAttend a)
+template <typename T, int J, int B, bool VEC>
+static int launch_prompt_kernel(const PromptAttend& a, uint32_t units)
 {
-	constexpr int B = J <= 4 ? 2 : 1;
-	const uint64_t rows = (uint64_t)a.max_queries * a.group;
-	const uint64_t row_tiles = (rows + 128 * B - 1) / (128 * B), units = row_tiles < 0x80000000u ? row_tiles * a.heads * a.sequences : ~0ull;
-	if ((uint64_t)a.heads * a.sequences > 0x7FFFFFFFu || units > 0x7FFFFFFFu) return fail(KMX_ERR_UNSUPPORTED, "kmx_prompt_attend: too many queries for one call");
-	a.row_tiles = (uint32_t)row_tiles;
 	constexpr uint32_t bytes = prompt_lds<J>();
 	if (bytes > 65536 - 64) { /* more LDS than a launch may ask for unannounced, on this device */
 		static int allowed = -1;
@@ -348,13 +373,25 @@ static int launch_prompt_of(PromptAttend a)
 		const int rc = device_info(&dev);
 		if (rc) return rc;
 		if (allowed != dev->device) {
-			KMX_HIP(hipFuncSetAttribute((const void*)prompt_attend_kernel<T, J, B>, hipFuncAttributeMaxDynamicSharedMemorySize, (int)bytes));
+			KMX_HIP(hipFuncSetAttribute((const void*)prompt_attend_kernel<T, J, B, VEC>, hipFuncAttributeMaxDynamicSharedMemorySize, (int)bytes));
 			allowed = dev->device;
 		}
 	}
-	KMX_LAUNCH_KERNEL((prompt_attend_kernel<T, J, B>), dim3((unsigned)units), dim3(256), bytes, stream(), a);
+	KMX_LAUNCH_KERNEL((prompt_attend_kernel<T, J, B, VEC>), dim3(units), dim3(256), bytes, stream(), a);
 	KMX_LAUNCH_CHECK("prompt_attend_kernel");
 	return KMX_OK;
+}
+
+template <typename T, int J>
+static int launch_prompt_of(PromptAttend a)
+{
+	constexpr int B = J <= 4 ? 2 : 1;
+	const uint64_t rows = (uint64_t)a.max_queries * a.group, row_tiles = (rows + 128 * B - 1) / (128 * B);
+	if (rows > 0x7FFFFF00u || (uint64_t)a.heads * a.sequences > 0x7FFFFFFFu || row_tiles * a.heads * a.sequences > 0x7FFFFFFFu)
+		return fail(KMX_ERR_UNSUPPORTED, "kmx_prompt_attend: too many queries for one call");
+	a.row_tiles = (uint32_t)row_tiles;
+	const uint32_t units = (uint32_t)(row_tiles * a.heads * a.sequences);
+	return a.vec ? launch_prompt_kernel<T, J, B, true>(a, units) : launch_prompt_kernel<T, J, B, false>(a, units);
 }
 
 template <int J>
