@@ -102,7 +102,7 @@ template <int J> constexpr uint32_t prompt_lds() { return 2 * 32 * (key_row<J>()
  * their first operand (v_mfma_f32_32x32x16): scores come out as [token][row], a lane has 16 scores of its row, and its probabilities are, as they stand, its piece of the
  * second operand of [channel][row] = values . p; the values' columns are turned on the way from LDS (ds_read_b64_tr_b16).
  * While the vector units make a tile's probabilities, the matrix cores have the scores of the next one and the sums of the one before: nothing of these three waits for
- * another. The probabilities are made against the reference as it was; where a score passes it by too much they are made again.
+ * another. A reference that is raised counts for the tile's own probabilities; the sums get there once those of the tile before are in them.
  */
 template <typename T, int J, int B, bool VEC>
 __global__ void __launch_bounds__(256, J <= 2 ? 2 : 1)
@@ -149,6 +149,7 @@ prompt_attend_kernel(PromptAttend a)
 		for (int c = 0; c < 2 * J; ++c) {
 			q[b][c] = load_raw8(from + 16 * c, VEC);
 			for (int e = 0; e < 4; ++e) q[b][c][e] = (q[b][c][e] & a.q_keep) ^ a.q_turn; /* the sign of the scale; nothing of them where it is 0 */
+			if constexpr (J > 2) asm volatile("" : "+a"(q[b][c])); /* (the other half of the registers) */
 		}
 	}
 
@@ -156,11 +157,23 @@ prompt_attend_kernel(PromptAttend a)
 	const uint16_t* const key_rows = (const uint16_t*)a.k + (size_t)p.token_first * a.token_stride + (size_t)head * a.head_stride;
 	const uint16_t* const value_rows = (const uint16_t*)a.v + (size_t)p.token_first * a.token_stride + (size_t)head * a.head_stride;
 	struct Staged { u32x4 k[PIECES], v[PIECES]; };
+	const uint32_t last_tile = p.tokens ? (p.tokens - 1) / 32 : 0;
+	uint32_t at_piece[PIECES], at_last[PIECES]; /* bytes from the begin of a tile, and of the last one */
+#pragma unroll
+	for (int i = 0; i < PIECES; ++i) {
+		const uint32_t piece = min(tid + 256 * i, 4u * J * 32 - 1), token = piece / (4 * J), part = 16 * (piece % (4 * J)), stride = (uint32_t)(2 * a.token_stride);
+		at_piece[i] = token * stride + part;
+		at_last[i] = min(token, p.tokens - 1 - 32 * last_tile) * stride + part;
+	}
 	auto fetch = [&](u32x4 (&w)[PIECES], const uint16_t* from, uint32_t tile) {
+		const uint16_t* rows = from + (size_t)tile * 32 * a.token_stride;
 #pragma unroll
 		for (int i = 0; i < PIECES; ++i) {
-			const uint32_t piece = min(tid + 256 * i, 4u * J * 32 - 1), token = min(32 * tile + piece / (4 * J), p.tokens - 1);
-			w[i] = load_raw8(from + (size_t)token * a.token_stride + 8 * (piece % (4 * J)), VEC);
+			if constexpr (VEC) w[i] = *(const u32x4*)((const uint8_t*)rows + (tile < last_tile ? at_piece[i] : at_last[i]));
+			else {
+				const uint32_t piece = min(tid + 256 * i, 4u * J * 32 - 1), token = min(32 * tile + piece / (4 * J), p.tokens - 1);
+				w[i] = load_raw8(from + (size_t)token * a.token_stride + 8 * (piece % (4 * J)), false);
+			}
 		}
 	};
 	auto store = [&](uint8_t* to, uint32_t row, const u32x4 (&w)[PIECES]) {
@@ -191,7 +204,7 @@ prompt_attend_kernel(PromptAttend a)
 	}
 
 	struct Scores { f32x16 s[B]; };
-	struct Weights { u32x4 w[B][2]; float sum[B]; };
+	struct Weights { u32x4 w[B][2]; };
 	const uint8_t* const key_at = keys + n32 * KROW + 16 * h;
 	const uint8_t* const value_at = values + (4 * h + lane % 16 / 4) * VROW + 32 * (lane / 16 % 2) + 8 * (lane % 4);
 	auto score = [&](Scores& sc, uint32_t tile) {
@@ -206,33 +219,25 @@ prompt_attend_kernel(PromptAttend a)
 			for (int b = 0; b < B; ++b) sc.s[b] = product(w, q[b][c], sc.s[b], T{});
 		}
 	};
-	auto add = [&](const Weights& p, uint32_t tile) {
-		const uint8_t* const v = value_at + tile % 2 * VTILE;
-#pragma unroll
-		for (int j = 0; j < J; ++j)
-#pragma unroll
-			for (int c = 0; c < 2; ++c) {
-				const u32x2 low = read_turned(v + 16 * c * VROW + 64 * j), high = read_turned(v + (16 * c + 8) * VROW + 64 * j);
-				const u32x4 w{ low[0], low[1], high[0], high[1] };
-#pragma unroll
-				for (int b = 0; b < B; ++b) o[b][j] = product(w, p.w[b][c], o[b][j], T{});
-			}
-	};
-	auto weigh = [&](Weights& p, const Scores& sc) {
-#pragma unroll
-		for (int b = 0; b < B; ++b) {
-			float sum[2] = { 0.0f, 0.0f };
-#pragma unroll
-			for (int e = 0; e < 16; e += 2) {
-				const float x = __builtin_amdgcn_exp2f(fmaf(sc.s[b][e], a.factor, base[b])), y = __builtin_amdgcn_exp2f(fmaf(sc.s[b][e + 1], a.factor, base[b]));
-				sum[0] += x;
-				sum[1] += y;
-				p.w[b][e / 8][e % 8 / 2] = rounded_pair(x, y, T{});
-			}
-			p.sum[b] = sum[0] + sum[1];
-		}
-	};
+	float less[B]; /* what sums from before a raised reference are lowered by */
+	bool lower = false;
 	auto work = [&](uint32_t tile, Scores& now, Scores& next, const Weights& before, Weights& weights) {
+		const uint8_t* const k = key_at + (tile + 1) % 2 * KTILE;
+		const uint8_t* const v = value_at + (tile + 1) % 2 * VTILE;
+		auto key_operand = [&](int i) { return *(const u32x4*)(k + 32 * i); };
+		auto value_operand = [&](int i) {
+			const uint8_t* at = v + 16 * (i % 2) * VROW + 64 * (i / 2);
+			const u32x2 low = read_turned(at), high = read_turned(at + 8 * VROW);
+			return u32x4{ low[0], low[1], high[0], high[1] };
+		};
+		constexpr int AHEAD = 2, STEPS = 2 * J;
+		u32x4 kop[AHEAD + 1], vop[AHEAD + 1];
+#pragma unroll
+		for (int i = 0; i < AHEAD && i < STEPS; ++i) {
+			kop[i] = key_operand(i);
+			vop[i] = value_operand(i);
+		}
+		__builtin_amdgcn_sched_barrier(0);
 		const int32_t from = (int32_t)(32 * tile);
 		if (least - from < 32) {
 #pragma unroll
@@ -241,35 +246,75 @@ prompt_attend_kernel(PromptAttend a)
 				for (int e = 0; e < 16; ++e) now.s[b][e] = 8 * (e / 4) + 4 * (int32_t)h + e % 4 < sees[b] - from ? now.s[b][e] : -__builtin_inff();
 		}
 		float top[B];
+		bool rises = false;
 #pragma unroll
 		for (int b = 0; b < B; ++b) {
 			top[b] = now.s[b][0];
 #pragma unroll
 			for (int e = 1; e < 16; ++e) top[b] = fmaxf(top[b], now.s[b][e]);
-		}
-		score(next, tile + 1);
-		add(before, tile + 1);
-		weigh(weights, now);
-		bool rises = false;
-#pragma unroll
-		for (int b = 0; b < B; ++b) {
+			for (int e = 0; e < 16; ++e) next.s[b][e] = 0.0f;
 			top[b] = both_halves_most(top[b]) * a.factor;
 			rises = rises || top[b] > reference[b] + RISE;
 		}
 		if (__any(rises)) {
 #pragma unroll
 			for (int b = 0; b < B; ++b) {
-				const float higher = fmaxf(reference[b], top[b]), less = higher == reference[b] ? 1.0f : __builtin_amdgcn_exp2f(reference[b] - higher);
+				const float higher = fmaxf(reference[b], top[b]);
+				less[b] = higher == reference[b] ? 1.0f : __builtin_amdgcn_exp2f(reference[b] - higher);
 				reference[b] = higher;
 				base[b] = higher == -__builtin_inff() ? LIFT : LIFT - higher;
-				l[b] *= less;
-#pragma unroll
-				for (int j = 0; j < J; ++j) o[b][j] *= less;
+				l[b] *= less[b];
 			}
-			weigh(weights, now);
+			lower = true;
+		}
+		/*
+		 * In this order and no other (the compiler would have all products first): between two products, of 32 cycles each, one or two probabilities, each in three turns --
+		 * its exponent, the power, where it goes -- and the operands for the products two steps on.
+		 */
+		float sum[B], exponent[2], power[2], before_last = 0.0f;
+		auto turn = [&](int n) {
+			const int b2 = (n - 2) / 16, e2 = (n - 2) % 16;
+			if (n >= 2) {
+				sum[b2] = e2 ? sum[b2] + power[n % 2] : power[n % 2];
+				if (e2 % 2) weights.w[b2][e2 / 8][e2 % 8 / 2] = rounded_pair(before_last, power[n % 2], T{});
+				before_last = power[n % 2];
+			}
+			if (n >= 1 && n <= 16 * B) power[(n - 1) % 2] = __builtin_amdgcn_exp2f(exponent[(n - 1) % 2]);
+			if (n < 16 * B) {
+				exponent[n % 2] = fmaf(now.s[n / 16][n % 16], a.factor, base[n / 16]);
+				asm volatile("" : "+v"(exponent[n % 2])); /* (here: not all of them ahead) */
+			}
+		};
+		__builtin_amdgcn_sched_barrier(0);
+		constexpr int SLOTS = 2 * STEPS * B, TURNS = 16 * B + 2;
+#pragma unroll
+		for (int i = 0; i < STEPS; ++i) {
+			if (i + AHEAD < STEPS) kop[(i + AHEAD) % (AHEAD + 1)] = key_operand(i + AHEAD);
+#pragma unroll
+			for (int b = 0; b < B; ++b) {
+				next.s[b] = product(kop[i % (AHEAD + 1)], q[b][i], next.s[b], T{});
+#pragma unroll
+				for (int n = TURNS * (2 * B * i + b) / SLOTS; n < TURNS * (2 * B * i + b + 1) / SLOTS; ++n) turn(n);
+				__builtin_amdgcn_sched_barrier(0);
+			}
+			if (i + AHEAD < STEPS) vop[(i + AHEAD) % (AHEAD + 1)] = value_operand(i + AHEAD);
+#pragma unroll
+			for (int b = 0; b < B; ++b) {
+				o[b][i / 2] = product(vop[i % (AHEAD + 1)], before.w[b][i % 2], o[b][i / 2], T{});
+#pragma unroll
+				for (int n = TURNS * (2 * B * i + B + b) / SLOTS; n < TURNS * (2 * B * i + B + b + 1) / SLOTS; ++n) turn(n);
+				__builtin_amdgcn_sched_barrier(0);
+			}
 		}
 #pragma unroll
-		for (int b = 0; b < B; ++b) l[b] += weights.sum[b];
+		for (int b = 0; b < B; ++b) l[b] += sum[b];
+		if (lower) { /* (the tile's own weights, added up with the next tile, are against the reference that is) */
+#pragma unroll
+			for (int b = 0; b < B; ++b)
+#pragma unroll
+				for (int j = 0; j < J; ++j) o[b][j] *= less[b];
+			lower = false;
+		}
 	};
 
 	if (tid == 0) strange = 0;
