@@ -272,19 +272,28 @@ prompt_attend_kernel(PromptAttend a)
 		 * its exponent, the power, where it goes -- and the operands for the products two steps on.
 		 */
 		float sum[B], exponent[2], power[2], before_last = 0.0f;
-		auto turn = [&](int n) {
+		auto turn = [&](int n) { /* (the empty statements keep what they name here: left alone all of it goes to where it is used) */
 			const int b2 = (n - 2) / 16, e2 = (n - 2) % 16;
 			if (n >= 2) {
 				sum[b2] = e2 ? sum[b2] + power[n % 2] : power[n % 2];
-				if (e2 % 2) weights.w[b2][e2 / 8][e2 % 8 / 2] = rounded_pair(before_last, power[n % 2], T{});
+				asm volatile("" : "+v"(sum[b2]));
+				if (e2 % 2) {
+					uint32_t w = rounded_pair(before_last, power[n % 2], T{});
+					asm volatile("" : "+v"(w));
+					weights.w[b2][e2 / 8][e2 % 8 / 2] = w;
+				}
 				before_last = power[n % 2];
 			}
-			if (n >= 1 && n <= 16 * B) power[(n - 1) % 2] = __builtin_amdgcn_exp2f(exponent[(n - 1) % 2]);
+			if (n >= 1 && n <= 16 * B) {
+				power[(n - 1) % 2] = __builtin_amdgcn_exp2f(exponent[(n - 1) % 2]);
+				asm volatile("" : "+v"(power[(n - 1) % 2]));
+			}
 			if (n < 16 * B) {
 				exponent[n % 2] = fmaf(now.s[n / 16][n % 16], a.factor, base[n / 16]);
-				asm volatile("" : "+v"(exponent[n % 2])); /* (here: not all of them ahead) */
+				asm volatile("" : "+v"(exponent[n % 2]));
 			}
 		};
+		__builtin_amdgcn_sched_barrier(0);
 		__builtin_amdgcn_sched_barrier(0);
 		constexpr int SLOTS = 2 * STEPS * B, TURNS = 16 * B + 2;
 #pragma unroll
