@@ -20,7 +20,7 @@ typedef short i16x4 __attribute__((ext_vector_type(4)));
  * Probabilities are rounded to the type of the values for their product with them, sums are those of the floats. They are taken times 2^LIFT, and may pass the
  * reference by 2^RISE: half precision holds them up to 2^15, with 11 bits down to 2^-21 of the reference and none below 2^-32; bfloat16 has 8 bits of all of them.
  */
-constexpr float LIFT = 7.0f, RISE = 8.0f;
+constexpr float LIFT = 7.0f, MOST_SUM = 0x1p15f; /* 2^(LIFT + RISE), RISE = 8 */
 
 __device__ __forceinline__ f32x16 product(const u32x4& a, const u32x4& b, const f32x16& c, __bf16)
 {
@@ -102,7 +102,7 @@ template <int J> constexpr uint32_t prompt_lds() { return 2 * 32 * (key_row<J>()
  * their first operand (v_mfma_f32_32x32x16): scores come out as [token][row], a lane has 16 scores of its row, and its probabilities are, as they stand, its piece of the
  * second operand of [channel][row] = values . p; the values' columns are turned on the way from LDS (ds_read_b64_tr_b16).
  * While the vector units make a tile's probabilities, the matrix cores have the scores of the next one and the sums of the one before: nothing of these three waits for
- * another. A reference that is raised counts for the tile's own probabilities; the sums get there once those of the tile before are in them.
+ * another. Where a row's weights come to more than they may, its reference is raised and they are made again.
  */
 template <typename T, int J, int B, bool VEC>
 __global__ void __launch_bounds__(256, J <= 2 ? 2 : 1)
@@ -219,8 +219,42 @@ prompt_attend_kernel(PromptAttend a)
 			for (int b = 0; b < B; ++b) sc.s[b] = product(w, q[b][c], sc.s[b], T{});
 		}
 	};
-	float less[B]; /* what sums from before a raised reference are lowered by */
-	bool lower = false;
+	auto weigh = [&](Weights& p, float (&sum)[B], const Scores& sc) {
+#pragma unroll
+		for (int b = 0; b < B; ++b) {
+			sum[b] = 0.0f;
+#pragma unroll
+			for (int e = 0; e < 16; e += 2) {
+				const float x = __builtin_amdgcn_exp2f(fmaf(sc.s[b][e], a.factor, base[b])), y = __builtin_amdgcn_exp2f(fmaf(sc.s[b][e + 1], a.factor, base[b]));
+				sum[b] += x + y;
+				p.w[b][e / 8][e % 8 / 2] = rounded_pair(x, y, T{});
+			}
+		}
+	};
+	/* the references of rows whose scores pass them (all rows of the wavefront: what has not passed stays), with what was added up so far */
+	auto raise = [&](const Scores& sc) {
+#pragma unroll
+		for (int b = 0; b < B; ++b) {
+			float top = sc.s[b][0];
+#pragma unroll
+			for (int e = 1; e < 16; ++e) top = fmaxf(top, sc.s[b][e]);
+			top = both_halves_most(top) * a.factor;
+			const float higher = fmaxf(reference[b], top), less = higher == reference[b] ? 1.0f : __builtin_amdgcn_exp2f(reference[b] - higher);
+			reference[b] = higher;
+			base[b] = higher == -__builtin_inff() ? LIFT : LIFT - higher;
+			l[b] *= less;
+#pragma unroll
+			for (int j = 0; j < J; ++j) o[b][j] *= less;
+		}
+	};
+	auto hide = [&](Scores& sc, uint32_t tile) { /* tokens that a row does not see */
+		const int32_t from = (int32_t)(32 * tile);
+		if (least - from >= 32) return;
+#pragma unroll
+		for (int b = 0; b < B; ++b)
+#pragma unroll
+			for (int e = 0; e < 16; ++e) sc.s[b][e] = 8 * (e / 4) + 4 * (int32_t)h + e % 4 < sees[b] - from ? sc.s[b][e] : -__builtin_inff();
+	};
 	auto work = [&](uint32_t tile, Scores& now, Scores& next, const Weights& before, Weights& weights) {
 		const uint8_t* const k = key_at + (tile + 1) % 2 * KTILE;
 		const uint8_t* const v = value_at + (tile + 1) % 2 * VTILE;
@@ -238,35 +272,10 @@ prompt_attend_kernel(PromptAttend a)
 			vop[i] = value_operand(i);
 		}
 		__builtin_amdgcn_sched_barrier(0);
-		const int32_t from = (int32_t)(32 * tile);
-		if (least - from < 32) {
+		hide(now, tile);
 #pragma unroll
-			for (int b = 0; b < B; ++b)
-#pragma unroll
-				for (int e = 0; e < 16; ++e) now.s[b][e] = 8 * (e / 4) + 4 * (int32_t)h + e % 4 < sees[b] - from ? now.s[b][e] : -__builtin_inff();
-		}
-		float top[B];
-		bool rises = false;
-#pragma unroll
-		for (int b = 0; b < B; ++b) {
-			top[b] = now.s[b][0];
-#pragma unroll
-			for (int e = 1; e < 16; ++e) top[b] = fmaxf(top[b], now.s[b][e]);
+		for (int b = 0; b < B; ++b)
 			for (int e = 0; e < 16; ++e) next.s[b][e] = 0.0f;
-			top[b] = both_halves_most(top[b]) * a.factor;
-			rises = rises || top[b] > reference[b] + RISE;
-		}
-		if (__any(rises)) {
-#pragma unroll
-			for (int b = 0; b < B; ++b) {
-				const float higher = fmaxf(reference[b], top[b]);
-				less[b] = higher == reference[b] ? 1.0f : __builtin_amdgcn_exp2f(reference[b] - higher);
-				reference[b] = higher;
-				base[b] = higher == -__builtin_inff() ? LIFT : LIFT - higher;
-				l[b] *= less[b];
-			}
-			lower = true;
-		}
 		/*
 		 * In this order and no other (the compiler would have all products first): between two products, of 32 cycles each, one or two probabilities, each in three turns --
 		 * its exponent, the power, where it goes -- and the operands for the products two steps on.
@@ -315,15 +324,16 @@ prompt_attend_kernel(PromptAttend a)
 				__builtin_amdgcn_sched_barrier(0);
 			}
 		}
+		/* a sum that is no more than 2^(LIFT + RISE) has no weight above it: no need to look for the largest score */
+		bool rises = false;
+#pragma unroll
+		for (int b = 0; b < B; ++b) rises = rises || !(sum[b] <= MOST_SUM);
+		if (__any(rises)) {
+			raise(now);
+			weigh(weights, sum, now);
+		}
 #pragma unroll
 		for (int b = 0; b < B; ++b) l[b] += sum[b];
-		if (lower) { /* (the tile's own weights, added up with the next tile, are against the reference that is) */
-#pragma unroll
-			for (int b = 0; b < B; ++b)
-#pragma unroll
-				for (int j = 0; j < J; ++j) o[b][j] *= less[b];
-			lower = false;
-		}
 	};
 
 	if (tid == 0) strange = 0;
@@ -348,7 +358,11 @@ prompt_attend_kernel(PromptAttend a)
 		fetch(g1.k, key_rows, min(3u, last));
 		fetch(g1.v, value_rows, min(1u, last));
 		__syncthreads();
-		if (mine) score(s0, 0);
+		if (mine) {
+			score(s0, 0);
+			hide(s0, 0);
+			raise(s0);
+		}
 		__syncthreads();
 		/* a step stages the keys of two tiles on and the tile's own values, and works on the tile; the last one of a wavefront adds up the sums of its last tile (and sees no
 		 * tokens). All wavefronts make as many steps, an even number; those with fewer tiles only bring theirs. */
