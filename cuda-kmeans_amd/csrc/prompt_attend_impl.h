@@ -10,6 +10,8 @@
 
 #include "prompt_attend.h"
 
+#include <type_traits>
+
 namespace kmx {
 
 typedef float f32x16 __attribute__((ext_vector_type(16)));
@@ -69,6 +71,13 @@ __device__ __forceinline__ bool without_strange(u32x4& w)
 	return found;
 }
 
+/* an address that is the same in all lanes, in scalar registers */
+__device__ __forceinline__ void* same_in_all(const void* p)
+{
+	const uint64_t u = (uint64_t)p;
+	return (void*)((uint64_t)(uint32_t)__builtin_amdgcn_readfirstlane((int)(u >> 32)) << 32 | (uint32_t)__builtin_amdgcn_readfirstlane((int)u));
+}
+
 struct Prompt4 { uint32_t query_first, queries, token_first, tokens; };
 /* queries and tokens of sequence s, held to what there is */
 __device__ __forceinline__ Prompt4 prompt_of(const PromptAttend& a, uint32_t s)
@@ -94,11 +103,11 @@ __device__ __forceinline__ int32_t sees_of(const PromptAttend& a, const Prompt4&
 
 template <int J> constexpr uint32_t key_row() { return 64 * J + 16; }                       /* bytes: 8 tokens one below the other read 8 groups of banks */
 template <int J> constexpr uint32_t value_row() { return 64 * J + (J % 2 ? 0 : 64); }       /* 64 or 192 bytes on in the banks: 4 tokens side by side */
-template <int J> constexpr uint32_t prompt_lds() { return 2 * 32 * (key_row<J>() + value_row<J>()); }
+template <int J> constexpr uint32_t prompt_lds() { return 3 * 32 * (key_row<J>() + value_row<J>()); }
 
 /*
  * A work-group of four wavefronts takes 128 B rows of one head of the keys (the query heads of a query side by side, then the next query's), 32 B a wavefront. Tiles of
- * 32 tokens pass through LDS as they are, two of keys and two of values, from registers that were loaded two tiles before. Both products have the cache's side as
+ * 32 tokens pass through LDS as they are, three of keys and three of values, from registers that were loaded two tiles before. Both products have the keys' and values' side as
  * their first operand (v_mfma_f32_32x32x16): scores come out as [token][row], a lane has 16 scores of its row, and its probabilities are, as they stand, its piece of the
  * second operand of [channel][row] = values . p; the values' columns are turned on the way from LDS (ds_read_b64_tr_b16).
  * While the vector units make a tile's probabilities, the matrix cores have the scores of the next one and the sums of the one before: nothing of these three waits for
@@ -108,13 +117,10 @@ template <typename T, int J, int B, bool VEC>
 __global__ void __launch_bounds__(256, J <= 2 ? 2 : 1)
 prompt_attend_kernel(PromptAttend a)
 {
-	constexpr uint32_t KROW = key_row<J>(), VROW = value_row<J>(), KTILE = 32 * KROW, VTILE = 32 * VROW;
+	constexpr uint32_t KROW = key_row<J>(), VROW = value_row<J>(), KTILE = 32 * KROW, PLACE = KTILE + 32 * VROW;
 	constexpr int PIECES = (4 * J * 32 + 255) / 256; /* of 16 bytes that a lane brings of a tile */
-	constexpr bool UNEVEN = 4 * J * 32 % 256 != 0;
 	extern __shared__ __attribute__((aligned(16))) uint8_t lds[];
 	__shared__ uint32_t strange; /* values that are no numbers, where not all rows see them */
-	uint8_t* const keys = lds;
-	uint8_t* const values = lds + 2 * KTILE;
 	const uint32_t tid = threadIdx.x, wave = (uint32_t)__builtin_amdgcn_readfirstlane((int)(tid / WAVE)), lane = tid % WAVE, n32 = lane % 32, h = lane / 32;
 	/* heads take turns over the dies, and the rows that see the most come first */
 	const uint32_t head = blockIdx.x % a.heads, rest = blockIdx.x / a.heads, s = rest % a.sequences, row_tile = a.row_tiles - 1 - rest / a.sequences;
@@ -157,32 +163,36 @@ prompt_attend_kernel(PromptAttend a)
 	const uint16_t* const key_rows = (const uint16_t*)a.k + (size_t)p.token_first * a.token_stride + (size_t)head * a.head_stride;
 	const uint16_t* const value_rows = (const uint16_t*)a.v + (size_t)p.token_first * a.token_stride + (size_t)head * a.head_stride;
 	struct Staged { u32x4 k[PIECES], v[PIECES]; };
-	const uint32_t last_tile = p.tokens ? (p.tokens - 1) / 32 : 0;
-	uint32_t at_piece[PIECES], at_last[PIECES]; /* bytes from the begin of a tile, and of the last one */
+	/* pieces of 16 bytes of a tile: where they lie from the sequence's first token on, and in LDS. With whole pieces what lies behind the last token is zeros (the hardware's own check of
+	 * offsets in a buffer), else the last token again: no row sees it */
+	const uint32_t stride = (uint32_t)(2 * a.token_stride), size = p.tokens ? (p.tokens - 1) * stride + 64 * J : 0;
+	const auto key_buffer = __builtin_amdgcn_make_buffer_rsrc(same_in_all(key_rows), 0, __builtin_amdgcn_readfirstlane((int)size), 0x00020000);
+	const auto value_buffer = __builtin_amdgcn_make_buffer_rsrc(same_in_all(value_rows), 0, __builtin_amdgcn_readfirstlane((int)size), 0x00020000);
+	uint32_t at_key[PIECES], at_value[PIECES], to_key[PIECES], to_value[PIECES];
 #pragma unroll
 	for (int i = 0; i < PIECES; ++i) {
-		const uint32_t piece = min(tid + 256 * i, 4u * J * 32 - 1), token = piece / (4 * J), part = 16 * (piece % (4 * J)), stride = (uint32_t)(2 * a.token_stride);
-		at_piece[i] = token * stride + part;
-		at_last[i] = min(token, p.tokens - 1 - 32 * last_tile) * stride + part;
+		const uint32_t piece = min(tid + 256 * i, 4u * J * 32 - 1), token = piece / (4 * J), part = 16 * (piece % (4 * J));
+		at_key[i] = at_value[i] = VEC ? token * stride + part : token;
+		to_key[i] = token * KROW + part;
+		to_value[i] = KTILE + token * VROW + part;
 	}
-	auto fetch = [&](u32x4 (&w)[PIECES], const uint16_t* from, uint32_t tile) {
-		const uint16_t* rows = from + (size_t)tile * 32 * a.token_stride;
-#pragma unroll
-		for (int i = 0; i < PIECES; ++i) {
-			if constexpr (VEC) w[i] = *(const u32x4*)((const uint8_t*)rows + (tile < last_tile ? at_piece[i] : at_last[i]));
-			else {
-				const uint32_t piece = min(tid + 256 * i, 4u * J * 32 - 1), token = min(32 * tile + piece / (4 * J), p.tokens - 1);
-				w[i] = load_raw8(from + (size_t)token * a.token_stride + 8 * (piece % (4 * J)), false);
-			}
-		}
+	auto load_key = [&](int i) { /* and on to the next tile */
+		u32x4 w;
+		if constexpr (VEC) w = __builtin_bit_cast(u32x4, __builtin_amdgcn_raw_buffer_load_b128(key_buffer, (int)at_key[i], 0, 0));
+		else w = load_raw8(key_rows + (size_t)min(at_key[i], p.tokens - 1) * a.token_stride + 8 * (min(tid + 256 * i, 4u * J * 32 - 1) % (4 * J)), false);
+		at_key[i] += VEC ? 32 * stride : 32;
+		return w;
 	};
-	auto store = [&](uint8_t* to, uint32_t row, const u32x4 (&w)[PIECES]) {
-#pragma unroll
-		for (int i = 0; i < PIECES; ++i) {
-			const uint32_t piece = tid + 256 * i;
-			if (!UNEVEN || piece < 4 * J * 32) *(u32x4*)(to + piece / (4 * J) * row + 16 * (piece % (4 * J))) = w[i];
-		}
+	auto load_value = [&](int i) {
+		u32x4 w;
+		if constexpr (VEC) w = __builtin_bit_cast(u32x4, __builtin_amdgcn_raw_buffer_load_b128(value_buffer, (int)at_value[i], 0, 0));
+		else w = load_raw8(value_rows + (size_t)min(at_value[i], p.tokens - 1) * a.token_stride + 8 * (min(tid + 256 * i, 4u * J * 32 - 1) % (4 * J)), false);
+		at_value[i] += VEC ? 32 * stride : 32;
+		return w;
 	};
+	/* (of a tile that has no multiple of 256 pieces some lanes bring the last piece again) */
+	auto store_key = [&](uint32_t at, const u32x4& w, int i) { *(u32x4*)(lds + at + to_key[i]) = w; };
+	auto store_value = [&](uint32_t at, const u32x4& w, int i) { *(u32x4*)(lds + at + to_value[i]) = w; };
 	auto check = [&](u32x4 (&w)[PIECES], uint32_t tile) { /* 0 times an infinity must not come into rows that do not see it */
 		if ((int32_t)(32 * tile + 32) <= all_see) return;
 		bool found = false;
@@ -205,16 +215,21 @@ prompt_attend_kernel(PromptAttend a)
 
 	struct Scores { f32x16 s[B]; };
 	struct Weights { u32x4 w[B][2]; };
-	const uint8_t* const key_at = keys + n32 * KROW + 16 * h;
-	const uint8_t* const value_at = values + (4 * h + lane % 16 / 4) * VROW + 32 * (lane / 16 % 2) + 8 * (lane % 4);
-	auto score = [&](Scores& sc, uint32_t tile) {
-		const uint8_t* const k = key_at + tile % 2 * KTILE;
+	const uint8_t* const key_at = lds + n32 * KROW + 16 * h;
+	const uint8_t* const value_at = lds + KTILE + (4 * h + lane % 16 / 4) * VROW + 32 * (lane / 16 % 2) + 8 * (lane % 4);
+	auto key_operand = [&](uint32_t at, int i) { return *(const u32x4*)(key_at + at + 32 * i); };
+	auto value_operand = [&](u32x4& w, uint32_t at, int i, int half) { /* tokens 0 to 3 of 8, or the others */
+		const u32x2 v = read_turned(value_at + at + (16 * (i % 2) + 8 * half) * VROW + 64 * (i / 2));
+		w[2 * half] = v[0];
+		w[2 * half + 1] = v[1];
+	};
+	auto score = [&](Scores& sc, uint32_t at) {
 #pragma unroll
 		for (int b = 0; b < B; ++b)
 			for (int e = 0; e < 16; ++e) sc.s[b][e] = 0.0f;
 #pragma unroll
 		for (int c = 0; c < 2 * J; ++c) {
-			const u32x4 w = *(const u32x4*)(k + 32 * c);
+			const u32x4 w = key_operand(at, c);
 #pragma unroll
 			for (int b = 0; b < B; ++b) sc.s[b] = product(w, q[b][c], sc.s[b], T{});
 		}
@@ -255,31 +270,27 @@ prompt_attend_kernel(PromptAttend a)
 #pragma unroll
 			for (int e = 0; e < 16; ++e) sc.s[b][e] = 8 * (e / 4) + 4 * (int32_t)h + e % 4 < sees[b] - from ? sc.s[b][e] : -__builtin_inff();
 	};
-	auto work = [&](uint32_t tile, Scores& now, Scores& next, const Weights& before, Weights& weights) {
-		const uint8_t* const k = key_at + (tile + 1) % 2 * KTILE;
-		const uint8_t* const v = value_at + (tile + 1) % 2 * VTILE;
-		auto key_operand = [&](int i) { return *(const u32x4*)(k + 32 * i); };
-		auto value_operand = [&](int i) {
-			const uint8_t* at = v + 16 * (i % 2) * VROW + 64 * (i / 2);
-			const u32x2 low = read_turned(at), high = read_turned(at + 8 * VROW);
-			return u32x4{ low[0], low[1], high[0], high[1] };
-		};
-		constexpr int AHEAD = 2, STEPS = 2 * J;
-		u32x4 kop[AHEAD + 1], vop[AHEAD + 1];
-#pragma unroll
-		for (int i = 0; i < AHEAD && i < STEPS; ++i) {
-			kop[i] = key_operand(i);
-			vop[i] = value_operand(i);
-		}
-		__builtin_amdgcn_sched_barrier(0);
+	/* operands come in batches, one in use and one on its way */
+	constexpr int STEPS = 2 * J, BATCH = J == 2 ? 1 : J, SLOTS = 2 * STEPS * B, BATCH_SLOTS = 2 * BATCH * B;
+	u32x4 kop[2][BATCH], vop[2][BATCH];
+	Staged g0, g1; /* keys three tiles on and values one; then those of the next tile */
+	Scores s0, s1;
+	Weights w0, w1;
+	/*
+	 * A step: the scores of the tile behind, the sums of the tile before, the tile's own weights; the keys of three tiles on and the values of the next one go to LDS and those of
+	 * two tiles later are loaded. All in this order and no other (the compiler would have all products first): between two products, of 32 cycles each, one or two probabilities,
+	 * each in three turns -- its exponent, the power, where it goes --, operands for later products, a piece of what goes to LDS. One wavefront a SIMD issues an instruction in four
+	 * cycles: places in LDS are known when this is compiled (N is the tile's number modulo 6: three places, two sets of registers).
+	 */
+	auto work = [&](auto number, uint32_t tile) {
+		constexpr uint32_t N = decltype(number)::value, HERE = N % 3 * PLACE, ON1 = (N + 1) % 3 * PLACE, ON2 = (N + 2) % 3 * PLACE;
+		Staged& g = N % 2 ? g1 : g0;
+		Scores &now = N % 2 ? s1 : s0, &next = N % 2 ? s0 : s1;
+		Weights &before = N % 2 ? w0 : w1, &weights = N % 2 ? w1 : w0;
 		hide(now, tile);
 #pragma unroll
 		for (int b = 0; b < B; ++b)
 			for (int e = 0; e < 16; ++e) next.s[b][e] = 0.0f;
-		/*
-		 * In this order and no other (the compiler would have all products first): between two products, of 32 cycles each, one or two probabilities, each in three turns --
-		 * its exponent, the power, where it goes -- and the operands for the products two steps on.
-		 */
 		float sum[B], exponent[2], power[2], before_last = 0.0f;
 		auto turn = [&](int n) { /* (the empty statements keep what they name here: left alone all of it goes to where it is used) */
 			const int b2 = (n - 2) / 16, e2 = (n - 2) % 16;
@@ -302,26 +313,43 @@ prompt_attend_kernel(PromptAttend a)
 				asm volatile("" : "+v"(exponent[n % 2]));
 			}
 		};
+		constexpr int TURNS = 16 * B + 2, BATCHES = STEPS / BATCH, READS = 3 * BATCH, MOVES = 4 * PIECES / BATCHES, ITEMS = READS + MOVES;
+		auto slot = [&](int t) {
+#pragma unroll
+			for (int n = TURNS * t / SLOTS; n < TURNS * (t + 1) / SLOTS; ++n) turn(n);
+			/* one of a batch's reads of operands for the next, or of its moves -- first those to LDS, then those from memory --, evenly over its slots: all four wavefronts
+			 * are about here, and LDS takes a read of theirs in 5 cycles and a write in 13 */
+			const int batch = t / BATCH_SLOTS, in = t % BATCH_SLOTS, first = (batch + 1) * BATCH, at = (batch + 1) % 2;
+#pragma unroll
+			for (int p = ITEMS * in / BATCH_SLOTS; p < ITEMS * (in + 1) / BATCH_SLOTS; ++p) {
+				const int move = MOVES * p / ITEMS, read = p - move;
+				if (MOVES * (p + 1) / ITEMS > move) {
+					const int m = batch * MOVES + move, i = m % PIECES;
+					if (m / PIECES == 0) store_key(HERE, g.k[i], i);
+					else if (m / PIECES == 1) store_value(ON1, g.v[i], i);
+					else if (m / PIECES == 2) g.k[i] = load_key(i);
+					else g.v[i] = load_value(i);
+				} else {
+					const int n = read / 3, i = first < STEPS ? first + n : n;
+					if (read % 3 == 0) kop[at][n] = key_operand(first < STEPS ? ON1 : ON2, i);
+					else value_operand(vop[at][n], first < STEPS ? ON2 : HERE, i, read % 3 - 1);
+				}
+			}
+			__builtin_amdgcn_sched_barrier(0);
+		};
 		__builtin_amdgcn_sched_barrier(0);
-		__builtin_amdgcn_sched_barrier(0);
-		constexpr int SLOTS = 2 * STEPS * B, TURNS = 16 * B + 2;
 #pragma unroll
 		for (int i = 0; i < STEPS; ++i) {
-			if (i + AHEAD < STEPS) kop[(i + AHEAD) % (AHEAD + 1)] = key_operand(i + AHEAD);
+			const int batch = i / BATCH, n = i % BATCH;
 #pragma unroll
 			for (int b = 0; b < B; ++b) {
-				next.s[b] = product(kop[i % (AHEAD + 1)], q[b][i], next.s[b], T{});
-#pragma unroll
-				for (int n = TURNS * (2 * B * i + b) / SLOTS; n < TURNS * (2 * B * i + b + 1) / SLOTS; ++n) turn(n);
-				__builtin_amdgcn_sched_barrier(0);
+				next.s[b] = product(kop[batch % 2][n], q[b][i], next.s[b], T{});
+				slot(2 * B * i + b);
 			}
-			if (i + AHEAD < STEPS) vop[(i + AHEAD) % (AHEAD + 1)] = value_operand(i + AHEAD);
 #pragma unroll
 			for (int b = 0; b < B; ++b) {
-				o[b][i / 2] = product(vop[i % (AHEAD + 1)], before.w[b][i % 2], o[b][i / 2], T{});
-#pragma unroll
-				for (int n = TURNS * (2 * B * i + B + b) / SLOTS; n < TURNS * (2 * B * i + B + b + 1) / SLOTS; ++n) turn(n);
-				__builtin_amdgcn_sched_barrier(0);
+				o[b][i / 2] = product(vop[batch % 2][n], before.w[b][i % 2], o[b][i / 2], T{});
+				slot(2 * B * i + B + b);
 			}
 		}
 		/* a sum that is no more than 2^(LIFT + RISE) has no weight above it: no need to look for the largest score */
@@ -339,55 +367,72 @@ prompt_attend_kernel(PromptAttend a)
 	if (tid == 0) strange = 0;
 	__syncthreads();
 	if (end) {
-		Staged g0, g1; /* keys two tiles ahead of the one that is worked on, its own values; then those of the next tile */
-		Scores s0, s1;
-		Weights w0, w1;
-		const uint32_t last = end - 1;
 #pragma unroll
 		for (int b = 0; b < B; ++b)
 			for (int c = 0; c < 2; ++c) w1.w[b][c] = u32x4{ 0, 0, 0, 0 };
-		fetch(g0.k, key_rows, 0);
-		fetch(g1.k, key_rows, min(1u, last));
-		fetch(g0.v, value_rows, 0);
-		store(keys, KROW, g0.k);
-		store(keys + KTILE, KROW, g1.k);
+		u32x4 k[3][PIECES];
 #pragma unroll
-		for (int i = 0; i < PIECES; ++i) g1.v[i] = u32x4{ 0, 0, 0, 0 };
-		store(values + VTILE, VROW, g1.v); /* (nothing before the first tile) */
-		fetch(g0.k, key_rows, min(2u, last));
-		fetch(g1.k, key_rows, min(3u, last));
-		fetch(g1.v, value_rows, min(1u, last));
+		for (int n = 0; n < 3; ++n)
+			for (int i = 0; i < PIECES; ++i) k[n][i] = load_key(i);
+#pragma unroll
+		for (int i = 0; i < PIECES; ++i) g0.v[i] = load_value(i);
+#pragma unroll
+		for (int i = 0; i < PIECES; ++i) {
+			for (int n = 0; n < 3; ++n) store_key(n * PLACE, k[n][i], i);
+			store_value(2 * PLACE, u32x4{ 0, 0, 0, 0 }, i); /* (nothing before the first tile) */
+		}
+		check(g0.v, 0);
+#pragma unroll
+		for (int i = 0; i < PIECES; ++i) store_value(0, g0.v[i], i);
+		auto fetch = [&](Staged& g) {
+#pragma unroll
+			for (int i = 0; i < PIECES; ++i) g.k[i] = load_key(i);
+#pragma unroll
+			for (int i = 0; i < PIECES; ++i) g.v[i] = load_value(i);
+		};
+		fetch(g0);
+		fetch(g1);
 		__syncthreads();
+		/* the last step of a wavefront adds up its last tile (and sees no tokens itself); those with fewer tiles only bring theirs */
+		const uint32_t steps = end + 1, my_steps = mine ? mine + 1 : 0;
 		if (mine) {
 			score(s0, 0);
 			hide(s0, 0);
 			raise(s0);
+#pragma unroll
+			for (int n = 0; n < BATCH; ++n) {
+				kop[0][n] = key_operand(PLACE, n);
+				for (int half = 0; half < 2; ++half) value_operand(vop[0][n], 2 * PLACE, n, half);
+			}
 		}
 		__syncthreads();
-		/* a step stages the keys of two tiles on and the tile's own values, and works on the tile; the last one of a wavefront adds up the sums of its last tile (and sees no
-		 * tokens). All wavefronts make as many steps, an even number; those with fewer tiles only bring theirs. */
-		auto bring = [&](uint32_t tile, Staged& g) {
-			check(g.v, tile);
-			store(keys + tile % 2 * KTILE, KROW, g.k);
-			store(values + tile % 2 * VTILE, VROW, g.v);
-			fetch(g.k, key_rows, min(tile + 4, last));
-			fetch(g.v, value_rows, min(tile + 2, last));
-		};
-		const uint32_t steps = (end + 2) / 2 * 2, my_steps = mine ? (mine + 2) / 2 * 2 : 0;
 		uint32_t tile = 0;
-		for (; tile < my_steps; tile += 2) {
-			bring(tile, g0);
-			work(tile, s0, s1, w1, w0);
+		auto step = [&](auto number) {
+			check(decltype(number)::value % 2 ? g1.v : g0.v, tile + 1);
+			work(number, tile);
+			/* what was stored to LDS is there: of what LDS was asked for since, the last batch's reads are for the next step and need not be back */
+			constexpr int LATE = 3 * BATCH < 14 ? 3 * BATCH : 14;
+			asm volatile("s_waitcnt lgkmcnt(%0)\n\ts_barrier" :: "n"(LATE) : "memory");
+			return ++tile < my_steps;
+		};
+		while (tile < my_steps)
+			if (!step(std::integral_constant<uint32_t, 0>{}) || !step(std::integral_constant<uint32_t, 1>{}) || !step(std::integral_constant<uint32_t, 2>{}) ||
+			    !step(std::integral_constant<uint32_t, 3>{}) || !step(std::integral_constant<uint32_t, 4>{}) || !step(std::integral_constant<uint32_t, 5>{}))
+				break;
+		auto bring = [&](Staged& g) {
+			check(g.v, tile + 1);
+			const uint32_t here = tile % 3, on1 = (tile + 1) % 3;
+#pragma unroll
+			for (int i = 0; i < PIECES; ++i) {
+				store_key(here * PLACE, g.k[i], i);
+				store_value(on1 * PLACE, g.v[i], i);
+			}
+			fetch(g);
 			__syncthreads();
-			bring(tile + 1, g1);
-			work(tile + 1, s1, s0, w0, w1);
-			__syncthreads();
-		}
-		for (; tile < steps; tile += 2) {
-			bring(tile, g0);
-			__syncthreads();
-			bring(tile + 1, g1);
-			__syncthreads();
+		};
+		for (; tile < steps; ++tile) {
+			if (tile % 2) bring(g1);
+			else bring(g0);
 		}
 	}
 
