@@ -57,8 +57,8 @@ int kmx_prompt_attend(const kmx_prompt* prompt, int type, const void* q, size_t 
 	a.causal = causal != 0;
 	const auto aligned = [](const void* p, size_t token, size_t head) { return (uintptr_t)p % 16 == 0 && token % 8 == 0 && head % 8 == 0; };
 	a.vec = aligned(q, q_token_stride, q_head_stride) && aligned(keys, token_stride, head_stride) && aligned(values, token_stride, head_stride) && aligned(out, out_token_stride, out_head_stride);
-	/* offsets of pieces, five tiles behind the last token among them, are counted in 32 bits */
-	if ((uint64_t)a.max_tokens + 192 > 0xFFFFFFFFu / 2 / (token_stride ? token_stride : 1)) a.vec = false;
+	/* offsets of pieces are counted in 32 bits, from the end of a sequence as far on as it is long among them */
+	if ((uint64_t)a.max_tokens + 192 > 0x7FFFFFFFu / 2 / (token_stride ? token_stride : 1)) a.vec = false;
 	switch (b.dim / 32) {
 	case 1: return launch_prompt_attend<1>(a, type == KMX_BF16);
 	case 2: return launch_prompt_attend<2>(a, type == KMX_BF16);

@@ -103,7 +103,9 @@ __device__ __forceinline__ int32_t sees_of(const PromptAttend& a, const Prompt4&
 
 template <int J> constexpr uint32_t key_row() { return 64 * J + 16; }                       /* bytes: 8 tokens one below the other read 8 groups of banks */
 template <int J> constexpr uint32_t value_row() { return 64 * J + (J % 2 ? 0 : 64); }       /* 64 or 192 bytes on in the banks: 4 tokens side by side */
-template <int J> constexpr uint32_t prompt_lds() { return 3 * 32 * (key_row<J>() + value_row<J>()); }
+template <int J, int W> constexpr int prompt_waves() { return J <= 6 ? 2 : 1; } /* wavefronts a SIMD: 256 registers each, or 512 */
+template <int J, int W> constexpr int prompt_batch() { return J <= 6 ? 1 : J; }
+template <int J> constexpr uint32_t prompt_lds() { return 3 * 32 * (key_row<J>() + value_row<J>()) + 1024; } /* (and a place for what wavefronts without pieces store) */
 
 /*
  * A work-group of four wavefronts takes 128 B rows of one head of the keys (the query heads of a query side by side, then the next query's), 32 B a wavefront. Tiles of
@@ -113,21 +115,23 @@ template <int J> constexpr uint32_t prompt_lds() { return 3 * 32 * (key_row<J>()
  * While the vector units make a tile's probabilities, the matrix cores have the scores of the next one and the sums of the one before: nothing of these three waits for
  * another. Where a row's weights come to more than they may, its reference is raised and they are made again.
  */
-template <typename T, int J, int B, bool VEC>
-__global__ void __launch_bounds__(256, J <= 2 ? 2 : 1)
+template <typename T, int J, int W, int B, bool VEC>
+__global__ void __launch_bounds__(64 * W, (prompt_waves<J, W>()))
 prompt_attend_kernel(PromptAttend a)
 {
 	constexpr uint32_t KROW = key_row<J>(), VROW = value_row<J>(), KTILE = 32 * KROW, PLACE = KTILE + 32 * VROW;
-	constexpr int PIECES = (4 * J * 32 + 255) / 256; /* of 16 bytes that a lane brings of a tile */
+	constexpr uint32_t THREADS = 64 * W, ROWS = 32 * W * B;
+	constexpr uint32_t TILE_PIECES = 4 * J * 32; /* of 16 bytes, of keys, and as many of values */
+	constexpr int PIECES = (2 * TILE_PIECES + THREADS - 1) / THREADS; /* that a lane brings each step */
 	extern __shared__ __attribute__((aligned(16))) uint8_t lds[];
 	__shared__ uint32_t strange; /* values that are no numbers, where not all rows see them */
 	const uint32_t tid = threadIdx.x, wave = (uint32_t)__builtin_amdgcn_readfirstlane((int)(tid / WAVE)), lane = tid % WAVE, n32 = lane % 32, h = lane / 32;
 	/* heads take turns over the dies, and the rows that see the most come first */
 	const uint32_t head = blockIdx.x % a.heads, rest = blockIdx.x / a.heads, s = rest % a.sequences, row_tile = a.row_tiles - 1 - rest / a.sequences;
 	const Prompt4 p = prompt_of(a, s);
-	const uint32_t all_rows = p.queries * a.group, first_row = row_tile * (128 * B); /* (31 bits) */
+	const uint32_t all_rows = p.queries * a.group, first_row = row_tile * ROWS; /* (31 bits) */
 	if (first_row >= all_rows) return;
-	const uint32_t rows = min(128u * B, all_rows - first_row);
+	const uint32_t rows = min(ROWS, all_rows - first_row);
 	const uint32_t end = ((uint32_t)sees_of(a, p, (first_row + rows - 1) / a.group) + 31) / 32; /* tiles */
 	const int32_t all_see = sees_of(a, p, first_row / a.group);
 
@@ -155,49 +159,58 @@ prompt_attend_kernel(PromptAttend a)
 		for (int c = 0; c < 2 * J; ++c) {
 			q[b][c] = load_raw8(from + 16 * c, VEC);
 			for (int e = 0; e < 4; ++e) q[b][c][e] = (q[b][c][e] & a.q_keep) ^ a.q_turn; /* the sign of the scale; nothing of them where it is 0 */
-			if constexpr (J > 2) asm volatile("" : "+a"(q[b][c])); /* (the other half of the registers) */
+			if constexpr (prompt_waves<J, W>() == 1) asm volatile("" : "+a"(q[b][c])); /* (the other half of the registers) */
 		}
 	}
 
 	/* what lies behind the last token is the last token again: no row sees it */
 	const uint16_t* const key_rows = (const uint16_t*)a.k + (size_t)p.token_first * a.token_stride + (size_t)head * a.head_stride;
 	const uint16_t* const value_rows = (const uint16_t*)a.v + (size_t)p.token_first * a.token_stride + (size_t)head * a.head_stride;
-	struct Staged { u32x4 k[PIECES], v[PIECES]; };
-	/* pieces of 16 bytes of a tile: where they lie from the sequence's first token on, and in LDS. With whole pieces what lies behind the last token is zeros (the hardware's own check of
-	 * offsets in a buffer), else the last token again: no row sees it */
+	/*
+	 * Pieces of 16 bytes of a step: a tile's keys, then (another tile's) values, shared out over the lanes; whole wavefronts bring the one or the other. `at`: where they lie from the
+	 * sequence's first token on, `to`: where they go in LDS, in the three places in turn. With whole pieces what lies behind the last token is zeros (the hardware's own check of
+	 * offsets in a buffer), else the last token again: no row sees it.
+	 */
+	struct Staged { u32x4 w[PIECES]; };
 	const uint32_t stride = (uint32_t)(2 * a.token_stride), size = p.tokens ? (p.tokens - 1) * stride + 64 * J : 0;
-	const auto key_buffer = __builtin_amdgcn_make_buffer_rsrc(same_in_all(key_rows), 0, __builtin_amdgcn_readfirstlane((int)size), 0x00020000);
-	const auto value_buffer = __builtin_amdgcn_make_buffer_rsrc(same_in_all(value_rows), 0, __builtin_amdgcn_readfirstlane((int)size), 0x00020000);
-	uint32_t at_key[PIECES], at_value[PIECES], to_key[PIECES], to_value[PIECES];
+	const auto size_in_all = __builtin_amdgcn_readfirstlane((int)size);
+	constexpr uint32_t AHEAD_KEYS = 3, AHEAD_VALUES = 1; /* tiles on */
+	bool values[PIECES];
+	void* rows_of[PIECES];
+	uint32_t at[PIECES], to[PIECES], to0[PIECES], to1[PIECES], to2[PIECES];
 #pragma unroll
 	for (int i = 0; i < PIECES; ++i) {
-		const uint32_t piece = min(tid + 256 * i, 4u * J * 32 - 1), token = piece / (4 * J), part = 16 * (piece % (4 * J));
-		at_key[i] = at_value[i] = VEC ? token * stride + part : token;
-		to_key[i] = token * KROW + part;
-		to_value[i] = KTILE + token * VROW + part;
+		const uint32_t first = __builtin_amdgcn_readfirstlane((int)(WAVE * wave + THREADS * i)), piece = tid + THREADS * i;
+		values[i] = first >= TILE_PIECES;
+		rows_of[i] = same_in_all(values[i] ? value_rows : key_rows);
+		const bool none = first >= 2 * TILE_PIECES; /* (those fetch nothing, and store to a place of their own) */
+		const uint32_t n = none ? 0 : values[i] ? piece - TILE_PIECES : piece, token = n / (4 * J), part = 16 * (n % (4 * J));
+		const uint32_t from = token + 32 * (values[i] ? AHEAD_VALUES : AHEAD_KEYS);
+		at[i] = VEC ? (none ? size : from * stride + part) : (none ? 0xFFFFFFFFu : from);
+		to[i] = none ? 3 * PLACE + 16 * lane : values[i] ? KTILE + token * VROW + part : token * KROW + part; /* and in a place: */
+		to0[i] = to[i] + (none ? 0 : values[i] ? PLACE : 0);
+		to1[i] = to[i] + (none ? 0 : values[i] ? 2 * PLACE : PLACE);
+		to2[i] = to[i] + (none ? 0 : values[i] ? 0 : 2 * PLACE);
 	}
-	auto load_key = [&](int i) { /* and on to the next tile */
+	auto load = [&](int i) { /* and on to the next tile */
 		u32x4 w;
-		if constexpr (VEC) w = __builtin_bit_cast(u32x4, __builtin_amdgcn_raw_buffer_load_b128(key_buffer, (int)at_key[i], 0, 0));
-		else w = load_raw8(key_rows + (size_t)min(at_key[i], p.tokens - 1) * a.token_stride + 8 * (min(tid + 256 * i, 4u * J * 32 - 1) % (4 * J)), false);
-		at_key[i] += VEC ? 32 * stride : 32;
+		if constexpr (VEC) {
+			const auto buffer = __builtin_amdgcn_make_buffer_rsrc(rows_of[i], 0, size_in_all, 0x00020000);
+			w = __builtin_bit_cast(u32x4, __builtin_amdgcn_raw_buffer_load_b128(buffer, (int)at[i], 0, 0));
+			at[i] += 32 * stride;
+			asm volatile("" : "+v"(at[i])); /* (one register, not one for each of six steps) */
+		} else {
+			w = load_raw8((const uint16_t*)rows_of[i] + (size_t)min(at[i], p.tokens - 1) * a.token_stride + 8 * ((tid + THREADS * i) % (4 * J)), false);
+			at[i] = at[i] > 0xFFFFFFFFu - 32 ? at[i] : at[i] + 32;
+		}
 		return w;
 	};
-	auto load_value = [&](int i) {
-		u32x4 w;
-		if constexpr (VEC) w = __builtin_bit_cast(u32x4, __builtin_amdgcn_raw_buffer_load_b128(value_buffer, (int)at_value[i], 0, 0));
-		else w = load_raw8(value_rows + (size_t)min(at_value[i], p.tokens - 1) * a.token_stride + 8 * (min(tid + 256 * i, 4u * J * 32 - 1) % (4 * J)), false);
-		at_value[i] += VEC ? 32 * stride : 32;
-		return w;
-	};
-	/* (of a tile that has no multiple of 256 pieces some lanes bring the last piece again) */
-	auto store_key = [&](uint32_t at, const u32x4& w, int i) { *(u32x4*)(lds + at + to_key[i]) = w; };
-	auto store_value = [&](uint32_t at, const u32x4& w, int i) { *(u32x4*)(lds + at + to_value[i]) = w; };
-	auto check = [&](u32x4 (&w)[PIECES], uint32_t tile) { /* 0 times an infinity must not come into rows that do not see it */
+	auto check = [&](Staged& g, uint32_t tile) { /* of values: 0 times an infinity must not come into rows that do not see it */
 		if ((int32_t)(32 * tile + 32) <= all_see) return;
 		bool found = false;
 #pragma unroll
-		for (int i = 0; i < PIECES; ++i) found = without_strange<T>(w[i]) || found;
+		for (int i = 0; i < PIECES; ++i)
+			if (values[i]) found = without_strange<T>(g.w[i]) || found;
 		if (found) strange = 1;
 	};
 
@@ -266,12 +279,14 @@ prompt_attend_kernel(PromptAttend a)
 		const int32_t from = (int32_t)(32 * tile);
 		if (least - from >= 32) return;
 #pragma unroll
-		for (int b = 0; b < B; ++b)
+		for (int b = 0; b < B; ++b) {
+			const int32_t some = sees[b] - from - 4 * (int32_t)h; /* (compared with numbers that stand in the instructions) */
 #pragma unroll
-			for (int e = 0; e < 16; ++e) sc.s[b][e] = 8 * (e / 4) + 4 * (int32_t)h + e % 4 < sees[b] - from ? sc.s[b][e] : -__builtin_inff();
+			for (int e = 0; e < 16; ++e) sc.s[b][e] = some > 8 * (e / 4) + e % 4 ? sc.s[b][e] : -__builtin_inff();
+		}
 	};
 	/* operands come in batches, one in use and one on its way */
-	constexpr int STEPS = 2 * J, BATCH = J == 2 ? 1 : J, SLOTS = 2 * STEPS * B, BATCH_SLOTS = 2 * BATCH * B;
+	constexpr int STEPS = 2 * J, BATCH = prompt_batch<J, W>(), SLOTS = 2 * STEPS * B, BATCH_SLOTS = 2 * BATCH * B;
 	u32x4 kop[2][BATCH], vop[2][BATCH];
 	Staged g0, g1; /* keys three tiles on and values one; then those of the next tile */
 	Scores s0, s1;
@@ -313,7 +328,7 @@ prompt_attend_kernel(PromptAttend a)
 				asm volatile("" : "+v"(exponent[n % 2]));
 			}
 		};
-		constexpr int TURNS = 16 * B + 2, BATCHES = STEPS / BATCH, READS = 3 * BATCH, MOVES = 4 * PIECES / BATCHES, ITEMS = READS + MOVES;
+		constexpr int TURNS = 16 * B + 2, BATCHES = STEPS / BATCH, READS = 3 * BATCH, MOVES = (2 * PIECES + BATCHES - 1) / BATCHES, ITEMS = READS + MOVES;
 		auto slot = [&](int t) {
 #pragma unroll
 			for (int n = TURNS * t / SLOTS; n < TURNS * (t + 1) / SLOTS; ++n) turn(n);
@@ -325,10 +340,8 @@ prompt_attend_kernel(PromptAttend a)
 				const int move = MOVES * p / ITEMS, read = p - move;
 				if (MOVES * (p + 1) / ITEMS > move) {
 					const int m = batch * MOVES + move, i = m % PIECES;
-					if (m / PIECES == 0) store_key(HERE, g.k[i], i);
-					else if (m / PIECES == 1) store_value(ON1, g.v[i], i);
-					else if (m / PIECES == 2) g.k[i] = load_key(i);
-					else g.v[i] = load_value(i);
+					if (m < PIECES) *(u32x4*)(lds + (N % 3 == 0 ? to0[i] : N % 3 == 1 ? to1[i] : to2[i])) = g.w[i];
+					else if (m < 2 * PIECES) g.w[i] = load(i);
 				} else {
 					const int n = read / 3, i = first < STEPS ? first + n : n;
 					if (read % 3 == 0) kop[at][n] = key_operand(first < STEPS ? ON1 : ON2, i);
@@ -370,25 +383,22 @@ prompt_attend_kernel(PromptAttend a)
 #pragma unroll
 		for (int b = 0; b < B; ++b)
 			for (int c = 0; c < 2; ++c) w1.w[b][c] = u32x4{ 0, 0, 0, 0 };
-		u32x4 k[3][PIECES];
-#pragma unroll
-		for (int n = 0; n < 3; ++n)
-			for (int i = 0; i < PIECES; ++i) k[n][i] = load_key(i);
-#pragma unroll
-		for (int i = 0; i < PIECES; ++i) g0.v[i] = load_value(i);
-#pragma unroll
-		for (int i = 0; i < PIECES; ++i) {
-			for (int n = 0; n < 3; ++n) store_key(n * PLACE, k[n][i], i);
-			store_value(2 * PLACE, u32x4{ 0, 0, 0, 0 }, i); /* (nothing before the first tile) */
-		}
-		check(g0.v, 0);
-#pragma unroll
-		for (int i = 0; i < PIECES; ++i) store_value(0, g0.v[i], i);
+		/* the first tiles: three of keys, one of values */
+		auto bring_tile = [&](const uint16_t* rows, uint32_t tile, uint32_t place, uint32_t row, bool checked) {
+			for (uint32_t piece = tid; piece < TILE_PIECES; piece += THREADS) {
+				const uint32_t token = piece / (4 * J), part = piece % (4 * J);
+				u32x4 w = load_raw8(rows + (size_t)min(32 * tile + token, p.tokens - 1) * a.token_stride + 8 * part, VEC);
+				if (checked && (int32_t)(32 * tile + 32) > all_see && without_strange<T>(w)) strange = 1;
+				*(u32x4*)(lds + place + token * row + 16 * part) = w;
+			}
+		};
+		for (uint32_t n = 0; n < 3; ++n) bring_tile(key_rows, n, n * PLACE, KROW, false);
+		bring_tile(value_rows, 0, KTILE, VROW, true);
+		for (uint32_t piece = tid; piece < TILE_PIECES; piece += THREADS) /* (nothing before the first tile) */
+			*(u32x4*)(lds + 2 * PLACE + KTILE + piece / (4 * J) * VROW + 16 * (piece % (4 * J))) = u32x4{ 0, 0, 0, 0 };
 		auto fetch = [&](Staged& g) {
 #pragma unroll
-			for (int i = 0; i < PIECES; ++i) g.k[i] = load_key(i);
-#pragma unroll
-			for (int i = 0; i < PIECES; ++i) g.v[i] = load_value(i);
+			for (int i = 0; i < PIECES; ++i) g.w[i] = load(i);
 		};
 		fetch(g0);
 		fetch(g1);
@@ -408,7 +418,7 @@ prompt_attend_kernel(PromptAttend a)
 		__syncthreads();
 		uint32_t tile = 0;
 		auto step = [&](auto number) {
-			check(decltype(number)::value % 2 ? g1.v : g0.v, tile + 1);
+			check(decltype(number)::value % 2 ? g1 : g0, tile + 1);
 			work(number, tile);
 			/* what was stored to LDS is there: of what LDS was asked for since, the last batch's reads are for the next step and need not be back */
 			constexpr int LATE = 3 * BATCH < 14 ? 3 * BATCH : 14;
@@ -420,12 +430,11 @@ prompt_attend_kernel(PromptAttend a)
 			    !step(std::integral_constant<uint32_t, 3>{}) || !step(std::integral_constant<uint32_t, 4>{}) || !step(std::integral_constant<uint32_t, 5>{}))
 				break;
 		auto bring = [&](Staged& g) {
-			check(g.v, tile + 1);
-			const uint32_t here = tile % 3, on1 = (tile + 1) % 3;
+			check(g, tile + 1);
 #pragma unroll
 			for (int i = 0; i < PIECES; ++i) {
-				store_key(here * PLACE, g.k[i], i);
-				store_value(on1 * PLACE, g.v[i], i);
+				const uint32_t place = (tile + (values[i] ? AHEAD_VALUES : 0)) % 3;
+				*(u32x4*)(lds + to[i] + (WAVE * wave + THREADS * i < 2 * TILE_PIECES ? place * PLACE : 0)) = g.w[i];
 			}
 			fetch(g);
 			__syncthreads();
@@ -476,7 +485,7 @@ prompt_attend_kernel(PromptAttend a)
 	}
 }
 
-template <typename T, int J, int B, bool VEC>
+template <typename T, int J, int W, int B, bool VEC>
 static int launch_prompt_kernel(const PromptAttend& a, uint32_t units)
 {
 	constexpr uint32_t bytes = prompt_lds<J>();
@@ -486,25 +495,37 @@ static int launch_prompt_kernel(const PromptAttend& a, uint32_t units)
 		const int rc = device_info(&dev);
 		if (rc) return rc;
 		if (allowed != dev->device) {
-			KMX_HIP(hipFuncSetAttribute((const void*)prompt_attend_kernel<T, J, B, VEC>, hipFuncAttributeMaxDynamicSharedMemorySize, (int)bytes));
+			KMX_HIP(hipFuncSetAttribute((const void*)prompt_attend_kernel<T, J, W, B, VEC>, hipFuncAttributeMaxDynamicSharedMemorySize, (int)bytes));
 			allowed = dev->device;
 		}
 	}
-	KMX_LAUNCH_KERNEL((prompt_attend_kernel<T, J, B, VEC>), dim3(units), dim3(256), bytes, stream(), a);
+	KMX_LAUNCH_KERNEL((prompt_attend_kernel<T, J, W, B, VEC>), dim3(units), dim3(64 * W), bytes, stream(), a);
 	KMX_LAUNCH_CHECK("prompt_attend_kernel");
 	return KMX_OK;
 }
 
-template <typename T, int J>
-static int launch_prompt_of(PromptAttend a)
+template <typename T, int J, int W>
+static int launch_prompt_rows(PromptAttend a)
 {
-	constexpr int B = J <= 4 ? 2 : 1;
-	const uint64_t rows = (uint64_t)a.max_queries * a.group, row_tiles = (rows + 128 * B - 1) / (128 * B);
+	constexpr int B = 1;
+	const uint64_t rows = (uint64_t)a.max_queries * a.group, row_tiles = (rows + 32 * W * B - 1) / (32 * W * B);
 	if (rows > 0x7FFFFF00u || (uint64_t)a.heads * a.sequences > 0x7FFFFFFFu || row_tiles * a.heads * a.sequences > 0x7FFFFFFFu)
 		return fail(KMX_ERR_UNSUPPORTED, "kmx_prompt_attend: too many queries for one call");
 	a.row_tiles = (uint32_t)row_tiles;
 	const uint32_t units = (uint32_t)(row_tiles * a.heads * a.sequences);
-	return a.vec ? launch_prompt_kernel<T, J, B, true>(a, units) : launch_prompt_kernel<T, J, B, false>(a, units);
+	return a.vec ? launch_prompt_kernel<T, J, W, B, true>(a, units) : launch_prompt_kernel<T, J, W, B, false>(a, units);
+}
+
+template <typename T, int J>
+static int launch_prompt_of(const PromptAttend& a)
+{
+	if constexpr (J >= 3 && J <= 6) {
+		const DeviceInfo* dev = nullptr;
+		const int rc = device_info(&dev);
+		if (rc) return rc;
+		if ((uint64_t)a.max_queries * a.group * a.heads * a.sequences > 512 * (uint64_t)dev->compute_units) return launch_prompt_rows<T, J, 8>(a);
+	}
+	return launch_prompt_rows<T, J, 4>(a);
 }
 
 template <int J>
