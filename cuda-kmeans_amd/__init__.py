@@ -40,7 +40,7 @@ ABI_SYMBOLS = [
     "kmx_event_elapsed_ms", "kmx_set_profiling", "kmx_last_kernel_ms", "kmx_last_error", "kmx_certificate_tau", "kmx_certificate_unmoved_threshold",
     "kmx_update_f32_noalloc", "kmx_reserve_f32", "kmx_prepare_points_f64", "kmx_forget_points_f64", "kmx_probe_matrix_chain", "kmx_set_two_level_sweep", "kmx_iteration_f32", "kmx_iteration_last_passes",
     "kmx_cache4_sizes", "kmx_cache4_round_levels", "kmx_cache4_write", "kmx_cache4_read", "kmx_cache4_bound", "kmx_cache4_select", "kmx_cache4_attend", "kmx_cache4_reserve",
-    "kmx_cache4_attend_shared", "kmx_cache4_reserve_shared", "kmx_cache4_weigh", "kmx_cache4_evict", "kmx_rotary_turns", "kmx_rotary", "kmx_prompt_attend",
+    "kmx_cache4_attend_shared", "kmx_cache4_reserve_shared", "kmx_cache4_weigh", "kmx_cache4_evict", "kmx_rotary_turns", "kmx_rotary", "kmx_prompt_attend", "kmx_prompt_reserve",
 ]
 
 
@@ -184,6 +184,7 @@ def hip_lib():
         f64 = ctypes.c_double
         lib.kmx_rotary_turns.argtypes = [u32, f64, f64, f64, f64, f64, vp]
         lib.kmx_rotary.argtypes = [ctypes.c_int, ctypes.POINTER(RotaryRowsStruct), u32, u32, u32, u32, vp, vp, ctypes.c_int, ctypes.c_int, ctypes.c_float]
+        lib.kmx_prompt_reserve.argtypes = [u32]
         lib.kmx_prompt_attend.argtypes = [ctypes.POINTER(PromptStruct), ctypes.c_int, vp, sz, sz, vp, vp, sz, sz, vp, sz, sz, vp, ctypes.c_float, ctypes.c_int]
         _hip = lib
     return _hip
@@ -695,6 +696,11 @@ class Prompt:
         out_strides = self._strides(self.query_heads, out_token_stride, out_head_stride)
         check(hip_lib().kmx_prompt_attend(self.ref, element_type, q.ptr, *strides, keys.ptr, values.ptr, *key_strides, out.ptr, *out_strides,
                                           lse.ptr if lse is not None else None, scale, int(causal)))
+
+    @staticmethod
+    def reserve(dim):
+        """Sizes the work space for attention over prompts with heads of `dim` channels (kmx_prompt_reserve)."""
+        check(hip_lib().kmx_prompt_reserve(dim))
 
 
 # ---------------------------------------------------------------- algorithm objects --------------

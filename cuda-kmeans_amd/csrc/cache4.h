@@ -193,7 +193,7 @@ int check_cache4(const char* who, const kmx_cache4* cache, Cache4* out);
 int check_batch4(const char* who, const kmx_cache4* cache, const kmx_cache4_batch* batch, int causal, Batch4* out);
 int check_type(const char* who, int type, bool floats);
 bool aligned_rows(const void* p, size_t token_stride, size_t head_stride, size_t size);
-int place_cache4(const char* who, size_t floats, float** partials);
+int place_cache4(const char* who, size_t floats, float** partials, const char* reserve = "kmx_cache4_reserve");
 
 /* cache4_attend_impl.h, one object per J: see there */
 struct Attend4 {

@@ -824,7 +824,7 @@ int kmx::check_batch4(const char* who, const kmx_cache4* cache, const kmx_cache4
  * Work space of a call. A recording keeps the addresses of its moment, and the work space moves when a later call needs more of it: recorded calls take the static
  * scratch array of recorded updates where it has room (64 MB: all attention of few rows, and choices of 16M scores), else the work space.
  */
-int kmx::place_cache4(const char* who, size_t floats, float** partials)
+int kmx::place_cache4(const char* who, size_t floats, float** partials, const char* reserve)
 {
 	const bool recorded = launches_recorded();
 	const Workspace* fixed = recorded ? fixed_scratch() : nullptr;
@@ -837,7 +837,7 @@ int kmx::place_cache4(const char* who, size_t floats, float** partials)
 	int rc = workspace(&ws);
 	if (rc) return rc;
 	if (recorded && floats > ws->partials_cap)
-		return fail(KMX_ERR_INVALID_ARGUMENT, "%s: the call needs a larger work space, which cannot be allocated while it is recorded: kmx_cache4_reserve, or the same call once before", who);
+		return fail(KMX_ERR_INVALID_ARGUMENT, "%s: the call needs a larger work space, which cannot be allocated while it is recorded: %s, or the same call once before", who, reserve);
 	if (recorded) scratch_recorded();
 	rc = reserve_partials(ws, floats);
 	*partials = ws->partials;

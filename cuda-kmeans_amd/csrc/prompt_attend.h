@@ -5,6 +5,7 @@
 #define KMX_PROMPT_ATTEND_H
 
 #include "cache4.h"
+#include "prompt_plan.h"
 
 namespace kmx {
 
@@ -19,9 +20,10 @@ struct PromptAttend {
 	float factor;             /* |scale| log2(e) */
 	uint32_t q_keep, q_turn;  /* bits of two queries that stay, and those that are turned over */
 	bool causal, vec;         /* vec: rows of 16-byte pieces */
-	uint32_t row_tiles;       /* (filled in by the launcher) */
+	uint32_t row_tiles, units, parts, tiles_per_part; /* (filled in by the launcher) */
+	float* partial;           /* sums of parts, where there are any */
 };
-template <int J> int launch_prompt_attend(const PromptAttend& a, bool bf16);
+template <int J> int launch_prompt_attend(const PromptAttend& a, bool bf16, const PromptPlan& plan);
 
 } // namespace kmx
 

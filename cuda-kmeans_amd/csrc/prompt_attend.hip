@@ -59,16 +59,41 @@ int kmx_prompt_attend(const kmx_prompt* prompt, int type, const void* q, size_t 
 	a.vec = aligned(q, q_token_stride, q_head_stride) && aligned(keys, token_stride, head_stride) && aligned(values, token_stride, head_stride) && aligned(out, out_token_stride, out_head_stride);
 	/* offsets of pieces are counted in 32 bits, from the end of a sequence as far on as it is long among them */
 	if ((uint64_t)a.max_tokens + 192 > 0x7FFFFFFFu / 2 / (token_stride ? token_stride : 1)) a.vec = false;
-	switch (b.dim / 32) {
-	case 1: return launch_prompt_attend<1>(a, type == KMX_BF16);
-	case 2: return launch_prompt_attend<2>(a, type == KMX_BF16);
-	case 3: return launch_prompt_attend<3>(a, type == KMX_BF16);
-	case 4: return launch_prompt_attend<4>(a, type == KMX_BF16);
-	case 5: return launch_prompt_attend<5>(a, type == KMX_BF16);
-	case 6: return launch_prompt_attend<6>(a, type == KMX_BF16);
-	case 7: return launch_prompt_attend<7>(a, type == KMX_BF16);
-	default: return launch_prompt_attend<8>(a, type == KMX_BF16);
+	const DeviceInfo* dev = nullptr;
+	const int rc = device_info(&dev);
+	if (rc) return rc;
+	const uint32_t J = b.dim / 32;
+	const PromptPlan plan = plan_prompt(PromptShape{ J, a.heads, a.group, a.sequences, a.max_queries, a.max_tokens, dev->compute_units });
+	if (plan.units == 0) return fail(KMX_ERR_UNSUPPORTED, "kmx_prompt_attend: too many queries for one call");
+	if (const size_t floats = prompt_floats(plan, J)) {
+		const int rc2 = place_cache4("kmx_prompt_attend", floats, &a.partial, "kmx_prompt_reserve");
+		if (rc2) return rc2;
 	}
+	const bool bf16 = type == KMX_BF16;
+	switch (J) {
+	case 1: return launch_prompt_attend<1>(a, bf16, plan);
+	case 2: return launch_prompt_attend<2>(a, bf16, plan);
+	case 3: return launch_prompt_attend<3>(a, bf16, plan);
+	case 4: return launch_prompt_attend<4>(a, bf16, plan);
+	case 5: return launch_prompt_attend<5>(a, bf16, plan);
+	case 6: return launch_prompt_attend<6>(a, bf16, plan);
+	case 7: return launch_prompt_attend<7>(a, bf16, plan);
+	default: return launch_prompt_attend<8>(a, bf16, plan);
+	}
+}
+
+int kmx_prompt_reserve(uint32_t dim)
+{
+	clear_error();
+	if (recording_graph()) return fail(KMX_ERR_INVALID_ARGUMENT, "kmx_prompt_reserve: not allowed between kmx_graph_begin and kmx_graph_end");
+	if (dim == 0 || dim % 32 || dim > 256) return fail(KMX_ERR_UNSUPPORTED, "kmx_prompt_reserve: dim %u is no multiple of 32 up to 256", dim);
+	const DeviceInfo* dev = nullptr;
+	const int rc = device_info(&dev);
+	if (rc) return rc;
+	Workspace* scratch = nullptr;
+	if (noalloc_workspace(&scratch)) clear_error(); /* the address of the scratch array that recorded calls use (they do without if it has none) */
+	float* partials = nullptr;
+	return place_cache4("kmx_prompt_reserve", most_prompt_floats(dim / 32, dev->compute_units), &partials);
 }
 
 } // extern "C"

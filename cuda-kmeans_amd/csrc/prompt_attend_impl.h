@@ -108,59 +108,56 @@ template <int J, int W> constexpr int prompt_batch() { return J <= 6 ? 1 : J; }
 template <int J> constexpr uint32_t prompt_lds() { return 3 * 32 * (key_row<J>() + value_row<J>()) + 1024; } /* (and a place for what wavefronts without pieces store) */
 
 /*
- * A work-group of four wavefronts takes 128 B rows of one head of the keys (the query heads of a query side by side, then the next query's), 32 B a wavefront. Tiles of
- * 32 tokens pass through LDS as they are, three of keys and three of values, from registers that were loaded two tiles before. Both products have the keys' and values' side as
- * their first operand (v_mfma_f32_32x32x16): scores come out as [token][row], a lane has 16 scores of its row, and its probabilities are, as they stand, its piece of the
- * second operand of [channel][row] = values . p; the values' columns are turned on the way from LDS (ds_read_b64_tr_b16).
- * While the vector units make a tile's probabilities, the matrix cores have the scores of the next one and the sums of the one before: nothing of these three waits for
- * another. Where a row's weights come to more than they may, its reference is raised and they are made again.
+ * Attention over prompts: out = sum_t exp(scale q . k_t) v_t / sum_t exp(scale q . k_t) in one pass, with a reference for the exponents that is raised where a row's weights come to
+ * more than 2^15. A work-group of W wavefronts takes 32 W rows of one head of the keys (the query heads of a query side by side, then the next query's), 32 a wavefront, over all
+ * tokens or a part of them. Tiles of 32 tokens pass through LDS as they are, three of keys and three of values, from registers that were loaded two tiles before. Both products have the
+ * keys' and values' side as their first operand (v_mfma_f32_32x32x16): scores come out as [token][row], a lane has 16 scores of its row, and its probabilities are, as they stand, its
+ * piece of the second operand of [channel][row] = values . p; the values' columns are turned on the way from LDS (ds_read_b64_tr_b16).
+ * While the vector units make a tile's probabilities, the matrix cores have the scores of the next one and the sums of the one before: nothing of these three waits for another.
+ *
+ * Bound: products of 4 rows tokens channels operations, at 128 channels. 8192 tokens, 32 heads of 128 over 8 in bf16, causal: 513 us, 1.07 of the 1.18 PFLOP/s that a large product of
+ * matrices reaches here. At 64 channels the vector units have as much to do (a power a score) as the matrix cores: 6 prompts of up to 4096 in half precision 202 us. A single query over
+ * 8192 tokens: 129 us by one work-group a head, 18 by parts (its keys and values take 7). Steps on the way, at 8192 tokens: scores, powers and sums one after the other 1191 us; side by
+ * side 733; operands two products ahead 606; powers between the products 564; sums in place of the largest score 528; three places in LDS and buffer loads 521; eight wavefronts 513.
  */
-template <typename T, int J, int W, int B, bool VEC>
+template <typename T, int J, int W, bool VEC>
 __global__ void __launch_bounds__(64 * W, (prompt_waves<J, W>()))
 prompt_attend_kernel(PromptAttend a)
 {
 	constexpr uint32_t KROW = key_row<J>(), VROW = value_row<J>(), KTILE = 32 * KROW, PLACE = KTILE + 32 * VROW;
-	constexpr uint32_t THREADS = 64 * W, ROWS = 32 * W * B;
+	constexpr uint32_t THREADS = 64 * W, ROWS = 32 * W;
 	constexpr uint32_t TILE_PIECES = 4 * J * 32; /* of 16 bytes, of keys, and as many of values */
 	constexpr int PIECES = (2 * TILE_PIECES + THREADS - 1) / THREADS; /* that a lane brings each step */
 	extern __shared__ __attribute__((aligned(16))) uint8_t lds[];
 	__shared__ uint32_t strange; /* values that are no numbers, where not all rows see them */
 	const uint32_t tid = threadIdx.x, wave = (uint32_t)__builtin_amdgcn_readfirstlane((int)(tid / WAVE)), lane = tid % WAVE, n32 = lane % 32, h = lane / 32;
 	/* heads take turns over the dies, and the rows that see the most come first */
-	const uint32_t head = blockIdx.x % a.heads, rest = blockIdx.x / a.heads, s = rest % a.sequences, row_tile = a.row_tiles - 1 - rest / a.sequences;
+	const uint32_t part = blockIdx.x / a.units, unit = blockIdx.x - part * a.units, head = unit % a.heads, rest = unit / a.heads, s = rest % a.sequences, row_tile = a.row_tiles - 1 - rest / a.sequences;
 	const Prompt4 p = prompt_of(a, s);
 	const uint32_t all_rows = p.queries * a.group, first_row = row_tile * ROWS; /* (31 bits) */
 	if (first_row >= all_rows) return;
 	const uint32_t rows = min(ROWS, all_rows - first_row);
-	const uint32_t end = ((uint32_t)sees_of(a, p, (first_row + rows - 1) / a.group) + 31) / 32; /* tiles */
-	const int32_t all_see = sees_of(a, p, first_row / a.group);
+	const uint32_t all_tiles = ((uint32_t)sees_of(a, p, (first_row + rows - 1) / a.group) + 31) / 32, start = part * a.tiles_per_part;
+	if (part && start >= all_tiles) return;
+	const uint32_t end = min(all_tiles - start, a.tiles_per_part); /* tiles, from the part's first one on */
+	const int32_t limit = (int32_t)min(32 * (start + end), 0x7FFFFFFFu); /* tokens behind are another part's */
+	const int32_t all_see = min(sees_of(a, p, first_row / a.group), limit);
 
 	/* the rows of the lane, what those of its wavefront see at least, and the tiles they look at */
-	const uint32_t wave_first = 32 * B * wave, wave_rows = rows > wave_first ? min(32u * B, rows - wave_first) : 0;
-	uint32_t query[B], query_head[B];
-	int32_t sees[B];
-	bool there[B];
-#pragma unroll
-	for (int b = 0; b < B; ++b) {
-		there[b] = 32 * b + n32 < wave_rows;
-		const uint32_t x = first_row + (there[b] ? wave_first + 32 * b + n32 : 0);
-		query[b] = x / a.group;
-		query_head[b] = head * a.group + (x - query[b] * a.group);
-		sees[b] = there[b] ? sees_of(a, p, query[b]) : 0;
-	}
-	const int32_t least = wave_rows ? sees_of(a, p, (first_row + wave_first) / a.group) : 0;
-	const uint32_t mine = wave_rows ? ((uint32_t)sees_of(a, p, (first_row + wave_first + wave_rows - 1) / a.group) + 31) / 32 : 0;
+	const uint32_t wave_first = 32 * wave, wave_rows = rows > wave_first ? min(32u, rows - wave_first) : 0;
+	const bool there = n32 < wave_rows;
+	const uint32_t x = first_row + (there ? wave_first + n32 : 0), query = x / a.group, query_head = head * a.group + (x - query * a.group);
+	const int32_t sees = there ? min(sees_of(a, p, query), limit) : 0;
+	const int32_t least = wave_rows ? min(sees_of(a, p, (first_row + wave_first) / a.group), limit) : 0;
+	const uint32_t seen = wave_rows ? ((uint32_t)min(sees_of(a, p, (first_row + wave_first + wave_rows - 1) / a.group), limit) + 31) / 32 : 0, mine = seen > start ? seen - start : 0;
 
-	u32x4 q[B][2 * J]; /* channels 16 c + 8 h .. + 7 */
+	u32x4 q[2 * J]; /* channels 16 c + 8 h .. + 7 */
+	const uint16_t* from = (const uint16_t*)a.q + (size_t)(p.query_first + query) * a.q_token + (size_t)query_head * a.q_head + 8 * h;
 #pragma unroll
-	for (int b = 0; b < B; ++b) {
-		const uint16_t* from = (const uint16_t*)a.q + (size_t)(p.query_first + query[b]) * a.q_token + (size_t)query_head[b] * a.q_head + 8 * h;
-#pragma unroll
-		for (int c = 0; c < 2 * J; ++c) {
-			q[b][c] = load_raw8(from + 16 * c, VEC);
-			for (int e = 0; e < 4; ++e) q[b][c][e] = (q[b][c][e] & a.q_keep) ^ a.q_turn; /* the sign of the scale; nothing of them where it is 0 */
-			if constexpr (prompt_waves<J, W>() == 1) asm volatile("" : "+a"(q[b][c])); /* (the other half of the registers) */
-		}
+	for (int c = 0; c < 2 * J; ++c) {
+		q[c] = load_raw8(from + 16 * c, VEC);
+		for (int e = 0; e < 4; ++e) q[c][e] = (q[c][e] & a.q_keep) ^ a.q_turn; /* the sign of the scale; nothing of them where it is 0 */
+		if constexpr (prompt_waves<J, W>() == 1) asm volatile("" : "+a"(q[c])); /* (the other half of the registers) */
 	}
 
 	/* what lies behind the last token is the last token again: no row sees it */
@@ -185,7 +182,7 @@ prompt_attend_kernel(PromptAttend a)
 		rows_of[i] = same_in_all(values[i] ? value_rows : key_rows);
 		const bool none = first >= 2 * TILE_PIECES; /* (those fetch nothing, and store to a place of their own) */
 		const uint32_t n = none ? 0 : values[i] ? piece - TILE_PIECES : piece, token = n / (4 * J), part = 16 * (n % (4 * J));
-		const uint32_t from = token + 32 * (values[i] ? AHEAD_VALUES : AHEAD_KEYS);
+		const uint32_t from = token + 32 * (start + (values[i] ? AHEAD_VALUES : AHEAD_KEYS));
 		at[i] = VEC ? (none ? size : from * stride + part) : (none ? 0xFFFFFFFFu : from);
 		to[i] = none ? 3 * PLACE + 16 * lane : values[i] ? KTILE + token * VROW + part : token * KROW + part; /* and in a place: */
 		to0[i] = to[i] + (none ? 0 : values[i] ? PLACE : 0);
@@ -206,7 +203,7 @@ prompt_attend_kernel(PromptAttend a)
 		return w;
 	};
 	auto check = [&](Staged& g, uint32_t tile) { /* of values: 0 times an infinity must not come into rows that do not see it */
-		if ((int32_t)(32 * tile + 32) <= all_see) return;
+		if ((int32_t)(32 * (start + tile) + 32) <= all_see) return;
 		bool found = false;
 #pragma unroll
 		for (int i = 0; i < PIECES; ++i)
@@ -214,20 +211,14 @@ prompt_attend_kernel(PromptAttend a)
 		if (found) strange = 1;
 	};
 
-	float reference[B], base[B], l[B];
-	f32x16 o[B][J];
+	float reference = -__builtin_inff(), base = LIFT, l = 0.0f;
+	f32x16 o[J];
 #pragma unroll
-	for (int b = 0; b < B; ++b) {
-		reference[b] = -__builtin_inff();
-		base[b] = LIFT;
-		l[b] = 0.0f;
-#pragma unroll
-		for (int j = 0; j < J; ++j)
-			for (int e = 0; e < 16; ++e) o[b][j][e] = 0.0f;
-	}
+	for (int j = 0; j < J; ++j)
+		for (int e = 0; e < 16; ++e) o[j][e] = 0.0f;
 
-	struct Scores { f32x16 s[B]; };
-	struct Weights { u32x4 w[B][2]; };
+	struct Scores { f32x16 s; };
+	struct Weights { u32x4 w[2]; };
 	const uint8_t* const key_at = lds + n32 * KROW + 16 * h;
 	const uint8_t* const value_at = lds + KTILE + (4 * h + lane % 16 / 4) * VROW + 32 * (lane / 16 % 2) + 8 * (lane % 4);
 	auto key_operand = [&](uint32_t at, int i) { return *(const u32x4*)(key_at + at + 32 * i); };
@@ -237,56 +228,44 @@ prompt_attend_kernel(PromptAttend a)
 		w[2 * half + 1] = v[1];
 	};
 	auto score = [&](Scores& sc, uint32_t at) {
-#pragma unroll
-		for (int b = 0; b < B; ++b)
-			for (int e = 0; e < 16; ++e) sc.s[b][e] = 0.0f;
+		for (int e = 0; e < 16; ++e) sc.s[e] = 0.0f;
 #pragma unroll
 		for (int c = 0; c < 2 * J; ++c) {
 			const u32x4 w = key_operand(at, c);
-#pragma unroll
-			for (int b = 0; b < B; ++b) sc.s[b] = product(w, q[b][c], sc.s[b], T{});
+			sc.s = product(w, q[c], sc.s, T{});
 		}
 	};
-	auto weigh = [&](Weights& p, float (&sum)[B], const Scores& sc) {
+	auto weigh = [&](Weights& p, float& sum, const Scores& sc) {
+		sum = 0.0f;
 #pragma unroll
-		for (int b = 0; b < B; ++b) {
-			sum[b] = 0.0f;
-#pragma unroll
-			for (int e = 0; e < 16; e += 2) {
-				const float x = __builtin_amdgcn_exp2f(fmaf(sc.s[b][e], a.factor, base[b])), y = __builtin_amdgcn_exp2f(fmaf(sc.s[b][e + 1], a.factor, base[b]));
-				sum[b] += x + y;
-				p.w[b][e / 8][e % 8 / 2] = rounded_pair(x, y, T{});
-			}
+		for (int e = 0; e < 16; e += 2) {
+			const float x = __builtin_amdgcn_exp2f(fmaf(sc.s[e], a.factor, base)), y = __builtin_amdgcn_exp2f(fmaf(sc.s[e + 1], a.factor, base));
+			sum += x + y;
+			p.w[e / 8][e % 8 / 2] = rounded_pair(x, y, T{});
 		}
 	};
 	/* the references of rows whose scores pass them (all rows of the wavefront: what has not passed stays), with what was added up so far */
 	auto raise = [&](const Scores& sc) {
+		float top = sc.s[0];
 #pragma unroll
-		for (int b = 0; b < B; ++b) {
-			float top = sc.s[b][0];
+		for (int e = 1; e < 16; ++e) top = fmaxf(top, sc.s[e]);
+		top = both_halves_most(top) * a.factor;
+		const float higher = fmaxf(reference, top), less = higher == reference ? 1.0f : __builtin_amdgcn_exp2f(reference - higher);
+		reference = higher;
+		base = higher == -__builtin_inff() ? LIFT : LIFT - higher;
+		l *= less;
 #pragma unroll
-			for (int e = 1; e < 16; ++e) top = fmaxf(top, sc.s[b][e]);
-			top = both_halves_most(top) * a.factor;
-			const float higher = fmaxf(reference[b], top), less = higher == reference[b] ? 1.0f : __builtin_amdgcn_exp2f(reference[b] - higher);
-			reference[b] = higher;
-			base[b] = higher == -__builtin_inff() ? LIFT : LIFT - higher;
-			l[b] *= less;
-#pragma unroll
-			for (int j = 0; j < J; ++j) o[b][j] *= less;
-		}
+		for (int j = 0; j < J; ++j) o[j] *= less;
 	};
 	auto hide = [&](Scores& sc, uint32_t tile) { /* tokens that a row does not see */
-		const int32_t from = (int32_t)(32 * tile);
+		const int32_t from = (int32_t)(32 * (start + tile));
 		if (least - from >= 32) return;
+		const int32_t some = sees - from - 4 * (int32_t)h; /* (compared with numbers that stand in the instructions) */
 #pragma unroll
-		for (int b = 0; b < B; ++b) {
-			const int32_t some = sees[b] - from - 4 * (int32_t)h; /* (compared with numbers that stand in the instructions) */
-#pragma unroll
-			for (int e = 0; e < 16; ++e) sc.s[b][e] = some > 8 * (e / 4) + e % 4 ? sc.s[b][e] : -__builtin_inff();
-		}
+		for (int e = 0; e < 16; ++e) sc.s[e] = some > 8 * (e / 4) + e % 4 ? sc.s[e] : -__builtin_inff();
 	};
 	/* operands come in batches, one in use and one on its way */
-	constexpr int STEPS = 2 * J, BATCH = prompt_batch<J, W>(), SLOTS = 2 * STEPS * B, BATCH_SLOTS = 2 * BATCH * B;
+	constexpr int STEPS = 2 * J, BATCH = prompt_batch<J, W>(), SLOTS = 2 * STEPS, BATCH_SLOTS = 2 * BATCH;
 	u32x4 kop[2][BATCH], vop[2][BATCH];
 	Staged g0, g1; /* keys three tiles on and values one; then those of the next tile */
 	Scores s0, s1;
@@ -303,32 +282,30 @@ prompt_attend_kernel(PromptAttend a)
 		Scores &now = N % 2 ? s1 : s0, &next = N % 2 ? s0 : s1;
 		Weights &before = N % 2 ? w0 : w1, &weights = N % 2 ? w1 : w0;
 		hide(now, tile);
-#pragma unroll
-		for (int b = 0; b < B; ++b)
-			for (int e = 0; e < 16; ++e) next.s[b][e] = 0.0f;
-		float sum[B], exponent[2], power[2], before_last = 0.0f;
+		for (int e = 0; e < 16; ++e) next.s[e] = 0.0f;
+		float sum, exponent[2], power[2], before_last = 0.0f;
 		auto turn = [&](int n) { /* (the empty statements keep what they name here: left alone all of it goes to where it is used) */
-			const int b2 = (n - 2) / 16, e2 = (n - 2) % 16;
+			const int e2 = n - 2;
 			if (n >= 2) {
-				sum[b2] = e2 ? sum[b2] + power[n % 2] : power[n % 2];
-				asm volatile("" : "+v"(sum[b2]));
+				sum = e2 ? sum + power[n % 2] : power[n % 2];
+				asm volatile("" : "+v"(sum));
 				if (e2 % 2) {
 					uint32_t w = rounded_pair(before_last, power[n % 2], T{});
 					asm volatile("" : "+v"(w));
-					weights.w[b2][e2 / 8][e2 % 8 / 2] = w;
+					weights.w[e2 / 8][e2 % 8 / 2] = w;
 				}
 				before_last = power[n % 2];
 			}
-			if (n >= 1 && n <= 16 * B) {
+			if (n >= 1 && n <= 16) {
 				power[(n - 1) % 2] = __builtin_amdgcn_exp2f(exponent[(n - 1) % 2]);
 				asm volatile("" : "+v"(power[(n - 1) % 2]));
 			}
-			if (n < 16 * B) {
-				exponent[n % 2] = fmaf(now.s[n / 16][n % 16], a.factor, base[n / 16]);
+			if (n < 16) {
+				exponent[n % 2] = fmaf(now.s[n], a.factor, base);
 				asm volatile("" : "+v"(exponent[n % 2]));
 			}
 		};
-		constexpr int TURNS = 16 * B + 2, BATCHES = STEPS / BATCH, READS = 3 * BATCH, MOVES = (2 * PIECES + BATCHES - 1) / BATCHES, ITEMS = READS + MOVES;
+		constexpr int TURNS = 16 + 2, BATCHES = STEPS / BATCH, READS = 3 * BATCH, MOVES = (2 * PIECES + BATCHES - 1) / BATCHES, ITEMS = READS + MOVES;
 		auto slot = [&](int t) {
 #pragma unroll
 			for (int n = TURNS * t / SLOTS; n < TURNS * (t + 1) / SLOTS; ++n) turn(n);
@@ -354,42 +331,30 @@ prompt_attend_kernel(PromptAttend a)
 #pragma unroll
 		for (int i = 0; i < STEPS; ++i) {
 			const int batch = i / BATCH, n = i % BATCH;
-#pragma unroll
-			for (int b = 0; b < B; ++b) {
-				next.s[b] = product(kop[batch % 2][n], q[b][i], next.s[b], T{});
-				slot(2 * B * i + b);
-			}
-#pragma unroll
-			for (int b = 0; b < B; ++b) {
-				o[b][i / 2] = product(vop[batch % 2][n], before.w[b][i % 2], o[b][i / 2], T{});
-				slot(2 * B * i + B + b);
-			}
+			next.s = product(kop[batch % 2][n], q[i], next.s, T{});
+			slot(2 * i);
+			o[i / 2] = product(vop[batch % 2][n], before.w[i % 2], o[i / 2], T{});
+			slot(2 * i + 1);
 		}
 		/* a sum that is no more than 2^(LIFT + RISE) has no weight above it: no need to look for the largest score */
-		bool rises = false;
-#pragma unroll
-		for (int b = 0; b < B; ++b) rises = rises || !(sum[b] <= MOST_SUM);
-		if (__any(rises)) {
+		if (__any(!(sum <= MOST_SUM))) {
 			raise(now);
 			weigh(weights, sum, now);
 		}
-#pragma unroll
-		for (int b = 0; b < B; ++b) l[b] += sum[b];
+		l += sum;
 	};
 
 	if (tid == 0) strange = 0;
 	__syncthreads();
 	if (end) {
-#pragma unroll
-		for (int b = 0; b < B; ++b)
-			for (int c = 0; c < 2; ++c) w1.w[b][c] = u32x4{ 0, 0, 0, 0 };
+		for (int c = 0; c < 2; ++c) w1.w[c] = u32x4{ 0, 0, 0, 0 };
 		/* the first tiles: three of keys, one of values */
 		auto bring_tile = [&](const uint16_t* rows, uint32_t tile, uint32_t place, uint32_t row, bool checked) {
 			for (uint32_t piece = tid; piece < TILE_PIECES; piece += THREADS) {
-				const uint32_t token = piece / (4 * J), part = piece % (4 * J);
-				u32x4 w = load_raw8(rows + (size_t)min(32 * tile + token, p.tokens - 1) * a.token_stride + 8 * part, VEC);
-				if (checked && (int32_t)(32 * tile + 32) > all_see && without_strange<T>(w)) strange = 1;
-				*(u32x4*)(lds + place + token * row + 16 * part) = w;
+				const uint32_t token = piece / (4 * J), at_row = piece % (4 * J);
+				u32x4 w = load_raw8(rows + (size_t)min(32 * (start + tile) + token, p.tokens - 1) * a.token_stride + 8 * at_row, VEC);
+				if (checked && (int32_t)(32 * (start + tile) + 32) > all_see && without_strange<T>(w)) strange = 1;
+				*(u32x4*)(lds + place + token * row + 16 * at_row) = w;
 			}
 		};
 		for (uint32_t n = 0; n < 3; ++n) bring_tile(key_rows, n, n * PLACE, KROW, false);
@@ -447,7 +412,7 @@ prompt_attend_kernel(PromptAttend a)
 
 	if (strange) { /* infinities and NaN come to the rows that see them (their weights are above 0, however small) */
 #pragma unroll 1
-		for (uint32_t t = (uint32_t)all_see / 32 * 32; t < p.tokens && t < 32 * end; ++t) {
+		for (uint32_t t = max((uint32_t)all_see / 32, start) * 32; t < p.tokens && t < (uint32_t)limit; ++t) {
 			const uint16_t* from = value_rows + (size_t)t * a.token_stride;
 #pragma unroll
 			for (int j = 0; j < J; ++j)
@@ -455,37 +420,96 @@ prompt_attend_kernel(PromptAttend a)
 				for (int e = 0; e < 16; ++e) {
 					const float x = raw_element(from[32 * j + 8 * (e / 4) + 4 * h + e % 4], false, __is_same(T, __bf16));
 					const bool number = fabsf(x) <= 3.4028235e38f;
-#pragma unroll
-					for (int b = 0; b < B; ++b) o[b][j][e] += !number && (int32_t)t < sees[b] ? x : 0.0f;
+					o[j][e] += !number && (int32_t)t < sees ? x : 0.0f;
 				}
 		}
 	}
 
-#pragma unroll
-	for (int b = 0; b < B; ++b) {
-		l[b] += __shfl_xor(l[b], 32);
-		if (!there[b]) continue;
-		const float by = l[b] > 0.0f ? 1.0f / l[b] : l[b] == l[b] ? 0.0f : l[b]; /* a row that sees nothing is zero; NaN stays */
-		uint16_t* to = (uint16_t*)a.out + (size_t)(p.query_first + query[b]) * a.out_token + (size_t)query_head[b] * a.out_head;
+	/* what the end needs is read and worked out here, and takes up no registers in the loop */
+	auto last = (const __attribute__((address_space(4))) PromptAttend*)__builtin_amdgcn_kernarg_segment_ptr();
+	asm volatile("" : "+s"(last));
+	const uint32_t id = __builtin_amdgcn_mbcnt_hi(~0u, __builtin_amdgcn_mbcnt_lo(~0u, 0)), n = id % 32, half = id / 32, r = wave_first + n;
+	l += __shfl_xor(l, 32);
+	if (r >= rows) return;
+	if (last->parts > 1) { /* [unit][part]: [ROWS][channel] sums, [ROWS] of reference and sum of weights, for prompt_join_kernel */
+		float* const to = last->partial + ((size_t)unit * last->parts + part) * (ROWS * (32 * J + 2));
 #pragma unroll
 		for (int j = 0; j < J; ++j)
-			for (int e = 0; e < 4; ++e) {
-				const uint32_t low = rounded_pair(o[b][j][4 * e] * by, o[b][j][4 * e + 1] * by, T{}), high = rounded_pair(o[b][j][4 * e + 2] * by, o[b][j][4 * e + 3] * by, T{});
-				uint16_t* at = to + 32 * j + 8 * e + 4 * h;
-				if constexpr (VEC) *(u32x2*)at = u32x2{ low, high };
-				else {
-					at[0] = (uint16_t)low;
-					at[1] = (uint16_t)(low >> 16);
-					at[2] = (uint16_t)high;
-					at[3] = (uint16_t)(high >> 16);
-				}
-			}
-		if (h == 0 && a.lse)
-			a.lse[(size_t)(p.query_first + query[b]) * a.query_heads + query_head[b]] = l[b] == 0.0f ? -__builtin_inff() : (reference[b] + log2f(l[b]) - LIFT) * 0.693147180559945309f;
+			for (int e = 0; e < 4; ++e)
+				*(f32x4*)(to + (size_t)r * (32 * J) + 32 * j + 8 * e + 4 * half) = f32x4{ o[j][4 * e], o[j][4 * e + 1], o[j][4 * e + 2], o[j][4 * e + 3] };
+		if (half == 0) *(float2*)(to + ROWS * (32 * J) + 2 * r) = float2{ reference, l };
+		return;
 	}
+	const float by = l > 0.0f ? 1.0f / l : l == l ? 0.0f : l; /* a row that sees nothing is zero; NaN stays */
+	const uint32_t in = (first_row + r) / last->group, out_head = head * last->group + (first_row + r - in * last->group);
+	uint16_t* const row = (uint16_t*)last->out + (size_t)(p.query_first + in) * last->out_token + (size_t)out_head * last->out_head;
+#pragma unroll
+	for (int j = 0; j < J; ++j)
+		for (int e = 0; e < 4; ++e) {
+			const uint32_t low = rounded_pair(o[j][4 * e] * by, o[j][4 * e + 1] * by, T{}), high = rounded_pair(o[j][4 * e + 2] * by, o[j][4 * e + 3] * by, T{});
+			uint16_t* at = row + 32 * j + 8 * e + 4 * half;
+			if constexpr (VEC) *(u32x2*)at = u32x2{ low, high };
+			else {
+				at[0] = (uint16_t)low;
+				at[1] = (uint16_t)(low >> 16);
+				at[2] = (uint16_t)high;
+				at[3] = (uint16_t)(high >> 16);
+			}
+		}
+	if (half == 0 && last->lse)
+		last->lse[(size_t)(p.query_first + in) * last->query_heads + out_head] = l == 0.0f ? -__builtin_inff() : (reference + log2f(l) - LIFT) * 0.693147180559945309f;
 }
 
-template <typename T, int J, int W, int B, bool VEC>
+/* The parts of 32 W rows: a wavefront a row, 8 J lanes 4 channels each of every (64 / 8 J)-th part. */
+template <typename T, int J, int W>
+__global__ void __launch_bounds__(256)
+prompt_join_kernel(PromptAttend a)
+{
+	constexpr uint32_t D = 32 * J, ROWS = 32 * W, LANES = 8 * J, GROUPS = WAVE / LANES;
+	constexpr size_t PART = ROWS * (D + 2);
+	const uint32_t wave = (uint32_t)__builtin_amdgcn_readfirstlane((int)(threadIdx.x / WAVE)), lane = threadIdx.x % WAVE;
+	const uint32_t unit = blockIdx.x / (ROWS / 4), r = blockIdx.x % (ROWS / 4) * 4 + wave;
+	const uint32_t head = unit % a.heads, rest = unit / a.heads, s = rest % a.sequences, row_tile = a.row_tiles - 1 - rest / a.sequences;
+	const Prompt4 p = prompt_of(a, s);
+	const uint32_t all_rows = p.queries * a.group, first_row = row_tile * ROWS;
+	if (first_row + r >= all_rows) return;
+	const uint32_t rows = min(ROWS, all_rows - first_row), tiles = ((uint32_t)sees_of(a, p, (first_row + rows - 1) / a.group) + 31) / 32;
+	const uint32_t parts = tiles ? (tiles + a.tiles_per_part - 1) / a.tiles_per_part : 1, group = lane / LANES, at = lane % LANES;
+	const float* const left = a.partial + (size_t)unit * a.parts * PART;
+	float top = -__builtin_inff();
+	for (uint32_t n = lane; n < parts; n += WAVE) top = fmaxf(top, left[n * PART + ROWS * D + 2 * r]);
+	for (int d = 1; d < WAVE; d *= 2) top = fmaxf(top, __shfl_xor(top, d));
+	const float lowest = top == -__builtin_inff() ? 0.0f : top;
+	float sum = 0.0f;
+	f32x4 mine{ 0.0f, 0.0f, 0.0f, 0.0f };
+	if (group < GROUPS)
+#pragma unroll 4
+		for (uint32_t n = group; n < parts; n += GROUPS) {
+			const float* from = left + n * PART;
+			const float2 ml = *(const float2*)(from + ROWS * D + 2 * r);
+			const float weight = __builtin_amdgcn_exp2f(ml.x - lowest);
+			sum += ml.y * weight;
+			mine += *(const f32x4*)(from + (size_t)r * D + 4 * at) * weight;
+		}
+	for (uint32_t g = 1; g < GROUPS; ++g) { /* the groups' sums, in their order */
+		const int other = (int)(at + g * LANES);
+		const f32x4 more{ __shfl(mine[0], other), __shfl(mine[1], other), __shfl(mine[2], other), __shfl(mine[3], other) };
+		const float more_sum = __shfl(sum, other);
+		if (group == 0) { mine += more; sum += more_sum; }
+	}
+	if (group != 0) return;
+	const float by = sum > 0.0f ? 1.0f / sum : sum == sum ? 0.0f : sum;
+	const uint32_t query = (first_row + r) / a.group, query_head = head * a.group + (first_row + r - query * a.group);
+	uint16_t* to = (uint16_t*)a.out + (size_t)(p.query_first + query) * a.out_token + (size_t)query_head * a.out_head + 4 * at;
+	const uint32_t low = rounded_pair(mine[0] * by, mine[1] * by, T{}), high = rounded_pair(mine[2] * by, mine[3] * by, T{});
+	to[0] = (uint16_t)low;
+	to[1] = (uint16_t)(low >> 16);
+	to[2] = (uint16_t)high;
+	to[3] = (uint16_t)(high >> 16);
+	if (at == 0 && a.lse) a.lse[(size_t)(p.query_first + query) * a.query_heads + query_head] = sum == 0.0f ? -__builtin_inff() : (top + log2f(sum) - LIFT) * 0.693147180559945309f;
+}
+
+template <typename T, int J, int W, bool VEC>
 static int launch_prompt_kernel(const PromptAttend& a, uint32_t units)
 {
 	constexpr uint32_t bytes = prompt_lds<J>();
@@ -495,43 +519,42 @@ static int launch_prompt_kernel(const PromptAttend& a, uint32_t units)
 		const int rc = device_info(&dev);
 		if (rc) return rc;
 		if (allowed != dev->device) {
-			KMX_HIP(hipFuncSetAttribute((const void*)prompt_attend_kernel<T, J, W, B, VEC>, hipFuncAttributeMaxDynamicSharedMemorySize, (int)bytes));
+			KMX_HIP(hipFuncSetAttribute((const void*)prompt_attend_kernel<T, J, W, VEC>, hipFuncAttributeMaxDynamicSharedMemorySize, (int)bytes));
 			allowed = dev->device;
 		}
 	}
-	KMX_LAUNCH_KERNEL((prompt_attend_kernel<T, J, W, B, VEC>), dim3(units), dim3(64 * W), bytes, stream(), a);
+	KMX_LAUNCH_KERNEL((prompt_attend_kernel<T, J, W, VEC>), dim3(units), dim3(64 * W), bytes, stream(), a);
 	KMX_LAUNCH_CHECK("prompt_attend_kernel");
 	return KMX_OK;
 }
 
 template <typename T, int J, int W>
-static int launch_prompt_rows(PromptAttend a)
+static int launch_prompt_rows(PromptAttend a, const PromptPlan& plan)
 {
-	constexpr int B = 1;
-	const uint64_t rows = (uint64_t)a.max_queries * a.group, row_tiles = (rows + 32 * W * B - 1) / (32 * W * B);
-	if (rows > 0x7FFFFF00u || (uint64_t)a.heads * a.sequences > 0x7FFFFFFFu || row_tiles * a.heads * a.sequences > 0x7FFFFFFFu)
-		return fail(KMX_ERR_UNSUPPORTED, "kmx_prompt_attend: too many queries for one call");
-	a.row_tiles = (uint32_t)row_tiles;
-	const uint32_t units = (uint32_t)(row_tiles * a.heads * a.sequences);
-	return a.vec ? launch_prompt_kernel<T, J, W, B, true>(a, units) : launch_prompt_kernel<T, J, W, B, false>(a, units);
+	a.row_tiles = plan.row_tiles;
+	a.units = plan.units;
+	a.parts = plan.parts;
+	a.tiles_per_part = plan.tiles_per_part;
+	const int rc = a.vec ? launch_prompt_kernel<T, J, W, true>(a, plan.units * plan.parts) : launch_prompt_kernel<T, J, W, false>(a, plan.units * plan.parts);
+	if (rc || plan.parts == 1) return rc;
+	KMX_LAUNCH_KERNEL((prompt_join_kernel<T, J, W>), dim3(plan.units * (32 * W / 4)), dim3(256), 0, stream(), a);
+	KMX_LAUNCH_CHECK("prompt_join_kernel");
+	return KMX_OK;
 }
 
 template <typename T, int J>
-static int launch_prompt_of(const PromptAttend& a)
+static int launch_prompt_of(const PromptAttend& a, const PromptPlan& plan)
 {
-	if constexpr (J >= 3 && J <= 6) {
-		const DeviceInfo* dev = nullptr;
-		const int rc = device_info(&dev);
-		if (rc) return rc;
-		if ((uint64_t)a.max_queries * a.group * a.heads * a.sequences > 512 * (uint64_t)dev->compute_units) return launch_prompt_rows<T, J, 8>(a);
-	}
-	return launch_prompt_rows<T, J, 4>(a);
+	if constexpr (J == 5 || J == 6) return launch_prompt_rows<T, J, 8>(a, plan);
+	if constexpr (J == 3 || J == 4)
+		if (plan.wide) return launch_prompt_rows<T, J, 8>(a, plan);
+	return launch_prompt_rows<T, J, 4>(a, plan);
 }
 
 template <int J>
-int launch_prompt_attend(const PromptAttend& a, bool bf16)
+int launch_prompt_attend(const PromptAttend& a, bool bf16, const PromptPlan& plan)
 {
-	return bf16 ? launch_prompt_of<__bf16, J>(a) : launch_prompt_of<_Float16, J>(a);
+	return bf16 ? launch_prompt_of<__bf16, J>(a, plan) : launch_prompt_of<_Float16, J>(a, plan);
 }
 
 } // namespace kmx

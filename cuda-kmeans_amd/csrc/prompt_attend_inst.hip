@@ -7,6 +7,6 @@
 
 namespace kmx {
 
-template int launch_prompt_attend<KMX_J>(const PromptAttend& a, bool bf16);
+template int launch_prompt_attend<KMX_J>(const PromptAttend& a, bool bf16, const PromptPlan& plan);
 
 } // namespace kmx

@@ -575,6 +575,10 @@ int kmx_prompt_attend(const kmx_prompt* prompt, int type, const void* q, size_t 
                       const void* keys, const void* values, size_t token_stride, size_t head_stride,
                       void* out, size_t out_token_stride, size_t out_head_stride, float* lse, float scale, int causal);
 
+/* Sizes the work space for every kmx_prompt_attend on heads of `dim` channels (few rows take their tokens in parts), so that they allocate nothing afterwards, under the rules of
+ * kmx_cache4_reserve's. */
+int kmx_prompt_reserve(uint32_t dim);
+
 /* Message of the last failed call on this thread ("" if none). */
 const char* kmx_last_error(void);
 

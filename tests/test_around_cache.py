@@ -129,6 +129,7 @@ def test_prompts_that_are_refused(km):
     call(invalid, b"token stride", ots=63)
     for nothing in (dict(sequences=0), dict(queries=0), dict(max_queries=0)):
         call(km.KMX_OK, b"", q=None, k=None, v=None, out=None, query_starts=None, token_starts=None, **nothing)
+    assert lib.kmx_prompt_reserve(48) == lib.kmx_prompt_reserve(0) == lib.kmx_prompt_reserve(288) == unsupported and b"multiple of 32" in lib.kmx_last_error()
 
 
 def test_shared_prefixes_that_are_refused(km):

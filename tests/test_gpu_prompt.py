@@ -3,6 +3,7 @@ import numpy as np
 import pytest
 
 from test_gpu_cache4 import BF16, F16, UNIT, device, from_bits, to_bits
+from test_zz_no_alloc import device_memory_in_use
 
 pytestmark = pytest.mark.gpu
 
@@ -242,6 +243,81 @@ def test_starts_that_say_nothing(km, gpu):
         assert np.array_equal(got[:30], want[0][:30]) and not got[30:].any() and np.isneginf(lse[30:]).all()
     got, lse = s.attend(starts=(np.int32([-3, 30, 70]), np.int32([0, 30, 70])))
     assert (s.bits[:30] == 0x5A5A).all() and np.array_equal(got[30:], want[0][30:])
+
+
+@pytest.mark.parametrize("kind", [F16, BF16])
+@pytest.mark.parametrize("causal", [True, False])
+@pytest.mark.parametrize("heads,group,dim,counts,lengths", [
+    (2, 4, 128, [1, 3, 1, 0, 2], [3000, 33, 0, 500, 2999]), (1, 1, 32, [200], [2100]), (1, 3, 192, [2, 100], [1500, 40]), (1, 1, 160, [300], [1025]), (1, 2, 256, [5], [2000]),
+    (2, 1, 96, [31, 1], [1999, 2000]), (1, 8, 64, [40], [4097]), (1, 1, 224, [90, 90], [64, 1600])])
+def test_tokens_in_parts(km, gpu, kind, causal, heads, group, dim, counts, lengths):
+    """Few rows over many tokens: work-groups share out the tokens, also of sequences much shorter than the longest, whose last parts are empty."""
+    rng = np.random.default_rng(dim + len(counts))
+    s = Prompts(km, rng, heads, group, dim, counts, lengths, kind, extra=(1, 0))
+    first = s.check(causal)
+    again = s.attend(causal, gaps=(1, 0), key_gaps=(0, 1), out_gaps=(1, 1), offset=1)
+    assert np.array_equal(first[0], again[0][:len(first[0])]) and np.array_equal(first[1], again[1][:len(first[1])])
+
+
+@pytest.mark.parametrize("kind", [F16, BF16])
+@pytest.mark.parametrize("where", [(0, 0), (1023, 63), (1900, 7), (1999, 40)])
+def test_parts_with_values_that_are_no_numbers(km, gpu, kind, where):
+    rng = np.random.default_rng(13)
+    s = Prompts(km, rng, 2, 2, 64, [120], [2000], kind)
+    for what in (np.inf, np.nan):
+        s.v[where[0], 1, where[1]] = what
+        got, _ = s.check()
+        assert np.isfinite(got[:, 0]).all() and (~np.isfinite(got[:, 1])).any()
+    s.k[500, 0] = np.nan
+    got, lse = s.check()
+    assert np.isnan(got[:, 0]).all() and np.isnan(lse[:, 0]).all()
+
+
+def test_parts_below_one_that_stands_out(km, gpu):
+    """Parts whose references are far apart, also further than 32 bits reach."""
+    rng = np.random.default_rng(14)
+    for far in (10.0, 300.0):
+        s = Prompts(km, rng, 1, 1, 32, [3], [3000], BF16)
+        s.q[:] = 1
+        s.k[:] = from_bits(to_bits(0.01 * rng.normal(size=s.k.shape), BF16), BF16)
+        s.k[700] = far / 32
+        s.check(causal=False, scale=1.0)
+
+
+def test_reserved_recorded_and_replayed(km, gpu):
+    """Nothing is allocated after kmx_prompt_reserve; recordings outlive the work space."""
+    rng = np.random.default_rng(15)
+    shapes = [Prompts(km, rng, 2, 4, 128, [1, 2], [3000, 100], BF16), Prompts(km, rng, 1, 4, 128, [60], [2500], F16)]
+    want = [(s.attend(), s.results[0].read(np.uint16, s.results[0].nbytes // 2)) for s in shapes]
+    shapes[0].results[0].zero()  # (all code is on the device)
+    km.check(km.hip_lib().kmx_shutdown())
+    km.Prompt.reserve(128)
+    km.sync()
+    before = device_memory_in_use()
+
+    def same(s, bits):
+        km.sync()
+        return np.array_equal(s.results[0].read(np.uint16, s.results[0].nbytes // 2), bits)
+
+    for s, (_, bits) in zip(shapes, want):
+        s.results[0].write(np.zeros(s.results[0].nbytes, np.uint8))
+        s.call()
+        assert same(s, bits)
+    assert device_memory_in_use() == before
+    graphs = []
+    for s in shapes:
+        with km.Graph() as g:
+            s.call()
+        graphs.append(g)
+    km.check(km.hip_lib().kmx_shutdown())
+    for _ in range(3):
+        for s, g, (_, bits) in zip(shapes, graphs, want):
+            s.results[0].write(np.zeros(s.results[0].nbytes, np.uint8))
+            g.launch()
+            assert same(s, bits)
+            s.call()
+    for g in graphs:
+        g.destroy()
 
 
 def test_recorded_and_on_a_stream_of_the_callers(km, gpu):
