@@ -162,12 +162,15 @@ struct Evict4 {
 	int32_t* kept; /* [sequence][head][keep] */
 	int32_t* left; /* [sequence] */
 	uint32_t sequences, table_stride, max_length, keep, first, recent;
-	uint32_t cached; /* tokens whose keys LDS holds */
+	uint32_t words, cached; /* LDS: words of 64 places, weights */
 };
 
 constexpr uint32_t EVICT_THREADS = 1024, EVICT_WAVES = EVICT_THREADS / WAVE, EVICT_BINS = 2048;
-constexpr uint32_t EVICT_CACHED = 24576;   /* keys of a sequence that LDS holds: 96 KB */
-constexpr uint32_t EVICT_TOKENS = 1 << 18; /* of a sequence: a bit for each place, and a count for each 64 */
+constexpr uint32_t EVICT_CACHED = 24576;   /* weights of a sequence that LDS holds: 96 KB, and 24 KB for which of them move */
+constexpr uint32_t EVICT_TOKENS = 1 << 18; /* of a sequence */
+constexpr uint32_t EVICT_WORD = 24;        /* bytes for 64 places: those that stay, those at the threshold, free and moving ones before */
+constexpr uint32_t evict_bytes(uint32_t words, uint32_t cached) { return EVICT_WORD * words + 4 * cached + 2 * ((cached / 2 + 1) / 2 * 2); }
+constexpr uint32_t MOST_EVICT_BYTES = EVICT_TOKENS / 64 * EVICT_WORD > evict_bytes(EVICT_CACHED / 64, EVICT_CACHED) ? EVICT_TOKENS / 64 * EVICT_WORD : evict_bytes(EVICT_CACHED / 64, EVICT_CACHED);
 
 __device__ __forceinline__ uint32_t evict_length(const Evict4& e, uint32_t s)
 {
@@ -196,17 +199,31 @@ __device__ __forceinline__ uint32_t sum_below(const uint32_t* counts, uint32_t w
 }
 __device__ __forceinline__ uint64_t lanes_below(uint32_t lane) { return ((uint64_t)1 << lane) - 1; }
 
+/* sums of what the threads before have; EVICT_WAVES counts */
+__device__ __forceinline__ uint32_t sum_before(uint32_t mine, uint32_t* counts, uint32_t wave, uint32_t lane)
+{
+	uint32_t upto = mine;
+	for (uint32_t d = 1; d < WAVE; d *= 2) {
+		const uint32_t v = (uint32_t)__shfl_up((int)upto, d);
+		if (lane >= d) upto += v;
+	}
+	if (lane == WAVE - 1) counts[wave] = upto;
+	__syncthreads();
+	return sum_below(counts, wave) + upto - mine;
+}
+
 /*
  * One work-group a sequence and head. The threshold of the weights by counting them in 2048 equal shares of the range of their keys, then of the share that it lies in:
- * three rounds at most. Then all places in order, each wavefront a run of them: which stay (of those at the threshold the first ones), which of the places below the
- * edge become free, which tokens from the edge on have to move. The moving ones are listed at the begin of `kept` and go from there to the free places, the
- * highest first: none of them lies below where it is listed.
+ * three rounds at most. Then, for 64 places a word: which stay (of those at the threshold the first ones), how many places below the edge become free before them and how many
+ * tokens from the edge on have to move. The n-th moving one goes to the n-th free place. Up to 24576 weights stay in LDS, with the list of those that move; else the list is the begin of
+ * `kept`, from where it goes to the free places, the highest first: none of them lies below where it is listed.
+ * Bound by latency (one work-group a compute unit, few of them): weights come eight at a time, all that is written depends on LDS alone. MEASURED
  */
 __global__ void __launch_bounds__(EVICT_THREADS)
 evict4_choose_kernel(Evict4 e)
 {
-	extern __shared__ __attribute__((aligned(16))) uint32_t lds[]; /* bits of the places that stay, free places before each 64, keys */
-	__shared__ uint32_t bins[EVICT_BINS], counts[3][EVICT_WAVES], found[3];
+	extern __shared__ __attribute__((aligned(16))) uint32_t lds[]; /* words of 64 places, weights, a list of tokens */
+	__shared__ uint32_t bins[EVICT_BINS], counts[4][EVICT_WAVES], found[3];
 	const uint32_t tid = threadIdx.x, wave = (uint32_t)__builtin_amdgcn_readfirstlane((int)(tid / WAVE)), lane = tid % WAVE;
 	const uint32_t head = blockIdx.x, s = blockIdx.y, n = evict_length(e, s);
 	int32_t* const kept = e.kept + ((size_t)s * e.cache.heads + head) * e.keep;
@@ -217,26 +234,44 @@ evict4_choose_kernel(Evict4 e)
 	}
 	const int32_t* table = e.table + (size_t)s * e.table_stride;
 	const uint32_t edge = e.keep - e.recent, places = edge - e.first, rest = n - e.first - e.recent; /* `places` of the `rest` tokens stay: fewer */
-	const uint32_t words = (places + 63) / 64;
-	uint64_t* const bits = (uint64_t*)lds;
-	uint32_t* const before = lds + 2 * words;
-	uint32_t* const cache = before + words + words % 2;
+	const uint32_t words = (rest + 63) / 64;
+	uint64_t *const bits = (uint64_t*)lds, *const level = bits + e.words;
+	uint32_t *const freed = (uint32_t*)(level + e.words), *const moved = freed + e.words;
+	float* const cache = (float*)(moved + e.words);
+	uint16_t* const list = (uint16_t*)(cache + e.cached);
 	const bool cached = rest <= e.cached;
-	auto key_at = [&](uint32_t x) {
+	auto weight_at = [&](uint32_t t) {
 		size_t at;
-		return weight_of(e, table, head, e.first + x, &at) ? key_of(e.weights[at]) : 0u;
+		return weight_of(e, table, head, t, &at) ? e.weights[at] : __builtin_nanf("");
 	};
-	auto key = [&](uint32_t x) { return cached ? cache[x] : key_at(x); };
+	auto key = [&](uint32_t x) { return key_of(cached ? cache[x] : weight_at(e.first + x)); };
 
-	/* the range of the keys */
+	/* the weights, and the range of their keys */
+	const float recent = tid < e.recent ? weight_at(n - e.recent + tid) : 0.0f; /* (the first of them) */
 	if (tid < 2) found[tid] = tid ? 0u : ~0u;
+	for (uint32_t i = tid; i < EVICT_BINS; i += EVICT_THREADS) bins[i] = 0;
 	__syncthreads();
 	uint32_t low = ~0u, high = 0;
-	for (uint32_t x = tid; x < rest; x += EVICT_THREADS) {
-		const uint32_t k = key_at(x);
-		if (cached) cache[x] = k;
-		low = min(low, k);
-		high = max(high, k);
+	constexpr int AT_ONCE = 8;
+	for (uint32_t x = tid; x < rest; x += AT_ONCE * EVICT_THREADS) {
+		uint32_t page[AT_ONCE];
+		float w[AT_ONCE];
+#pragma unroll
+		for (int i = 0; i < AT_ONCE; ++i) page[i] = (uint32_t)table[(e.first + min(x + i * EVICT_THREADS, rest - 1)) >> e.cache.page_shift];
+#pragma unroll
+		for (int i = 0; i < AT_ONCE; ++i) {
+			const uint32_t t = e.first + min(x + i * EVICT_THREADS, rest - 1);
+			const size_t at = (((size_t)(page[i] < e.cache.page_count ? page[i] : 0) * e.cache.heads + head) << e.cache.page_shift) + (t & ((1u << e.cache.page_shift) - 1));
+			w[i] = e.weights[at];
+		}
+#pragma unroll
+		for (int i = 0; i < AT_ONCE; ++i) {
+			const float mine = page[i] < e.cache.page_count ? w[i] : __builtin_nanf("");
+			const uint32_t k = key_of(mine), at = x + i * EVICT_THREADS;
+			if (cached && at < rest) cache[at] = mine;
+			low = min(low, k); /* (the last one counts again) */
+			high = max(high, k);
+		}
 	}
 	for (int d = 1; d < WAVE; d *= 2) {
 		low = min(low, (uint32_t)__shfl_xor((int)low, d));
@@ -250,11 +285,9 @@ evict4_choose_kernel(Evict4 e)
 	low = found[0];
 	high = found[1];
 	uint32_t need = places; /* of the tokens between low and high */
-	while (need && low != high) {
+	while (need && low != high) { /* (the shares are zero here) */
 		uint32_t shift = 0;
 		while ((high - low) >> shift >= EVICT_BINS) ++shift;
-		for (uint32_t i = tid; i < EVICT_BINS; i += EVICT_THREADS) bins[i] = 0;
-		__syncthreads();
 		for (uint32_t x = tid; x < rest; x += EVICT_THREADS) {
 			const uint32_t k = key(x);
 			if (k >= low && k <= high) atomicAdd(&bins[(k - low) >> shift], 1u);
@@ -262,14 +295,8 @@ evict4_choose_kernel(Evict4 e)
 		__syncthreads();
 		/* the share that holds the need-th largest: thread t has shares 2047 - 2 t and the one below */
 		const uint32_t upper = bins[EVICT_BINS - 1 - 2 * tid], lower = bins[EVICT_BINS - 2 - 2 * tid];
-		uint32_t upto = upper + lower;
-		for (uint32_t d = 1; d < WAVE; d *= 2) {
-			const uint32_t v = (uint32_t)__shfl_up((int)upto, d);
-			if (lane >= d) upto += v;
-		}
-		if (lane == WAVE - 1) counts[0][wave] = upto;
-		__syncthreads();
-		const uint32_t above = sum_below(counts[0], wave) + upto - upper - lower;
+		bins[EVICT_BINS - 1 - 2 * tid] = bins[EVICT_BINS - 2 - 2 * tid] = 0;
+		const uint32_t above = sum_before(upper + lower, counts[0], wave, lane);
 		if (above < need && above + upper + lower >= need) {
 			const bool first = above + upper >= need;
 			found[0] = EVICT_BINS - (first ? 1 : 2) - 2 * tid;
@@ -282,77 +309,96 @@ evict4_choose_kernel(Evict4 e)
 	}
 	const uint32_t threshold = need ? low : ~0u; /* above it all stay, at it the first `need` (without places: none) */
 
-	/* runs of places, whole 64s, a wavefront each */
-	const uint32_t run = ((rest + EVICT_WAVES - 1) / EVICT_WAVES + 63) / 64 * 64, begin = min(rest, wave * run), end = min(rest, begin + run);
-	uint32_t equal = 0;
-	for (uint32_t x0 = begin; x0 < end; x0 += WAVE) equal += (uint32_t)__popcll(__ballot(x0 + lane < end && key(x0 + lane) == threshold));
-	if (lane == 0) counts[0][wave] = equal;
+	for (uint32_t x0 = WAVE * wave; x0 < rest; x0 += EVICT_THREADS) {
+		const uint32_t k = x0 + lane < rest ? key(x0 + lane) : 0;
+		const uint64_t at = __ballot(x0 + lane < rest && k == threshold), above = __ballot(k > threshold);
+		if (lane == 0) {
+			bits[x0 / 64] = above;
+			level[x0 / 64] = at;
+		}
+	}
 	__syncthreads();
-	const uint32_t equal_before = sum_below(counts[0], wave);
-	auto stays = [&](uint32_t x, uint32_t& seen) { /* bits of 64 places; seen: those at the threshold so far */
-		const uint32_t k = x < end ? key(x) : 0;
-		const uint64_t at = __ballot(x < end && k == threshold);
-		const uint64_t bit = __ballot(x < end && (k > threshold || (k == threshold && seen + (uint32_t)__popcll(at & lanes_below(lane)) < need)));
-		seen += (uint32_t)__popcll(at);
-		return bit;
+	/* threads have words side by side, four at most */
+	const uint32_t each = (words + EVICT_THREADS - 1) / EVICT_THREADS, word = tid * each, word_end = min(words, word + each);
+	auto below_edge = [&](uint32_t w) { return 64 * w >= places ? (uint64_t)0 : places - 64 * w >= 64 ? ~(uint64_t)0 : lanes_below(places - 64 * w); };
+	uint32_t mine = 0;
+	for (uint32_t w = word; w < word_end; ++w) mine += (uint32_t)__popcll(level[w]);
+	uint32_t before = sum_before(mine, counts[1], wave, lane), free_here = 0, move_here = 0;
+	for (uint32_t w = word; w < word_end; ++w) {
+		uint64_t at = level[w];
+		const uint32_t count = (uint32_t)__popcll(at);
+		for (uint32_t more = before >= need ? count : before + count > need ? before + count - need : 0; more; --more) at &= ~((uint64_t)1 << (63 - __clzll((long long)at))); /* the last ones go */
+		before += count;
+		const uint64_t bit = bits[w] | at, below = below_edge(w);
+		bits[w] = bit;
+		free_here += (uint32_t)__popcll(~bit & below);
+		move_here += (uint32_t)__popcll(bit & ~below);
+	}
+	uint32_t free_before = sum_before(free_here, counts[2], wave, lane), move_before = sum_before(move_here, counts[3], wave, lane);
+	for (uint32_t w = word; w < word_end; ++w) {
+		const uint64_t bit = bits[w], below = below_edge(w);
+		freed[w] = free_before;
+		moved[w] = move_before;
+		free_before += (uint32_t)__popcll(~bit & below);
+		move_before += (uint32_t)__popcll(bit & ~below);
+	}
+	__syncthreads();
+	for (uint32_t x = places / EVICT_THREADS * EVICT_THREADS + tid; x < rest; x += EVICT_THREADS) {
+		const uint64_t beyond = bits[x / 64] & ~below_edge(x / 64);
+		if (!(beyond >> lane & 1)) continue;
+		const uint32_t to = moved[x / 64] + (uint32_t)__popcll(beyond & lanes_below(lane));
+		if (cached) list[to] = (uint16_t)x;
+		else kept[e.first + to] = (int32_t)(e.first + x);
+	}
+	__syncthreads();
+	auto put = [&](uint32_t t, float w) {
+		size_t at;
+		if (weight_of(e, table, head, t, &at)) e.weights[at] = w;
 	};
-	uint32_t seen = equal_before, freed = 0, moved = 0;
-	for (uint32_t x0 = begin; x0 < end; x0 += WAVE) {
-		const uint64_t bit = stays(x0 + lane, seen), below = x0 >= places ? 0 : places - x0 >= 64 ? ~(uint64_t)0 : lanes_below(places - x0);
-		if (x0 < places && lane == 0) {
-			bits[x0 / 64] = bit;
-			before[x0 / 64] = freed;
+	if (cached) {
+#pragma unroll 4
+		for (uint32_t x = tid; x < places; x += EVICT_THREADS) {
+			const uint64_t bit = bits[x / 64];
+			uint32_t from = x;
+			if (!(bit >> lane & 1)) {
+				from = list[freed[x / 64] + (uint32_t)__popcll(~bit & lanes_below(lane))];
+				size_t at;
+				put(e.first + x, weight_of(e, table, head, e.first + from, &at) ? cache[from] : 0.0f);
+			}
+			kept[e.first + x] = (int32_t)(e.first + from);
 		}
-		freed += (uint32_t)__popcll(~bit & below);
-		moved += (uint32_t)__popcll(bit & ~below);
-	}
-	if (lane == 0) {
-		counts[1][wave] = freed;
-		counts[2][wave] = moved;
-	}
-	__syncthreads();
-	const uint32_t freed_before = sum_below(counts[1], wave);
-	moved = sum_below(counts[2], wave);
-	seen = equal_before;
-	for (uint32_t x0 = begin; x0 < end; x0 += WAVE) {
-		if (x0 < places && lane == 0) before[x0 / 64] += freed_before;
-		const uint64_t bit = stays(x0 + lane, seen), beyond = bit & (x0 >= places ? ~(uint64_t)0 : places - x0 >= 64 ? 0 : ~lanes_below(places - x0));
-		if (beyond >> lane & 1) kept[e.first + moved + (uint32_t)__popcll(beyond & lanes_below(lane))] = (int32_t)(e.first + x0 + lane);
-		moved += (uint32_t)__popcll(beyond);
-	}
-	__syncthreads();
-	for (uint32_t top = (places + EVICT_THREADS - 1) / EVICT_THREADS; top-- > 0;) {
-		const uint32_t x = top * EVICT_THREADS + tid;
-		int32_t from = (int32_t)(e.first + x);
-		bool free = false;
-		if (x < places) {
-			free = !(bits[x / 64] >> lane & 1);
-			if (free) from = kept[e.first + before[x / 64] + (uint32_t)__popcll(~bits[x / 64] & lanes_below(lane))];
+	} else {
+		for (uint32_t top = (places + EVICT_THREADS - 1) / EVICT_THREADS; top-- > 0;) {
+			const uint32_t x = top * EVICT_THREADS + tid;
+			int32_t from = (int32_t)(e.first + x);
+			bool free = false;
+			if (x < places) {
+				free = !(bits[x / 64] >> lane & 1);
+				if (free) from = kept[e.first + freed[x / 64] + (uint32_t)__popcll(~bits[x / 64] & lanes_below(lane))];
+			}
+			__syncthreads();
+			if (x < places) {
+				kept[e.first + x] = from;
+				size_t at;
+				if (free) put(e.first + x, weight_of(e, table, head, (uint32_t)from, &at) ? e.weights[at] : 0.0f);
+			}
 		}
-		__syncthreads();
-		if (x < places) {
-			kept[e.first + x] = from;
-			size_t a, b;
-			if (free && weight_of(e, table, head, e.first + x, &b)) e.weights[b] = weight_of(e, table, head, (uint32_t)from, &a) ? e.weights[a] : 0.0f;
-		}
+		__syncthreads(); /* (what moved from where the recent ones go) */
 	}
 	for (uint32_t i = tid; i < e.first; i += EVICT_THREADS) kept[i] = (int32_t)i;
 	for (uint32_t i = tid; i < e.recent; i += EVICT_THREADS) kept[edge + i] = (int32_t)(n - e.recent + i);
-	__syncthreads();
 	/* the recent ones move down in their order, later ones from places that earlier ones do not go to */
 	for (uint32_t i0 = 0; i0 < e.recent; i0 += EVICT_THREADS) {
 		const uint32_t i = i0 + tid;
-		float w = 0.0f;
+		float w = recent;
 		size_t at;
-		if (i < e.recent && weight_of(e, table, head, n - e.recent + i, &at)) w = e.weights[at];
+		if (i0 && i < e.recent) w = weight_at(n - e.recent + i);
 		__syncthreads();
-		if (i < e.recent && weight_of(e, table, head, edge + i, &at)) e.weights[at] = w;
+		if (i < e.recent) put(edge + i, weight_of(e, table, head, n - e.recent + i, &at) ? w : 0.0f);
 	}
 	__syncthreads();
-	for (uint32_t t = e.keep + tid; t < n; t += EVICT_THREADS) {
-		size_t at;
-		if (weight_of(e, table, head, t, &at)) e.weights[at] = 0.0f;
-	}
+#pragma unroll 4
+	for (uint32_t t = e.keep + tid; t < n; t += EVICT_THREADS) put(t, 0.0f);
 }
 
 /* ---------------------------------------------------------------- moves -------------------------- */
@@ -397,62 +443,57 @@ evict4_move_kernel(Evict4 e)
 	const int32_t* table = e.table + (size_t)s * e.table_stride;
 	const int32_t* kept = e.kept + ((size_t)s * e.cache.heads + head) * e.keep;
 	const uint32_t edge = e.keep - e.recent, page_mask = (1u << e.cache.page_shift) - 1;
-	auto block_of = [&](uint32_t t, bool* there) { /* t: the same in all lanes */
-		const uint32_t page = (uint32_t)__builtin_amdgcn_readfirstlane(table[t >> e.cache.page_shift]);
-		*there = page < e.cache.page_count;
-		return e.cache.blocks + block_offset<J>(e.cache, *there ? page : 0, head, (t & page_mask) / 16);
-	};
+	auto page_of = [&](uint32_t t) { return (uint32_t)table[t >> e.cache.page_shift]; };
+	auto block_of = [&](uint32_t page, uint32_t t) { return e.cache.blocks + block_offset<J>(e.cache, page, head, (t & page_mask) / 16); };
+	constexpr int AT_ONCE = 8;
 	const bool begins = blockIdx.z == 0;
 	const uint32_t waves = begins ? 4 : 4 * (gridDim.z - 1), number = begins ? wave : 4 * (blockIdx.z - 1) + wave;
-	for (uint32_t i0 = e.first + 64 * number; i0 < edge; i0 += 64 * waves) {
-		const uint32_t from = i0 + lane < edge ? (uint32_t)kept[i0 + lane] : 0;
-		uint64_t moves = __ballot(i0 + lane < edge && (begins ? from >= edge && from < e.keep : from >= e.keep));
+	constexpr uint32_t RUN = 64;
+	for (uint32_t i0 = e.first + RUN * number; i0 < edge; i0 += RUN * waves) {
+		const uint32_t i = i0 + lane, from = lane < RUN && i < edge ? (uint32_t)kept[i] : i;
+		const bool mine = begins ? from >= edge && from < e.keep : from >= e.keep;
+		const bool moving = lane < RUN && i < edge && mine;
+		const uint32_t source = moving ? page_of(from) : ~0u, target = moving ? page_of(i) : ~0u;
+		uint64_t moves = __ballot(source < e.cache.page_count && target < e.cache.page_count);
 		while (moves) {
-			constexpr int AT_ONCE = 4;
 			Row16<J> row[AT_ONCE];
-			uint32_t to[AT_ONCE];
-			bool good[AT_ONCE];
+			int bit[AT_ONCE];
 #pragma unroll
 			for (int k = 0; k < AT_ONCE; ++k) {
-				good[k] = moves != 0;
-				if (!good[k]) continue;
-				const int bit = __ffsll((unsigned long long)moves) - 1;
+				bit[k] = moves ? __ffsll((unsigned long long)moves) - 1 : -1;
+				if (bit[k] < 0) continue;
 				moves &= moves - 1;
-				to[k] = i0 + (uint32_t)bit;
-				const uint32_t t = (uint32_t)__builtin_amdgcn_readlane((int)from, bit);
-				const uint8_t* block = block_of(t, &good[k]);
-				if (good[k]) row[k] = take_row<J>(block, t % 16, lane);
+				const uint32_t t = (uint32_t)__builtin_amdgcn_readlane((int)from, bit[k]);
+				row[k] = take_row<J>(block_of((uint32_t)__builtin_amdgcn_readlane((int)source, bit[k]), t), t % 16, lane);
 			}
 #pragma unroll
 			for (int k = 0; k < AT_ONCE; ++k) {
-				if (!good[k]) continue;
-				bool there;
-				uint8_t* block = block_of(to[k], &there);
-				if (there) put_row<J>(block, to[k] % 16, lane, row[k]);
+				if (bit[k] < 0) continue;
+				const uint32_t t = i0 + (uint32_t)bit[k];
+				put_row<J>(block_of((uint32_t)__builtin_amdgcn_readlane((int)target, bit[k]), t), t % 16, lane, row[k]);
 			}
 		}
 	}
 	if (!begins) return;
-	for (uint32_t i0 = 0; i0 < e.recent; i0 += 32) {
+	for (uint32_t i0 = 0; i0 < e.recent; i0 += 4 * AT_ONCE) {
+		const uint32_t first = i0 + AT_ONCE * wave, i = first + lane % AT_ONCE;
+		const uint32_t source = i < e.recent ? page_of(n - e.recent + i) : ~0u, target = i < e.recent ? page_of(edge + i) : ~0u;
+		const bool good = source < e.cache.page_count && target < e.cache.page_count;
+		const uint32_t moves = (uint32_t)__ballot(good) & ((1u << AT_ONCE) - 1);
 		__syncthreads(); /* what lay there has been read */
-		Row16<J> row[8];
-		bool good[8];
+		Row16<J> row[AT_ONCE];
 #pragma unroll
-		for (int k = 0; k < 8; ++k) {
-			const uint32_t i = i0 + 8 * wave + k, t = n - e.recent + i;
-			good[k] = i < e.recent;
-			if (!good[k]) continue;
-			const uint8_t* block = block_of(t, &good[k]);
-			if (good[k]) row[k] = take_row<J>(block, t % 16, lane);
+		for (int k = 0; k < AT_ONCE; ++k) {
+			if (!(moves >> k & 1)) continue;
+			const uint32_t t = n - e.recent + first + k;
+			row[k] = take_row<J>(block_of((uint32_t)__builtin_amdgcn_readlane((int)source, k), t), t % 16, lane);
 		}
 		__syncthreads();
 #pragma unroll
-		for (int k = 0; k < 8; ++k) {
-			if (!good[k]) continue;
-			const uint32_t t = edge + i0 + 8 * wave + k;
-			bool there;
-			uint8_t* block = block_of(t, &there);
-			if (there) put_row<J>(block, t % 16, lane, row[k]);
+		for (int k = 0; k < AT_ONCE; ++k) {
+			if (!(moves >> k & 1)) continue;
+			const uint32_t t = edge + first + k;
+			put_row<J>(block_of((uint32_t)__builtin_amdgcn_readlane((int)target, k), t), t % 16, lane, row[k]);
 		}
 	}
 }
@@ -527,15 +568,18 @@ int kmx_cache4_evict(const kmx_cache4* cache, const kmx_cache4_batch* batch, flo
 	e.keep = keep;
 	e.first = first;
 	e.recent = recent;
-	const uint32_t places = keep < longest ? keep - recent - first : 0, words = (places + 63) / 64;
-	e.cached = longest < EVICT_CACHED ? longest : EVICT_CACHED;
-	const uint32_t bytes = 4 * (2 * words + words + words % 2 + e.cached);
+	const uint32_t places = keep < longest ? keep - recent - first : 0, rest = keep < longest ? longest - recent - first : 0;
+	e.words = (rest + 63) / 64;
+	const uint32_t room = (MOST_EVICT_BYTES - EVICT_WORD * e.words) / 6; /* beside the words: of 262144 tokens, for 6000 weights */
+	e.cached = rest < EVICT_CACHED ? rest : EVICT_CACHED;
+	if (e.cached > room) e.cached = room;
+	const uint32_t bytes = evict_bytes(e.words, e.cached);
 	static int allowed = -1;
 	const DeviceInfo* dev = nullptr;
 	rc = device_info(&dev);
 	if (rc) return rc;
 	if (bytes > 32768 && allowed != dev->device) { /* more LDS than a launch may ask for unannounced, on this device */
-		KMX_HIP(hipFuncSetAttribute((const void*)evict4_choose_kernel, hipFuncAttributeMaxDynamicSharedMemorySize, (int)(4 * (EVICT_TOKENS / 64 * 3 + 2 + EVICT_CACHED))));
+		KMX_HIP(hipFuncSetAttribute((const void*)evict4_choose_kernel, hipFuncAttributeMaxDynamicSharedMemorySize, (int)MOST_EVICT_BYTES));
 		allowed = dev->device;
 	}
 	KMX_LAUNCH_KERNEL(evict4_choose_kernel, dim3(cache->heads, batch->sequences), dim3(EVICT_THREADS), bytes, stream(), e);
