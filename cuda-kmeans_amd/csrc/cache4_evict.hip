@@ -41,6 +41,25 @@ weigh4_kernel(Weigh4 a)
 	if (seq.queries == 0 || from >= visible_to(a.batch, seq, seq.queries - 1)) return;
 	const int32_t least = (int32_t)visible_to(a.batch, seq, 0);
 
+	/* a row of 16 for the wavefront, of those from `first` on: asked for before what is to be done in the meantime */
+	const uint64_t rows = (uint64_t)seq.queries * a.batch.group;
+	u32x4 raw[J];
+	float lse = 0.0f;
+	int32_t look = 0;
+	bool there = false;
+	auto fetch = [&](uint64_t first) {
+		if (first + 16 * wave >= rows) return;
+		const uint64_t row = first + 16 * wave + i16;
+		there = row < rows;
+		const uint32_t token = there ? (uint32_t)row / a.batch.group : 0, query_head = head * a.batch.group + (there ? (uint32_t)row - token * a.batch.group : 0);
+		const uint16_t* p = (const uint16_t*)a.q + (size_t)(seq.first + token) * a.q_token + (size_t)query_head * a.q_head + 8 * kg;
+		lse = a.lse[(size_t)(seq.first + token) * a.batch.query_heads + query_head];
+#pragma unroll
+		for (int j = 0; j < J; ++j) raw[j] = a.vec ? load_raw8(p + 32 * j, true) : load_raw8(p + 32 * j, false);
+		look = there ? (int32_t)visible_to(a.batch, seq, token) : 0;
+	};
+	fetch(0);
+
 	/* the wavefront's blocks */
 	const Constant4 table = constant4(a.batch.table) + (size_t)s * a.batch.table_stride;
 	const uint32_t sub_bits = a.cache.page_shift - 4, begin = from + 64 * wave;
@@ -76,20 +95,14 @@ weigh4_kernel(Weigh4 a)
 	}
 	float w[4] = { 0.0f, 0.0f, 0.0f, 0.0f };
 	const bool cut = (int32_t)(begin + 64) > least; /* not all queries see all of the wavefront's tokens */
-	const uint64_t rows = (uint64_t)seq.queries * a.batch.group;
 	for (uint64_t first = 0; first < rows; first += 64) {
 		__syncthreads(); /* (the rows before are done with) */
 		if (first + 16 * wave < rows) {
-			const uint64_t row = first + 16 * wave + i16;
-			const bool there = row < rows;
-			const uint32_t token = there ? (uint32_t)(row / a.batch.group) : 0, query_head = head * a.batch.group + (there ? (uint32_t)(row % a.batch.group) : 0);
-			const uint16_t* p = (const uint16_t*)a.q + (size_t)(seq.first + token) * a.q_token + (size_t)query_head * a.q_head + 8 * kg;
 			float x[J][8], largest = 0.0f;
 #pragma unroll
 			for (int j = 0; j < J; ++j) {
-				const u32x4 raw = a.vec ? load_raw8(p + 32 * j, true) : load_raw8(p + 32 * j, false);
 				for (int e = 0; e < 8; ++e) {
-					x[j][e] = there ? raw_element(raw[e / 2], e % 2, a.bf16) : 0.0f;
+					x[j][e] = there ? raw_element(raw[j][e / 2], e % 2, a.bf16) : 0.0f;
 					largest = fmaxf(largest, fabsf(x[j][e]));
 				}
 			}
@@ -105,9 +118,10 @@ weigh4_kernel(Weigh4 a)
 			}
 			if (kg == 0) {
 				factors[wave][i16] = factor;
-				sums[wave][i16] = there ? -1.44269504088896341f * a.lse[(size_t)(seq.first + token) * a.batch.query_heads + query_head] : -__builtin_inff(); /* no such row: no weight */
-				looks[wave][i16] = there ? (int32_t)visible_to(a.batch, seq, token) : 0;
+				sums[wave][i16] = there ? -1.44269504088896341f * lse : -__builtin_inff(); /* no such row: no weight */
+				looks[wave][i16] = look;
 			}
+			fetch(first + 64);
 		}
 		__syncthreads();
 		if (!some) continue;
@@ -448,11 +462,11 @@ evict4_move_kernel(Evict4 e)
 	constexpr int AT_ONCE = 8;
 	const bool begins = blockIdx.z == 0;
 	const uint32_t waves = begins ? 4 : 4 * (gridDim.z - 1), number = begins ? wave : 4 * (blockIdx.z - 1) + wave;
-	constexpr uint32_t RUN = 64;
-	for (uint32_t i0 = e.first + RUN * number; i0 < edge; i0 += RUN * waves) {
-		const uint32_t i = i0 + lane, from = lane < RUN && i < edge ? (uint32_t)kept[i] : i;
+	const uint32_t run = begins ? 64 : 16; /* places of a wavefront at a time */
+	for (uint32_t i0 = e.first + run * number; i0 < edge; i0 += run * waves) {
+		const uint32_t i = i0 + lane, from = lane < run && i < edge ? (uint32_t)kept[i] : i;
 		const bool mine = begins ? from >= edge && from < e.keep : from >= e.keep;
-		const bool moving = lane < RUN && i < edge && mine;
+		const bool moving = lane < run && i < edge && mine;
 		const uint32_t source = moving ? page_of(from) : ~0u, target = moving ? page_of(i) : ~0u;
 		uint64_t moves = __ballot(source < e.cache.page_count && target < e.cache.page_count);
 		while (moves) {
@@ -473,6 +487,7 @@ evict4_move_kernel(Evict4 e)
 				put_row<J>(block_of((uint32_t)__builtin_amdgcn_readlane((int)target, bit[k]), t), t % 16, lane, row[k]);
 			}
 		}
+		if (begins && __any(from >= e.keep)) break; /* the lowest places have what came from the lowest: no more of its own behind */
 	}
 	if (!begins) return;
 	for (uint32_t i0 = 0; i0 < e.recent; i0 += 4 * AT_ONCE) {
