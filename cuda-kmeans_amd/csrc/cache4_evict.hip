@@ -260,6 +260,22 @@ evict4_choose_kernel(Evict4 e)
 	};
 	auto key = [&](uint32_t x) { return key_of(cached ? cache[x] : weight_at(e.first + x)); };
 
+	/* one more in a share. Many weights are alike (tokens that nothing has looked at yet have 0): those of the first two lanes' shares are counted before they are added, since LDS adds
+	 * to one address one after the other */
+	auto count = [&](bool mine, uint32_t share) {
+#pragma unroll
+		for (int i = 0; i < 2; ++i) {
+			const uint64_t some = __ballot(mine);
+			if (!some) return;
+			const int first = __ffsll((unsigned long long)some) - 1;
+			const bool same = mine && share == (uint32_t)__builtin_amdgcn_readlane((int)share, first);
+			const uint32_t many = (uint32_t)__popcll(__ballot(same));
+			if ((int)lane == first) atomicAdd(&bins[share], many);
+			mine = mine && !same;
+		}
+		if (mine) atomicAdd(&bins[share], 1u);
+	};
+
 	/* the weights, and the range of their keys */
 	const float recent = tid < e.recent ? weight_at(n - e.recent + tid) : 0.0f; /* (the first of them) */
 	if (tid < 2) found[tid] = tid ? 0u : ~0u;
@@ -302,9 +318,10 @@ evict4_choose_kernel(Evict4 e)
 	while (need && low != high) { /* (the shares are zero here) */
 		uint32_t shift = 0;
 		while ((high - low) >> shift >= EVICT_BINS) ++shift;
+#pragma unroll 4
 		for (uint32_t x = tid; x < rest; x += EVICT_THREADS) {
 			const uint32_t k = key(x);
-			if (k >= low && k <= high) atomicAdd(&bins[(k - low) >> shift], 1u);
+			count(k >= low && k <= high, (k - low) >> shift);
 		}
 		__syncthreads();
 		/* the share that holds the need-th largest: thread t has shares 2047 - 2 t and the one below */
