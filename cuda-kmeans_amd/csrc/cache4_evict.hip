@@ -25,7 +25,9 @@ constexpr uint32_t WEIGH_TOKENS = 256; /* of a work-group, 64 a wavefront */
 /*
  * A work-group takes 256 tokens of one head of a sequence, whose keys its wavefronts unpack once and keep, four blocks each; the rows (query heads of the head, of all queries)
  * come by 64 at a time through LDS, a tile of 16 from each wavefront. The keys are the second operand (v_mfma_f32_16x16x32_f16): scores come out as [row][token], so that
- * the weights of a token, 2^(c s - log2(e) lse), are added up in the lane that has it, and four lanes at the end.
+ * the weights of a token, 2^(c s - log2(e) lse), are added up in the lane that has it, and four lanes at the end. Rows are asked for before the keys are unpacked.
+ * Bound by the chain length - table - codes - products of its work-groups, three rounds of them, at 32 sequences of up to 2048 tokens (16 us; the packed keys alone take 5); 32 queries over
+ * 32768 tokens 22 us, half of it powers.
  */
 template <int J>
 __global__ void __launch_bounds__(256)
@@ -208,7 +210,8 @@ __device__ __forceinline__ uint32_t key_of(float w)
 __device__ __forceinline__ uint32_t sum_below(const uint32_t* counts, uint32_t wave)
 {
 	uint32_t sum = 0;
-	for (uint32_t w = 0; w < wave; ++w) sum += counts[w];
+#pragma unroll
+	for (uint32_t w = 0; w < EVICT_WAVES; ++w) sum += w < wave ? counts[w] : 0; /* (all are read at once) */
 	return sum;
 }
 __device__ __forceinline__ uint64_t lanes_below(uint32_t lane) { return ((uint64_t)1 << lane) - 1; }
@@ -216,11 +219,14 @@ __device__ __forceinline__ uint64_t lanes_below(uint32_t lane) { return ((uint64
 /* sums of what the threads before have; EVICT_WAVES counts */
 __device__ __forceinline__ uint32_t sum_before(uint32_t mine, uint32_t* counts, uint32_t wave, uint32_t lane)
 {
-	uint32_t upto = mine;
-	for (uint32_t d = 1; d < WAVE; d *= 2) {
-		const uint32_t v = (uint32_t)__shfl_up((int)upto, d);
-		if (lane >= d) upto += v;
-	}
+	int v = (int)mine; /* within rows of 16 lanes, then from row to row */
+	v += __builtin_amdgcn_update_dpp(0, v, 0x111, 0xF, 0xF, false);
+	v += __builtin_amdgcn_update_dpp(0, v, 0x112, 0xF, 0xF, false);
+	v += __builtin_amdgcn_update_dpp(0, v, 0x114, 0xF, 0xF, false);
+	v += __builtin_amdgcn_update_dpp(0, v, 0x118, 0xF, 0xF, false);
+	v += __builtin_amdgcn_update_dpp(0, v, 0x142, 0xA, 0xF, false);
+	v += __builtin_amdgcn_update_dpp(0, v, 0x143, 0xC, 0xF, false);
+	const uint32_t upto = (uint32_t)v;
 	if (lane == WAVE - 1) counts[wave] = upto;
 	__syncthreads();
 	return sum_below(counts, wave) + upto - mine;
@@ -231,7 +237,8 @@ __device__ __forceinline__ uint32_t sum_before(uint32_t mine, uint32_t* counts, 
  * three rounds at most. Then, for 64 places a word: which stay (of those at the threshold the first ones), how many places below the edge become free before them and how many
  * tokens from the edge on have to move. The n-th moving one goes to the n-th free place. Up to 24576 weights stay in LDS, with the list of those that move; else the list is the begin of
  * `kept`, from where it goes to the free places, the highest first: none of them lies below where it is listed.
- * Bound by latency (one work-group a compute unit, few of them): weights come eight at a time, all that is written depends on LDS alone. MEASURED
+ * Bound by latency (one work-group a compute unit, few of them): weights come eight at a time, all that is written depends on LDS alone.
+ * 16384 tokens to 4096, 32 work-groups: 24 us (weights 4, the threshold 10 in three rounds, words 4, places and lists 3, what is written 3); 1025 to 1024: 10 (5 of them the threshold).
  */
 __global__ void __launch_bounds__(EVICT_THREADS)
 evict4_choose_kernel(Evict4 e)
@@ -258,22 +265,29 @@ evict4_choose_kernel(Evict4 e)
 		size_t at;
 		return weight_of(e, table, head, t, &at) ? e.weights[at] : __builtin_nanf("");
 	};
-	auto key = [&](uint32_t x) { return key_of(cached ? cache[x] : weight_at(e.first + x)); };
 
-	/* one more in a share. Many weights are alike (tokens that nothing has looked at yet have 0): those of the first two lanes' shares are counted before they are added, since LDS adds
-	 * to one address one after the other */
+	/* one more in a share. Many weights are alike (tokens that nothing has looked at yet have 0): those of the first lane's share are counted before they are added, since LDS adds to one
+	 * address one after the other */
 	auto count = [&](bool mine, uint32_t share) {
+		const uint64_t some = __ballot(mine);
+		if (!some) return;
+		const int first = __ffsll((unsigned long long)some) - 1;
+		const bool same = mine & (share == (uint32_t)__builtin_amdgcn_readlane((int)share, first));
+		const uint32_t many = (uint32_t)__popcll(__ballot(same));
+		if (mine & (!same | ((int)lane == first))) atomicAdd(&bins[share], same ? many : 1u);
+	};
+	constexpr int KEYS = 4; /* that a thread has at a time */
+	auto keys_at = [&](uint32_t (&k)[KEYS], uint32_t x0) {
+		float w[KEYS];
+		if (cached) {
 #pragma unroll
-		for (int i = 0; i < 2; ++i) {
-			const uint64_t some = __ballot(mine);
-			if (!some) return;
-			const int first = __ffsll((unsigned long long)some) - 1;
-			const bool same = mine && share == (uint32_t)__builtin_amdgcn_readlane((int)share, first);
-			const uint32_t many = (uint32_t)__popcll(__ballot(same));
-			if ((int)lane == first) atomicAdd(&bins[share], many);
-			mine = mine && !same;
+			for (int i = 0; i < KEYS; ++i) w[i] = cache[min(x0 + i * EVICT_THREADS + tid, rest - 1)];
+		} else {
+#pragma unroll
+			for (int i = 0; i < KEYS; ++i) w[i] = weight_at(e.first + min(x0 + i * EVICT_THREADS + tid, rest - 1));
 		}
-		if (mine) atomicAdd(&bins[share], 1u);
+#pragma unroll
+		for (int i = 0; i < KEYS; ++i) k[i] = key_of(w[i]);
 	};
 
 	/* the weights, and the range of their keys */
@@ -318,10 +332,11 @@ evict4_choose_kernel(Evict4 e)
 	while (need && low != high) { /* (the shares are zero here) */
 		uint32_t shift = 0;
 		while ((high - low) >> shift >= EVICT_BINS) ++shift;
-#pragma unroll 4
-		for (uint32_t x = tid; x < rest; x += EVICT_THREADS) {
-			const uint32_t k = key(x);
-			count(k >= low && k <= high, (k - low) >> shift);
+		for (uint32_t x0 = 0; x0 < rest; x0 += KEYS * EVICT_THREADS) {
+			uint32_t k[KEYS];
+			keys_at(k, x0);
+#pragma unroll
+			for (int i = 0; i < KEYS; ++i) count((x0 + i * EVICT_THREADS + tid < rest) & (k[i] >= low) & (k[i] <= high), (k[i] - low) >> shift);
 		}
 		__syncthreads();
 		/* the share that holds the need-th largest: thread t has shares 2047 - 2 t and the one below */
@@ -340,12 +355,17 @@ evict4_choose_kernel(Evict4 e)
 	}
 	const uint32_t threshold = need ? low : ~0u; /* above it all stay, at it the first `need` (without places: none) */
 
-	for (uint32_t x0 = WAVE * wave; x0 < rest; x0 += EVICT_THREADS) {
-		const uint32_t k = x0 + lane < rest ? key(x0 + lane) : 0;
-		const uint64_t at = __ballot(x0 + lane < rest && k == threshold), above = __ballot(k > threshold);
-		if (lane == 0) {
-			bits[x0 / 64] = above;
-			level[x0 / 64] = at;
+	for (uint32_t x0 = 0; x0 < rest; x0 += KEYS * EVICT_THREADS) {
+		uint32_t k[KEYS];
+		keys_at(k, x0);
+#pragma unroll
+		for (int i = 0; i < KEYS; ++i) {
+			const uint32_t x = x0 + i * EVICT_THREADS + tid;
+			const uint64_t above = __ballot((x < rest) & (k[i] > threshold)), at = __ballot((x < rest) & (k[i] == threshold));
+			if (lane == 0 && x < rest) {
+				bits[x / 64] = above;
+				level[x / 64] = at;
+			}
 		}
 	}
 	__syncthreads();
@@ -461,8 +481,9 @@ __device__ __forceinline__ void put_row(uint8_t* block, uint32_t t, uint32_t lan
 }
 
 /*
- * Rows to their new places, a wavefront a row. Of a sequence and head the first work-group moves those that come from the places which the recent ones are about to
- * take, and then these, in their order; the others share the rest, which come from behind all new places.
+ * Rows to their new places, a wavefront a row, eight rows on their way at a time. Of a sequence and head the first work-group moves those that come from the places which the recent ones
+ * are about to take (the lowest places have them), and then these, in their order; the others share the rest, which come from behind all new places, by runs of 16 places.
+ * Bound by the chain kept - table - row - place of each run: 4096 of 16384 tokens, 4 sequences, 8 heads of 128: 11 us.
  */
 template <int J>
 __global__ void __launch_bounds__(256)
