@@ -26,8 +26,8 @@ constexpr uint32_t WEIGH_TOKENS = 256; /* of a work-group, 64 a wavefront */
  * A work-group takes 256 tokens of one head of a sequence, whose keys its wavefronts unpack once and keep, four blocks each; the rows (query heads of the head, of all queries)
  * come by 64 at a time through LDS, a tile of 16 from each wavefront. The keys are the second operand (v_mfma_f32_16x16x32_f16): scores come out as [row][token], so that
  * the weights of a token, 2^(c s - log2(e) lse), are added up in the lane that has it, and four lanes at the end. Rows are asked for before the keys are unpacked.
- * Bound by the chain length - table - codes - products of its work-groups, three rounds of them, at 32 sequences of up to 2048 tokens (16 us; the packed keys alone take 5); 32 queries over
- * 32768 tokens 22 us, half of it powers.
+ * Bound by the chain length - table - codes - products of its work-groups, three rounds of them, at 32 sequences of up to 2048 tokens (13.8 us; the packed keys alone take 5); 32 queries over
+ * 32768 tokens 18.8 us, half of it powers. 128 tokens a work-group instead of 256: 16.9 for 15.6 and 141 for 116 (64 x 8192); 256 after 256 by the same work-groups: 17.5 for 15.6.
  */
 template <int J>
 __global__ void __launch_bounds__(256)
@@ -56,8 +56,13 @@ weigh4_kernel(Weigh4 a)
 		const uint32_t token = there ? (uint32_t)row / a.batch.group : 0, query_head = head * a.batch.group + (there ? (uint32_t)row - token * a.batch.group : 0);
 		const uint16_t* p = (const uint16_t*)a.q + (size_t)(seq.first + token) * a.q_token + (size_t)query_head * a.q_head + 8 * kg;
 		lse = a.lse[(size_t)(seq.first + token) * a.batch.query_heads + query_head];
+		if (a.vec) {
 #pragma unroll
-		for (int j = 0; j < J; ++j) raw[j] = a.vec ? load_raw8(p + 32 * j, true) : load_raw8(p + 32 * j, false);
+			for (int j = 0; j < J; ++j) raw[j] = load_raw8(p + 32 * j, true);
+		} else {
+#pragma unroll
+			for (int j = 0; j < J; ++j) raw[j] = load_raw8(p + 32 * j, false);
+		}
 		look = there ? (int32_t)visible_to(a.batch, seq, token) : 0;
 	};
 	fetch(0);
@@ -71,11 +76,13 @@ weigh4_kernel(Weigh4 a)
 	size_t to[4];
 	const bool some = begin < seq.length;
 	if (some) {
+		uint32_t pages[4];
+#pragma unroll
+		for (int b = 0; b < 4; ++b) pages[b] = (uint32_t)table[min((begin / 16 + b) >> sub_bits, a.batch.table_stride - 1)];
 #pragma unroll
 		for (int b = 0; b < 4; ++b) {
-			const uint32_t n = begin / 16 + b, entry = n >> sub_bits, sub = n & ((1u << sub_bits) - 1);
-			const uint32_t page = entry < a.batch.table_stride ? (uint32_t)table[entry] : ~0u;
-			known[b] = 16 * n < seq.length && page < a.cache.page_count;
+			const uint32_t n = begin / 16 + b, entry = n >> sub_bits, sub = n & ((1u << sub_bits) - 1), page = pages[b];
+			known[b] = 16 * n < seq.length && entry < a.batch.table_stride && page < a.cache.page_count;
 			const uint8_t* block = a.cache.blocks + block_offset<J>(a.cache, known[b] ? page : 0, head, known[b] ? sub : 0);
 			to[b] = (((size_t)(known[b] ? page : 0) * a.cache.heads + head) << a.cache.page_shift) + 16 * sub;
 			uint32_t codes[J];
@@ -101,13 +108,16 @@ weigh4_kernel(Weigh4 a)
 		__syncthreads(); /* (the rows before are done with) */
 		if (first + 16 * wave < rows) {
 			float x[J][8], largest = 0.0f;
+			auto take = [&](bool bf16) { /* (one question for all of them) */
 #pragma unroll
-			for (int j = 0; j < J; ++j) {
-				for (int e = 0; e < 8; ++e) {
-					x[j][e] = there ? raw_element(raw[j][e / 2], e % 2, a.bf16) : 0.0f;
-					largest = fmaxf(largest, fabsf(x[j][e]));
-				}
-			}
+				for (int j = 0; j < J; ++j)
+					for (int e = 0; e < 8; ++e) x[j][e] = raw_element(there ? raw[j][e / 2] : 0u, e % 2, bf16);
+			};
+			if (a.bf16) take(true);
+			else take(false);
+#pragma unroll
+			for (int j = 0; j < J; ++j)
+				for (int e = 0; e < 8; ++e) largest = fmaxf(largest, fabsf(x[j][e]));
 			largest = fmaxf(largest, __shfl_xor(largest, 16));
 			largest = fmaxf(largest, __shfl_xor(largest, 32));
 			float factor;
