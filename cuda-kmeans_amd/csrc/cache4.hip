@@ -1103,7 +1103,7 @@ int kmx_cache4_attend_shared(const kmx_cache4* cache, const kmx_cache4_batch* pr
 	const size_t rows = any ? shared_floats(batch, cache->dim) : 0, mine = plan_floats(plan, J), theirs = any ? plan_floats(ahead, J) : 0;
 	float* space = nullptr;
 	if (rows + mine + theirs) {
-		rc = place_cache4("kmx_cache4_attend_shared", rows + (mine > theirs ? mine : theirs), &space);
+		rc = place_cache4("kmx_cache4_attend_shared", rows + (mine > theirs ? mine : theirs), &space, "kmx_cache4_reserve_shared");
 		if (rc) return rc;
 	}
 	a.partial = space + rows;

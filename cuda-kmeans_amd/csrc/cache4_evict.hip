@@ -583,6 +583,7 @@ int kmx_cache4_weigh(const kmx_cache4* cache, const kmx_cache4_batch* batch, int
 	const uint32_t longest = a.batch.max_length < most ? a.batch.max_length : (uint32_t)most;
 	if (batch->sequences == 0 || batch->tokens == 0 || batch->max_queries == 0 || longest == 0) return KMX_OK;
 	if (!q || !lse || !weights) return fail(KMX_ERR_INVALID_ARGUMENT, "kmx_cache4_weigh: null device pointer");
+	if ((uint64_t)(batch->max_queries < batch->tokens ? batch->max_queries : batch->tokens) * a.batch.group > 0x7FFFFFFFu) return fail(KMX_ERR_UNSUPPORTED, "kmx_cache4_weigh: rows of a head are counted in 31 bits");
 	if ((uintptr_t)q % 2 || (uintptr_t)lse % 4 || (uintptr_t)weights % 4) return fail(KMX_ERR_INVALID_ARGUMENT, "kmx_cache4_weigh: rows start at multiples of their element's size");
 	a.q = q;
 	a.q_token = q_token_stride;

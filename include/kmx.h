@@ -511,7 +511,8 @@ int kmx_cache4_reserve_shared(const kmx_cache4* cache, const kmx_cache4_batch* p
 /*
  * Attention weights added up: weights[page][head][token of the page] += sum over the queries that see the token, and the query heads of the head, of
  * exp(scale q . k - lse), lse as kmx_cache4_attend (or _attend_shared, for prefix and own tokens each) has written it for the same queries. Tokens of a page that several
- * sequences have get all of their weights. Floats; nothing is added for pages that are not there.
+ * sequences have get all of their weights, each sequence's in one addition and in the order in which they come: with such pages the last bits may differ from call to call. Floats; nothing
+ * is added for pages that are not there.
  */
 int kmx_cache4_weigh(const kmx_cache4* cache, const kmx_cache4_batch* batch, int type, const void* q, size_t q_token_stride, size_t q_head_stride,
                      const float* lse, float scale, int causal, float* weights);
@@ -556,7 +557,7 @@ int kmx_rotary(int type, const kmx_rotary_rows* rows, uint32_t sets, uint32_t to
  * token_starts[s] .. token_starts[s + 1] - 1 of the rows handed over; its queries are those of its last tokens: with `causal` query i of n sees the first tokens - n + i + 1 of
  * them, else all. out and lse as for kmx_cache4_attend; nothing that a query does not see, infinities and NaN among it, comes into its row. dim: a multiple of 32 up to 256.
  * F16 or BF16, products of numbers as they are, probabilities rounded to the type before the second product, sums in floats. Starts on the device are not trusted: a sequence whose
- * starts are not within the rows has none. max_queries and max_tokens bound queries and tokens of a sequence (more is cut off).
+ * starts are not within the rows has none. out and lse lie apart from what is read. max_queries and max_tokens bound queries and tokens of a sequence (more is cut off).
  */
 typedef struct kmx_prompt {
 	uint32_t sequences;

@@ -180,6 +180,7 @@ def test_weighing_and_eviction_that_are_refused(km):
     weigh(invalid, b"null device", weights=None)
     weigh(invalid, b"element", weights=ctypes.c_void_p((1 << 20) + 2))
     weigh(unsupported, b"too many", b=batch_of(km, sequences=70000))
+    weigh(unsupported, b"31 bits", b=batch_of(km, tokens=1 << 31, max_queries=1 << 31))
     for nothing in (dict(sequences=0), dict(tokens=0), dict(max_queries=0), dict(max_length=0), dict(table_stride=0)):
         weigh(km.KMX_OK, b"", b=batch_of(km, **nothing), q=None)
 
