@@ -208,7 +208,7 @@ prompt_attend_kernel(PromptAttend a)
 #pragma unroll
 		for (int i = 0; i < PIECES; ++i)
 			if (values[i]) found = without_strange<T>(g.w[i]) || found;
-		if (found) strange = 1;
+		if (__any(found)) strange = 1;
 	};
 
 	float reference = -__builtin_inff(), base = LIFT, l = 0.0f;
@@ -309,7 +309,7 @@ prompt_attend_kernel(PromptAttend a)
 		auto slot = [&](int t) {
 #pragma unroll
 			for (int n = TURNS * t / SLOTS; n < TURNS * (t + 1) / SLOTS; ++n) turn(n);
-			/* one of a batch's reads of operands for the next, or of its moves -- first those to LDS, then those from memory --, evenly over its slots: all four wavefronts
+			/* one of a batch's reads of operands for the next, or of its moves -- first those to LDS, then those from memory --, evenly over its slots: all wavefronts
 			 * are about here, and LDS takes a read of theirs in 5 cycles and a write in 13 */
 			const int batch = t / BATCH_SLOTS, in = t % BATCH_SLOTS, first = (batch + 1) * BATCH, at = (batch + 1) % 2;
 #pragma unroll
@@ -344,23 +344,26 @@ prompt_attend_kernel(PromptAttend a)
 		l += sum;
 	};
 
-	if (tid == 0) strange = 0;
+	if (wave == 0) strange = 0;
 	__syncthreads();
 	if (end) {
 		for (int c = 0; c < 2; ++c) w1.w[c] = u32x4{ 0, 0, 0, 0 };
-		/* the first tiles: three of keys, one of values */
+		/* the first tiles: three of keys, one of values. (Whole wavefronts take part or do not: where lanes leave a loop one by one the compiler has put copies of registers behind it, to the
+		 * other half of the file, before the lanes are back.) */
 		auto bring_tile = [&](const uint16_t* rows, uint32_t tile, uint32_t place, uint32_t row, bool checked) {
-			for (uint32_t piece = tid; piece < TILE_PIECES; piece += THREADS) {
-				const uint32_t token = piece / (4 * J), at_row = piece % (4 * J);
+			for (uint32_t first = WAVE * wave; first < TILE_PIECES; first += THREADS) {
+				const uint32_t piece = first + lane, token = piece / (4 * J), at_row = piece % (4 * J);
 				u32x4 w = load_raw8(rows + (size_t)min(32 * (start + tile) + token, p.tokens - 1) * a.token_stride + 8 * at_row, VEC);
-				if (checked && (int32_t)(32 * (start + tile) + 32) > all_see && without_strange<T>(w)) strange = 1;
+				if (checked && (int32_t)(32 * (start + tile) + 32) > all_see && __any(without_strange<T>(w))) strange = 1;
 				*(u32x4*)(lds + place + token * row + 16 * at_row) = w;
 			}
 		};
 		for (uint32_t n = 0; n < 3; ++n) bring_tile(key_rows, n, n * PLACE, KROW, false);
 		bring_tile(value_rows, 0, KTILE, VROW, true);
-		for (uint32_t piece = tid; piece < TILE_PIECES; piece += THREADS) /* (nothing before the first tile) */
+		for (uint32_t first = WAVE * wave; first < TILE_PIECES; first += THREADS) { /* (nothing before the first tile) */
+			const uint32_t piece = first + lane;
 			*(u32x4*)(lds + 2 * PLACE + KTILE + piece / (4 * J) * VROW + 16 * (piece % (4 * J))) = u32x4{ 0, 0, 0, 0 };
+		}
 		auto fetch = [&](Staged& g) {
 #pragma unroll
 			for (int i = 0; i < PIECES; ++i) g.w[i] = load(i);
@@ -546,9 +549,11 @@ template <typename T, int J>
 static int launch_prompt_of(const PromptAttend& a, const PromptPlan& plan)
 {
 	if constexpr (J == 5 || J == 6) return launch_prompt_rows<T, J, 8>(a, plan);
-	if constexpr (J == 3 || J == 4)
-		if (plan.wide) return launch_prompt_rows<T, J, 8>(a, plan);
-	return launch_prompt_rows<T, J, 4>(a, plan);
+	else {
+		if constexpr (J == 3 || J == 4)
+			if (plan.wide) return launch_prompt_rows<T, J, 8>(a, plan);
+		return launch_prompt_rows<T, J, 4>(a, plan);
+	}
 }
 
 template <int J>
