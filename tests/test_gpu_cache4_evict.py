@@ -255,6 +255,13 @@ def test_long_sequences(km, gpu, length, keep, first, recent):
     Evict(km, rng, 1, 32, 256, [length, 50], keep, first, recent).check()
 
 
+def test_long_and_short_sequences_in_one_call(km, gpu):
+    """Weights that stay in LDS beside others that are read again for every pass, and sequences that stay as they are."""
+    rng = np.random.default_rng(21)
+    e = Evict(km, rng, 2, 32, 64, [50000, 3000, 700, 12000, 1001], 1000, 4, 64)
+    e.check()
+
+
 def test_the_longest_sequences(km, gpu):
     rng = np.random.default_rng(7)
     e = Evict(km, rng, 1, 32, 256, [262144], 262000, 1000, 100)
