@@ -202,3 +202,46 @@ def test_weighing_and_eviction_that_are_refused(km):
     evict(invalid, b"element", kept=ctypes.c_void_p((1 << 20) + 2))
     evict(unsupported, b"too many", b=batch_of(km, sequences=70000))
     evict(km.KMX_OK, b"", b=batch_of(km, sequences=0, lengths=None, table=None), weights=None, kept=None, left=None)
+
+
+def test_prompts_are_shared_out_whole_and_within_the_reserved_room(tmp_path):
+    """Launch shapes of the attention over prompts (csrc/prompt_plan.h): every tile in one part, none of the longest sequence's parts empty, room as kmx_prompt_reserve makes it."""
+    source = tmp_path / "plan.cpp"
+    source.write_text(r"""
+#include "prompt_plan.h"
+#include <initializer_list>
+#include <cstdio>
+using namespace kmx;
+int main()
+{
+	unsigned parts = 0;
+	for (uint32_t J = 1; J <= 8; ++J)
+		for (uint32_t heads : { 1u, 3u, 8u, 64u })
+			for (uint32_t group : { 1u, 4u, 7u })
+				for (uint32_t sequences : { 1u, 5u, 300u })
+					for (uint32_t queries : { 1u, 31u, 500u, 8192u, 0x7FFFFFFFu })
+						for (uint32_t tokens : { 0u, 1u, 33u, 64u, 129u, 1000u, 8192u, 100001u, 0x7FFFFFFFu }) {
+							const PromptPlan p = plan_prompt(PromptShape{ J, heads, group, sequences, queries, tokens, 256 });
+							const uint64_t rows = (uint64_t)queries * group, tile = p.wide ? 256 : 128, tiles = ((uint64_t)tokens + 31) / 32;
+							const uint64_t units = (rows + tile - 1) / tile * heads * sequences;
+							if (p.units == 0) {
+								if (rows <= 0x7FFFFF00u && units <= 0x7FFFFFFFu) return printf("refused %u %u %u %u %u\n", J, heads, group, sequences, queries), 1;
+								continue;
+							}
+							if (p.units != units || (uint64_t)p.units * p.parts > 0x7FFFFFFFu || (p.wide ? J < 3 || J > 6 : J == 5 || J == 6)) return printf("units\n"), 1;
+							if ((uint64_t)p.parts * p.tiles_per_part < tiles || p.parts == 0 || (p.parts > 1 && (uint64_t)(p.parts - 1) * p.tiles_per_part >= tiles)) return printf("parts\n"), 1;
+							if (p.parts > 1 && p.tiles_per_part < PROMPT_LEAST) return printf("short parts\n"), 1;
+							if (prompt_floats(p, J) > most_prompt_floats(J, 256) || 4 * prompt_floats(p, J) > (64u << 20)) return printf("room\n"), 1;
+							parts += p.parts > 1;
+						}
+	printf("%u", parts);
+	return parts < 100;
+}
+""")
+    import os
+    import subprocess
+    csrc = os.path.join(os.path.dirname(os.path.dirname(os.path.abspath(__file__))), "cuda-kmeans_amd", "csrc")
+    program = tmp_path / "plan"
+    subprocess.run(["g++", "-std=c++17", "-O1", "-I", csrc, str(source), "-o", str(program)], check=True)
+    ran = subprocess.run([str(program)], capture_output=True, text=True)
+    assert ran.returncode == 0, ran.stdout
