@@ -211,7 +211,7 @@ prompt_attend_kernel(PromptAttend a)
 		if (__any(found)) strange = 1;
 	};
 
-	float reference = -__builtin_inff(), base = LIFT, l = 0.0f;
+	float reference = -__builtin_inff(), base = 0.0f, l = 0.0f; /* (the first tile's raise makes them) */
 	f32x16 o[J];
 #pragma unroll
 	for (int j = 0; j < J; ++j)
@@ -252,7 +252,7 @@ prompt_attend_kernel(PromptAttend a)
 		top = both_halves_most(top) * a.factor;
 		const float higher = fmaxf(reference, top), less = higher == reference ? 1.0f : __builtin_amdgcn_exp2f(reference - higher);
 		reference = higher;
-		base = higher == -__builtin_inff() ? LIFT : LIFT - higher;
+		base = higher == -__builtin_inff() ? 3.4028235e38f : LIFT - higher; /* (nothing with a weight so far: the first score that is a number raises) */
 		l *= less;
 #pragma unroll
 		for (int j = 0; j < J; ++j) o[j] *= less;

@@ -557,7 +557,8 @@ int kmx_rotary(int type, const kmx_rotary_rows* rows, uint32_t sets, uint32_t to
  * token_starts[s] .. token_starts[s + 1] - 1 of the rows handed over; its queries are those of its last tokens: with `causal` query i of n sees the first tokens - n + i + 1 of
  * them, else all. out and lse as for kmx_cache4_attend; nothing that a query does not see, infinities and NaN among it, comes into its row. dim: a multiple of 32 up to 256.
  * F16 or BF16, products of numbers as they are, probabilities rounded to the type before the second product, sums in floats. Starts on the device are not trusted: a sequence whose
- * starts are not within the rows has none. out and lse lie apart from what is read. max_queries and max_tokens bound queries and tokens of a sequence (more is cut off).
+ * starts are not within the rows has none. Tokens whose score is minus infinity have no weight; a query that sees no others sees nothing.
+ * out and lse lie apart from what is read. max_queries and max_tokens bound queries and tokens of a sequence (more is cut off).
  */
 typedef struct kmx_prompt {
 	uint32_t sequences;
