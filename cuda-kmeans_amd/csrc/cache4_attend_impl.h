@@ -186,9 +186,14 @@ __device__ __forceinline__ bool has_prefix(const Attend4& a, size_t token)
 	return from >= 0 && to <= (int64_t)a.batch.tokens && (int64_t)token < to && (int64_t)token - from < (int64_t)a.prefix_queries;
 }
 
+/* what the sums of a row over `l` are multiplied with: a row that sees nothing is zero; NaN stays */
+__device__ __forceinline__ float part_of(float l) { return l > 0.0f ? 1.0f / l : l == l ? 0.0f : l; }
+
 /*
  * The end of a row: its sums over `l`, the largest score m scale (to the base of 2); with a prefix these are joined with what the prefix has left, of a prefix they
  * are left as they are. `by` is what sums are multiplied with, `theirs` the prefix's sums at `from`.
+ * Kernels that know of no prefix (SHARED false) are others, with their ends written out: through here these cost registers, and a wait in the chain at the end of the parts' last
+ * work-group (1 sequence of 131072 tokens, heads of 64: 27.5 us for 25.8; 64 of up to 8192, of 128: 103.3 for 101.4).
  */
 struct End4 { float by, theirs; float* from; };
 template <uint32_t D>
@@ -196,12 +201,12 @@ __device__ __forceinline__ End4 end_of(const Attend4& a, size_t token, size_t qu
 {
 	const size_t row = token * a.batch.query_heads + query_head;
 	End4 e{ 1.0f, 0.0f, nullptr };
-	if (a.rows && !a.prefix_starts) {
+	if (!a.prefix_starts) {
 		e.from = a.rows + row * D;
 		if (says) *(float2*)(a.row_sums + 2 * row) = float2{ m * scale, l };
 		return e;
 	}
-	if (a.rows && has_prefix(a, token)) {
+	if (has_prefix(a, token)) {
 		const float2 p = *(const float2*)(a.row_sums + 2 * row);
 		const float mine = m * scale, top = fmaxf(mine, p.x), lowest = top == -__builtin_inff() ? 0.0f : top;
 		e.by = exp2_(mine - lowest);
@@ -211,7 +216,7 @@ __device__ __forceinline__ End4 end_of(const Attend4& a, size_t token, size_t qu
 		m = top;
 		scale = 1.0f;
 	}
-	const float by = l > 0.0f ? 1.0f / l : l == l ? 0.0f : l; /* a row that sees nothing is zero; NaN stays */
+	const float by = part_of(l);
 	e.by *= by;
 	e.theirs *= by;
 	if (says && a.lse) a.lse[row] = l == 0.0f ? -__builtin_inff() : (m * scale + log2f(l * LOWERED)) * 0.693147180559945309f;
@@ -219,7 +224,7 @@ __device__ __forceinline__ End4 end_of(const Attend4& a, size_t token, size_t qu
 }
 __device__ __forceinline__ void put4(const Attend4& a, const End4& e, char* to, uint32_t channel, const f32x4& sums)
 {
-	if (a.rows && !a.prefix_starts) {
+	if (!a.prefix_starts) {
 		*(f32x4*)(e.from + channel) = sums;
 		return;
 	}
@@ -254,7 +259,7 @@ struct Tile4 {
  * end last. Short sequences: 7 to 9 us, of which 4.5 are a launch with its first load and last store, the rest loads that wait for each other
  * (length, table, codes).
  */
-template <int J>
+template <int J, bool SHARED>
 __global__ void __launch_bounds__(256, J <= 4 ? 3 : 2)
 attend4_kernel(Attend4 a)
 {
@@ -498,10 +503,21 @@ attend4_kernel(Attend4 a)
 	if (parts == 1) {
 		if (wave != 0 || !row.there) return;
 		const size_t token = seq.first + row.token, query_head = (size_t)head * a.batch.group + row.head;
-		const End4 e = end_of<D>(a, token, query_head, all, row_scale, sum, kg == 0);
 		char* to = (char*)a.out + 2 * (token * a.out_token + query_head * a.out_head);
+		if constexpr (SHARED) {
+			const End4 e = end_of<D>(a, token, query_head, all, row_scale, sum, kg == 0);
 #pragma unroll
-		for (int c = 0; c < 2 * J; ++c) put4(a, e, to, 16 * c + 4 * kg, o[c]);
+			for (int c = 0; c < 2 * J; ++c) put4(a, e, to, 16 * c + 4 * kg, o[c]);
+		} else {
+			const float by = part_of(sum);
+#pragma unroll
+			for (int c = 0; c < 2 * J; ++c) {
+				float v[4];
+				for (int r = 0; r < 4; ++r) v[r] = o[c][r] * by;
+				store_out4(a, to, 16 * c + 4 * kg, v);
+			}
+			if (kg == 0 && a.lse) a.lse[token * a.batch.query_heads + query_head] = sum == 0.0f ? -__builtin_inff() : (all * row_scale + log2f(sum * LOWERED)) * 0.693147180559945309f;
+		}
 		return;
 	}
 
@@ -579,10 +595,20 @@ attend4_kernel(Attend4 a)
 				for (uint32_t g = 1; g < groups; ++g) mine += shares[g * across + tid];
 		}
 		if (group != 0 || e >= quads) continue;
+		const float s1 = total[0][r];
+		[[maybe_unused]] const float by = part_of(s1);
 		const Row4 to_row = row_of(a, seq, row_tile, r);
 		const size_t token = seq.first + to_row.token, query_head = (size_t)head * a.batch.group + to_row.head;
-		const End4 end_row = end_of<D>(a, token, query_head, most[0][r], 1.0f, total[0][r], e % (D / 4) == 0);
-		put4(a, end_row, (char*)a.out + 2 * (token * a.out_token + query_head * a.out_head), 4 * (e % (D / 4)), mine);
+		char* to = (char*)a.out + 2 * (token * a.out_token + query_head * a.out_head);
+		if constexpr (SHARED) {
+			const End4 end_row = end_of<D>(a, token, query_head, most[0][r], 1.0f, s1, e % (D / 4) == 0);
+			put4(a, end_row, to, 4 * (e % (D / 4)), mine);
+		} else {
+			float v[4];
+			for (int i = 0; i < 4; ++i) v[i] = mine[i] * by;
+			store_out4(a, to, 4 * (e % (D / 4)), v);
+			if (e % (D / 4) == 0 && a.lse) a.lse[token * a.batch.query_heads + query_head] = s1 == 0.0f ? -__builtin_inff() : (most[0][r] + log2f(s1 * LOWERED)) * 0.693147180559945309f;
+		}
 	}
 }
 
@@ -687,7 +713,7 @@ __device__ __forceinline__ Share4 share_of(const Attend4& a, uint32_t g)
  * 32 and 64 channels have two work-groups on a compute unit (376 and 405 us with one, 321 and 375 with two, before the shares), for which 64 channels keep 4 to 12
  * registers in memory. So do wide heads, whose sums and queries are more than the registers hold: 192 channels 2, 224 19 to 33, 256 50 to 72 (1277 us, 635 TFLOP/s).
  */
-template <int J>
+template <int J, bool SHARED>
 __device__ __forceinline__ void many_unit(const Attend4& a, uint8_t* many, uint32_t (*blocks_there)[4], uint32_t entry, uint32_t head, uint32_t begin, uint32_t until,
                                           bool whole, uint32_t parts, uint32_t slot)
 {
@@ -890,11 +916,23 @@ __device__ __forceinline__ void many_unit(const Attend4& a, uint8_t* many, uint3
 		((uint2*)(a.partial + (size_t)(a.tiles_per_split ? 1 : 2) * a.splits * (256 * (D + 2))))[entry * a.cache.heads + head] = uint2{ blockIdx.x, parts };
 	if (!there) return;
 	if (whole) {
-		const End4 end_row = end_of<D>(a, seq.first + token, query_head, m, row_scale, l, h == 0);
 		char* to = (char*)a.out + 2 * ((size_t)(seq.first + token) * a.out_token + (size_t)query_head * a.out_head);
+		if constexpr (SHARED) {
+			const End4 end_row = end_of<D>(a, seq.first + token, query_head, m, row_scale, l, h == 0);
 #pragma unroll
-		for (int j = 0; j < J; ++j)
-			for (int e = 0; e < 4; ++e) put4(a, end_row, to, 32 * j + 8 * e + 4 * h, f32x4{ o[j][4 * e], o[j][4 * e + 1], o[j][4 * e + 2], o[j][4 * e + 3] });
+			for (int j = 0; j < J; ++j)
+				for (int e = 0; e < 4; ++e) put4(a, end_row, to, 32 * j + 8 * e + 4 * h, f32x4{ o[j][4 * e], o[j][4 * e + 1], o[j][4 * e + 2], o[j][4 * e + 3] });
+		} else {
+			const float by = part_of(l);
+#pragma unroll
+			for (int j = 0; j < J; ++j)
+				for (int e = 0; e < 4; ++e) {
+					float v[4];
+					for (int r = 0; r < 4; ++r) v[r] = o[j][4 * e + r] * by;
+					store_out4(a, to, 32 * j + 8 * e + 4 * h, v);
+				}
+			if (h == 0 && a.lse) a.lse[(size_t)(seq.first + token) * a.batch.query_heads + query_head] = l == 0.0f ? -__builtin_inff() : (m * row_scale + log2f(l * LOWERED)) * 0.693147180559945309f;
+		}
 		return;
 	}
 
@@ -907,7 +945,7 @@ __device__ __forceinline__ void many_unit(const Attend4& a, uint8_t* many, uint3
 	if (h == 0) *(float2*)(to + 256 * D + 2 * r) = float2{ m * row_scale, l };
 }
 
-template <int J, bool SHARES>
+template <int J, bool SHARES, bool SHARED>
 __global__ void __launch_bounds__(512, J <= 2 ? 4 : 2)
 attend4_many_kernel(Attend4 a)
 {
@@ -919,7 +957,7 @@ attend4_many_kernel(Attend4 a)
 		const uint32_t weight = many_tiles(a, entry / a.row_tiles, entry % a.row_tiles), begin = part * a.tiles_per_split;
 		if (begin >= weight) return;
 		const uint32_t parts = (weight + a.tiles_per_split - 1) / a.tiles_per_split;
-		many_unit<J>(a, many, blocks_there, entry, unit % heads, begin, min(weight, begin + a.tiles_per_split), parts == 1, parts, blockIdx.x);
+		many_unit<J, SHARED>(a, many, blocks_there, entry, unit % heads, begin, min(weight, begin + a.tiles_per_split), parts == 1, parts, blockIdx.x);
 	} else {
 		__shared__ Share4 share; /* (in registers it would be there through all the work) */
 		const Share4 mine = share_of(a, blockIdx.x);
@@ -937,7 +975,7 @@ attend4_many_kernel(Attend4 a)
 			const bool whole = begin == 0 && until == weight;
 			uint32_t parts = 1;
 			if (!whole && begin == 0) parts = share_with(share.total, share.to - left + weight - 1, share.shares) - blockIdx.x + 1;
-			if (weight) many_unit<J>(a, many, blocks_there, entry, head, begin, until, whole, parts, 2 * blockIdx.x + (begin == 0));
+			if (weight) many_unit<J, SHARED>(a, many, blocks_there, entry, head, begin, until, whole, parts, 2 * blockIdx.x + (begin == 0));
 			if (!shared) {
 				const uint32_t next = entry * heads + head + gridDim.x;
 				entry = next / heads;
@@ -958,7 +996,7 @@ attend4_many_kernel(Attend4 a)
 /* Joins the parts of many rows: 256 rows of sums are more than one work-group should read alone, so they have a kernel. A wavefront takes a row, 8 J
  * lanes 4 channels each of every (64 / 8 J)-th part. */
 constexpr uint32_t JOIN_GROUPS = 64; /* work-groups a unit */
-template <int J>
+template <int J, bool SHARED>
 __global__ void __launch_bounds__(256)
 join4_kernel(Attend4 a)
 {
@@ -1000,11 +1038,52 @@ join4_kernel(Attend4 a)
 			if (group == 0) { mine += more; sum += more_sum; }
 		}
 		if (group != 0) continue;
+		[[maybe_unused]] const float by = part_of(sum);
 		const uint64_t x = first_row + r;
 		const size_t to_token = seq.first + x / a.batch.group, to_head = (size_t)head * a.batch.group + x % a.batch.group;
-		const End4 end_row = end_of<D>(a, to_token, to_head, top, 1.0f, sum, at == 0);
-		put4(a, end_row, (char*)a.out + 2 * (to_token * a.out_token + to_head * a.out_head), 4 * at, mine);
+		char* to = (char*)a.out + 2 * (to_token * a.out_token + to_head * a.out_head);
+		if constexpr (SHARED) {
+			const End4 end_row = end_of<D>(a, to_token, to_head, top, 1.0f, sum, at == 0);
+			put4(a, end_row, to, 4 * at, mine);
+		} else {
+			float v[4];
+			for (int e = 0; e < 4; ++e) v[e] = mine[e] * by;
+			store_out4(a, to, 4 * at, v);
+			if (at == 0 && a.lse) a.lse[to_token * a.batch.query_heads + to_head] = sum == 0.0f ? -__builtin_inff() : (top + log2f(sum * LOWERED)) * 0.693147180559945309f;
+		}
 	}
+}
+
+template <int J, bool SHARED>
+static int launch_attend4_of(const Attend4& a, const Plan4& plan)
+{
+	if (plan.many) {
+		constexpr uint32_t bytes = 2 * (64 * (64 * J + 16) + 32 * J * 144);
+		if (bytes > 65536) { /* more LDS than a launch may ask for unannounced, on this device */
+			static int allowed = -1;
+			const DeviceInfo* dev = nullptr;
+			const int rc = device_info(&dev);
+			if (rc) return rc;
+			if (allowed != dev->device) {
+				KMX_HIP(hipFuncSetAttribute((const void*)attend4_many_kernel<J, false, SHARED>, hipFuncAttributeMaxDynamicSharedMemorySize, (int)bytes));
+				KMX_HIP(hipFuncSetAttribute((const void*)attend4_many_kernel<J, true, SHARED>, hipFuncAttributeMaxDynamicSharedMemorySize, (int)bytes));
+				allowed = dev->device;
+			}
+		}
+		if (a.tiles_per_split == 0) KMX_LAUNCH_KERNEL((attend4_many_kernel<J, true, SHARED>), dim3(a.splits), dim3(512), bytes, stream(), a);
+		else KMX_LAUNCH_KERNEL((attend4_many_kernel<J, false, SHARED>), dim3(a.splits), dim3(512), bytes, stream(), a);
+		KMX_LAUNCH_CHECK("attend4_many_kernel");
+		if (a.joined) {
+			KMX_LAUNCH_KERNEL((join4_kernel<J, SHARED>), dim3((unsigned)(plan.units * JOIN_GROUPS)), dim3(256), 0, stream(), a);
+			KMX_LAUNCH_CHECK("join4_kernel");
+		}
+		return KMX_OK;
+	}
+	if (a.batch.sequences > 65535 || (uint64_t)a.row_tiles * a.splits > 65535)
+		return fail(KMX_ERR_UNSUPPORTED, "kmx_cache4_attend: %u sequences of %u queries are too many for one call", a.batch.sequences, a.batch.max_queries);
+	KMX_LAUNCH_KERNEL((attend4_kernel<J, SHARED>), dim3(a.cache.heads, a.batch.sequences, a.row_tiles * a.splits), dim3(256), 0, stream(), a);
+	KMX_LAUNCH_CHECK("attend4_kernel");
+	return KMX_OK;
 }
 
 template <int J>
@@ -1014,33 +1093,7 @@ int launch_attend4(Attend4 a, const Plan4& plan)
 	a.splits = plan.splits;
 	a.tiles_per_split = plan.tiles_per_split;
 	a.joined = plan.joined;
-	if (plan.many) {
-		constexpr uint32_t bytes = 2 * (64 * (64 * J + 16) + 32 * J * 144);
-		if (bytes > 65536) { /* more LDS than a launch may ask for unannounced, on this device */
-			static int allowed = -1;
-			const DeviceInfo* dev = nullptr;
-			const int rc = device_info(&dev);
-			if (rc) return rc;
-			if (allowed != dev->device) {
-				KMX_HIP(hipFuncSetAttribute((const void*)attend4_many_kernel<J, false>, hipFuncAttributeMaxDynamicSharedMemorySize, (int)bytes));
-				KMX_HIP(hipFuncSetAttribute((const void*)attend4_many_kernel<J, true>, hipFuncAttributeMaxDynamicSharedMemorySize, (int)bytes));
-				allowed = dev->device;
-			}
-		}
-		if (a.tiles_per_split == 0) KMX_LAUNCH_KERNEL((attend4_many_kernel<J, true>), dim3(a.splits), dim3(512), bytes, stream(), a);
-		else KMX_LAUNCH_KERNEL((attend4_many_kernel<J, false>), dim3(a.splits), dim3(512), bytes, stream(), a);
-		KMX_LAUNCH_CHECK("attend4_many_kernel");
-		if (a.joined) {
-			KMX_LAUNCH_KERNEL((join4_kernel<J>), dim3((unsigned)(plan.units * JOIN_GROUPS)), dim3(256), 0, stream(), a);
-			KMX_LAUNCH_CHECK("join4_kernel");
-		}
-		return KMX_OK;
-	}
-	if (a.batch.sequences > 65535 || (uint64_t)a.row_tiles * a.splits > 65535)
-		return fail(KMX_ERR_UNSUPPORTED, "kmx_cache4_attend: %u sequences of %u queries are too many for one call", a.batch.sequences, a.batch.max_queries);
-	KMX_LAUNCH_KERNEL((attend4_kernel<J>), dim3(a.cache.heads, a.batch.sequences, a.row_tiles * a.splits), dim3(256), 0, stream(), a);
-	KMX_LAUNCH_CHECK("attend4_kernel");
-	return KMX_OK;
+	return a.rows ? launch_attend4_of<J, true>(a, plan) : launch_attend4_of<J, false>(a, plan);
 }
 
 } // namespace kmx
