@@ -64,7 +64,7 @@ int kmx_prompt_attend(const kmx_prompt* prompt, int type, const void* q, size_t 
 	if (rc) return rc;
 	const uint32_t J = b.dim / 32;
 	const PromptPlan plan = plan_prompt(PromptShape{ J, a.heads, a.group, a.sequences, a.max_queries, a.max_tokens, dev->compute_units });
-	if (plan.units == 0) return fail(KMX_ERR_UNSUPPORTED, "kmx_prompt_attend: too many queries for one call");
+	if (!prompt_launches(plan)) return fail(KMX_ERR_UNSUPPORTED, "kmx_prompt_attend: %u sequences of up to %u queries are too many for one call", b.sequences, a.max_queries);
 	if (const size_t floats = prompt_floats(plan, J)) {
 		const int rc2 = place_cache4("kmx_prompt_attend", floats, &a.partial, "kmx_prompt_reserve");
 		if (rc2) return rc2;

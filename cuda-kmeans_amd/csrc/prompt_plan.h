@@ -50,6 +50,9 @@ inline PromptPlan plan_prompt(const PromptShape& s)
 	return plan;
 }
 
+/* a launch has fewer than 2^32 threads: 2^24 work-groups of 128 rows, 2^23 of 256 */
+inline bool prompt_launches(const PromptPlan& plan) { return plan.units && (uint64_t)plan.units * plan.parts <= 0xFFFFFFFFu / (plan.wide ? 512u : 256u); }
+
 /* floats of work space of a call, and the most of any (no more work-groups than the chip holds have parts: 51 MB at 192 channels) */
 inline size_t prompt_floats(const PromptPlan& plan, uint32_t J) { return plan.parts > 1 ? (size_t)plan.units * plan.parts * (plan.wide ? 256 : 128) * (32 * (size_t)J + 2) : 0; }
 inline size_t most_prompt_floats(uint32_t J, uint32_t compute_units) { return (J <= 6 ? 256 : 128) * (size_t)compute_units * (32 * (size_t)J + 2); }
