@@ -156,12 +156,17 @@ int kmx_rotary_turns(uint32_t channels, double base, double stretch, double leng
 	if (!(length >= 0.0 && std::isfinite(length)) || !(slow >= 0.0 && std::isfinite(slow)) || !(fast >= slow && std::isfinite(fast)))
 		return fail(KMX_ERR_INVALID_ARGUMENT, "kmx_rotary_turns: length %g, slow %g and fast %g: not negative, fast not below slow", length, slow, fast);
 	if (channels && !turns) return fail(KMX_ERR_INVALID_ARGUMENT, "kmx_rotary_turns: null pointer");
-	for (uint32_t i = 0; i < channels / 2; ++i) {
+	const auto frequency = [&](uint32_t i) {
 		const double f = std::pow(base, -2.0 * i / channels) / 6.283185307179586476925286766559; /* turns a position */
 		const double made = length * f;
 		double share = 0.0; /* of the frequency as it is */
 		if (length > 0.0) share = made >= fast ? 1.0 : made <= slow ? 0.0 : (made - slow) / (fast - slow);
-		const double g = f * (share + (1.0 - share) / stretch), part = g - std::floor(g); /* whole turns are none */
+		return f * (share + (1.0 - share) / stretch);
+	};
+	for (uint32_t i = 0; i < channels / 2; ++i)
+		if (!std::isfinite(frequency(i))) return fail(KMX_ERR_INVALID_ARGUMENT, "kmx_rotary_turns: base %g and stretch %g: the frequency of pair %u is not finite", base, stretch, i);
+	for (uint32_t i = 0; i < channels / 2; ++i) {
+		const double g = frequency(i), part = g - std::floor(g); /* whole turns are none */
 		const double scaled = std::nearbyint(std::ldexp(part, 64));
 		turns[i] = scaled >= 18446744073709551616.0 ? 0 : (uint64_t)scaled;
 	}
