@@ -208,6 +208,7 @@ int kmx_rotary(int type, const kmx_rotary_rows* rows, uint32_t sets, uint32_t to
 	}
 	if (heads == 0 || (channels == 0 && !copies)) return KMX_OK;
 	if (!positions || (channels && !turns)) return fail(KMX_ERR_INVALID_ARGUMENT, "kmx_rotary: null positions or turns");
+	if ((uintptr_t)positions % 4 || (uintptr_t)turns % 8) return fail(KMX_ERR_INVALID_ARGUMENT, "kmx_rotary: positions start at multiples of 4 bytes, turns of 8");
 	a.positions = positions;
 	a.turns = turns;
 	a.tokens = tokens;

@@ -532,7 +532,8 @@ int kmx_cache4_evict(const kmx_cache4* cache, const kmx_cache4_batch* batch, flo
  * Rotary positions: of each row the first `channels` channels are pairs (a, b) -- i and i + channels / 2 with `halves`, else 2 i and 2 i + 1 -- that become
  * gain (a cos x - b sin x), gain (a sin x + b cos x), x = 2 pi positions[token] turns[i] / 2^64, with `inverse` -x (times gain^2 that is the way back, and for a gradient the
  * transpose). The other channels stay. In floats, rounded to the type once. Up to 4 sets of rows (queries, keys) with the positions of the same tokens in one call; out is in, with its
- * strides, or apart from it. F32, F16, BF16; element (token, head, channel) as for kmx_cache4_write. positions may be negative.
+ * strides, or apart from it; the sets' outputs lie apart from one another. F32, F16, BF16; element (token, head, channel) as for kmx_cache4_write. positions may be negative.
+ * positions (4-byte aligned) and turns (8-byte aligned) lie in device memory.
  */
 typedef struct kmx_rotary_rows {
 	const void* in;
@@ -544,7 +545,7 @@ typedef struct kmx_rotary_rows {
 	uint32_t heads;
 } kmx_rotary_rows;
 
-/* turns[channels / 2] as kmx_rotary takes them, host arrays: the frequency of pair i, f = base^(-2 i / channels) radians a position, in 2^-64 of a turn. Stretched for contexts
+/* turns[channels / 2], a host array, which the caller copies to the device for kmx_rotary: the frequency of pair i, f = base^(-2 i / channels) radians a position, in 2^-64 of a turn. Stretched for contexts
  * longer than the `length` that was trained on: f (share + (1 - share) / stretch), where share goes from 0, at `slow` turns over that length and less, to 1, at `fast` and more
  * (length 0: share is 0, all frequencies are divided; stretch 1: none). Host only. */
 int kmx_rotary_turns(uint32_t channels, double base, double stretch, double length, double slow, double fast, uint64_t* turns);
