@@ -885,6 +885,15 @@ static int take_rows(const char* who, const kmx_cache4* cache, const kmx_cache4_
 	return KMX_OK;
 }
 
+/* what a launch has room for, asked before anything is launched */
+static int check_launch(const char* who, const Batch4& b, const Plan4& plan)
+{
+	if (plan.units >= MOST_UNITS) return fail(KMX_ERR_UNSUPPORTED, "%s: too many queries for one call", who);
+	if (!plan.many && (b.sequences > 65535 || (uint64_t)plan.row_tiles * plan.splits > 65535))
+		return fail(KMX_ERR_UNSUPPORTED, "%s: %u sequences of %u queries are too many for one call", who, b.sequences, b.max_queries);
+	return KMX_OK;
+}
+
 static int launch_attend(const Attend4& a, const Plan4& plan, uint32_t J)
 {
 	switch (J) {
@@ -1067,7 +1076,8 @@ int kmx_cache4_attend(const kmx_cache4* cache, const kmx_cache4_batch* batch, in
 	rc = device_info(&dev);
 	if (rc) return rc;
 	const Plan4 plan = plan_attend4(shape_of(cache, batch, a.batch.table_stride, a.top, *dev));
-	if (plan.units >= MOST_UNITS) return fail(KMX_ERR_UNSUPPORTED, "kmx_cache4_attend: too many queries for one call");
+	rc = check_launch("kmx_cache4_attend", a.batch, plan);
+	if (rc) return rc;
 	const size_t floats = plan_floats(plan, cache->dim / 32);
 	if (floats) {
 		rc = place_cache4("kmx_cache4_attend", floats, &a.partial);
@@ -1099,7 +1109,9 @@ int kmx_cache4_attend_shared(const kmx_cache4* cache, const kmx_cache4_batch* pr
 	const bool any = prefix->sequences && prefix->max_queries;
 	const Plan4 plan = plan_attend4(shape_of(cache, batch, a.batch.table_stride, 0, *dev));
 	const Plan4 ahead = plan_attend4(shape_of(cache, prefix, front.batch.table_stride, 0, *dev));
-	if (plan.units >= MOST_UNITS || (any && ahead.units >= MOST_UNITS)) return fail(KMX_ERR_UNSUPPORTED, "kmx_cache4_attend_shared: too many queries for one call");
+	rc = check_launch("kmx_cache4_attend_shared", a.batch, plan);
+	if (rc == KMX_OK && any) rc = check_launch("kmx_cache4_attend_shared", front.batch, ahead);
+	if (rc) return rc;
 	const size_t rows = any ? shared_floats(batch, cache->dim) : 0, mine = plan_floats(plan, J), theirs = any ? plan_floats(ahead, J) : 0;
 	float* space = nullptr;
 	if (rows + mine + theirs) {

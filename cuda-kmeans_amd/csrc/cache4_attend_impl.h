@@ -1079,8 +1079,6 @@ static int launch_attend4_of(const Attend4& a, const Plan4& plan)
 		}
 		return KMX_OK;
 	}
-	if (a.batch.sequences > 65535 || (uint64_t)a.row_tiles * a.splits > 65535)
-		return fail(KMX_ERR_UNSUPPORTED, "kmx_cache4_attend: %u sequences of %u queries are too many for one call", a.batch.sequences, a.batch.max_queries);
 	KMX_LAUNCH_KERNEL((attend4_kernel<J, SHARED>), dim3(a.cache.heads, a.batch.sequences, a.row_tiles * a.splits), dim3(256), 0, stream(), a);
 	KMX_LAUNCH_CHECK("attend4_kernel");
 	return KMX_OK;
