@@ -3,7 +3,8 @@
  *
  * For a row r (a query head of a query) that sees the tokens t < vis: o_r = sum_t p_rt v_t / l_r, p_rt = 2^(c s_rt - m_r), s_rt = +- q_r . k_t, c = |scale| log2(e),
  * l_r = sum_t p_rt; lse_r = ln 2 (m_r + log2 l_r). m_r is any number near the largest c s_rt: it is raised when one passes it by more than 2^RISE, and what
- * was added up before is lowered by as much.
+ * was added up before is lowered by as much. Exponents are c s + base, base = LIFT - m; where c s is far from zero that difference of two roundings is no small number any more, and they
+ * are c (s - shift) + LIFT, shift the score itself.
  */
 #ifndef KMX_PROMPT_ATTEND_IMPL_H
 #define KMX_PROMPT_ATTEND_IMPL_H
@@ -23,6 +24,8 @@ typedef short i16x4 __attribute__((ext_vector_type(4)));
  * reference by 2^RISE: half precision holds them up to 2^15, with 11 bits down to 2^-21 of the reference and none below 2^-32; bfloat16 has 8 bits of all of them.
  */
 constexpr float LIFT = 7.0f, MOST_SUM = 0x1p15f; /* 2^(LIFT + RISE), RISE = 8 */
+constexpr float FAR = 0x1p20f;            /* exponents of 2 from here on: below it the base is off by 2^-5 at most, the same for all tokens */
+constexpr float NOTHING = 3.4028235e38f; /* the base of rows that have no token with a weight so far: the first score that is a number comes to an infinity, and raises */
 
 __device__ __forceinline__ f32x16 product(const u32x4& a, const u32x4& b, const f32x16& c, __bf16)
 {
@@ -211,7 +214,8 @@ prompt_attend_kernel(PromptAttend a)
 		if (__any(found)) strange = 1;
 	};
 
-	float reference = -__builtin_inff(), base = 0.0f, l = 0.0f; /* (the first tile's raise makes them) */
+	float base = NOTHING, shift = 0.0f, l = 0.0f;
+	float most_sum = MOST_SUM; /* no sum is small enough where rows of the wavefront have a shift */
 	f32x16 o[J];
 #pragma unroll
 	for (int j = 0; j < J; ++j)
@@ -249,13 +253,22 @@ prompt_attend_kernel(PromptAttend a)
 		float top = sc.s[0];
 #pragma unroll
 		for (int e = 1; e < 16; ++e) top = fmaxf(top, sc.s[e]);
-		top = both_halves_most(top) * a.factor;
-		const float higher = fmaxf(reference, top), less = higher == reference ? 1.0f : __builtin_amdgcn_exp2f(reference - higher);
-		reference = higher;
-		base = higher == -__builtin_inff() ? 3.4028235e38f : LIFT - higher; /* (nothing with a weight so far: the first score that is a number raises) */
+		top = both_halves_most(top);
+		const float most = top * a.factor, old_base = base, old_shift = shift;
+		if (fmaf(top - shift, a.factor, base) > LIFT) {
+			const bool away = !(fabsf(most) < FAR);
+			shift = away ? top : 0.0f;
+			base = away ? LIFT : LIFT - most;
+		}
+		const float less = __builtin_amdgcn_exp2f(fminf(fmaf(old_shift - shift, a.factor, base - old_base), 0.0f)); /* (1 where there was nothing, or an infinity) */
+		most_sum = __builtin_bit_cast(float, __builtin_amdgcn_readfirstlane(__builtin_bit_cast(int, __any(shift != 0.0f) ? -1.0f : MOST_SUM)));
 		l *= less;
 #pragma unroll
 		for (int j = 0; j < J; ++j) o[j] *= less;
+	};
+	auto lower = [&](Scores& sc) { /* scores that are not looked at again */
+#pragma unroll
+		for (int e = 0; e < 16; ++e) sc.s[e] -= shift;
 	};
 	auto hide = [&](Scores& sc, uint32_t tile) { /* tokens that a row does not see */
 		const int32_t from = (int32_t)(32 * (start + tile));
@@ -336,9 +349,10 @@ prompt_attend_kernel(PromptAttend a)
 			o[i / 2] = product(vop[batch % 2][n], before.w[i % 2], o[i / 2], T{});
 			slot(2 * i + 1);
 		}
-		/* a sum that is no more than 2^(LIFT + RISE) has no weight above it: no need to look for the largest score */
-		if (__any(!(sum <= MOST_SUM))) {
+		/* a sum that is no more than 2^(LIFT + RISE) has no weight above it: no need to look for the largest score. (Weights of scores far from zero are made here only.) */
+		if (__any(!(sum <= most_sum))) {
 			raise(now);
+			lower(now);
 			weigh(weights, sum, now);
 		}
 		l += sum;
@@ -434,6 +448,7 @@ prompt_attend_kernel(PromptAttend a)
 	const uint32_t id = __builtin_amdgcn_mbcnt_hi(~0u, __builtin_amdgcn_mbcnt_lo(~0u, 0)), n = id % 32, half = id / 32, r = wave_first + n;
 	l += __shfl_xor(l, 32);
 	if (r >= rows) return;
+	const float reference = fminf(fmaf(shift, last->factor, LIFT - base), NOTHING); /* (of a row without a weight the lowest number) */
 	if (last->parts > 1) { /* [unit][part]: [ROWS][channel] sums, [ROWS] of reference and sum of weights, for prompt_join_kernel */
 		float* const to = last->partial + ((size_t)unit * last->parts + part) * (ROWS * (32 * J + 2));
 #pragma unroll
@@ -482,7 +497,6 @@ prompt_join_kernel(PromptAttend a)
 	float top = -__builtin_inff();
 	for (uint32_t n = lane; n < parts; n += WAVE) top = fmaxf(top, left[n * PART + ROWS * D + 2 * r]);
 	for (int d = 1; d < WAVE; d *= 2) top = fmaxf(top, __shfl_xor(top, d));
-	const float lowest = top == -__builtin_inff() ? 0.0f : top;
 	float sum = 0.0f;
 	f32x4 mine{ 0.0f, 0.0f, 0.0f, 0.0f };
 	if (group < GROUPS)
@@ -490,7 +504,7 @@ prompt_join_kernel(PromptAttend a)
 		for (uint32_t n = group; n < parts; n += GROUPS) {
 			const float* from = left + n * PART;
 			const float2 ml = *(const float2*)(from + ROWS * D + 2 * r);
-			const float weight = __builtin_amdgcn_exp2f(ml.x - lowest);
+			const float weight = __builtin_amdgcn_exp2f(ml.x - top);
 			sum += ml.y * weight;
 			mine += *(const f32x4*)(from + (size_t)r * D + 4 * at) * weight;
 		}
