@@ -27,7 +27,7 @@ constexpr uint32_t WEIGH_TOKENS = 256; /* of a work-group, 64 a wavefront */
  * come by 64 at a time through LDS, a tile of 16 from each wavefront. The keys are the second operand (v_mfma_f32_16x16x32_f16): scores come out as [row][token], so that
  * the weights of a token, 2^(c s - log2(e) lse), are added up in the lane that has it, and four lanes at the end. Rows are asked for before the keys are unpacked.
  * Bound by the chain length - table - codes - products of its work-groups, three rounds of them, at 32 sequences of up to 2048 tokens (13.8 us; the packed keys alone take 5); 32 queries over
- * 32768 tokens 18.8 us, half of it powers. 128 tokens a work-group instead of 256: 16.9 for 15.6 and 141 for 116 (64 x 8192); 256 after 256 by the same work-groups: 17.5 for 15.6.
+ * 32768 tokens 18.8 us, vector units busy 42 % of it (powers 13 %), matrix cores 13 %: each work-group makes halves of the same rows of queries, 64 between two barriers. 128 tokens a work-group instead of 256: 16.9 for 15.6 and 141 for 116 (64 x 8192); 256 after 256 by the same work-groups: 17.5 for 15.6.
  */
 template <int J>
 __global__ void __launch_bounds__(256)
@@ -634,7 +634,7 @@ int kmx_cache4_evict(const kmx_cache4* cache, const kmx_cache4_batch* batch, flo
 	e.recent = recent;
 	const uint32_t places = keep < longest ? keep - recent - first : 0, rest = keep < longest ? longest - recent - first : 0;
 	e.words = (rest + 63) / 64;
-	const uint32_t room = (MOST_EVICT_BYTES - EVICT_WORD * e.words) / 6; /* beside the words: of 262144 tokens, for 6000 weights */
+	const uint32_t room = (MOST_EVICT_BYTES - EVICT_WORD * e.words) / 6; /* beside the words: of 262144 tokens, for 5632 weights */
 	e.cached = rest < EVICT_CACHED ? rest : EVICT_CACHED;
 	if (e.cached > room) e.cached = room;
 	const uint32_t bytes = evict_bytes(e.words, e.cached);

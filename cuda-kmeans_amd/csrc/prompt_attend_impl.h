@@ -118,10 +118,11 @@ template <int J> constexpr uint32_t prompt_lds() { return 3 * 32 * (key_row<J>()
  * piece of the second operand of [channel][row] = values . p; the values' columns are turned on the way from LDS (ds_read_b64_tr_b16).
  * While the vector units make a tile's probabilities, the matrix cores have the scores of the next one and the sums of the one before: nothing of these three waits for another.
  *
- * Bound: products of 4 rows tokens channels operations, at 128 channels. 8192 tokens, 32 heads of 128 over 8 in bf16, causal: 513 us, 1.07 of the 1.18 PFLOP/s that a large product of
- * matrices reaches here. At 64 channels the vector units have as much to do (a power a score) as the matrix cores: 6 prompts of up to 4096 in half precision 202 us. A single query over
- * 8192 tokens: 129 us by one work-group a head, 18 by parts (its keys and values take 7). Steps on the way, at 8192 tokens: scores, powers and sums one after the other 1191 us; side by
- * side 733; operands two products ahead 606; powers between the products 564; sums in place of the largest score 528; three places in LDS and buffer loads 521; eight wavefronts 513.
+ * 8192 tokens, 32 heads of 128 over 8 in bf16, causal: 525 us (cards differ, 515 to 537), 1.05 of the 1.33 PFLOP/s that a large product of matrices reaches here. The matrix cores are busy
+ * 52 % of that time, the vector units 43 %; LDS hands each operand to one product only, 128 KiB a tile and work-group, which at 128 bytes a cycle takes as long as the products. At 64
+ * channels no unit is full: 6 prompts of up to 4096 in half precision 206 us, matrix cores 25 %, vector units 40 %. A single query over 8192 tokens: 129 us by one work-group a head, 18 by
+ * parts (its keys and values take 7). Steps on the way, at 8192 tokens on one card: scores, powers and sums one after the other 1191 us; side by side 733; operands two products ahead 606;
+ * powers between the products 564; sums in place of the largest score 528; three places in LDS and buffer loads 521; eight wavefronts 513; scores far from zero, 1 more.
  */
 template <typename T, int J, int W, bool VEC>
 __global__ void __launch_bounds__(64 * W, (prompt_waves<J, W>()))

@@ -19,7 +19,7 @@ constexpr uint32_t PROMPT_LEAST = 2; /* tiles of a part at least */
 
 /*
  * Rows of 256 a work-group where heads have 160 or 192 channels (128 of them do not have the registers), and where heads have 96 or 128 and there are more than two rounds of
- * work-groups of 256; else 128. 8192 tokens, 32 heads of 128: 513 us by 256, 537 by 128; 4 x 500: 23.0 and 20.6; 6 prompts of up to 4096, 24 heads of 64 channels, 268 and 202.
+ * work-groups of 256; else 128. 8192 tokens, 32 heads of 128: 525 us by 256, 550 by 128; 4 x 500: 25.4 and 22.9; 6 prompts of up to 4096, 24 heads of 64 channels, 268 and 202 when both were built.
  *
  * Parts where the work-groups do not fill the chip. A tile takes a work-group about STEP us, so P parts save STEP tiles (1 - 1 / P); their sums, in 32 bits, are written and read again
  * and joined in a launch of its own, ROWS us for each part of all rows and 4 us once. P is where both together are least: sqrt(STEP tiles / ROWS).

@@ -317,17 +317,17 @@ int kmx_event_elapsed_ms(void* start, void* stop, float* ms); /* waits for `stop
  * ---- recorded iterations (no counterpart in the reference, whose loop launches kernel by kernel,
  *      cuda.hpp:70-88) ----
  * Between kmx_graph_begin and kmx_graph_end the launching calls (kmx_assign_f32, kmx_update_f32, kmx_fused_f32, kmx_iteration_f32,
- * kmx_bucket_sum_f32, kmx_fill_zero_u32, kmx_cache4_write, _read, _bound, _select and _attend) run nothing: their kernels, with the arguments of that moment, are recorded into
- * a HIP graph. kmx_graph_launch enqueues the whole recording on the library's stream as one unit, any number of times
+ * kmx_bucket_sum_f32, kmx_fill_zero_u32, kmx_cache4_write, _read, _bound, _select, _attend, _attend_shared, _weigh and _evict, kmx_rotary, kmx_prompt_attend) run nothing: their kernels, with the
+ * arguments of that moment, are recorded into a HIP graph. kmx_graph_launch enqueues the whole recording on the library's stream as one unit, any number of times
  * (the host driver records two ping-pong iterations once and replays them). Everything that allocates, copies or
  * waits is refused while recording; a call whose work space would have to grow is refused too -- make the same
  * calls once before recording. Per-kernel profiling events are not recorded.
  * A recording holds the addresses of its moment: those of its buffers, and of the work space where a call uses it, which a later call that needs more
  * of it, and kmx_shutdown, release. It is not launched after that; kmx_reserve_f32 for the largest shape beforehand keeps the work space where it is.
  * Updates with KMX_UPDATE_ATOMIC_SHM (kmx_update_f32, kmx_update_f64) whose sums fit LDS take their scratch memory from the static array of kmx_update_f32_noalloc instead, as do
- * kmx_cache4_select and kmx_cache4_attend where it has room (attention with up to 64 rows of a head, or to chosen pages, always), so
+ * kmx_cache4_select, kmx_cache4_attend and _attend_shared where it has room (attention with up to 64 rows of a head, or to chosen pages, always) and kmx_prompt_attend, so
  * recordings of nothing else stay valid. The same holds where the caller records the stream of kmx_set_stream with the runtime's own means, except that kmx_set_device,
- * kmx_reserve_f32, kmx_cache4_reserve or kmx_graph_begin has to come first (the array's address) and that replays are the caller's to keep from overlapping with other users of the array.
+ * kmx_reserve_f32, kmx_cache4_reserve, kmx_cache4_reserve_shared, kmx_prompt_reserve or kmx_graph_begin has to come first (the array's address) and that replays are the caller's to keep from overlapping with other users of the array.
  */
 int kmx_graph_begin(void);
 int kmx_graph_end(void** graph);
@@ -424,7 +424,7 @@ int kmx_probe_matrix_chain(int kind, const float* a, const float* b, const float
  * Bounds, where they are kept: for each page and head the largest and the smallest value of each channel of the keys, outwards in 127ths of
  * their largest magnitude m (dim + dim bytes: up(hi (1/m 127)), down(lo (1/m 127)) in floats), behind all of them those largest magnitudes over 127 (floats).
  * Places, pages and lengths on the device are not trusted: a place or page outside the cache is left out (reads as zeros, is not attended to).
- * kmx_cache4_select and kmx_cache4_attend use the library's work space (see kmx_cache4_reserve), recorded ones the static scratch array (see kmx_graph_begin), under the
+ * kmx_cache4_select, kmx_cache4_attend and kmx_cache4_attend_shared use the library's work space (see kmx_cache4_reserve), recorded ones the static scratch array (see kmx_graph_begin), under the
  * rules of the updates.
  */
 typedef enum kmx_type { KMX_F32 = 0, KMX_F16 = 1, KMX_BF16 = 2 } kmx_type;
@@ -510,16 +510,16 @@ int kmx_cache4_reserve_shared(const kmx_cache4* cache, const kmx_cache4_batch* p
 
 /*
  * Attention weights added up: weights[page][head][token of the page] += sum over the queries that see the token, and the query heads of the head, of
- * exp(scale q . k - lse), lse as kmx_cache4_attend (or _attend_shared, for prefix and own tokens each) has written it for the same queries. Tokens of a page that several
- * sequences have get all of their weights, each sequence's in one addition and in the order in which they come: with such pages the last bits may differ from call to call. Floats; nothing
- * is added for pages that are not there.
+ * exp(scale q . k - lse), lse as kmx_cache4_attend (or _attend_shared, for prefix and own tokens each) has written it for the same queries: a float, to whose rounding
+ * weights are exact (scores of some 2^20 and more: no longer to a tenth). Tokens of a page that several sequences have get all of their weights, each sequence's in one addition and in the
+ * order in which they come: with such pages the last bits may differ from call to call. Floats; nothing is added for pages that are not there.
  */
 int kmx_cache4_weigh(const kmx_cache4* cache, const kmx_cache4_batch* batch, int type, const void* q, size_t q_token_stride, size_t q_head_stride,
                      const float* lse, float scale, int causal, float* weights);
 
 /*
- * Sequences of more than `keep` tokens back to that many, for each head its own. Of the batch sequences, max_length (at most 262144), lengths and table are looked at; its pages
- * belong to one sequence each. The `first` first and `recent` last tokens stay, and of the others those of the largest weights, the lower place of two as heavy (NaN
+ * Sequences of more than `keep` tokens back to that many, for each head its own. Of the batch sequences, max_length (at most 262144, also where the table has room for less), lengths and
+ * table are looked at; its pages belong to one sequence each. The `first` first and `recent` last tokens stay, and of the others those of the largest weights, the lower place of two as heavy (NaN
  * are the lightest). The recent ones become the last ones, in their order; of the others those below keep - recent stay where they are, and what has to leave there makes room for
  * the others, the lowest place for the lowest: no more rows move than have to, and a sequence's tokens are not in their order any more but for the recent ones. Weights
  * move with their rows, and are zero at the places behind. kept[sequence][head][i] is the place that the token of place i had, -1 behind the last; left[sequence] what is left of
@@ -530,7 +530,7 @@ int kmx_cache4_evict(const kmx_cache4* cache, const kmx_cache4_batch* batch, flo
 /*
  * ---- around the cache (no counterpart in the reference) ----
  * Rotary positions: of each row the first `channels` channels are pairs (a, b) -- i and i + channels / 2 with `halves`, else 2 i and 2 i + 1 -- that become
- * gain (a cos x - b sin x), gain (a sin x + b cos x), x = 2 pi positions[token] turns[i] / 2^64, with `inverse` -x (times gain^2 that is the way back, and for a gradient the
+ * gain (a cos x - b sin x), gain (a sin x + b cos x), x = 2 pi positions[token] turns[i] / 2^64, with `inverse` -x (the way back but for a factor of gain^2, and for a gradient the
  * transpose). The other channels stay. In floats, rounded to the type once. Up to 4 sets of rows (queries, keys) with the positions of the same tokens in one call; out is in, with its
  * strides, or apart from it; the sets' outputs lie apart from one another. F32, F16, BF16; element (token, head, channel) as for kmx_cache4_write. positions may be negative.
  * positions (4-byte aligned) and turns (8-byte aligned) lie in device memory.
