@@ -87,3 +87,26 @@ def test_equal_scores_far_from_zero(km, gpu, kind, power, sign, dim, counts, len
                 assert np.all(np.abs(got[t, 0] - want) <= off), (t, causal, (np.abs(got[t, 0] - want) / off).max())
                 top = sign * 2.0 ** power + steps.max() * 2.0 ** step
                 assert np.all(np.abs(lse[t, 0] - (top + np.log(p.sum()))) <= 2.0 ** -21 * abs(top))
+
+
+@pytest.mark.parametrize("kind,loud", [(BF16, 2.0 ** 40), (F16, 2.0 ** 13)])
+@pytest.mark.parametrize("dim,counts,lengths", [(64, [100, 40], [300, 40]), (128, [70], [500]), (256, [40], [200]), (192, [3], [2500])])
+def test_rows_far_from_zero_beside_others(km, gpu, kind, loud, dim, counts, lengths):
+    """Every third query is so loud that its scores are far from zero: the others of its wavefront stay within the bounds that they have without it."""
+    rng = np.random.default_rng(dim)
+    s = Prompts(km, rng, 1, 2, dim, counts, lengths, kind)
+    s.q[::3] = from_bits(to_bits(s.q[::3] * loud, kind), kind)
+    got, lse = s.check(scale=1.0 if kind == F16 else None)
+    assert np.isfinite(got).all() and np.isfinite(lse).all()
+
+
+@pytest.mark.parametrize("kind", [F16, BF16])
+@pytest.mark.parametrize("token", [0, 31, 40, 79])
+def test_scores_of_plus_infinity(km, gpu, kind, token):
+    """A softmax over them is no number: rows that see one are NaN, and no others."""
+    rng = np.random.default_rng(5)
+    s = Prompts(km, rng, 1, 2, 64, [80], [80], kind)
+    s.q[..., 0] = 1
+    s.k[token, 0, 0] = np.inf
+    got, lse = s.attend()
+    assert np.isfinite(got[:token]).all() and np.isfinite(lse[:token]).all() and np.isnan(got[token:]).all() and not np.isfinite(lse[token:]).any()
