@@ -24,7 +24,7 @@ typedef short i16x4 __attribute__((ext_vector_type(4)));
  * reference by 2^RISE: half precision holds them up to 2^15, with 11 bits down to 2^-21 of the reference and none below 2^-32; bfloat16 has 8 bits of all of them.
  */
 constexpr float LIFT = 7.0f, MOST_SUM = 0x1p15f; /* 2^(LIFT + RISE), RISE = 8 */
-constexpr float FAR = 0x1p20f;            /* exponents of 2 from here on: below it the base is off by 2^-5 at most, the same for all tokens */
+constexpr float FAR = 0x1p20f;           /* exponents of 2 from here on: below it the base has two roundings of 2^-5 at most, the same for all tokens of a row */
 constexpr float NOTHING = 3.4028235e38f; /* the base of rows that have no token with a weight so far: the first score that is a number comes to an infinity, and raises */
 
 __device__ __forceinline__ f32x16 product(const u32x4& a, const u32x4& b, const f32x16& c, __bf16)
