@@ -558,9 +558,8 @@ int kmx_rotary(int type, const kmx_rotary_rows* rows, uint32_t sets, uint32_t to
  * token_starts[s] .. token_starts[s + 1] - 1 of the rows handed over; its queries are those of its last tokens: with `causal` query i of n sees the first tokens - n + i + 1 of
  * them, else all. out and lse as for kmx_cache4_attend; nothing that a query does not see, infinities and NaN among it, comes into its row. dim: a multiple of 32 up to 256.
  * F16 or BF16, products of numbers as they are, probabilities rounded to the type before the second product, sums in floats. Starts on the device are not trusted: a sequence whose
- * starts are not within the rows has none. Scores are floats, whatever their size; tokens whose score is minus infinity have no weight, and a query that sees
- * no others sees nothing.
- * out and lse lie apart from what is read. max_queries and max_tokens bound queries and tokens of a sequence (more is cut off). A bound on queries far above them costs
+ * starts are not within the rows has none. Scores are floats, whatever their size; tokens whose score is minus infinity have no weight (their values have to
+ * be numbers all the same), and a query that sees no others sees nothing. out and lse lie apart from what is read. max_queries and max_tokens bound queries and tokens of a sequence (more is cut off). A bound on queries far above them costs
  * work-groups that find nothing to do, and from 2^31 rows on -- that bound, held to the queries there are, times query heads and sequences -- the call is refused.
  */
 typedef struct kmx_prompt {
